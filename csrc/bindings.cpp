@@ -66,6 +66,17 @@ void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, c10::opt
 void opt_tick(at::Tensor clk, at::Tensor bc, double b1, double b2, bool bump_epoch);
 void lion_step(at::Tensor master, at::Tensor grad, at::Tensor mom, double lr, double b1, double b2,
                double wd, int64_t seed);
+// rotary.cu
+void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
+            c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign);
+// distill.cu
+void distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets,
+             at::Tensor rows, at::Tensor sums, c10::optional<at::Tensor> grad, c10::optional<at::Tensor> loss,
+             int64_t vocab, int64_t ignore_index, double temperature, double alpha);
+void distill_grad(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets,
+                  at::Tensor sums, at::Tensor g, at::Tensor grad, int64_t vocab, int64_t ignore_index,
+                  double temperature, double alpha);
+void scale_by_scalar(at::Tensor x, at::Tensor g);
 // p2p.cu
 std::vector<int64_t> peer_alloc(int64_t bytes);
 at::Tensor peer_handle(int64_t ptr);
@@ -150,6 +161,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope", &rope);
   m.def("rope_into", &rope_into);
   m.def("rope_into2", &rope_into2, "rope_into for two (x, out) pairs in one launch");
+  m.def("rotary", &rotary, "rotary positions for q and k: explicit positions, either layout, part of the head");
+  m.def("distill", &distill, "distillation loss rows, and in the same launch the mean and its gradient");
+  m.def("distill_grad", &distill_grad, "gradient of the distillation loss rows from their log-sum-exps");
+  m.def("scale_by_scalar", &scale_by_scalar, "x *= g[0] in place; nothing is touched where g[0] is 1");
   m.def("gelu_fwd", &gelu_fwd);
   m.def("gelu_bwd", &gelu_bwd);
   m.def("gelu_cdf_pdf", &gelu_cdf_pdf);

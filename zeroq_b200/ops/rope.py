@@ -4,9 +4,19 @@
 position-dependent angles ``pos * theta^(-2i/D)``; the backward is the rotation
 by the negated angle.  CUDA tensors run ``csrc/elementwise.cu``'s kernel, which
 computes the angles in fp32 per element (no cos/sin table in HBM).
+
+``rotary_embedding(q, k, positions, ...)`` is the general form: an explicit position
+for every token (packed documents, continued sequences), half or interleaved pairs,
+a rotary width below the head's, and :class:`RopeScaling` for contexts longer than
+the model was trained on.  CUDA tensors run ``csrc/rotary.cu``.
 """
 
 from __future__ import annotations
+
+import functools
+import math
+from dataclasses import dataclass
+from typing import Optional, Tuple
 
 import torch
 
@@ -125,3 +135,162 @@ class _RopeRows(torch.autograd.Function):
 
 def rope_rows_autograd(x: torch.Tensor, rope) -> torch.Tensor:
     return _RopeRows.apply(x, rope)
+
+
+# ---------------------------------------------------------------------------
+# explicit positions, pair layouts, part of the head, context scaling
+# ---------------------------------------------------------------------------
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the frequencies ``w_i = theta^(-2i/R)`` change for contexts ``factor`` times
+    longer than the ``original_max_position`` tokens a model was trained on.
+
+    * ``linear``: ``w_i / factor`` (positions are interpolated).
+    * ``ntk``: theta becomes ``theta * factor^(R/(R-2))``: the fastest pair keeps its
+      frequency, the slowest is divided by ``factor``.
+    * ``yarn``: pairs that turn more than ``beta_fast`` times within the original
+      context keep their frequency, those that turn less than ``beta_slow`` times are
+      divided by ``factor``, with a linear ramp over the pair index between them; cos
+      and sin are multiplied by ``attention_factor`` (default ``0.1 ln(factor) + 1``).
+      (Peng et al., "YaRN: Efficient Context Window Extension", 2023.)
+    """
+
+    kind: str
+    factor: float = 1.0
+    original_max_position: int = 4096
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: Optional[float] = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"RopeScaling: unknown kind {self.kind!r} (linear, ntk or yarn)")
+        if not (math.isfinite(self.factor) and self.factor >= 1.0):
+            raise ValueError(f"RopeScaling: factor must be at least 1, got {self.factor}")
+        if self.original_max_position < 1 or not 0 < self.beta_slow <= self.beta_fast:
+            raise ValueError("RopeScaling: original_max_position >= 1 and 0 < beta_slow <= beta_fast")
+
+
+@functools.lru_cache(maxsize=256)
+def _rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[RopeScaling]) -> Tuple[tuple, float]:
+    """(frequency of each pair in radians per position, factor of cos and sin), 64 bits."""
+    R, s = rotary_dim, 1.0 if scaling is None else scaling.factor
+    kind = None if scaling is None else scaling.kind
+    if kind == "ntk" and R > 2:
+        theta = theta * s ** (R / (R - 2))
+    freq = [theta ** (-2.0 * i / R) for i in range(R // 2)]
+    if kind == "linear":
+        return tuple(f / s for f in freq), 1.0
+    if kind != "yarn":
+        return tuple(freq), 1.0
+
+    def pair_of(turns):   # the (fractional) pair that turns so many times within the original context
+        return R * math.log(scaling.original_max_position / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low = max(0, math.floor(pair_of(scaling.beta_fast)))
+    high = min(R - 1, math.ceil(pair_of(scaling.beta_slow)))
+    out = []
+    for i, f in enumerate(freq):
+        ramp = min(1.0, max(0.0, (i - low) / max(high - low, 0.001)))
+        out.append(f * (1.0 - ramp) + f / s * ramp)
+    factor = scaling.attention_factor
+    return tuple(out), (0.1 * math.log(s) + 1.0 if factor is None else float(factor))
+
+
+@functools.lru_cache(maxsize=256)
+def _rope_turns(rotary_dim: int, theta: float, scaling: Optional[RopeScaling]) -> Tuple[torch.Tensor, float]:
+    """The frequencies in turns per position, as the CPU tensor that the kernel's
+    parameters are filled from (nothing of it is kept on a device)."""
+    freq, factor = _rope_frequencies(rotary_dim, theta, scaling)
+    return torch.tensor([f / (2 * math.pi) for f in freq], dtype=torch.float64, device="cpu"), factor
+
+
+def rotary_reference(x: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0,
+                     rotary_dim: Optional[int] = None, interleaved: bool = False,
+                     scaling: Optional[RopeScaling] = None) -> torch.Tensor:
+    """PyTorch form of :func:`rotary_embedding` for one tensor ``[..., S, H, D]``."""
+    R = x.shape[-1] if rotary_dim is None else rotary_dim
+    freq, factor = _rope_frequencies(R, float(theta), scaling)
+    ang = positions.double()[..., None, None] * torch.tensor(freq, dtype=torch.float64, device=x.device)
+    dt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    cos, sin = (torch.cos(ang) * factor).to(dt), (torch.sin(ang) * factor).to(dt)
+    xf = x.to(dt)
+    if interleaved:
+        a, b = xf[..., 0:R:2], xf[..., 1:R:2]
+        y = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+    else:
+        a, b = xf[..., : R // 2], xf[..., R // 2: R]
+        y = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return torch.cat([y, xf[..., R:]], dim=-1).to(x.dtype)
+
+
+def _rotary_launch(xs, positions, turns, factor, sign, interleaved):
+    """The kernel over one or two ``[..., H, D]`` tensors; contiguous outputs."""
+    flat = [t.flatten(0, -3) for t in xs]
+    flat = [t if t.stride(-1) == 1 else t.contiguous() for t in flat]
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+    out_flat = [t.flatten(0, -3) for t in outs]
+    two = len(xs) == 2
+    _ext.ext().rotary(flat[0], flat[1] if two else None, positions, turns, out_flat[0],
+                      out_flat[1] if two else None, bool(interleaved), factor, sign)
+    return outs
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, turns, factor, interleaved):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.meta = (turns, factor, interleaved)
+        if k is None:
+            return _rotary_launch([q], positions, turns, factor, 1.0, interleaved)[0], None
+        return tuple(_rotary_launch([q, k], positions, turns, factor, 1.0, interleaved))
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, = ctx.saved_tensors
+        turns, factor, interleaved = ctx.meta
+        given = [g for g in (gq, gk) if g is not None]
+        outs = iter(_rotary_launch(given, positions, turns, factor, -1.0, interleaved) if given else ())
+        dq = next(outs) if gq is not None else None
+        dk = next(outs) if gk is not None else None
+        return dq, dk, None, None, None, None
+
+
+def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                     theta: float = 10000.0, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                     scaling: Optional[RopeScaling] = None):
+    """Rotate ``q [..., S, Hq, D]`` and ``k [..., S, Hk, D]`` (or ``None``) by their tokens'
+    positions; returns new tensors ``(q', k')``, differentiable in q and k.
+
+    ``positions``: whole numbers, ``q.shape[:-2]`` or ``[S]`` (shared by the rows before
+    it).  Pair ``i`` of the first ``rotary_dim`` columns (default: all) turns by
+    ``position * w_i`` with ``w_i = theta^(-2i/rotary_dim)`` changed by ``scaling``;
+    pairs are columns ``(i, i + rotary_dim/2)``, or ``(2i, 2i + 1)`` with ``interleaved``.
+    The other columns pass through.  Angles are formed in 64 bits, so positions may be
+    far; the products are in 32 bits with one rounding.  bf16, fp16 or fp32, any strides."""
+    if q.dim() < 3:
+        raise ValueError(f"rotary_embedding: q must be [..., S, H, D], got {tuple(q.shape)}")
+    D = q.shape[-1]
+    R = D if rotary_dim is None else int(rotary_dim)
+    if R < 2 or R % 2 or R > D or R > 256:
+        raise ValueError(f"rotary_embedding: rotary_dim must be even, at most the head's {D} and at most 256, got {R}")
+    if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != D or k.dtype != q.dtype
+                          or k.device != q.device):
+        raise ValueError(f"rotary_embedding: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float64):
+        raise TypeError(f"rotary_embedding: bf16, fp16 or fp32 tensors, got {q.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rotary_embedding: positions must be int32 or int64, got {positions.dtype}")
+    if positions.device != q.device:
+        raise ValueError("rotary_embedding: positions must be on q's device")
+    if positions.shape != q.shape[:-2] and positions.shape != q.shape[-3:-2]:
+        raise ValueError(f"rotary_embedding: positions {tuple(positions.shape)} must be {tuple(q.shape[:-2])} "
+                         f"or {tuple(q.shape[-3:-2])}")
+    if not theta > 1.0:
+        raise ValueError(f"rotary_embedding: theta must be above 1, got {theta}")
+    if not q.is_cuda or q.dtype == torch.float64:
+        args = (positions, float(theta), R, interleaved, scaling)
+        return rotary_reference(q, *args), None if k is None else rotary_reference(k, *args)
+    turns, factor = _rope_turns(R, float(theta), scaling)
+    return _Rotary.apply(q, k, positions.reshape(-1).contiguous(), turns, factor, bool(interleaved))
