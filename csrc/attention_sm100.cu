@@ -49,7 +49,7 @@
 
 #include <cstdlib>
 
-#include "common.cuh"
+#include "attention_common.cuh"
 
 // defined in gemm_sm100.cu
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
@@ -81,12 +81,6 @@ struct AttSmem {
   static constexpr int kBar = kXSum + 2 * 128 * 4;
   static constexpr int kBytes = kBar + 256 + 1024;      // barriers + alignment slack
 };
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __global__ void __launch_bounds__(kAttThreads, 1)
 attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -460,60 +454,6 @@ struct Fwd2Smem {
   static constexpr int kBytes = kBar + 256 + 1024;
 };
 
-// Packed fp32 pairs (Blackwell f32x2 arithmetic: one instruction for two values).
-__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// 2^x for a pair, x <= 64, by range reduction and a degree-3 polynomial (see
-// above); x below -120 is clamped there (2^-120 ~ 7.5e-37 instead of 0).
-__device__ __forceinline__ void exp2_poly3_x2(float a0, float a1, float& p0, float& p1) {
-  const uint64_t x = f2_pack(fmaxf(a0, -120.0f), fmaxf(a1, -120.0f));
-  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);   // 1.5 * 2^23
-  const uint64_t t = f2_add(x, magic);        // round(x) in the low mantissa bits
-  const uint64_t f = f2_sub(x, f2_sub(t, magic));   // [-1/2, 1/2]
-  uint64_t p = f2_fma(f2_pack(0.05508868396282196f, 0.05508868396282196f), f,
-                      f2_pack(0.24260404706001282f, 0.24260404706001282f));
-  p = f2_fma(p, f, f2_pack(0.6932762265205383f, 0.6932762265205383f));
-  p = f2_fma(p, f, f2_pack(0.9999289512634277f, 0.9999289512634277f));
-  float q0, q1, t0, t1;
-  f2_unpack(p, q0, q1);
-  f2_unpack(t, t0, t1);
-  // the bits of t are (0x4B400000 + round(x)); shifted by 23 only round(x) << 23 remains
-  p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
-  p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
-}
-
 template <int POLY_EVERY, bool TRACE>
 __global__ void __launch_bounds__(kF2Threads, 1)
 attn_fwd2_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -880,26 +820,6 @@ constexpr int kBwdKStages = 3;     // dQ kernel K ring
 constexpr int kBwdVStages = 2;     // dQ kernel V ring
 constexpr int kBwdQStages = 2;     // dK/dV kernel Q and dO rings
 enum AttBwdErr { kErrBwdLoad = 311, kErrBwdMma = 312, kErrBwdCompute = 313 };
-
-// 64 consecutive columns of one TMEM row (this thread's lane) -> registers
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
-  tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-  tmem_ld_32x32b_x32(taddr + 32u, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-}
-
-// one 128-byte row of a 128-byte-swizzled smem atom (64 bf16) -> 32 TMEM columns
-__device__ __forceinline__ void copy_row_to_tmem(const uint8_t* atom_row, int row, uint32_t taddr) {
-  uint32_t v[32];
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const uint4 u = *reinterpret_cast<const uint4*>(atom_row + ((c ^ (row & 7)) << 4));
-    v[4 * c + 0] = u.x;
-    v[4 * c + 1] = u.y;
-    v[4 * c + 2] = u.z;
-    v[4 * c + 3] = u.w;
-  }
-  tmem_st_32x32b_x32(taddr, v);
-}
 
 struct BwdDqSmem {
   static constexpr int kTile = AttSmem::kTile, kAtom = AttSmem::kAtom;

@@ -1,0 +1,1241 @@
+// Attention over packed sequences on the 5th-generation tensor cores (sm_100a):
+// forward, and the backward that recomputes the probabilities.
+//
+// q, o: [T, Hq, D], k, v: [T, Hk, D], bf16 or fp16, D <= 128 a multiple of 8 (q, k,
+// v, do through TMA maps: any 16-byte-multiple strides), GQA (Hq a multiple of Hk).
+// Sequence i holds rows [cu[i], cu[i+1]); a query sees the keys of its own sequence,
+// with `causal` those up to its own position.  lse: [Hq, T] fp32, natural log.
+//
+//   S = scale·Q Kᵀ, P = softmax(S), O = P V
+//   dP = dO Vᵀ, dS = P ∘ (dP - delta), delta = rowsum(dO ∘ O)
+//   dQ = scale·dS K, dK = scale·dSᵀ Q, dV = Pᵀ dO
+//
+// A plan (packed_plan below) lists the row tiles of all sequences, longest work
+// first: the grid is (entries, heads) with as many entries as any division of T
+// rows into n sequences can have; blocks past the real count leave at once, but
+// for the first of them, which writes zeros to the rows of no sequence.
+//
+// Ragged ends: tiles are loaded whole, so rows past a sequence's end hold the next
+// sequence's values (or the TMA fill).  Scores of such keys are replaced (never
+// multiplied) and such queries' outputs are not stored; rows that enter a product
+// as its K dimension (V forward, K in dQ, Q and dO in dK/dV) are zeroed in shared
+// memory first, so that 0 · NaN of a neighbour or of unset padding cannot arise.
+//
+// MMAs are issued by a whole warp that stays converged, with one elected lane
+// inside: the descriptors then are warp-uniform values.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cudaTypedefs.h>
+
+#include "attention_common.cuh"
+
+// defined in gemm_sm100.cu
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
+zq::DeviceStatus* status_buffer(int device);
+
+namespace zq {
+
+constexpr int kVlRows = 128;
+enum VlErr { kErrVlLoad = 321, kErrVlMma = 322, kErrVlCompute = 323, kErrVlPlan = 324 };
+
+// One tile of a sequence.  slot: number of this 128-row tile over all sequences
+// (row statistics of the backward live in slots of 128 rows).
+struct __align__(16) VlTile {
+  int start, len, tile, slot;
+};
+// meta words: [0] 256-row tiles, [1] 128-row query tiles, [2] 128-row key tiles,
+// [3] first row of a sequence, [4] row behind the last sequence
+constexpr int kVlMeta = 8;
+
+struct VlParams {
+  const VlTile* tiles;
+  const int* meta;        // the plan's meta words
+  int count_at;           // which of them counts these tiles
+  int T, Hq, Hk, D, causal, slots;
+  float scale, scale_log2;
+  DeviceStatus* status;
+};
+
+template <bool FP16>
+__device__ __forceinline__ uint32_t vl_pack(float lo, float hi) {
+  if constexpr (FP16) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+template <bool FP16>
+__device__ __forceinline__ float2 vl_unpack(uint32_t w) {
+  if constexpr (FP16) {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+  } else {
+    return bf16x2_to_f2(w);
+  }
+}
+// kind::f16, fp32 accumulators; both operands of one type; `bmn`: B MN-major
+template <bool FP16>
+__host__ __device__ constexpr uint32_t vl_idesc(int M, int N, bool bmn) {
+  return (1u << 4) | (FP16 ? 0u : (1u << 7) | (1u << 10)) | (bmn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1,
+                                            int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// a tile of ROWS rows x DP columns: one swizzled atom per 64 columns
+template <int DP, int ROWS>
+__device__ __forceinline__ void vl_load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+#pragma unroll
+  for (int a = 0; a < DP / 64; ++a) tma_load_3d(dst + a * ROWS * 128, map, bar, a * 64, head, row);
+}
+
+// zeros to rows [from, ROWS) of such a tile, by 128 threads; then visible to the MMAs
+template <int DP, int ROWS>
+__device__ __forceinline__ void vl_zero_rows(uint8_t* tile, int from, int thread) {
+  for (int i = thread; i < (DP / 64) * ROWS; i += 128) {
+    const int row = i % ROWS;
+    if (row >= from) {
+      uint4* r = reinterpret_cast<uint4*>(tile + (i / ROWS) * ROWS * 128 + row * 128);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) r[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_proxy_async_smem();
+}
+
+// wait by all lanes, decided as one
+__device__ __forceinline__ bool vl_wait(uint64_t* bar, uint32_t parity, DeviceStatus* st, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, st, code));
+}
+
+// zeros to the rows of no sequence of one head of out [T, H, D] (contiguous)
+__device__ __forceinline__ void vl_zero_outside(uint16_t* out, int T, int H, int h, int D, const int* meta) {
+  const int first = meta[3], last = meta[4], per = D / 8;
+  const int64_t n = (int64_t)(first + (T - last)) * per;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    int row = (int)(i / per);
+    if (row >= first) row = row - first + last;
+    *reinterpret_cast<uint4*>(out + ((int64_t)row * H + h) * D + (i % per) * 8) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// N accumulator columns of this lane times f, rounded, to out; columns from D on do not exist
+template <bool FP16, int N>
+__device__ __forceinline__ void vl_store_row(uint32_t taddr, float f, uint16_t* out, int col0, int D, bool store) {
+#pragma unroll 1
+  for (int c = 0; c < N; c += 32) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(taddr + (uint32_t)c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 v;
+      v.x = vl_pack<FP16>(__uint_as_float(o[8 * i + 0]) * f, __uint_as_float(o[8 * i + 1]) * f);
+      v.y = vl_pack<FP16>(__uint_as_float(o[8 * i + 2]) * f, __uint_as_float(o[8 * i + 3]) * f);
+      v.z = vl_pack<FP16>(__uint_as_float(o[8 * i + 4]) * f, __uint_as_float(o[8 * i + 5]) * f);
+      v.w = vl_pack<FP16>(__uint_as_float(o[8 * i + 6]) * f, __uint_as_float(o[8 * i + 7]) * f);
+      if (store && col0 + c + 8 * i < D) *reinterpret_cast<uint4*>(out + col0 + c + 8 * i) = v;
+    }
+  }
+}
+
+// ============================================================================
+// Plan: tile tables of the packed sequences and each row's position.
+//
+// Blocks 0-2 build the tables (256-row tiles, 128-row query tiles, 128-row key
+// tiles), each sorted by the tile's causal work, longest first (a counting sort
+// over at most 1024 classes; the order inside a class only moves blocks about).
+// The other blocks write positions.  cu is taken as it is on the device: values
+// are clamped to [0, T] and to rising order, and a division that needs more tiles
+// than the table has loses what does not fit, with an error status.
+// ============================================================================
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanClasses = 1024;
+
+__device__ __forceinline__ int plan_bound(const int* cu, int i, int T) { return min(max(cu[i], 0), T); }
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __restrict__ cu, int n, int T, int cap256,
+                                                                   int cap128, VlTile* __restrict__ tiles,
+                                                                   int* __restrict__ base, int* __restrict__ meta,
+                                                                   int* __restrict__ positions, DeviceStatus* status) {
+  const int tid = threadIdx.x;
+  if (blockIdx.x >= 3) {
+    const int row = (blockIdx.x - 3) * kPlanThreads + tid;
+    if (row >= T) return;
+    int lo = 0, hi = n;   // the last i with cu[i] <= row
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cu[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    const int begin = plan_bound(cu, lo, T);
+    positions[row] = (lo < n && row >= begin) ? row - begin : 0;
+    return;
+  }
+  __shared__ int s_warp[32];
+  __shared__ int s_class[kPlanClasses];
+  __shared__ int s_run;
+  const int kind = blockIdx.x;                       // 0: 256-row tiles, 1: queries, 2: keys
+  const int rows = kind == 0 ? 256 : 128, cap = kind == 0 ? cap256 : cap128;
+  VlTile* out = tiles + (kind == 0 ? 0 : cap256 + (kind - 1) * cap128);
+  int* b = base + kind * (n + 1);
+  auto bounds = [&](int i, int& begin, int& len) {
+    begin = plan_bound(cu, i, T);
+    len = max(plan_bound(cu, i + 1, T) - begin, 0);
+  };
+  // b[i] = tiles of the sequences before i
+  if (tid == 0) s_run = 0;
+  for (int i = tid; i < kPlanClasses; i += kPlanThreads) s_class[i] = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int c = 0;
+    if (i < n) {
+      int begin, len;
+      bounds(i, begin, len);
+      c = (len + rows - 1) / rows;
+    }
+    int x = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if ((tid & 31) >= o) x += y;
+    }
+    if ((tid & 31) == 31) s_warp[tid >> 5] = x;
+    __syncthreads();
+    int before = s_run;
+    for (int w = 0; w < (tid >> 5); ++w) before += s_warp[w];
+    if (i < n) b[i] = before + x - c;
+    __syncthreads();
+    if (tid == kPlanThreads - 1) s_run = before + x;
+    __syncthreads();
+  }
+  const int want = s_run, total = min(want, cap);
+  if (tid == 0) {
+    b[n] = want;
+    meta[kind] = 0;
+    if (kind == 0) {
+      meta[3] = n > 0 ? plan_bound(cu, 0, T) : 0;
+      meta[4] = n > 0 ? max(plan_bound(cu, n, T), plan_bound(cu, 0, T)) : 0;
+    }
+    bool bad = want > cap;
+    if (bad) record_error(status, kErrVlPlan, want);
+  }
+  __syncthreads();
+  // classes of work, in units of 64 rows, halved until they fit
+  int shift = 0;
+  while (((T + 63) / 64 >> shift) >= kPlanClasses) ++shift;
+  auto tile_at = [&](int s, VlTile& t, int& cls) -> bool {
+    int lo = 0, hi = n - 1;   // the last sequence with b[i] <= s
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (b[mid] <= s) lo = mid; else hi = mid - 1;
+    }
+    bounds(lo, t.start, t.len);
+    t.tile = s - b[lo];
+    t.slot = s;
+    // a sequence whose tiles do not all fit is left out (its row statistics would not either)
+    if (b[lo + 1] > cap || t.tile * rows >= t.len) return false;
+    const int row = t.tile * rows;
+    const int work = kind == 2 ? t.len - row : min(row + rows, t.len);
+    cls = kPlanClasses - 1 - min(kPlanClasses - 1, (work + 63) / 64 >> shift);   // longest first
+    return true;
+  };
+  for (int s = tid; s < total; s += kPlanThreads) {
+    VlTile t;
+    int cls;
+    if (tile_at(s, t, cls)) atomicAdd(&s_class[cls], 1);
+  }
+  __syncthreads();
+  {   // exclusive scan over the classes (one per thread)
+    static_assert(kPlanClasses == kPlanThreads, "one class per thread");
+    const int c = s_class[tid];
+    int x = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if ((tid & 31) >= o) x += y;
+    }
+    if ((tid & 31) == 31) s_warp[tid >> 5] = x;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < (tid >> 5); ++w) before += s_warp[w];
+    s_class[tid] = before + x - c;
+    if (tid == kPlanThreads - 1) meta[kind] = before + x;
+  }
+  __syncthreads();
+  for (int s = tid; s < total; s += kPlanThreads) {
+    VlTile t;
+    int cls;
+    if (tile_at(s, t, cls)) out[atomicAdd(&s_class[cls], 1)] = t;
+  }
+}
+
+// ============================================================================
+// Forward: two query tiles (256 rows of one sequence and head) per CTA.
+//
+// Tensor memory: S_A 0-127, S_B 128-255, O_A 256.., O_B 384..; P (16-bit pairs)
+// is written over the first 64 columns of its tile's S.  Q_A and Q_B stay in
+// shared memory, K and V tiles of 128 keys stream through two-stage rings read by
+// both query tiles.  320 threads: warps 0-3 / 4-7 are the softmax warpgroup of
+// tile A / B (thread = query row = TMEM lane), warp 8 issues the MMAs in the order
+//     PV_A(j), S_A(j+1) | PV_B(j), S_B(j+1) | ...
+// so one tile's exponentials run beside the other's products; warp 9 loads.
+// The running maximum moves only when a row's maximum grows by more than 2^8 (O is
+// rescaled then); O / l and lse use the same one, so the result is exact.
+// When the sequence ends inside tile A, tile B does not exist and is skipped.
+// ============================================================================
+constexpr int kVfThreads = 320;
+constexpr int kVfStages = 2;
+constexpr float kVlRescale = 8.0f;
+
+template <int DP>
+struct VfSmem {
+  static constexpr int kTile = 128 * DP * 2;
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kVfStages * kTile;
+  static constexpr int kBar = kV + kVfStages * kTile;
+  static constexpr int kBytes = kBar + 256 + 1024;
+};
+
+template <bool FP16, int DP>
+__global__ void __launch_bounds__(kVfThreads, 1)
+attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ VlParams p,
+                       uint16_t* __restrict__ O, float* __restrict__ lse) {
+  using L = VfSmem<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* q_full = bars;
+  uint64_t* k_full = bars + 1;     // [kVfStages]
+  uint64_t* k_empty = bars + 3;
+  uint64_t* v_full = bars + 5;
+  uint64_t* v_empty = bars + 7;
+  uint64_t* s_full = bars + 9;     // [tile]
+  uint64_t* p_full = bars + 11;    // [tile], one arrival per softmax warp
+  uint64_t* pv_done = bars + 13;   // [tile]
+  uint64_t* drain = bars + 15;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int entry = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+  const int count = p.meta[p.count_at];
+  if (entry >= count) {
+    if (entry == count) vl_zero_outside(O, p.T, p.Hq, h, p.D, p.meta);
+    return;
+  }
+  const VlTile w = p.tiles[entry];
+  const int hk = h / (p.Hq / p.Hk);
+  const int row_a = w.tile * 256, row_b = row_a + 128;
+  const int nkt = (w.len + 127) / 128;
+  const int n_a = p.causal ? min(2 * w.tile + 1, nkt) : nkt;
+  const int n_b = row_b >= w.len ? 0 : p.causal ? min(2 * w.tile + 2, nkt) : nkt;   // n_b >= n_a, or none
+  const int n_max = max(n_a, n_b);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kVfStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 9) {
+    // ------------------------------------------------------------ TMA loader (one thread)
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, (n_b > 0 ? 2 : 1) * L::kTile);
+      vl_load_tile<DP, 128>(smem + L::kQ, &tmQ, q_full, h, w.start + row_a);
+      if (n_b > 0) vl_load_tile<DP, 128>(smem + L::kQ + L::kTile, &tmQ, q_full, h, w.start + row_b);
+      int k_issued = 0, v_issued = 0;
+      bool ok = true;
+      for (int j = 0; j < n_max && ok; ++j) {
+        const int st = j % kVfStages;
+        const uint32_t ph = ((j / kVfStages) & 1) ^ 1;
+        if (!mbar_wait(&k_empty[st], ph, p.status, kErrVlLoad)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[st], L::kTile);
+        vl_load_tile<DP, 128>(smem + L::kK + st * L::kTile, &tmK, &k_full[st], hk, w.start + j * 128);
+        k_issued = j + 1;
+        if (!mbar_wait(&v_empty[st], ph, p.status, kErrVlLoad)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[st], L::kTile);
+        vl_load_tile<DP, 128>(smem + L::kV + st * L::kTile, &tmV, &v_full[st], hk, w.start + j * 128);
+        v_issued = j + 1;
+      }
+      if (!ok) {  // let every copy this thread issued land before the CTA can exit
+        mbar_wait(q_full, 0, nullptr, 0);
+        for (int j = max(k_issued - kVfStages, 0); j < k_issued; ++j)
+          mbar_wait(&k_full[j % kVfStages], (j / kVfStages) & 1, nullptr, 0);
+        for (int j = max(v_issued - kVfStages, 0); j < v_issued; ++j)
+          mbar_wait(&v_full[j % kVfStages], (j / kVfStages) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer (whole warp)
+    constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 128, false);
+    constexpr uint32_t idesc_pv = vl_idesc<FP16>(128, DP, true);
+    const uint32_t q_base = smem_u32(smem + L::kQ), k_base = smem_u32(smem + L::kK), v_base = smem_u32(smem + L::kV);
+    auto wait_k = [&](int j) { return vl_wait(&k_full[j % kVfStages], (j / kVfStages) & 1, p.status, kErrVlMma); };
+    // S_x = Q_x K_jᵀ; `last`: nobody reads K_j after it
+    auto issue_s = [&](int x, int j, bool last) {
+      const uint64_t qd = umma_desc_sw128_kmajor(q_base + x * L::kTile);
+      const uint64_t kd = umma_desc_sw128_kmajor(k_base + (j % kVfStages) * L::kTile);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t off = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+          umma_f16_ss(tmem + (uint32_t)(x * 128), qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[x]);
+        if (last) umma_commit(&k_empty[j % kVfStages]);
+      }
+      __syncwarp();
+    };
+    // O_x += P_x V_j: P from tensor memory, V read MN-major
+    auto issue_pv = [&](int x, int j, bool last) {
+      const uint64_t vd = umma_desc_sw128_mnmajor(v_base + (j % kVfStages) * L::kTile, 16384u);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16_ts(tmem + 256u + (uint32_t)(x * 128), tmem + (uint32_t)(x * 128 + kk * 8), vd + (uint64_t)(kk * 128),
+                      idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&pv_done[x]);
+        if (last) umma_commit(&v_empty[j % kVfStages]);
+      }
+      __syncwarp();
+    };
+    bool ok = vl_wait(q_full, 0, p.status, kErrVlMma) && wait_k(0);
+    if (ok) {
+      tc_fence_after();
+      issue_s(0, 0, n_b == 0);
+      if (n_b > 0) issue_s(1, 0, true);
+    }
+    for (int j = 0; j < n_max && ok; ++j) {
+      if (!vl_wait(&v_full[j % kVfStages], (j / kVfStages) & 1, p.status, kErrVlMma)) { ok = false; break; }
+      if (j < n_a) {
+        if (!vl_wait(&p_full[0], j & 1, p.status, kErrVlMma)) { ok = false; break; }
+        tc_fence_after();
+        issue_pv(0, j, n_b == 0);
+        if (j + 1 < n_a) {
+          if (!wait_k(j + 1)) { ok = false; break; }
+          tc_fence_after();
+          issue_s(0, j + 1, n_b == 0);
+        }
+      }
+      if (j < n_b) {
+        if (!vl_wait(&p_full[1], j & 1, p.status, kErrVlMma)) { ok = false; break; }
+        tc_fence_after();
+        issue_pv(1, j, true);
+        if (j + 1 < n_b) {
+          if (!wait_k(j + 1)) { ok = false; break; }
+          tc_fence_after();
+          issue_s(1, j + 1, true);
+        }
+      }
+    }
+    // every MMA issued has completed before TMEM can be freed
+    if (elect_one_sync()) umma_commit(drain);
+    __syncwarp();
+    mbar_wait(drain, 0, nullptr, 0);
+  } else {
+    // ------------------------------------------------------------ softmax + epilogue
+    const int x = warp >> 2;                        // 0: tile A, 1: tile B
+    const int quad = warp & 3;                      // TMEM lane quadrant
+    const int row = quad * 32 + lane;               // row in the tile = TMEM lane
+    const int q = (x == 0 ? row_a : row_b) + row;   // row in the sequence
+    const int n_kv = x == 0 ? n_a : n_b;
+    const int limit = p.causal ? min(q + 1, w.len) : w.len;   // keys that the row sees
+    const uint32_t t_s = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(x * 128);
+    const uint32_t t_o = t_s + 256u;
+    float m_used = -INFINITY;
+    float l = 0.0f;
+    bool ok = n_kv > 0;
+    for (int j = 0; j < n_kv; ++j) {
+      if (!vl_wait(&s_full[x], j & 1, p.status, kErrVlCompute)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t r[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        tmem_ld_32x32b_x32(t_s + (uint32_t)(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+      tmem_ld_wait();
+      const int seen = limit - j * 128;
+      if (__any_sync(0xffffffffu, seen < 128)) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c >= seen) r[c] = __float_as_uint(-INFINITY);
+      }
+      // row max: 8 independent chains of 3-input maxima over columns 8..119, then the rest
+      float pm[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[i]);
+#pragma unroll
+      for (int c = 8; c < 120; c += 16)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          pm[i] = fmax3(pm[i], __uint_as_float(r[c + i]), __uint_as_float(r[c + 8 + i]));
+      const float mx = fmax3(fmax3(pm[0], pm[1], __uint_as_float(r[120])),
+                             fmax3(pm[2], pm[3], __uint_as_float(r[121])),
+                             fmax3(fmax3(pm[4], pm[5], __uint_as_float(r[122])),
+                                   fmax3(pm[6], pm[7], __uint_as_float(r[123])),
+                                   fmax3(__uint_as_float(r[124]), __uint_as_float(r[125]),
+                                         fmaxf(__uint_as_float(r[126]), __uint_as_float(r[127]))))) *
+                       p.scale_log2;
+      const bool need = mx > m_used + kVlRescale;
+      const bool rescale = __any_sync(0xffffffffu, need);
+      float factor = 1.0f;
+      if (rescale) {
+        const float m_new = need ? mx : m_used;
+        factor = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
+        m_used = m_new;
+      }
+      const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-m_used, -m_used);
+      uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+      uint32_t pk[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {  // masked keys hold -inf: 2^x gives 0 (the polynomial 2^-120)
+        float a0, a1;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, nm2), a0, a1);
+        float p0, p1;
+        if (i % 4 == 3) {
+          exp2_poly3_x2(a0, a1, p0, p1);
+        } else {
+          p0 = fast_exp2(a0);
+          p1 = fast_exp2(a1);
+        }
+        ps2[i & 3] = f2_add(ps2[i & 3], f2_pack(p0, p1));
+        pk[i] = vl_pack<FP16>(p0, p1);
+      }
+      tmem_st_32x32b_x32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+      tmem_st_32x32b_x32(t_s + 32u, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+      float ps[4];
+      f2_unpack(f2_add(ps2[0], ps2[1]), ps[0], ps[1]);
+      f2_unpack(f2_add(ps2[2], ps2[3]), ps[2], ps[3]);
+      l = l * factor + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+      if (rescale && j > 0) {
+        // O holds PV_0..PV_{j-1}: wait for PV_{j-1}, then scale this thread's row
+        if (!vl_wait(&pv_done[x], (j - 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + (uint32_t)(c * 32), o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+          tmem_st_32x32b_x32(t_o + (uint32_t)(c * 32), o);
+        }
+      }
+      // the sequence ends inside this key tile: zero V's other rows, by the first
+      // query tile that uses it (PV_B(j) is issued after PV_A(j))
+      if (w.len - j * 128 < 128 && (x == 0 || j >= n_a)) {
+        if (!vl_wait(&v_full[j % kVfStages], (j / kVfStages) & 1, p.status, kErrVlCompute)) { ok = false; break; }
+        vl_zero_rows<DP, 128>(smem + L::kV + (j % kVfStages) * L::kTile, w.len - j * 128, threadIdx.x & 127);
+      }
+      tmem_st_wait();
+      tc_fence_before();          // TMEM loads/stores of this step ordered before the arrive
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+    if (ok) {
+      const int jl = n_kv - 1;
+      if (vl_wait(&pv_done[x], jl & 1, p.status, kErrVlCompute)) {
+        tc_fence_after();
+        const bool store = q < w.len;
+        const int64_t at = (int64_t)(w.start + q) * p.Hq + h;
+        vl_store_row<FP16, DP>(t_o, 1.0f / l, O + at * p.D, 0, p.D, store);
+        if (store) lse[(int64_t)h * p.T + w.start + q] = (m_used + __log2f(l)) * 0.69314718055994531f;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ============================================================================
+// dQ: one CTA per (128-query tile, head), key tiles of 64.
+//
+// Q and dO are copied into tensor memory once, so that S = Q Kᵀ and dP = dO Vᵀ
+// (N = 64) read only K and V from shared memory.  S and dP are double-buffered:
+// two warpgroups take alternate key tiles (thread = query row, all 64 columns of
+// it: no exchange between warps), the MMA warp issues the scores of tile t + 1
+// before it waits for dS of tile t.  dS (16-bit pairs, over S's own columns) times
+// K (read MN-major) adds into dQ; dQ is written once: no atomics.
+// Tensor memory: S 64 b, dP 128 + 64 b (b = t & 1), dQ 256.., Q 384.., dO 448...
+// The kernel also forms delta = rowsum(dO ∘ O) and lse·log2(e) of its rows and
+// stores them by slots of 128 rows for the dK/dV kernel, which runs after it.
+// ============================================================================
+constexpr int kVbThreads = 352;     // two compute warpgroups, MMA warp, two loader warps
+
+template <int DP>
+struct VqSmem {
+  static constexpr int kKStages = 5, kVStages = 3;
+  static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2;
+  static constexpr int kQ = 0, kDO = kTile, kK = 2 * kTile, kV = kK + kKStages * kHalf;
+  static constexpr int kX = kV + kVStages * kHalf;       // [2][128] fp32
+  static constexpr int kBar = kX + 1024;
+  static constexpr int kBytes = kBar + 256 + 1024;
+};
+
+template <bool FP16, int DP>
+__global__ void __launch_bounds__(kVbThreads, 1)
+attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                      const __grid_constant__ VlParams p, const uint16_t* __restrict__ O,
+                      const float* __restrict__ lse, float* __restrict__ delta, float* __restrict__ lse2,
+                      uint16_t* __restrict__ dQ) {
+  using L = VqSmem<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* q_full = bars;                     // Q and dO landed
+  uint64_t* in_tmem = bars + 1;                // Q and dO copied (one arrival per compute warp)
+  uint64_t* k_full = bars + 2;                 // [kKStages]
+  uint64_t* k_empty = k_full + L::kKStages;
+  uint64_t* v_full = k_empty + L::kKStages;    // [kVStages]
+  uint64_t* v_empty = v_full + L::kVStages;
+  uint64_t* s_full = v_empty + L::kVStages;    // [2]
+  uint64_t* ds_full = s_full + 2;              // [2], four arrivals
+  uint64_t* dq_done = ds_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int entry = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+  const int count = p.meta[p.count_at];
+  if (entry >= count) {
+    if (entry == count) vl_zero_outside(dQ, p.T, p.Hq, h, p.D, p.meta);
+    return;
+  }
+  const VlTile w = p.tiles[entry];
+  const int hk = h / (p.Hq / p.Hk);
+  const int row0 = w.tile * 128;
+  const int keys = p.causal ? min(row0 + 128, w.len) : w.len;
+  const int n_kv = (keys + 63) / 64;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(in_tmem, 8);
+    for (int i = 0; i < L::kKStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < L::kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&ds_full[i], 4); }
+    mbar_init(dq_done, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmDO);
+  }
+  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 9) {
+    // ------------------------------------------------------------ TMA loaders (K with Q and dO; V)
+    if (lane == 0) {
+      const bool is_k = warp == 9;
+      if (is_k) {
+        mbar_arrive_expect_tx(q_full, 2 * L::kTile);
+        vl_load_tile<DP, 128>(smem + L::kQ, &tmQ, q_full, h, w.start + row0);
+        vl_load_tile<DP, 128>(smem + L::kDO, &tmDO, q_full, h, w.start + row0);
+      }
+      const CUtensorMap* map = is_k ? &tmK : &tmV;
+      uint64_t* empty = is_k ? k_empty : v_empty;
+      uint64_t* full = is_k ? k_full : v_full;
+      uint8_t* ring = smem + (is_k ? L::kK : L::kV);
+      const int nst = is_k ? L::kKStages : L::kVStages;
+      int issued = 0;
+      bool ok = true;
+      for (int t = 0; t < n_kv; ++t) {
+        const int st = t % nst;
+        if (!mbar_wait(&empty[st], ((t / nst) & 1) ^ 1, p.status, kErrVlLoad)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full[st], L::kHalf);
+        vl_load_tile<DP, 64>(ring + st * L::kHalf, map, &full[st], hk, w.start + t * 64);
+        issued = t + 1;
+      }
+      if (!ok) {  // let every copy this thread issued land before the CTA can exit
+        if (is_k) mbar_wait(q_full, 0, nullptr, 0);
+        for (int t = max(issued - nst, 0); t < issued; ++t) mbar_wait(&full[t % nst], (t / nst) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer (whole warp)
+    constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 64, false);
+    constexpr uint32_t idesc_q = vl_idesc<FP16>(128, DP, true);
+    const uint32_t k_base = smem_u32(smem + L::kK), v_base = smem_u32(smem + L::kV);
+    auto issue_scores = [&](int t) -> bool {
+      const int ks = t % L::kKStages, vs = t % L::kVStages, b = t & 1;
+      if (!vl_wait(&k_full[ks], (t / L::kKStages) & 1, p.status, kErrVlMma)) return false;
+      if (!vl_wait(&v_full[vs], (t / L::kVStages) & 1, p.status, kErrVlMma)) return false;
+      tc_fence_after();
+      const uint64_t kd = umma_desc_sw128_kmajor(k_base + ks * L::kHalf), vd = umma_desc_sw128_kmajor(v_base + vs * L::kHalf);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t off = (uint64_t)(((kk >> 2) * 8192 + (kk & 3) * 32) >> 4);
+          umma_f16_ts(tmem + (uint32_t)(64 * b), tmem + 384u + (uint32_t)(kk * 8), kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          umma_f16_ts(tmem + 128u + (uint32_t)(64 * b), tmem + 448u + (uint32_t)(kk * 8), vd + off, idesc_s,
+                      kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[b]);
+        umma_commit(&v_empty[vs]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = vl_wait(in_tmem, 0, p.status, kErrVlMma) && issue_scores(0);
+    for (int t = 0; t < n_kv && ok; ++t) {
+      if (t + 1 < n_kv && !issue_scores(t + 1)) { ok = false; break; }
+      const int b = t & 1, ks = t % L::kKStages;
+      if (!vl_wait(&ds_full[b], (t >> 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
+      tc_fence_after();
+      const uint64_t kd = umma_desc_sw128_mnmajor(k_base + ks * L::kHalf, 8192u);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f16_ts(tmem + 256u, tmem + (uint32_t)(64 * b + kk * 8), kd + (uint64_t)(kk * 128), idesc_q,
+                      (t > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&k_empty[ks]);
+      }
+      __syncwarp();
+    }
+    if (elect_one_sync()) umma_commit(dq_done);
+    __syncwarp();
+    mbar_wait(dq_done, 0, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
+  } else {
+    // ------------------------------------------------------------ dS + epilogue
+    const int quad = warp & 3, g = warp >> 2;
+    const int row = quad * 32 + lane, q = row0 + row;
+    const bool live = q < w.len;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const int limit = live ? (p.causal ? q + 1 : w.len) : 0;     // keys that the row sees
+    const float l2 = live ? lse[(int64_t)h * p.T + w.start + q] * 1.4426950408889634f : 0.0f;
+    // delta: this warpgroup's half of the columns, O from global (before the wait), dO from the tile
+    constexpr int CH = DP / 16;                                  // 8-column chunks of the half
+    uint4 ov[CH];
+    {
+      const uint16_t* orow = O + ((int64_t)(w.start + q) * p.Hq + h) * p.D;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = g * (DP / 2) + c * 8;
+        ov[c] = live && col < p.D ? *reinterpret_cast<const uint4*>(orow + col) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    bool ok = vl_wait(q_full, 0, p.status, kErrVlCompute);
+    float dl = 0.0f;
+    {
+      float acc = 0.0f;
+      const int a0 = DP == 128 ? g : 0;                          // atom of the half's columns
+      const uint8_t* drow = smem + L::kDO + a0 * 16384 + row * 128;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int chunk = (DP == 128 ? 0 : g * CH) + c;
+        const uint4 du = *reinterpret_cast<const uint4*>(drow + ((chunk ^ (row & 7)) << 4));
+        const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[c].x, ov[c].y, ov[c].z, ov[c].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 a = vl_unpack<FP16>(dw[j]), b = vl_unpack<FP16>(ow[j]);
+          acc = fmaf(a.x, b.x, acc);
+          acc = fmaf(a.y, b.y, acc);
+        }
+      }
+      float* xs = reinterpret_cast<float*>(smem + L::kX);
+      xs[g * 128 + row] = acc;
+      named_barrier(1, 256);
+      dl = live ? xs[row] + xs[128 + row] : 0.0f;
+      if (g == 0) {
+        const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
+        delta[at] = dl;
+        lse2[at] = l2;
+      }
+    }
+    if (ok) {  // warpgroup 0 copies Q, warpgroup 1 dO
+      const uint8_t* src = smem + (g == 0 ? L::kQ : L::kDO) + row * 128;
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a)
+        copy_row_to_tmem(src + a * 16384, row, lane_base + 384u + (uint32_t)(64 * g + 32 * a));
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(in_tmem);
+    }
+    const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(-l2, -l2), dl2 = f2_pack(dl, dl);
+    for (int t = g; t < n_kv && ok; t += 2) {
+      if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t s[64], dp[64];
+      tmem_ld64(lane_base + (uint32_t)(64 * g), s);
+      tmem_ld64(lane_base + 128u + (uint32_t)(64 * g), dp);
+      tmem_ld_wait();
+      const int seen = limit - t * 64;
+      const bool cut = __any_sync(0xffffffffu, seen < 64);
+      uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int c = 2 * i;
+        float a0, a1, g0, g1;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
+        f2_unpack(f2_mul(f2_pack(fast_exp2(a0), fast_exp2(a1)),
+                         f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl2)), g0, g1);
+        if (cut) {
+          if (c >= seen) g0 = 0.0f;
+          if (c + 1 >= seen) g1 = 0.0f;
+        }
+        pk[i] = vl_pack<FP16>(g0, g1);
+      }
+      tmem_st_32x32b_x32(lane_base + (uint32_t)(64 * g), pk);
+      if (w.len - t * 64 < 64)   // the sequence ends inside this key tile (K_t has given its scores)
+        vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, w.len - t * 64, threadIdx.x & 127);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_full[g]);
+    }
+    if (ok && vl_wait(dq_done, 0, p.status, kErrVlCompute)) {
+      tc_fence_after();
+      uint16_t* out = dQ + ((int64_t)(w.start + q) * p.Hq + h) * p.D;
+      vl_store_row<FP16, DP / 2>(lane_base + 256u + (uint32_t)(g * (DP / 2)), p.scale, out, g * (DP / 2), p.D, live);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ============================================================================
+// dK and dV: one CTA per (128-key tile, kv head), over the query heads that share
+// the kv head and their query tiles of 64.
+//
+//   Sᵀ_t = K Q_tᵀ, dPᵀ_t = V dO_tᵀ       M = 128 keys, N = 64 queries
+//   dV += Pᵀ_t dO_t, dK += dSᵀ_t Q_t      A = Pᵀ / dSᵀ from tensor memory, B MN-major
+// Two warpgroups take alternate query tiles (thread = key row, its 64 columns);
+// the scores of tile t + 1 are issued before the wait for Pᵀ/dSᵀ of tile t.
+// Tensor memory: dV 0.., dK 128.., Sᵀ 256 + 128 b, dPᵀ 320 + 128 b (b = t & 1),
+// Pᵀ and dSᵀ over the first 32 columns of theirs.  Q and dO come through rings of
+// four tiles with the tile's lse·log2(e) and delta.
+// ============================================================================
+template <int DP>
+struct VkSmem {
+  static constexpr int kStages = 4;
+  static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2;
+  static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kDO = kQ + kStages * kHalf;
+  static constexpr int kLD = kDO + kStages * kHalf;      // per stage: lse2[64], delta[64]
+  static constexpr int kBar = kLD + kStages * 512;
+  static constexpr int kBytes = kBar + 256 + 1024;
+};
+
+template <bool FP16, int DP>
+__global__ void __launch_bounds__(kVbThreads, 1)
+attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                       const __grid_constant__ VlParams p, const float* __restrict__ lse2,
+                       const float* __restrict__ delta, uint16_t* __restrict__ dK, uint16_t* __restrict__ dV) {
+  using L = VkSmem<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* kv_full = bars;                          // K and V landed
+  uint64_t* q_full = bars + 1;                       // [kStages]
+  uint64_t* q_empty = q_full + L::kStages;
+  uint64_t* o_full = q_empty + L::kStages;           // dO with lse2 and delta
+  uint64_t* o_empty = o_full + L::kStages;
+  uint64_t* s_full = o_empty + L::kStages;           // [2]
+  uint64_t* p_full = s_full + 2;                     // [2], four arrivals
+  uint64_t* acc_done = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_done + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int entry = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  const int count = p.meta[p.count_at];
+  if (entry >= count) {
+    if (entry == count) {
+      vl_zero_outside(dK, p.T, p.Hk, hk, p.D, p.meta);
+      vl_zero_outside(dV, p.T, p.Hk, hk, p.D, p.meta);
+    }
+    return;
+  }
+  const VlTile w = p.tiles[entry];
+  const int group = p.Hq / p.Hk, key0 = w.tile * 128;
+  const int i0 = p.causal ? 2 * w.tile : 0;          // first 64-query tile that sees this key tile
+  const int per_head = (w.len + 63) / 64 - i0;
+  const int n_it = group * per_head;
+  const int slot0 = w.slot - w.tile;                 // the sequence's first slot
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
+      mbar_init(&o_full[i], 1); mbar_init(&o_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+    mbar_init(acc_done, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmDO);
+  }
+  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 9) {
+    // ------------------------------------------------------------ TMA loaders (Q with K and V; dO)
+    if (lane == 0) {
+      const bool is_q = warp == 9;
+      if (is_q) {
+        mbar_arrive_expect_tx(kv_full, 2 * L::kTile);
+        vl_load_tile<DP, 128>(smem + L::kK, &tmK, kv_full, hk, w.start + key0);
+        vl_load_tile<DP, 128>(smem + L::kV, &tmV, kv_full, hk, w.start + key0);
+      }
+      const CUtensorMap* map = is_q ? &tmQ : &tmDO;
+      uint64_t* empty = is_q ? q_empty : o_empty;
+      uint64_t* full = is_q ? q_full : o_full;
+      uint8_t* ring = smem + (is_q ? L::kQ : L::kDO);
+      int issued = 0, h = hk * group, it = i0;
+      bool ok = true;
+      for (int t = 0; t < n_it; ++t) {
+        const int st = t % L::kStages;
+        if (!mbar_wait(&empty[st], ((t / L::kStages) & 1) ^ 1, p.status, kErrVlLoad)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full[st], L::kHalf + (is_q ? 0 : 512));
+        vl_load_tile<DP, 64>(ring + st * L::kHalf, map, &full[st], h, w.start + it * 64);
+        if (!is_q) {  // this query tile's lse2 and delta (256 B each)
+          const int64_t at = ((int64_t)h * p.slots + slot0) * 128 + it * 64;
+          bulk_load(smem + L::kLD + st * 512, lse2 + at, 256, &full[st]);
+          bulk_load(smem + L::kLD + st * 512 + 256, delta + at, 256, &full[st]);
+        }
+        issued = t + 1;
+        if (++it == i0 + per_head) { it = i0; ++h; }
+      }
+      if (!ok) {  // let every copy this thread issued land before the CTA can exit
+        if (is_q) mbar_wait(kv_full, 0, nullptr, 0);
+        for (int t = max(issued - L::kStages, 0); t < issued; ++t)
+          mbar_wait(&full[t % L::kStages], (t / L::kStages) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer (whole warp)
+    constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 64, false);
+    constexpr uint32_t idesc_g = vl_idesc<FP16>(128, DP, true);
+    const uint64_t kd = umma_desc_sw128_kmajor(smem_u32(smem + L::kK)), vd = umma_desc_sw128_kmajor(smem_u32(smem + L::kV));
+    const uint32_t q_base = smem_u32(smem + L::kQ), o_base = smem_u32(smem + L::kDO);
+    auto issue_scores = [&](int t) -> bool {
+      const int st = t % L::kStages;
+      const uint32_t ph = (t / L::kStages) & 1, sc = tmem + 256u + 128u * (uint32_t)(t & 1);
+      if (!vl_wait(&q_full[st], ph, p.status, kErrVlMma)) return false;
+      if (!vl_wait(&o_full[st], ph, p.status, kErrVlMma)) return false;
+      tc_fence_after();
+      const uint64_t qd = umma_desc_sw128_kmajor(q_base + st * L::kHalf), od = umma_desc_sw128_kmajor(o_base + st * L::kHalf);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ka = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+          const uint64_t qa = (uint64_t)(((kk >> 2) * 8192 + (kk & 3) * 32) >> 4);
+          umma_f16_ss(sc, kd + ka, qd + qa, idesc_s, kk > 0 ? 1u : 0u);
+          umma_f16_ss(sc + 64u, vd + ka, od + qa, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[t & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = vl_wait(kv_full, 0, p.status, kErrVlMma) && issue_scores(0);
+    for (int t = 0; t < n_it && ok; ++t) {
+      if (t + 1 < n_it && !issue_scores(t + 1)) { ok = false; break; }
+      if (!vl_wait(&p_full[t & 1], (t >> 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
+      tc_fence_after();
+      const int st = t % L::kStages;
+      const uint32_t sc = tmem + 256u + 128u * (uint32_t)(t & 1);
+      const uint64_t qd = umma_desc_sw128_mnmajor(q_base + st * L::kHalf, 8192u);
+      const uint64_t od = umma_desc_sw128_mnmajor(o_base + st * L::kHalf, 8192u);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {   // dV += Pᵀ dO and dK += dSᵀ Q
+          umma_f16_ts(tmem, sc + (uint32_t)(kk * 8), od + (uint64_t)(kk * 128), idesc_g, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_f16_ts(tmem + 128u, sc + 64u + (uint32_t)(kk * 8), qd + (uint64_t)(kk * 128), idesc_g,
+                      (t > 0 || kk > 0) ? 1u : 0u);
+        }
+        umma_commit(&q_empty[st]);
+        umma_commit(&o_empty[st]);
+      }
+      __syncwarp();
+    }
+    if (elect_one_sync()) umma_commit(acc_done);
+    __syncwarp();
+    mbar_wait(acc_done, 0, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
+  } else {
+    // ------------------------------------------------------------ Pᵀ, dSᵀ + epilogue
+    const int quad = warp & 3, g = warp >> 2;
+    const int row = quad * 32 + lane, key = key0 + row;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t sc = lane_base + 256u + 128u * (uint32_t)g;
+    bool ok = true;
+    int it = i0 + g % per_head;
+    for (int t = g; t < n_it; t += 2) {
+      const int st = t % L::kStages;
+      const float* sl = reinterpret_cast<const float*>(smem + L::kLD + st * 512);
+      // (o_full has completed by then; waiting on it makes lse2 and delta visible here)
+      if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute) ||
+          !vl_wait(&o_full[st], (t / L::kStages) & 1, p.status, kErrVlCompute)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[64], dp[64];
+      tmem_ld64(sc, s);
+      tmem_ld64(sc + 64u, dp);
+      tmem_ld_wait();
+      // queries [from, to) of the tile see this key
+      const int to = w.len - it * 64;
+      const int from = p.causal ? key - it * 64 : 0;
+      const bool cut = to < 64 || __any_sync(0xffffffffu, from > 0);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {   // 4 queries per step: shared-memory broadcasts
+        const float4 l4 = reinterpret_cast<const float4*>(sl)[i];
+        const float4 d4 = reinterpret_cast<const float4*>(sl + 64)[i];
+        const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dv4[4] = {d4.x, d4.y, d4.z, d4.w};
+        float pr[4], ds[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = 4 * i + u;
+          pr[u] = fast_exp2(fmaf(__uint_as_float(s[c]), p.scale_log2, -lv[u]));
+          ds[u] = pr[u] * (__uint_as_float(dp[c]) - dv4[u]);
+          if (cut && (c < from || c >= to)) pr[u] = ds[u] = 0.0f;
+        }
+        s[2 * i] = vl_pack<FP16>(pr[0], pr[1]);
+        s[2 * i + 1] = vl_pack<FP16>(pr[2], pr[3]);
+        dp[2 * i] = vl_pack<FP16>(ds[0], ds[1]);
+        dp[2 * i + 1] = vl_pack<FP16>(ds[2], ds[3]);
+      }
+      tmem_st_32x32b_x32(sc, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
+      tmem_st_32x32b_x32(sc + 64u, *reinterpret_cast<const uint32_t(*)[32]>(&dp[0]));
+      if (to < 64) {   // the sequence ends inside this query tile (it has given its scores)
+        vl_zero_rows<DP, 64>(smem + L::kQ + st * L::kHalf, to, threadIdx.x & 127);
+        vl_zero_rows<DP, 64>(smem + L::kDO + st * L::kHalf, to, threadIdx.x & 127);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[g]);
+      it += 2;
+      while (it >= i0 + per_head) it -= per_head;
+    }
+    if (ok && vl_wait(acc_done, 0, p.status, kErrVlCompute)) {
+      tc_fence_after();
+      const int64_t at = ((int64_t)(w.start + key) * p.Hk + hk) * p.D;
+      const bool live = key < w.len;
+      // warpgroup 0 writes dV, warpgroup 1 dK
+      vl_store_row<FP16, DP>(lane_base + (uint32_t)(128 * g), g == 0 ? 1.0f : p.scale, (g == 0 ? dV : dK) + at, 0, p.D, live);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+}  // namespace zq
+
+using namespace zq;
+
+// The plan's integers: tile tables, scratch, meta (see the sizes in packed_plan_words).
+static int64_t vl_cap(int64_t T, int64_t n, int rows) { return (T + rows - 1) / rows + n; }
+
+int64_t packed_plan_words(int64_t T, int64_t n) {
+  return 4 * (vl_cap(T, n, 256) + 2 * vl_cap(T, n, 128)) + kVlMeta + 3 * (n + 1);
+}
+
+// plan: int32 [packed_plan_words(T, n)], 16-byte aligned; positions: int32 [T]
+void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions) {
+  TORCH_CHECK(cu.is_cuda() && cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.dim() == 1 && cu.numel() >= 1,
+              "packed_plan: cu_seqlens int32 [n + 1] on the GPU");
+  const int64_t n = cu.numel() - 1;
+  TORCH_CHECK(T >= 0 && T < (1LL << 30) && n < (1 << 24), "packed_plan: too many rows or sequences");
+  TORCH_CHECK(plan.is_cuda() && plan.get_device() == cu.get_device() && plan.scalar_type() == at::kInt && plan.is_contiguous() &&
+                  plan.numel() == packed_plan_words(T, n) && (reinterpret_cast<uintptr_t>(plan.data_ptr()) & 15) == 0,
+              "packed_plan: plan int32 [packed_plan_words]");
+  TORCH_CHECK(positions.is_cuda() && positions.get_device() == cu.get_device() && positions.scalar_type() == at::kInt &&
+                  positions.is_contiguous() && positions.numel() == T,
+              "packed_plan: positions int32 [T]");
+  const c10::cuda::CUDAGuard guard(cu.device());
+  const int64_t c256 = vl_cap(T, n, 256), c128 = vl_cap(T, n, 128);
+  int* words = plan.data_ptr<int>();
+  int* meta = words + 4 * (c256 + 2 * c128);
+  const unsigned grid = 3 + (unsigned)((T + kPlanThreads - 1) / kPlanThreads);
+  packed_plan_kernel<<<grid, kPlanThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
+      cu.data_ptr<int>(), (int)n, (int)T, (int)c256, (int)c128, reinterpret_cast<VlTile*>(words), meta + kVlMeta, meta,
+      T > 0 ? positions.data_ptr<int>() : nullptr, status_buffer(cu.get_device()));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// [T, H, D] as a 3-D map (D, H, T) with boxes of 64 columns x 1 head x box_rows rows
+static CUtensorMap vl_tmap(const at::Tensor& t, int box_rows) {
+  CUtensorMap map;
+  const int64_t T = t.size(0), H = t.size(1), D = t.size(2);
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(2) == 1 && t.stride(1) % 8 == 0 &&
+                  t.stride(0) % 8 == 0 && t.stride(1) >= 0 && t.stride(0) >= 0,
+              "attention: 16-byte aligned rows with unit stride");
+  // the stride of an axis of one is never taken; the map wants a real one all the same
+  const int64_t sh = H > 1 ? t.stride(1) : D, st = T > 1 ? t.stride(0) : H * D;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)(sh * 2), (cuuint64_t)(st * 2)};
+  cuuint32_t box[3] = {64u, 1u, (cuuint32_t)box_rows};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  const auto type = t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUresult r = get_encode_fn()(&map, type, 3, t.data_ptr(), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "attention: cuTensorMapEncodeTiled failed with code ", (int)r);
+  return map;
+}
+
+struct VlCall {
+  VlParams p;
+  int64_t c256, c128;
+  bool fp16, narrow;
+};
+
+static VlCall vl_check(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& plan, int64_t n,
+                       bool causal, double scale) {
+  TORCH_CHECK(q.is_cuda() && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && q.dim() == 3,
+              "attention: bf16 or fp16 [T, H, D] CUDA tensors");
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), Hk = k.dim() == 3 ? k.size(1) : 0;
+  for (const at::Tensor* t : {&k, &v})
+    TORCH_CHECK(t->is_cuda() && t->get_device() == q.get_device() && t->scalar_type() == q.scalar_type() && t->dim() == 3 &&
+                    t->size(0) == T && t->size(1) == Hk && t->size(2) == D,
+                "attention: k and v [T, Hk, D] like q");
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention: head width a multiple of 8 up to 128");
+  TORCH_CHECK(T > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0, "attention: rows, and Hq a multiple of Hk");
+  TORCH_CHECK(scale > 0, "attention: scale must be positive");
+  TORCH_CHECK(plan.is_cuda() && plan.get_device() == q.get_device() && plan.scalar_type() == at::kInt && plan.is_contiguous() &&
+                  n >= 0 && plan.numel() == packed_plan_words(T, n),
+              "attention: the plan is another division's");
+  VlCall c;
+  c.c256 = vl_cap(T, n, 256);
+  c.c128 = vl_cap(T, n, 128);
+  TORCH_CHECK((c.c128 + 1) * Hq < (1LL << 31), "attention: grid too large");
+  const int* words = plan.data_ptr<int>();
+  c.p = VlParams{reinterpret_cast<const VlTile*>(words), words + 4 * (c.c256 + 2 * c.c128), 0, (int)T, (int)Hq, (int)Hk,
+                 (int)D, causal ? 1 : 0, (int)c.c128, (float)scale, (float)(scale * 1.4426950408889634),
+                 status_buffer(q.get_device())};
+  c.fp16 = q.scalar_type() == at::kHalf;
+  c.narrow = D <= 64;
+  return c;
+}
+
+static uint16_t* vl_out(const at::Tensor& t, const at::Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == like.scalar_type() && t.is_contiguous() &&
+                  t.sizes() == like.sizes() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
+              "attention: outputs are contiguous and like their inputs");
+  return reinterpret_cast<uint16_t*>(t.data_ptr());
+}
+
+template <typename K>
+static void vl_smem(K kern, int bytes, bool (&done)[64], int dev) {
+  if (done[dev]) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done[dev] = true;
+}
+
+template <bool FP16, int DP>
+static void vl_launch_fwd(const VlCall& c, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, uint16_t* o,
+                          float* lse, int dev) {
+  static bool done[64] = {false};
+  auto kern = attn_varlen_fwd_kernel<FP16, DP>;
+  vl_smem(kern, VfSmem<DP>::kBytes, done, dev);
+  kern<<<(unsigned)((c.c256 + 1) * c.p.Hq), kVfThreads, VfSmem<DP>::kBytes, at::cuda::getCurrentCUDAStream()>>>(tq, tk, tv, c.p,
+                                                                                                               o, lse);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// o [T, Hq, D] contiguous; lse [Hq, T] fp32 (rows of no sequence are not written)
+void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, at::Tensor o, at::Tensor lse,
+                     bool causal, double scale) {
+  VlCall c = vl_check(q, k, v, plan, n, causal, scale);
+  uint16_t* op = vl_out(o, q);
+  TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == q.size(0) * q.size(1),
+              "attention: lse [Hq, T] fp32");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const CUtensorMap tq = vl_tmap(q, 128), tk = vl_tmap(k, 128), tv = vl_tmap(v, 128);
+  c.p.count_at = 0;
+  auto go = c.fp16 ? (c.narrow ? vl_launch_fwd<true, 64> : vl_launch_fwd<true, 128>)
+                   : (c.narrow ? vl_launch_fwd<false, 64> : vl_launch_fwd<false, 128>);
+  go(c, tq, tk, tv, op, lse.data_ptr<float>(), q.get_device());
+}
+
+struct VlBwd {
+  CUtensorMap q128, do128, k64, v64, q64, do64, k128, v128;
+  const uint16_t* o;
+  const float* lse;
+  float *delta, *lse2;
+  uint16_t *dq, *dk, *dv;
+};
+
+template <bool FP16, int DP>
+static void vl_launch_bwd(VlCall& c, const VlBwd& b, int dev) {
+  static bool done_q[64] = {false}, done_k[64] = {false};
+  auto kq = attn_varlen_dq_kernel<FP16, DP>;
+  auto kk = attn_varlen_dkv_kernel<FP16, DP>;
+  vl_smem(kq, VqSmem<DP>::kBytes, done_q, dev);
+  vl_smem(kk, VkSmem<DP>::kBytes, done_k, dev);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const VlTile* tiles = c.p.tiles;
+  c.p.count_at = 1;
+  c.p.tiles = tiles + c.c256;
+  kq<<<(unsigned)((c.c128 + 1) * c.p.Hq), kVbThreads, VqSmem<DP>::kBytes, stream>>>(b.q128, b.k64, b.v64, b.do128, c.p, b.o, b.lse,
+                                                                                   b.delta, b.lse2, b.dq);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  c.p.count_at = 2;
+  c.p.tiles = tiles + c.c256 + c.c128;
+  kk<<<(unsigned)((c.c128 + 1) * c.p.Hk), kVbThreads, VkSmem<DP>::kBytes, stream>>>(b.q64, b.k128, b.v128, b.do64, c.p, b.lse2,
+                                                                                   b.delta, b.dk, b.dv);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// dq, dk, dv (contiguous) from dout, the forward's inputs, o and lse: two launches
+void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor plan,
+                     int64_t n, at::Tensor dq, at::Tensor dk, at::Tensor dv, bool causal, double scale) {
+  VlCall c = vl_check(q, k, v, plan, n, causal, scale);
+  TORCH_CHECK(dout.is_cuda() && dout.get_device() == q.get_device() && dout.scalar_type() == q.scalar_type() &&
+                  dout.sizes() == q.sizes(),
+              "attention backward: dout like q");
+  TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == q.size(0) * q.size(1),
+              "attention: lse [Hq, T] fp32");
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto stats = at::empty({2, q.size(1), c.c128 * 128}, lse.options());
+  VlBwd b{vl_tmap(q, 128), vl_tmap(dout, 128), vl_tmap(k, 64), vl_tmap(v, 64), vl_tmap(q, 64), vl_tmap(dout, 64), vl_tmap(k, 128),
+          vl_tmap(v, 128), vl_out(o, q), lse.data_ptr<float>(), stats.data_ptr<float>(),
+          stats.data_ptr<float>() + stats.numel() / 2, vl_out(dq, q), vl_out(dk, k), vl_out(dv, v)};
+  auto go = c.fp16 ? (c.narrow ? vl_launch_bwd<true, 64> : vl_launch_bwd<true, 128>)
+                   : (c.narrow ? vl_launch_bwd<false, 64> : vl_launch_bwd<false, 128>);
+  go(c, b, q.get_device());
+}

@@ -66,6 +66,13 @@ void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, c10::opt
 void opt_tick(at::Tensor clk, at::Tensor bc, double b1, double b2, bool bump_epoch);
 void lion_step(at::Tensor master, at::Tensor grad, at::Tensor mom, double lr, double b1, double b2,
                double wd, int64_t seed);
+// attention_varlen_sm100.cu
+int64_t packed_plan_words(int64_t T, int64_t n);
+void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions);
+void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, at::Tensor o, at::Tensor lse,
+                     bool causal, double scale);
+void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor plan,
+                     int64_t n, at::Tensor dq, at::Tensor dk, at::Tensor dv, bool causal, double scale);
 // rotary.cu
 void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
             c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign);
@@ -161,6 +168,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope", &rope);
   m.def("rope_into", &rope_into);
   m.def("rope_into2", &rope_into2, "rope_into for two (x, out) pairs in one launch");
+  m.def("packed_plan_words", &packed_plan_words);
+  m.def("packed_plan", &packed_plan, "tile tables and positions of packed sequences");
+  m.def("attn_varlen_fwd", &attn_varlen_fwd, "tcgen05 attention over packed sequences, forward");
+  m.def("attn_varlen_bwd", &attn_varlen_bwd, "its backward: dQ, then dK/dV");
   m.def("rotary", &rotary, "rotary positions for q and k: explicit positions, either layout, part of the head");
   m.def("distill", &distill, "distillation loss rows, and in the same launch the mean and its gradient");
   m.def("distill_grad", &distill_grad, "gradient of the distillation loss rows from their log-sum-exps");

@@ -1032,6 +1032,16 @@ using namespace zq;
 // host side
 // ----------------------------------------------------------------------------
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+  // The encoder is a driver call and needs the calling thread's context, which only a
+  // runtime call makes current: an autograd thread whose first work is one of this
+  // extension's backwards has made none (the driver then ends in a segmentation fault).
+  static thread_local bool bound = false;
+  if (!bound) {
+    int dev;
+    C10_CUDA_CHECK(cudaGetDevice(&dev));
+    C10_CUDA_CHECK(cudaSetDevice(dev));
+    bound = true;
+  }
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {

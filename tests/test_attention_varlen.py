@@ -1,0 +1,285 @@
+"""flash_attention_varlen and PackedSequences against the formulas in 64 bits.
+
+Tolerances, with u = half a step of the type and e = 2^-11 (the exponentials' 2^-13.6, as it
+enters P and, through the row sums, again; and the scores' 32-bit products):
+  O   (u + e) sum P|v| + u|O|
+  dV  (u + e) sum P|dO| + u|dV|
+  dS  (u + e)|dS| + P (sum |dO| tol(O)), since delta is formed from the rounded O
+  dQ  scale sum tol(dS)|K| + u|dQ|, dK likewise.
+fp16 P and dS below the normal range are off by up to 2^-25 each."""
+
+import math
+
+import pytest
+import torch
+
+from zeroq_b200.ops import PackedSequences, flash_attention_varlen
+from zeroq_b200.ops.attention import attention_varlen_reference
+
+E = 2.0 ** -11
+
+
+def inputs(lengths, tail, hq, hk, D, dtype, device, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    T = sum(lengths) + tail
+    qkv = (torch.randn(T, (hq + 2 * hk) * D, generator=g) * std).to(dtype).to(device)
+    q = qkv[:, : hq * D].view(T, hq, D)
+    k = qkv[:, hq * D: (hq + hk) * D].view(T, hk, D)
+    v = qkv[:, (hq + hk) * D:].view(T, hk, D)
+    do = torch.randn(T, hq, D, generator=g).to(dtype).to(device)
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(device)
+    return q, k, v, do, cu
+
+
+def exact(q, k, v, do, lengths, causal, scale):
+    """Outputs, gradients and their tolerances (as factors above) in 64 bits, on the inputs' device."""
+    u = torch.finfo(q.dtype).eps / 2
+    sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    dev = q.device
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    share = q.shape[1] // k.shape[1]
+    zero = lambda t: torch.zeros_like(t)  # noqa: E731
+    out = {n: (zero(t), zero(t)) for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    a = 0
+    for n in lengths:
+        r = slice(a, a + n)
+        a += n
+        hidden = torch.ones(n, n, dtype=torch.bool, device=dev).triu(1) if causal else None
+        for h in range(q.shape[1]):
+            hk = h // share
+            Q, K, V, G = q[r, h], k[r, hk], v[r, hk], do[r, h]
+            s = Q @ K.T * scale
+            if causal:
+                s = s.masked_fill(hidden, -math.inf)
+            p = torch.softmax(s, -1) if n else s
+            seen = (p > 0).double()
+            o = p @ V
+            to = (u + E) * (p @ V.abs()) + u * o.abs() + sub * (seen @ V.abs())
+            ds = p * (G @ V.T - (G * o).sum(-1, keepdim=True))
+            tds = (u + E) * ds.abs() + p * (G.abs() * to).sum(-1, keepdim=True) + sub * seen
+            for name, at, value, tol in (
+                    ("o", h, o, to),
+                    ("dq", h, scale * ds @ K, scale * tds @ K.abs()),
+                    ("dk", hk, scale * ds.T @ Q, scale * tds.T @ Q.abs()),
+                    ("dv", hk, p.T @ G, (u + E) * (p.T @ G.abs()) + sub * (seen.T @ G.abs()))):
+                out[name][0][r, at] += value
+                out[name][1][r, at] += tol
+    for name in ("dq", "dk", "dv"):
+        out[name][1].add_(u * out[name][0].abs())
+    if sub:
+        for name in out:
+            out[name][1].add_(sub)
+    return out
+
+
+def check(lengths, tail, hq, hk, D, dtype, device, causal=True, scale=None, seed=0, std=1.0, poison=False):
+    q, k, v, do, cu = inputs(lengths, tail, hq, hk, D, dtype, device, seed, std)
+    if poison:   # padding rows that hold anything
+        for t in (q, k, v, do):
+            t[sum(lengths):] = float("nan")
+            t[sum(lengths)::2] = float("inf")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = flash_attention_varlen(*leaves, cu, causal=causal, scale=scale)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, leaves, do)))
+    want = exact(q, k, v, do, lengths, causal, 1 / math.sqrt(D) if scale is None else scale)
+    for name, (value, tol) in want.items():
+        x = got[name]
+        assert x.dtype == dtype and x.shape == value.shape
+        assert (x[sum(lengths):] == 0).all(), name
+        off = (x.double() - value).abs()
+        assert (off <= tol).all(), (name, (off / tol.clamp_min(1e-300)).max().item(), off.max().item())
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("causal", [True, False])
+def test_reference_matches_formula(causal):
+    check([3, 0, 17, 1, 40], 5, 4, 2, 24, torch.float32, "cpu", causal)
+
+
+def test_reference_gradient_against_differences():
+    q, k, v, do, cu = inputs([3, 4], 1, 2, 1, 4, torch.float64, "cpu")
+    f = lambda *t: flash_attention_varlen(*t, cu)  # noqa: E731
+    assert torch.autograd.gradcheck(f, tuple(t.clone().requires_grad_() for t in (q, k, v)))
+
+
+def test_positions_and_bounds():
+    s = PackedSequences(torch.tensor([0, 3, 3, 7]), 9)
+    assert s.positions.tolist() == [0, 1, 2, 0, 1, 2, 3, 0, 0]
+    assert s.bounds() == [(0, 3), (3, 3), (3, 7)]
+
+
+@pytest.mark.parametrize("cu,total", [
+    (torch.tensor([1, 3]), 5), (torch.tensor([0, 4, 3]), 5), (torch.tensor([0, 6]), 5), (torch.tensor([[0, 3]]), 5),
+    (torch.tensor([0.0, 3.0]), 5), (torch.tensor([], dtype=torch.int32), 5), (torch.tensor([0]), -1)])
+def test_packed_refusals(cu, total):
+    with pytest.raises((ValueError, TypeError)):
+        PackedSequences(cu, total)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=torch.zeros(8, 4)), dict(k=torch.zeros(7, 2, 16)), dict(v=torch.zeros(8, 1, 16)),
+    dict(q=torch.zeros(8, 3, 16)), dict(k=torch.zeros(8, 2, 16).double()), dict(scale=0.0), dict(scale=-1.0),
+    dict(scale=float("nan")), dict(seqs=PackedSequences(torch.tensor([0, 9]), 9)), dict(seqs=torch.tensor([0, 9]))])
+def test_refusals(bad):
+    args = dict(q=torch.zeros(8, 4, 16), k=torch.zeros(8, 2, 16), v=torch.zeros(8, 2, 16), seqs=torch.tensor([0, 8]))
+    args.update(bad)
+    with pytest.raises((ValueError, TypeError)):
+        flash_attention_varlen(**args)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,tail", [
+    ([], 5), ([0, 0], 0), ([1], 0), ([128, 256, 0, 1, 300, 129], 17), ([5000, 3, 0, 700], 1),
+    ([i % 7 for i in range(3000)], 40), ([70000, 2000], 0)])
+def test_plan_tables(cuda, lengths, tail):
+    T = sum(lengths) + tail
+    cu = torch.tensor([0] + lengths).cumsum(0)
+    s = PackedSequences(cu.to(cuda), T)
+    host = PackedSequences(cu, T)
+    assert torch.equal(s.positions.cpu(), host.positions)
+    n = len(lengths)
+    words = s.plan.cpu()
+    caps = [(T + 255) // 256 + n] + [(T + 127) // 128 + n] * 2
+    tables, at = [], 0
+    for c in caps:
+        tables.append(words[at: at + 4 * c].view(c, 4))
+        at += 4 * c
+    meta = words[at: at + 5].tolist()
+    assert meta[3:] == [0, sum(lengths)]
+    for kind, rows in enumerate((256, 128, 128)):
+        want, slot = set(), 0
+        for a, b in host.bounds():
+            for t in range(0, (b - a + rows - 1) // rows):
+                want.add((a, b - a, t, slot))
+                slot += 1
+        got = [tuple(r) for r in tables[kind][: meta[kind]].tolist()]
+        assert len(got) == len(set(got)) == meta[kind] and set(got) == want
+        work = [(L - t * rows if kind == 2 else min(t * rows + rows, L)) for _, L, t, _ in got]
+        unit = 64
+        while (T + 63) // unit >= 1024:
+            unit *= 2
+        cls = [(w + 63) // 64 * 64 // unit for w in work]
+        assert cls == sorted(cls, reverse=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,tail,hq,hk,D", [
+    ([1], 0, 1, 1, 128),
+    ([128], 0, 2, 1, 128),
+    ([1, 63, 64, 65, 127, 128, 129], 3, 4, 2, 128),
+    ([255, 256, 257, 0, 383, 1], 0, 3, 1, 64),
+    ([700, 2, 513], 100, 7, 1, 80),
+    ([33, 300], 1, 2, 2, 8),
+    ([200, 129, 77], 0, 4, 4, 72),
+    ([1025], 0, 6, 3, 120)])
+def test_kernels_match_formula(cuda, dtype, causal, lengths, tail, hq, hk, D):
+    check(lengths, tail, hq, hk, D, dtype, cuda, causal, seed=sum(lengths) + D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_kernels_long_and_many(cuda, D):
+    check([4097, 100], 0, 2, 1, D, torch.bfloat16, cuda)
+    check([(i * 37) % 90 for i in range(60)], 9, 2, 2, D, torch.bfloat16, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+def test_unset_padding_does_not_enter(cuda, causal):
+    check([130, 1, 60, 255], 150, 4, 2, 128, torch.bfloat16, cuda, causal, poison=True)
+    check([130, 1, 60, 255], 150, 4, 2, 64, torch.float16, cuda, causal, poison=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_neighbour_does_not_enter(cuda, causal):
+    """A document of NaN and infinities between two others changes neither."""
+    lengths = [100, 77, 200]
+    q, k, v, do, cu = inputs(lengths, 0, 4, 2, 128, torch.bfloat16, cuda)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    o = flash_attention_varlen(*leaves, cu, causal=causal)
+    clean = (o.detach(),) + torch.autograd.grad(o, leaves, do)
+    for t in (q, k, v, do):
+        t[100:177] = float("nan")
+        t[120:130] = float("inf")
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    o = flash_attention_varlen(*leaves, cu, causal=causal)
+    dirty = (o.detach(),) + torch.autograd.grad(o, leaves, do)
+    for a, b in zip(clean, dirty):
+        assert torch.equal(a[:100], b[:100]) and torch.equal(a[177:], b[177:])
+
+
+@pytest.mark.gpu
+def test_large_scores_move_the_running_maximum(cuda):
+    check([600, 300], 0, 2, 1, 128, torch.bfloat16, cuda, seed=3, std=1.0, scale=1.0)
+    check([600, 300], 0, 2, 1, 64, torch.bfloat16, cuda, causal=False, seed=4, scale=0.01)
+
+
+@pytest.mark.gpu
+def test_strides_shared_plan_and_partial_gradients(cuda):
+    lengths = [150, 90]
+    q, k, v, do, cu = inputs(lengths, 0, 4, 2, 64, torch.bfloat16, cuda)
+    seqs = PackedSequences(cu.long().cpu(), 240, device=cuda)
+    want = flash_attention_varlen(q.contiguous(), k.contiguous(), v.contiguous(), cu)
+    heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert torch.equal(flash_attention_varlen(*heads_first, seqs), want)
+    odd = [torch.empty(240 * t.shape[1] * 64 + 1, device=cuda, dtype=t.dtype)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    assert torch.equal(flash_attention_varlen(*odd, seqs), want)
+    one = k[:, :1].expand(240, 2, 64)     # one kv head for both
+    assert torch.equal(flash_attention_varlen(q, one, one, seqs),
+                       flash_attention_varlen(q, one.contiguous(), one.contiguous(), seqs))
+    leaf = q.detach().requires_grad_()
+    flash_attention_varlen(leaf, k, v, seqs).sum().backward()     # an expanded gradient; k, v take none
+    full = q.detach().requires_grad_()
+    o = flash_attention_varlen(full, k, v, seqs)
+    o.backward(torch.ones_like(o))
+    assert torch.equal(leaf.grad, full.grad)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals(cuda):
+    q, k, v, do, cu = inputs([10], 0, 2, 2, 128, torch.bfloat16, cuda)
+    with pytest.raises(TypeError):
+        flash_attention_varlen(q.float(), k.float(), v.float(), cu)
+    for D in (4, 12, 136):
+        t = torch.zeros(10, 2, D, device=cuda, dtype=torch.bfloat16)
+        with pytest.raises(ValueError):
+            flash_attention_varlen(t, t, t, cu)
+    with pytest.raises(ValueError):
+        flash_attention_varlen(q, k, v, PackedSequences(torch.tensor([0, 10]), 10))   # on the CPU
+    from zeroq_b200.ops import _ext
+    s = PackedSequences(cu, 10)
+    with pytest.raises(RuntimeError, match="plan"):
+        _ext.ext().attn_varlen_fwd(q, k, v, s.plan, 2, torch.empty_like(q), torch.empty(2, 10, device=cuda), True, 0.1)
+
+
+@pytest.mark.gpu
+def test_repeatable_in_a_graph_with_changing_sequences(cuda):
+    q, k, v, do, cu = inputs([200, 300, 12], 0, 4, 2, 128, torch.bfloat16, cuda)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = flash_attention_varlen(*leaves, cu)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    first = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, side))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for lengths in ([200, 300, 12], [1, 500, 11], [512, 0, 0]):
+        cu.copy_(torch.tensor([0] + lengths).cumsum(0).to(torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+    from zeroq_b200.ops import _ext
+    assert _ext.ext().gemm_status(0)[0] == 0

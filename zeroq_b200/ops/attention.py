@@ -13,16 +13,22 @@ every head size up to 128 runs on the same kernels (at 128-wide cost).
 
 CPU tensors, ``S`` not a multiple of 128 and heads wider than 128 use PyTorch's
 SDPA (the oracle).
+
+``flash_attention_varlen`` is attention over packed sequences of any lengths
+(``csrc/attention_varlen_sm100.cu``): ``[T, H, D]`` rows, divided by a
+:class:`~zeroq_b200.ops.packed.PackedSequences`, bf16 or fp16, with its backward.
 """
 
 from __future__ import annotations
 
 import math
+from typing import Optional, Union
 
 import torch
 import torch.nn.functional as F
 
 from . import _ext
+from .packed import PackedSequences
 
 
 def attention_reference(q, k, v, causal: bool = True, scale=None):
@@ -120,3 +126,92 @@ def flash_attention(q, k, v, causal: bool = True, scale=None, rope=None):
     if q.is_cuda and q.dtype == torch.bfloat16 and _tc_ok(q):
         return _FlashAttn.apply(q, k, v, causal, scale, rope)
     return attention_reference(q, k, v, causal, scale)
+
+
+# ---------------------------------------------------------------------------
+# packed sequences
+# ---------------------------------------------------------------------------
+def attention_varlen_reference(q, k, v, seqs: PackedSequences, causal: bool = True, scale=None):
+    """PyTorch form of :func:`flash_attention_varlen`, a sequence at a time, in 32 bits
+    (64 for 64-bit inputs); differentiable."""
+    D, share = q.shape[-1], q.shape[1] // k.shape[1]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    parts, end = [], 0
+    for a, b in seqs.bounds():
+        qs, ks, vs = (t[a:b].to(dt).transpose(0, 1) for t in (q, k, v))
+        ks, vs = (t.repeat_interleave(share, dim=0) for t in (ks, vs))
+        s = (qs @ ks.transpose(1, 2)) * scale
+        if causal:
+            s = s.masked_fill(torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).triu(1), -math.inf)
+        parts.append((torch.softmax(s, -1) @ vs).transpose(0, 1).to(q.dtype))
+        end = b
+    parts.append(q.new_zeros(q.shape[0] - end, *q.shape[1:]))
+    return torch.cat(parts)
+
+
+def _rows_ok(t: torch.Tensor) -> bool:
+    """``t [T, H, D]`` can be read through a tensor map as it is (no repeated rows or heads)."""
+    return _tma_ok(t) and all(st > 0 or n == 1 for st, n in zip(t.stride(), t.shape))
+
+
+class _FlashAttnVarlen(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, seqs, causal, scale):
+        q, k, v = (t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+        T, Hq, _ = q.shape
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
+        _ext.ext().attn_varlen_fwd(q, k, v, seqs.plan, seqs.n, o, lse, causal, scale)
+        ctx.save_for_backward(q, k, v, o, lse, seqs.plan)
+        ctx.meta = (seqs.n, causal, scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, plan = ctx.saved_tensors
+        n, causal, scale = ctx.meta
+        do = do if _rows_ok(do) else do.clone(memory_format=torch.contiguous_format)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _ext.ext().attn_varlen_bwd(do, q, k, v, o, lse, plan, n, dq, dk, dv, causal, scale)
+        return dq, dk, dv, None, None, None
+
+
+def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           seqs: Union[PackedSequences, torch.Tensor], causal: bool = True,
+                           scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of each sequence of a packed row over itself.
+
+    ``q [T, Hq, D]``, ``k`` and ``v`` ``[T, Hk, D]`` with ``Hq`` a multiple of ``Hk``
+    (query head ``h`` reads kv head ``h // (Hq / Hk)``), any strides with a unit head-dim
+    stride; ``D`` a multiple of 8 up to 128; bf16 or fp16 on the GPU.  ``seqs``: the
+    :class:`~zeroq_b200.ops.packed.PackedSequences` of the ``T`` rows, or its
+    ``cu_seqlens`` (then its tables are built for this call).  ``causal``: a row sees its
+    sequence's rows up to itself, otherwise all of them.  ``scale`` (positive) defaults
+    to ``1/sqrt(D)``.  Rows of no sequence get an output and gradients of zero, whatever
+    they hold.  P and dS are rounded to the inputs' type before their products;
+    scores, softmax statistics and accumulators are in 32 bits."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"flash_attention_varlen: q [T, Hq, D], k and v [T, Hk, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    T, Hq, D = q.shape
+    if k.shape[1] < 1 or Hq < 1 or Hq % k.shape[1]:
+        raise ValueError(f"flash_attention_varlen: {Hq} query heads do not share {k.shape[1]} kv heads evenly")
+    if not (k.dtype == v.dtype == q.dtype) or not (k.device == v.device == q.device):
+        raise TypeError("flash_attention_varlen: q, k and v of one type on one device")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"flash_attention_varlen: scale must be positive, got {scale}")
+    if not isinstance(seqs, PackedSequences):
+        seqs = PackedSequences(seqs, T, device=q.device)
+    if seqs.total != T or seqs.device != q.device:
+        raise ValueError(f"flash_attention_varlen: the sequences divide {seqs.total} rows on {seqs.device}, "
+                         f"q has {T} on {q.device}")
+    if not q.is_cuda or T == 0:
+        return attention_varlen_reference(q, k, v, seqs, causal, scale)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"flash_attention_varlen: bf16 or fp16 on the GPU, got {q.dtype}")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"flash_attention_varlen: head width a multiple of 8 up to 128 on the GPU, got {D}")
+    return _FlashAttnVarlen.apply(q, k, v, seqs, bool(causal), scale)

@@ -1,0 +1,61 @@
+"""Packed rows: several sequences behind one another in one row of tokens.
+
+:class:`PackedSequences` holds the division ``cu_seqlens`` of ``total`` rows and what the
+kernels derive from it: the tile tables of the attention kernels and every row's
+position in its sequence.  Both are built on the device by one kernel, without a copy
+to the host, so a division may change from step to step (also in a captured graph:
+the tables are built again at each replay).  Make one for a batch and give it to
+every layer.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _ext
+
+
+class PackedSequences:
+    """Sequence ``i`` holds rows ``[cu_seqlens[i], cu_seqlens[i + 1])`` of ``total``;
+    rows behind the last sequence are padding.  Sequences may be empty.
+
+    ``cu_seqlens``: int32 or int64 ``[n + 1]``.  On the CPU it is checked here (it starts
+    at 0, does not fall and ends within ``total``) and copied to ``device``; on the GPU
+    it is not read by the host - values out of order are clamped by the kernel, and the
+    result for such a division is undefined."""
+
+    def __init__(self, cu_seqlens: torch.Tensor, total: int, device: Optional[torch.device] = None):
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError(f"PackedSequences: cu_seqlens must be [n + 1], got {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"PackedSequences: cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+        if not 0 <= total < 1 << 30:
+            raise ValueError(f"PackedSequences: total must be 0 to 2^30 - 1, got {total}")
+        device = cu_seqlens.device if device is None else torch.device(device)
+        if not cu_seqlens.is_cuda:
+            c = cu_seqlens.tolist()
+            if c[0] != 0 or any(b < a for a, b in zip(c, c[1:])) or c[-1] > total:
+                raise ValueError(f"PackedSequences: cu_seqlens must rise from 0 to at most total={total}")
+        self.total = int(total)
+        self.n = cu_seqlens.numel() - 1
+        self.device = device
+        self.cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+        self.plan = None
+        if device.type == "cuda":
+            E = _ext.ext()
+            words = E.packed_plan_words(self.total, self.n)
+            # the plan and the positions share one buffer
+            buf = torch.empty(words + self.total, dtype=torch.int32, device=device)
+            self.plan, self.positions = buf[:words], buf[words:]
+            E.packed_plan(self.cu_seqlens, self.total, self.plan, self.positions)
+        else:
+            self.positions = torch.zeros(self.total, dtype=torch.int32)
+            for a, b in self.bounds():
+                self.positions[a:b] = torch.arange(b - a, dtype=torch.int32)
+
+    def bounds(self):
+        """``[(first row, end row)]`` of the sequences (read from the device where they are there)."""
+        c = self.cu_seqlens.tolist()
+        return list(zip(c, c[1:]))
