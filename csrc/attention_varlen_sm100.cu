@@ -53,6 +53,7 @@ struct VlParams {
   const int* meta;        // the plan's meta words
   int count_at;           // which of them counts these tiles
   int T, Hq, Hk, D, causal, slots;
+  int split;              // CTAs of a cluster that share a key tile (dK/dV)
   float scale, scale_log2;
   DeviceStatus* status;
 };
@@ -127,9 +128,37 @@ __device__ __forceinline__ void vl_zero_outside(uint16_t* out, int T, int H, int
   }
 }
 
+// The forward's O in 32 bits, as its rounded value and one more byte: the 8 bits
+// behind the kept ones of the 32-bit pattern, read as a signed number they are the
+// difference to the value rounded to nearest (bits 8-15 for bf16, 5-12 for fp16; a tie
+// rounded down reads as one rounded up, and below fp16's normal range the byte is worth
+// 2^-11 of the value at most).  delta = rowsum(dO ∘ O) is formed from both: from the
+// rounded O alone it has an error of the size of dS's own rounding where a row sees few
+// keys (dQ and dK of 88-row sequences: 1.60 times the error of one rounding, with the
+// byte 1.41).
+// the bytes of four values
+template <bool FP16>
+__device__ __forceinline__ uint32_t vl_low_bytes(float a, float b, float c, float d) {
+  uint32_t x[4] = {__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)};
+  if constexpr (FP16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] <<= 3;   // to byte 1
+  }
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0051), __byte_perm(x[2], x[3], 0x0051), 0x5410);
+}
+// byte K of `bytes` back onto a rounded value
+template <bool FP16, int K>
+__device__ __forceinline__ float vl_with_low(float rounded, uint32_t bytes) {
+  int d;   // byte k, sign-extended, from byte 1 on (a selector's top bit copies the sign; __byte_perm has none)
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(d) : "r"(bytes), "n"(0x8804 | (K << 4) | (K << 8) | (K << 12)));
+  if constexpr (FP16) d >>= 3;
+  return rounded == 0.0f ? 0.0f : __int_as_float(__float_as_int(rounded) + d);   // (below 0's pattern lies NaN)
+}
+
 // N accumulator columns of this lane times f, rounded, to out; columns from D on do not exist
 template <bool FP16, int N>
-__device__ __forceinline__ void vl_store_row(uint32_t taddr, float f, uint16_t* out, int col0, int D, bool store) {
+__device__ __forceinline__ void vl_store_row(uint32_t taddr, float f, uint16_t* out, int col0, int D, bool store,
+                                             uint8_t* low = nullptr) {
 #pragma unroll 1
   for (int c = 0; c < N; c += 32) {
     uint32_t o[32];
@@ -143,6 +172,24 @@ __device__ __forceinline__ void vl_store_row(uint32_t taddr, float f, uint16_t* 
       v.z = vl_pack<FP16>(__uint_as_float(o[8 * i + 4]) * f, __uint_as_float(o[8 * i + 5]) * f);
       v.w = vl_pack<FP16>(__uint_as_float(o[8 * i + 6]) * f, __uint_as_float(o[8 * i + 7]) * f);
       if (store && col0 + c + 8 * i < D) *reinterpret_cast<uint4*>(out + col0 + c + 8 * i) = v;
+    }
+    if (low != nullptr) {
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        b[i] = vl_low_bytes<FP16>(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f,
+                                  __uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
+      uint8_t* to = low + col0 + c;
+      if ((D & 31) == 0) {   // whole 32-byte sectors
+        if (store && col0 + c < D) {
+          reinterpret_cast<uint4*>(to)[0] = make_uint4(b[0], b[1], b[2], b[3]);
+          reinterpret_cast<uint4*>(to)[1] = make_uint4(b[4], b[5], b[6], b[7]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (store && col0 + c + 8 * i < D) reinterpret_cast<uint2*>(to)[i] = make_uint2(b[2 * i], b[2 * i + 1]);
+      }
     }
   }
 }
@@ -308,7 +355,7 @@ template <bool FP16, int DP>
 __global__ void __launch_bounds__(kVfThreads, 1)
 attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ VlParams p,
-                       uint16_t* __restrict__ O, float* __restrict__ lse) {
+                       uint16_t* __restrict__ O, float* __restrict__ lse, uint8_t* __restrict__ low) {
   using L = VfSmem<DP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -567,7 +614,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         tc_fence_after();
         const bool store = q < w.len;
         const int64_t at = (int64_t)(w.start + q) * p.Hq + h;
-        vl_store_row<FP16, DP>(t_o, 1.0f / l, O + at * p.D, 0, p.D, store);
+        vl_store_row<FP16, DP>(t_o, 1.0f / l, O + at * p.D, 0, p.D, store, low != nullptr ? low + at * p.D : nullptr);
         if (store) lse[(int64_t)h * p.T + w.start + q] = (m_used + __log2f(l)) * 0.69314718055994531f;
       }
     }
@@ -594,6 +641,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 // The kernel also forms delta = rowsum(dO ∘ O) and lse·log2(e) of its rows and
 // stores them by slots of 128 rows for the dK/dV kernel, which runs after it.
 // ============================================================================
+constexpr int kVlMaxSplit = 4;      // CTAs that share a key tile at most (dK/dV)
 constexpr int kVbThreads = 352;     // two compute warpgroups, MMA warp, two loader warps
 
 template <int DP>
@@ -611,7 +659,7 @@ __global__ void __launch_bounds__(kVbThreads, 1)
 attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                       const __grid_constant__ VlParams p, const uint16_t* __restrict__ O,
-                      const float* __restrict__ lse, float* __restrict__ delta, float* __restrict__ lse2,
+                      const uint8_t* __restrict__ low, const float* __restrict__ lse, float* __restrict__ delta, float* __restrict__ lse2,
                       uint16_t* __restrict__ dQ) {
   using L = VqSmem<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -740,15 +788,28 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     // delta: this warpgroup's half of the columns, O from global (before the wait), dO from the tile
     constexpr int CH = DP / 16;                                  // 8-column chunks of the half
     uint4 ov[CH];
+    uint2 lv[CH];
     {
-      const uint16_t* orow = O + ((int64_t)(w.start + q) * p.Hq + h) * p.D;
+      const int64_t at = ((int64_t)(w.start + q) * p.Hq + h) * p.D;
+      const uint16_t* orow = O + at;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = g * (DP / 2) + c * 8;
         ov[c] = live && col < p.D ? *reinterpret_cast<const uint4*>(orow + col) : make_uint4(0, 0, 0, 0);
+        lv[c] = live && col < p.D ? *reinterpret_cast<const uint2*>(low + at + col) : make_uint2(0, 0);
       }
     }
     bool ok = vl_wait(q_full, 0, p.status, kErrVlCompute);
+    if (ok) {  // warpgroup 0 copies Q, warpgroup 1 dO: the first scores can start
+      const uint8_t* src = smem + (g == 0 ? L::kQ : L::kDO) + row * 128;
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a)
+        copy_row_to_tmem(src + a * 16384, row, lane_base + 384u + (uint32_t)(64 * g + 32 * a));
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(in_tmem);
+    }
     float dl = 0.0f;
     {
       float acc = 0.0f;
@@ -760,10 +821,14 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         const uint4 du = *reinterpret_cast<const uint4*>(drow + ((chunk ^ (row & 7)) << 4));
         const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[c].x, ov[c].y, ov[c].z, ov[c].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 a = vl_unpack<FP16>(dw[j]), b = vl_unpack<FP16>(ow[j]);
-          acc = fmaf(a.x, b.x, acc);
-          acc = fmaf(a.y, b.y, acc);
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t lw = j == 0 ? lv[c].x : lv[c].y;
+          const float2 a0 = vl_unpack<FP16>(dw[2 * j]), b0 = vl_unpack<FP16>(ow[2 * j]);
+          const float2 a1 = vl_unpack<FP16>(dw[2 * j + 1]), b1 = vl_unpack<FP16>(ow[2 * j + 1]);
+          acc = fmaf(a0.x, vl_with_low<FP16, 0>(b0.x, lw), acc);
+          acc = fmaf(a0.y, vl_with_low<FP16, 1>(b0.y, lw), acc);
+          acc = fmaf(a1.x, vl_with_low<FP16, 2>(b1.x, lw), acc);
+          acc = fmaf(a1.y, vl_with_low<FP16, 3>(b1.y, lw), acc);
         }
       }
       float* xs = reinterpret_cast<float*>(smem + L::kX);
@@ -775,16 +840,6 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         delta[at] = dl;
         lse2[at] = l2;
       }
-    }
-    if (ok) {  // warpgroup 0 copies Q, warpgroup 1 dO
-      const uint8_t* src = smem + (g == 0 ? L::kQ : L::kDO) + row * 128;
-#pragma unroll
-      for (int a = 0; a < DP / 64; ++a)
-        copy_row_to_tmem(src + a * 16384, row, lane_base + 384u + (uint32_t)(64 * g + 32 * a));
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(in_tmem);
     }
     const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(-l2, -l2), dl2 = f2_pack(dl, dl);
     for (int t = g; t < n_kv && ok; t += 2) {
@@ -841,6 +896,11 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 // Tensor memory: dV 0.., dK 128.., Sᵀ 256 + 128 b, dPᵀ 320 + 128 b (b = t & 1),
 // Pᵀ and dSᵀ over the first 32 columns of theirs.  Q and dO come through rings of
 // four tiles with the tile's lse·log2(e) and delta.
+//
+// Where there are few key tiles a cluster of S CTAs shares one: CTA r takes every
+// S-th of its query tiles, and at the end each writes its dV and dK (32 bits) into
+// its own rings' memory, and sums one S-th of the columns over the cluster, in rank
+// order - no atomics, the same result every time.
 // ============================================================================
 template <int DP>
 struct VkSmem {
@@ -859,6 +919,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
                        const __grid_constant__ VlParams p, const float* __restrict__ lse2,
                        const float* __restrict__ delta, uint16_t* __restrict__ dK, uint16_t* __restrict__ dV) {
   using L = VkSmem<DP>;
+  static_assert(2 * L::kStages * L::kHalf >= 2 * 128 * DP * 4, "the rings hold dV and dK in 32 bits");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
@@ -873,10 +934,11 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int entry = blockIdx.x / p.Hk, hk = blockIdx.x % p.Hk;
+  const int S = p.split, rank = (int)(blockIdx.x % (unsigned)S);
+  const int entry = blockIdx.x / (unsigned)S / p.Hk, hk = blockIdx.x / (unsigned)S % p.Hk;
   const int count = p.meta[p.count_at];
-  if (entry >= count) {
-    if (entry == count) {
+  if (entry >= count) {   // (all of a cluster)
+    if (entry == count && rank == 0) {
       vl_zero_outside(dK, p.T, p.Hk, hk, p.D, p.meta);
       vl_zero_outside(dV, p.T, p.Hk, hk, p.D, p.meta);
     }
@@ -886,7 +948,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   const int group = p.Hq / p.Hk, key0 = w.tile * 128;
   const int i0 = p.causal ? 2 * w.tile : 0;          // first 64-query tile that sees this key tile
   const int per_head = (w.len + 63) / 64 - i0;
-  const int n_it = group * per_head;
+  const int n_it = (group * per_head - rank + S - 1) / S;   // this CTA's; 0 where there are fewer tiles than CTAs
   const int slot0 = w.slot - w.tile;                 // the sequence's first slot
 
   if (threadIdx.x == 0) {
@@ -919,9 +981,10 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       uint64_t* empty = is_q ? q_empty : o_empty;
       uint64_t* full = is_q ? q_full : o_full;
       uint8_t* ring = smem + (is_q ? L::kQ : L::kDO);
-      int issued = 0, h = hk * group, it = i0;
+      int issued = 0, h = hk * group, it = i0 + rank;
       bool ok = true;
       for (int t = 0; t < n_it; ++t) {
+        while (it >= i0 + per_head) { it -= per_head; ++h; }
         const int st = t % L::kStages;
         if (!mbar_wait(&empty[st], ((t / L::kStages) & 1) ^ 1, p.status, kErrVlLoad)) { ok = false; break; }
         mbar_arrive_expect_tx(&full[st], L::kHalf + (is_q ? 0 : 512));
@@ -932,8 +995,9 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           bulk_load(smem + L::kLD + st * 512 + 256, delta + at, 256, &full[st]);
         }
         issued = t + 1;
-        if (++it == i0 + per_head) { it = i0; ++h; }
+        it += S;
       }
+      if (is_q && n_it == 0) mbar_wait(kv_full, 0, nullptr, 0);   // nobody else waits for K and V
       if (!ok) {  // let every copy this thread issued land before the CTA can exit
         if (is_q) mbar_wait(kv_full, 0, nullptr, 0);
         for (int t = max(issued - L::kStages, 0); t < issued; ++t)
@@ -966,7 +1030,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       __syncwarp();
       return true;
     };
-    bool ok = vl_wait(kv_full, 0, p.status, kErrVlMma) && issue_scores(0);
+    bool ok = n_it > 0 && vl_wait(kv_full, 0, p.status, kErrVlMma) && issue_scores(0);
     for (int t = 0; t < n_it && ok; ++t) {
       if (t + 1 < n_it && !issue_scores(t + 1)) { ok = false; break; }
       if (!vl_wait(&p_full[t & 1], (t >> 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
@@ -997,7 +1061,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t sc = lane_base + 256u + 128u * (uint32_t)g;
     bool ok = true;
-    int it = i0 + g % per_head;
+    int it = i0 + (rank + S * g) % per_head;
     for (int t = g; t < n_it; t += 2) {
       const int st = t % L::kStages;
       const float* sl = reinterpret_cast<const float*>(smem + L::kLD + st * 512);
@@ -1044,18 +1108,63 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[g]);
-      it += 2;
+      it += 2 * S;
       while (it >= i0 + per_head) it -= per_head;
     }
-    if (ok && vl_wait(acc_done, 0, p.status, kErrVlCompute)) {
-      tc_fence_after();
+    ok = ok && vl_wait(acc_done, 0, p.status, kErrVlCompute);
+    tc_fence_after();
+    // warpgroup 0 has dV, warpgroup 1 dK
+    const uint32_t acc = lane_base + (uint32_t)(128 * g);
+    if (S == 1) {
       const int64_t at = ((int64_t)(w.start + key) * p.Hk + hk) * p.D;
-      const bool live = key < w.len;
-      // warpgroup 0 writes dV, warpgroup 1 dK
-      vl_store_row<FP16, DP>(lane_base + (uint32_t)(128 * g), g == 0 ? 1.0f : p.scale, (g == 0 ? dV : dK) + at, 0, p.D, live);
+      if (ok) vl_store_row<FP16, DP>(acc, g == 0 ? 1.0f : p.scale, (g == 0 ? dV : dK) + at, 0, p.D, key < w.len);
+    } else {   // [column][row]: the lanes of a warp write one line
+      float* mine = reinterpret_cast<float*>(smem + L::kQ) + g * DP * 128 + row;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (n_it > 0) {
+          tmem_ld_32x32b_x32(acc + (uint32_t)c, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mine[(c + i) * 128] = n_it > 0 ? __uint_as_float(o[i]) : 0.0f;
+      }
     }
   }
 
+  if (S > 1) {
+    __syncwarp();
+    cluster_sync_all();   // every CTA's dV and dK are in its shared memory
+    if (warp < 8) {
+      const int g = warp >> 2, row = (warp & 3) * 32 + lane, key = key0 + row;
+      const float f = g == 0 ? 1.0f : p.scale;
+      const uint32_t mine = smem_u32(smem + L::kQ) + (uint32_t)((g * DP * 128 + row) * 4);
+      uint16_t* out = (g == 0 ? dV : dK) + ((int64_t)(w.start + key) * p.Hk + hk) * p.D;
+      const int cols = DP / S;
+#pragma unroll 1
+      for (int c = rank * cols; c < (rank + 1) * cols; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        for (int r = 0; r < S; ++r) {
+          const uint32_t from = map_to_cta(mine, (uint32_t)r) + (uint32_t)(c * 512);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from + (uint32_t)(i * 512)) : "memory");
+            v[i] += x;
+          }
+        }
+        if (key < w.len && c < p.D)
+          *reinterpret_cast<uint4*>(out + c) =
+              make_uint4(vl_pack<FP16>(v[0] * f, v[1] * f), vl_pack<FP16>(v[2] * f, v[3] * f),
+                         vl_pack<FP16>(v[4] * f, v[5] * f), vl_pack<FP16>(v[6] * f, v[7] * f));
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();   // read by all before a CTA's memory goes
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, 512); }
@@ -1118,7 +1227,7 @@ static CUtensorMap vl_tmap(const at::Tensor& t, int box_rows) {
 
 struct VlCall {
   VlParams p;
-  int64_t c256, c128;
+  int64_t c256, c128, n;
   bool fp16, narrow;
 };
 
@@ -1140,10 +1249,11 @@ static VlCall vl_check(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   VlCall c;
   c.c256 = vl_cap(T, n, 256);
   c.c128 = vl_cap(T, n, 128);
-  TORCH_CHECK((c.c128 + 1) * Hq < (1LL << 31), "attention: grid too large");
+  c.n = n;
+  TORCH_CHECK((c.c128 + 1) * Hq * kVlMaxSplit < (1LL << 31), "attention: grid too large");
   const int* words = plan.data_ptr<int>();
   c.p = VlParams{reinterpret_cast<const VlTile*>(words), words + 4 * (c.c256 + 2 * c.c128), 0, (int)T, (int)Hq, (int)Hk,
-                 (int)D, causal ? 1 : 0, (int)c.c128, (float)scale, (float)(scale * 1.4426950408889634),
+                 (int)D, causal ? 1 : 0, (int)c.c128, 1, (float)scale, (float)(scale * 1.4426950408889634),
                  status_buffer(q.get_device())};
   c.fp16 = q.scalar_type() == at::kHalf;
   c.narrow = D <= 64;
@@ -1166,18 +1276,26 @@ static void vl_smem(K kern, int bytes, bool (&done)[64], int dev) {
 
 template <bool FP16, int DP>
 static void vl_launch_fwd(const VlCall& c, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, uint16_t* o,
-                          float* lse, int dev) {
+                          float* lse, uint8_t* low, int dev) {
   static bool done[64] = {false};
   auto kern = attn_varlen_fwd_kernel<FP16, DP>;
   vl_smem(kern, VfSmem<DP>::kBytes, done, dev);
   kern<<<(unsigned)((c.c256 + 1) * c.p.Hq), kVfThreads, VfSmem<DP>::kBytes, at::cuda::getCurrentCUDAStream()>>>(tq, tk, tv, c.p,
-                                                                                                               o, lse);
+                                                                                                               o, lse, low);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// o [T, Hq, D] contiguous; lse [Hq, T] fp32 (rows of no sequence are not written)
+static uint8_t* vl_low(const at::Tensor& low, const at::Tensor& q) {
+  TORCH_CHECK(low.is_cuda() && low.get_device() == q.get_device() && low.scalar_type() == at::kChar && low.is_contiguous() &&
+                  low.sizes() == q.sizes() && (reinterpret_cast<uintptr_t>(low.data_ptr()) & 7) == 0,
+              "attention: the low bytes of o are int8, contiguous, like q");
+  return reinterpret_cast<uint8_t*>(low.data_ptr());
+}
+
+// o [T, Hq, D] contiguous; lse [Hq, T] fp32 and, for a backward, low [T, Hq, D] int8
+// (the rows of no sequence are not written in these)
 void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, at::Tensor o, at::Tensor lse,
-                     bool causal, double scale) {
+                     c10::optional<at::Tensor> low, bool causal, double scale) {
   VlCall c = vl_check(q, k, v, plan, n, causal, scale);
   uint16_t* op = vl_out(o, q);
   TORCH_CHECK(lse.is_cuda() && lse.get_device() == q.get_device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
@@ -1188,12 +1306,13 @@ void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, 
   c.p.count_at = 0;
   auto go = c.fp16 ? (c.narrow ? vl_launch_fwd<true, 64> : vl_launch_fwd<true, 128>)
                    : (c.narrow ? vl_launch_fwd<false, 64> : vl_launch_fwd<false, 128>);
-  go(c, tq, tk, tv, op, lse.data_ptr<float>(), q.get_device());
+  go(c, tq, tk, tv, op, lse.data_ptr<float>(), low.has_value() ? vl_low(*low, q) : nullptr, q.get_device());
 }
 
 struct VlBwd {
   CUtensorMap q128, do128, k64, v64, q64, do64, k128, v128;
   const uint16_t* o;
+  const uint8_t* low;
   const float* lse;
   float *delta, *lse2;
   uint16_t *dq, *dk, *dv;
@@ -1210,19 +1329,37 @@ static void vl_launch_bwd(VlCall& c, const VlBwd& b, int dev) {
   const VlTile* tiles = c.p.tiles;
   c.p.count_at = 1;
   c.p.tiles = tiles + c.c256;
-  kq<<<(unsigned)((c.c128 + 1) * c.p.Hq), kVbThreads, VqSmem<DP>::kBytes, stream>>>(b.q128, b.k64, b.v64, b.do128, c.p, b.o, b.lse,
+  kq<<<(unsigned)((c.c128 + 1) * c.p.Hq), kVbThreads, VqSmem<DP>::kBytes, stream>>>(b.q128, b.k64, b.v64, b.do128, c.p, b.o, b.low,
+                                                                                   b.lse,
                                                                                    b.delta, b.lse2, b.dq);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   c.p.count_at = 2;
   c.p.tiles = tiles + c.c256 + c.c128;
-  kk<<<(unsigned)((c.c128 + 1) * c.p.Hk), kVbThreads, VkSmem<DP>::kBytes, stream>>>(b.q64, b.k128, b.v128, b.do64, c.p, b.lse2,
-                                                                                   b.delta, b.dk, b.dv);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // A cluster to a key tile where the tiles are too few to even out over the SMs, as
+  // long as each of its CTAs keeps about eight query tiles of 64 on average (the exchange
+  // at the end takes about 3 us).
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int64_t work = c.c128 * c.p.Hk;
+  const int64_t each = (int64_t)(c.p.Hq / c.p.Hk) * c.p.T / std::max<int64_t>(c.n, 1) / (c.p.causal ? 128 : 64);
+  c.p.split = work <= sms && each >= 32 ? 4 : work <= 3 * sms && each >= 16 ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((c.c128 + 1) * c.p.Hk * c.p.split));
+  cfg.blockDim = dim3(kVbThreads);
+  cfg.dynamicSmemBytes = VkSmem<DP>::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c.p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kk, b.q64, b.k128, b.v128, b.do64, c.p, (const float*)b.lse2, (const float*)b.delta,
+                                    b.dk, b.dv));
 }
 
-// dq, dk, dv (contiguous) from dout, the forward's inputs, o and lse: two launches
-void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor plan,
-                     int64_t n, at::Tensor dq, at::Tensor dk, at::Tensor dv, bool causal, double scale) {
+// dq, dk, dv (contiguous) from dout, the forward's inputs, o, lse and low: two launches
+void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor low,
+                     at::Tensor plan, int64_t n, at::Tensor dq, at::Tensor dk, at::Tensor dv, bool causal, double scale) {
   VlCall c = vl_check(q, k, v, plan, n, causal, scale);
   TORCH_CHECK(dout.is_cuda() && dout.get_device() == q.get_device() && dout.scalar_type() == q.scalar_type() &&
                   dout.sizes() == q.sizes(),
@@ -1233,7 +1370,7 @@ void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, 
   const c10::cuda::CUDAGuard guard(q.device());
   auto stats = at::empty({2, q.size(1), c.c128 * 128}, lse.options());
   VlBwd b{vl_tmap(q, 128), vl_tmap(dout, 128), vl_tmap(k, 64), vl_tmap(v, 64), vl_tmap(q, 64), vl_tmap(dout, 64), vl_tmap(k, 128),
-          vl_tmap(v, 128), vl_out(o, q), lse.data_ptr<float>(), stats.data_ptr<float>(),
+          vl_tmap(v, 128), vl_out(o, q), vl_low(low, q), lse.data_ptr<float>(), stats.data_ptr<float>(),
           stats.data_ptr<float>() + stats.numel() / 2, vl_out(dq, q), vl_out(dk, k), vl_out(dv, v)};
   auto go = c.fp16 ? (c.narrow ? vl_launch_bwd<true, 64> : vl_launch_bwd<true, 128>)
                    : (c.narrow ? vl_launch_bwd<false, 64> : vl_launch_bwd<false, 128>);

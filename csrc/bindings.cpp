@@ -68,22 +68,18 @@ void lion_step(at::Tensor master, at::Tensor grad, at::Tensor mom, double lr, do
                double wd, int64_t seed);
 // attention_varlen_sm100.cu
 int64_t packed_plan_words(int64_t T, int64_t n);
-void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions);
 void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, at::Tensor o, at::Tensor lse,
-                     bool causal, double scale);
-void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor plan,
-                     int64_t n, at::Tensor dq, at::Tensor dk, at::Tensor dv, bool causal, double scale);
+                     c10::optional<at::Tensor> low, bool causal, double scale);
 // rotary.cu
 void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
             c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign);
-// distill.cu
-void distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets,
-             at::Tensor rows, at::Tensor sums, c10::optional<at::Tensor> grad, c10::optional<at::Tensor> loss,
-             int64_t vocab, int64_t ignore_index, double temperature, double alpha);
-void distill_grad(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets,
-                  at::Tensor sums, at::Tensor g, at::Tensor grad, int64_t vocab, int64_t ignore_index,
-                  double temperature, double alpha);
-void scale_by_scalar(at::Tensor x, at::Tensor g);
+// packed_autograd.cpp
+std::vector<at::Tensor> rotary_embedding(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns,
+                                         bool interleaved, double factor);
+std::vector<at::Tensor> packed_sequences(at::Tensor cu, int64_t T);
+at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, bool causal, double scale);
+at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets, int64_t vocab,
+                        int64_t ignore_index, double temperature, double alpha, bool mean, bool fused);
 // p2p.cu
 std::vector<int64_t> peer_alloc(int64_t bytes);
 at::Tensor peer_handle(int64_t ptr);
@@ -169,13 +165,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_into", &rope_into);
   m.def("rope_into2", &rope_into2, "rope_into for two (x, out) pairs in one launch");
   m.def("packed_plan_words", &packed_plan_words);
-  m.def("packed_plan", &packed_plan, "tile tables and positions of packed sequences");
+  m.def("packed_sequences", &packed_sequences, "tile tables and positions of packed sequences");
   m.def("attn_varlen_fwd", &attn_varlen_fwd, "tcgen05 attention over packed sequences, forward");
-  m.def("attn_varlen_bwd", &attn_varlen_bwd, "its backward: dQ, then dK/dV");
   m.def("rotary", &rotary, "rotary positions for q and k: explicit positions, either layout, part of the head");
-  m.def("distill", &distill, "distillation loss rows, and in the same launch the mean and its gradient");
-  m.def("distill_grad", &distill_grad, "gradient of the distillation loss rows from their log-sum-exps");
-  m.def("scale_by_scalar", &scale_by_scalar, "x *= g[0] in place; nothing is touched where g[0] is 1");
+  // the differentiable forms: kernels of the backward are launched from C++
+  m.def("rotary_embedding", &rotary_embedding);
+  m.def("attn_varlen", &attn_varlen);
+  m.def("distill_loss", &distill_loss);
   m.def("gelu_fwd", &gelu_fwd);
   m.def("gelu_bwd", &gelu_bwd);
   m.def("gelu_cdf_pdf", &gelu_cdf_pdf);

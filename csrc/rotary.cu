@@ -10,15 +10,16 @@
 // Angles: pos · turns[i] is formed in 64 bits and reduced to a fraction of a
 // turn there (at position 262144 an angle held in 32 bits is off by up to 2^-6
 // radians), then sin and cos are taken in 32 bits of an argument in [-1, 1] half
-// turns.  They are computed once for each (token, pair)
-// into shared memory and used by all heads of the token: R/2 evaluations for
-// (Hq + Hk) · D elements, so the kernel stays bound by memory.  turns travels in
-// the kernel's parameters: no table in global memory to keep or to fill.
+// turns.  turns travels in the kernel's parameters: no table in global memory to
+// keep or to fill.
 //
-// A block takes `tile` tokens at a time; a thread moves 16 bytes of each half of
-// the pair range (one 16-byte vector when interleaved).  Rows that are not
-// 16-byte aligned, or whose widths are not whole vectors, take the element-wise
-// form of the same code.
+// A thread owns one 16-byte column of one token (two of them, one in each half, in
+// the half layout): it evaluates its pairs' angles once, keeps them in registers and
+// walks over the heads, so there is no shared memory and no barrier, and the
+// evaluations are R/2 per token for (Hq + Hk) · D elements.  Bound by memory.  With
+// few tokens the heads are divided over the grid's second axis.  Rows that are not
+// 16-byte aligned, or whose widths are not whole vectors, take the element-wise form
+// of the same code.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -29,7 +30,6 @@ namespace zq {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxPairs = 128;   // rotary width up to 256
-constexpr int kRotMaxTile = 16;     // tokens per block iteration
 
 struct RotarySide {
   const void* x;
@@ -42,7 +42,7 @@ struct RotaryParams {
   RotarySide side[2];        // q, k
   const void* positions;
   int64_t tokens, pos_len;   // token t sits at positions[t % pos_len]
-  int dim, rot, tile, pos64;
+  int dim, rot, heads_per_block, pos64;
   float sin_factor, factor;
   double turns[kRotMaxPairs];
 };
@@ -74,84 +74,131 @@ __device__ __forceinline__ void rot_store(T* p, const float (&v)[VEC]) {
   }
 }
 
-// VEC elements per access: 16 bytes (WIDE), or 1 (half layout) / 2 (interleaved)
+// U heads of one side at once: loads, then turns, then stores.
+// VEC elements per access: 16 bytes (WIDE), or 1 (half layout) / 2 (interleaved).
+template <typename T, int VEC, bool WIDE, bool INTER, int U>
+__device__ __forceinline__ void rot_heads(const T* x, T* y, int64_t head_stride, int dim, int half, const float* c,
+                                          const float* s) {
+  float a[U][VEC], b[U][VEC];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    rot_load<T, VEC, WIDE>(x + u * head_stride, a[u]);
+    if constexpr (!INTER) rot_load<T, VEC, WIDE>(x + u * head_stride + half, b[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float lo[VEC], hi[VEC];
+    if constexpr (INTER) {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        lo[2 * i] = rope_lo(a[u][2 * i], a[u][2 * i + 1], c[i], s[i]);
+        lo[2 * i + 1] = rope_hi(a[u][2 * i], a[u][2 * i + 1], c[i], s[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        lo[i] = rope_lo(a[u][i], b[u][i], c[i], s[i]);
+        hi[i] = rope_hi(a[u][i], b[u][i], c[i], s[i]);
+      }
+      rot_store<T, VEC, WIDE>(y + (int64_t)u * dim + half, hi);
+    }
+    rot_store<T, VEC, WIDE>(y + (int64_t)u * dim, lo);
+  }
+}
+
 template <typename T, int VEC, bool WIDE, bool INTER>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 cs[];   // [tile][R/2] (cos, sin), times the factor
-  const int half = p.rot / 2;
-  const int turn_items = INTER ? p.rot / VEC : half / VEC;
+  constexpr int PAIRS = INTER ? VEC / 2 : VEC;       // pairs of one thread
   constexpr int PASS = (INTER && !WIDE) ? 1 : VEC;   // widths past R need not be whole pairs
+  const int half = p.rot / 2;
+  const int turn_items = half / PAIRS;
   const int items = turn_items + (p.dim - p.rot) / PASS;
+  // threads of one kind together: first all tokens' pairs, then all tokens' other columns
+  const int64_t n = (int64_t)blockIdx.x * kRotThreads + threadIdx.x;
+  const bool turns = n < p.tokens * turn_items;
+  const int kind = turns ? turn_items : items - turn_items;
+  const int64_t left = turns ? n : n - p.tokens * turn_items;
+  if (left >= p.tokens * kind) return;
+  const int64_t tok = left / kind;
+  const int it = (int)(left - tok * kind);
+  float c[PAIRS], s[PAIRS];
+  if (turns) {
+    const int64_t at = p.pos_len == p.tokens ? tok : tok % p.pos_len;
+    const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.positions)[at]
+                                : (int64_t)reinterpret_cast<const int32_t*>(p.positions)[at];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const double turn = (double)pos * p.turns[it * PAIRS + i];
+      sincospif(2.0f * (float)(turn - rint(turn)), &s[i], &c[i]);
+      c[i] *= p.factor;
+      s[i] *= p.sin_factor;
+    }
+  }
+  const int col = turns ? it * (INTER ? VEC : PAIRS) : p.rot + it * PASS;
+  // this block's heads [h0, h1) of both sides in a row
   const int heads = p.side[0].heads + p.side[1].heads;
-  const int per_token = heads * items;
-  for (int64_t t0 = (int64_t)blockIdx.x * p.tile; t0 < p.tokens; t0 += (int64_t)gridDim.x * p.tile) {
-    const int nt = (int)min((int64_t)p.tile, p.tokens - t0);
-    for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
-      const int64_t at = (t0 + i / half) % p.pos_len;
-      const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.positions)[at]
-                                  : (int64_t)reinterpret_cast<const int32_t*>(p.positions)[at];
-      const double turn = (double)pos * p.turns[i % half];
-      float s, c;
-      sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-      cs[i] = make_float2(c * p.factor, s * p.sin_factor);
-    }
-    __syncthreads();
-    for (int n = threadIdx.x; n < nt * per_token; n += kRotThreads) {
-      const int tok = n / per_token, in = n - tok * per_token;
-      const int hd = in / items, it = in - hd * items;
-      const bool second = hd >= p.side[0].heads;
-      const RotarySide& sd = p.side[second ? 1 : 0];
-      const int h = second ? hd - p.side[0].heads : hd;
-      const T* x = reinterpret_cast<const T*>(sd.x) + (t0 + tok) * sd.token_stride + h * sd.head_stride;
-      T* y = reinterpret_cast<T*>(sd.y) + ((t0 + tok) * sd.heads + h) * (int64_t)p.dim;
-      if (it >= turn_items) {   // columns past the rotary width
-        const int c = p.rot + (it - turn_items) * PASS;
+  const int h0 = blockIdx.y * p.heads_per_block, h1 = min(heads, h0 + p.heads_per_block);
+#pragma unroll
+  for (int sd = 0; sd < 2; ++sd) {
+    const RotarySide& side = p.side[sd];
+    const int first = sd == 0 ? 0 : p.side[0].heads;
+    int h = max(h0 - first, 0);
+    const int end = min(h1 - first, side.heads);
+    if (h >= end) continue;
+    const T* x = reinterpret_cast<const T*>(side.x) + tok * side.token_stride + h * side.head_stride + col;
+    T* y = reinterpret_cast<T*>(side.y) + (tok * side.heads + h) * (int64_t)p.dim + col;
+    if (turns) {
+      constexpr int U = 4;
+      for (; h + U <= end; h += U) {
+        rot_heads<T, VEC, WIDE, INTER, U>(x, y, side.head_stride, p.dim, half, c, s);
+        x += U * side.head_stride;
+        y += U * (int64_t)p.dim;
+      }
+      for (; h < end; ++h) {
+        rot_heads<T, VEC, WIDE, INTER, 1>(x, y, side.head_stride, p.dim, half, c, s);
+        x += side.head_stride;
+        y += p.dim;
+      }
+    } else {   // columns past the rotary width
+      constexpr int U = 4;
+      for (; h < end; h += U) {
+        const int m = min(U, end - h);
         if constexpr (WIDE) {
-          *reinterpret_cast<uint4*>(y + c) = *reinterpret_cast<const uint4*>(x + c);
+          uint4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (u < m) v[u] = *reinterpret_cast<const uint4*>(x + u * side.head_stride);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (u < m) *reinterpret_cast<uint4*>(y + u * (int64_t)p.dim) = v[u];
         } else {
-#pragma unroll
-          for (int i = 0; i < PASS; ++i) y[c + i] = x[c + i];
+          for (int u = 0; u < m; ++u)
+            for (int i = 0; i < PASS; ++i) y[u * (int64_t)p.dim + i] = x[u * side.head_stride + i];
         }
-        continue;
-      }
-      if constexpr (INTER) {
-        const float2* w = cs + tok * half + it * (VEC / 2);
-        float v[VEC], o[VEC];
-        rot_load<T, VEC, WIDE>(x + it * VEC, v);
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-          o[2 * i] = rope_lo(v[2 * i], v[2 * i + 1], w[i].x, w[i].y);
-          o[2 * i + 1] = rope_hi(v[2 * i], v[2 * i + 1], w[i].x, w[i].y);
-        }
-        rot_store<T, VEC, WIDE>(y + it * VEC, o);
-      } else {
-        const float2* w = cs + tok * half + it * VEC;
-        float a[VEC], b[VEC], lo[VEC], hi[VEC];
-        rot_load<T, VEC, WIDE>(x + it * VEC, a);
-        rot_load<T, VEC, WIDE>(x + half + it * VEC, b);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          lo[i] = rope_lo(a[i], b[i], w[i].x, w[i].y);
-          hi[i] = rope_hi(a[i], b[i], w[i].x, w[i].y);
-        }
-        rot_store<T, VEC, WIDE>(y + it * VEC, lo);
-        rot_store<T, VEC, WIDE>(y + half + it * VEC, hi);
+        x += U * side.head_stride;
+        y += U * (int64_t)p.dim;
       }
     }
-    __syncthreads();   // the next tokens' angles overwrite these
   }
 }
 
 template <typename T>
-static void launch_rotary(const RotaryParams& p, bool wide, bool inter, unsigned grid, cudaStream_t stream) {
+static void launch_rotary(RotaryParams& p, bool wide, bool inter, int sms, cudaStream_t stream) {
   constexpr int W = 16 / (int)sizeof(T);
-  const size_t smem = (size_t)p.tile * (p.rot / 2) * sizeof(float2);
-  if (wide)
-    inter ? rotary_kernel<T, W, true, true><<<grid, kRotThreads, smem, stream>>>(p)
-          : rotary_kernel<T, W, true, false><<<grid, kRotThreads, smem, stream>>>(p);
-  else
-    inter ? rotary_kernel<T, 2, false, true><<<grid, kRotThreads, smem, stream>>>(p)
-          : rotary_kernel<T, 1, false, false><<<grid, kRotThreads, smem, stream>>>(p);
+  const int vec = wide ? W : inter ? 2 : 1, pairs = inter ? vec / 2 : vec, pass = inter && !wide ? 1 : vec;
+  const int64_t items = p.rot / 2 / pairs + (p.dim - p.rot) / pass;
+  const int64_t blocks = (p.tokens * items + kRotThreads - 1) / kRotThreads;
+  const int heads = p.side[0].heads + p.side[1].heads;
+  // all heads in one thread where the tokens alone fill the SMs (eight blocks each);
+  // otherwise the heads are divided until they do, down to four (the angles are
+  // evaluated once for each part), or to one where that still leaves SMs idle
+  const int64_t least = blocks * ((heads + 3) / 4) < sms ? 1 : 4;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((heads + least - 1) / least, 8 * sms / blocks));
+  p.heads_per_block = (int)((heads + parts - 1) / parts);
+  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block));
+  auto kern = wide ? (inter ? rotary_kernel<T, W, true, true> : rotary_kernel<T, W, true, false>)
+                   : (inter ? rotary_kernel<T, 2, false, true> : rotary_kernel<T, 1, false, false>);
+  kern<<<grid, kRotThreads, 0, stream>>>(p);
 }
 
 }  // namespace zq
@@ -197,7 +244,7 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
     heads += x.size(1);
   }
   if (heads == 0) return;
-  TORCH_CHECK(heads * D < (1 << 24), "rotary: heads x width too large");
+  TORCH_CHECK(heads < 65536 && T * D < (1LL << 38), "rotary: too many rows or heads");
   p.positions = positions.data_ptr();
   p.pos64 = positions.scalar_type() == at::kLong;
   p.tokens = T;
@@ -209,18 +256,11 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
   for (int64_t i = 0; i < turns.numel(); ++i) p.turns[i] = turns.data_ptr<double>()[i];
   const c10::cuda::CUDAGuard guard(q.device());
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // few tokens: one a block, so that the call is spread over the SMs; many: enough
-  // of them that a block's threads have about four vectors each between two barriers
-  const int64_t vectors = heads * std::max<int64_t>(1, D / (wide ? 2 * W : 2));
-  const int64_t most = std::min<int64_t>(kRotMaxTile, (4 * kRotThreads + vectors - 1) / vectors);
-  p.tile = (int)std::max<int64_t>(1, std::min<int64_t>(most, T / (8 * (int64_t)sms)));
-  const int64_t tiles = (T + p.tile - 1) / p.tile;
-  const unsigned grid = (unsigned)std::min<int64_t>(tiles, 8 * (int64_t)sms);
   auto stream = at::cuda::getCurrentCUDAStream();
   switch (q.scalar_type()) {
-    case at::kBFloat16: launch_rotary<__nv_bfloat16>(p, wide, interleaved, grid, stream); break;
-    case at::kHalf: launch_rotary<__half>(p, wide, interleaved, grid, stream); break;
-    case at::kFloat: launch_rotary<float>(p, wide, interleaved, grid, stream); break;
+    case at::kBFloat16: launch_rotary<__nv_bfloat16>(p, wide, interleaved, sms, stream); break;
+    case at::kHalf: launch_rotary<__half>(p, wide, interleaved, sms, stream); break;
+    case at::kFloat: launch_rotary<float>(p, wide, interleaved, sms, stream); break;
     default: TORCH_CHECK(false, "rotary: bf16, fp16 or fp32");
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();

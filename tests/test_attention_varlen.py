@@ -253,7 +253,7 @@ def test_kernel_refusals(cuda):
     from zeroq_b200.ops import _ext
     s = PackedSequences(cu, 10)
     with pytest.raises(RuntimeError, match="plan"):
-        _ext.ext().attn_varlen_fwd(q, k, v, s.plan, 2, torch.empty_like(q), torch.empty(2, 10, device=cuda), True, 0.1)
+        _ext.ext().attn_varlen_fwd(q, k, v, s.plan, 2, torch.empty_like(q), torch.empty(2, 10, device=cuda), None, True, 0.1)
 
 
 @pytest.mark.gpu

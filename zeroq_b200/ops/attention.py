@@ -150,34 +150,6 @@ def attention_varlen_reference(q, k, v, seqs: PackedSequences, causal: bool = Tr
     return torch.cat(parts)
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    """``t [T, H, D]`` can be read through a tensor map as it is (no repeated rows or heads)."""
-    return _tma_ok(t) and all(st > 0 or n == 1 for st, n in zip(t.stride(), t.shape))
-
-
-class _FlashAttnVarlen(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, seqs, causal, scale):
-        q, k, v = (t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-        T, Hq, _ = q.shape
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
-        _ext.ext().attn_varlen_fwd(q, k, v, seqs.plan, seqs.n, o, lse, causal, scale)
-        ctx.save_for_backward(q, k, v, o, lse, seqs.plan)
-        ctx.meta = (seqs.n, causal, scale)
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, lse, plan = ctx.saved_tensors
-        n, causal, scale = ctx.meta
-        do = do if _rows_ok(do) else do.clone(memory_format=torch.contiguous_format)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _ext.ext().attn_varlen_bwd(do, q, k, v, o, lse, plan, n, dq, dk, dv, causal, scale)
-        return dq, dk, dv, None, None, None
-
-
 def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                            seqs: Union[PackedSequences, torch.Tensor], causal: bool = True,
                            scale: Optional[float] = None) -> torch.Tensor:
@@ -214,4 +186,4 @@ def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise TypeError(f"flash_attention_varlen: bf16 or fp16 on the GPU, got {q.dtype}")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"flash_attention_varlen: head width a multiple of 8 up to 128 on the GPU, got {D}")
-    return _FlashAttnVarlen.apply(q, k, v, seqs, bool(causal), scale)
+    return _ext.ext().attn_varlen(q, k, v, seqs.plan, seqs.n, bool(causal), scale)

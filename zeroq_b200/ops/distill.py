@@ -47,67 +47,6 @@ def distillation_reference(logits, teacher_ids, teacher_logits, targets=None, te
     return loss if reduction == "none" else loss.sum() / counted.sum().clamp_min(1)
 
 
-def _like_rows(logits: torch.Tensor) -> torch.Tensor:
-    """An empty gradient with the logits' row pitch."""
-    M, W = logits.shape
-    pitch = logits.stride(0) if M > 1 else W
-    return torch.empty(M * pitch, dtype=logits.dtype, device=logits.device).as_strided((M, W), (pitch, 1))
-
-
-class _Distill(torch.autograd.Function):
-    """``reduction="mean"`` with a gradient wanted: loss and gradient in one pass
-    over the logits.  The gradient is formed for an upstream gradient of 1 and kept
-    (the logits are not); the backward multiplies it by another one in place, with
-    a second rounding, and hands it over - so it can run once."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, targets, vocab, ignore_index, temperature, alpha):
-        M = logits.shape[0]
-        rows = torch.empty(M, dtype=torch.float32, device=logits.device)
-        sums = torch.empty(M, 3, dtype=torch.float32, device=logits.device)
-        loss = torch.empty((), dtype=torch.float32, device=logits.device)
-        grad = _like_rows(logits)
-        _ext.ext().distill(logits, ids, teacher, targets, rows, sums, grad, loss, vocab, ignore_index,
-                           temperature, alpha)
-        ctx.grad = grad
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            raise RuntimeError("distillation_loss: its gradient was handed over by the first backward; "
-                               "call it again for another one")
-        flat = grad if grad.is_contiguous() else grad.as_strided((grad.shape[0] * grad.stride(0),), (1,))
-        _ext.ext().scale_by_scalar(flat, g.float())
-        return (grad,) + (None,) * 7
-
-
-class _DistillRows(torch.autograd.Function):
-    """Loss rows; the backward forms their gradient from the saved row sums (one more
-    read of the logits), each with its own upstream gradient in 32 bits."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, targets, vocab, ignore_index, temperature, alpha):
-        M = logits.shape[0]
-        rows = torch.empty(M, dtype=torch.float32, device=logits.device)
-        sums = torch.empty(M, 3, dtype=torch.float32, device=logits.device)
-        _ext.ext().distill(logits, ids, teacher, targets, rows, sums, None, None, vocab, ignore_index,
-                           temperature, alpha)
-        ctx.save_for_backward(logits, ids, teacher, targets, sums)
-        ctx.meta = (vocab, ignore_index, temperature, alpha)
-        return rows
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        logits, ids, teacher, targets, sums = ctx.saved_tensors
-        grad = _like_rows(logits)
-        _ext.ext().distill_grad(logits, ids, teacher, targets, sums, g.float().contiguous(), grad, *ctx.meta)
-        return (grad,) + (None,) * 7
-
-
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
                       targets: Optional[torch.Tensor] = None, temperature: float = 1.0, alpha: float = 1.0,
                       vocab: Optional[int] = None, ignore_index: int = -100,
@@ -161,21 +100,12 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     teacher = teacher_logits.detach()
     if teacher.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         teacher = teacher.float()
-    tg = None if targets is None else targets.to(torch.int64).contiguous()
     W = logits.shape[1]
-    if logits.stride(1) != 1 or logits.stride(0) < W or logits.stride(0) > 2 * W:
+    if logits.stride(1) != 1 or not W <= logits.stride(0) <= 2 * W:
         logits = logits.contiguous()
     if logits.data_ptr() % 16:
         logits = logits.clone(memory_format=torch.contiguous_format)
-    args = (logits, teacher_ids.contiguous(), teacher.contiguous(), tg, vocab, int(ignore_index),
-            float(temperature), float(alpha))
     # fp16: a gradient formed before the upstream factor (a loss scale) is known would
     # underflow, so its rows take the form that reads the logits again
-    if reduction == "mean" and logits.dtype != torch.float16 and torch.is_grad_enabled() and logits.requires_grad:
-        return _Distill.apply(*args)
-    rows = _DistillRows.apply(*args)
-    if reduction == "none":
-        return rows
-    if tg is None:
-        return rows.sum() / M
-    return rows.sum() / ((tg >= 0) & (tg < vocab)).sum().clamp_min(1)
+    return _ext.ext().distill_loss(logits, teacher_ids, teacher, targets, vocab, int(ignore_index), float(temperature),
+                                   float(alpha), reduction == "mean", logits.dtype != torch.float16)

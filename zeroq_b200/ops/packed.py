@@ -41,15 +41,12 @@ class PackedSequences:
         self.total = int(total)
         self.n = cu_seqlens.numel() - 1
         self.device = device
-        self.cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.device != device or not cu_seqlens.is_contiguous():
+            cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+        self.cu_seqlens = cu_seqlens
         self.plan = None
         if device.type == "cuda":
-            E = _ext.ext()
-            words = E.packed_plan_words(self.total, self.n)
-            # the plan and the positions share one buffer
-            buf = torch.empty(words + self.total, dtype=torch.int32, device=device)
-            self.plan, self.positions = buf[:words], buf[words:]
-            E.packed_plan(self.cu_seqlens, self.total, self.plan, self.positions)
+            self.plan, self.positions = _ext.ext().packed_sequences(self.cu_seqlens, self.total)
         else:
             self.positions = torch.zeros(self.total, dtype=torch.int32)
             for a, b in self.bounds():

@@ -224,39 +224,6 @@ def rotary_reference(x: torch.Tensor, positions: torch.Tensor, theta: float = 10
     return torch.cat([y, xf[..., R:]], dim=-1).to(x.dtype)
 
 
-def _rotary_launch(xs, positions, turns, factor, sign, interleaved):
-    """The kernel over one or two ``[..., H, D]`` tensors; contiguous outputs."""
-    flat = [t.flatten(0, -3) for t in xs]
-    flat = [t if t.stride(-1) == 1 else t.contiguous() for t in flat]
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
-    out_flat = [t.flatten(0, -3) for t in outs]
-    two = len(xs) == 2
-    _ext.ext().rotary(flat[0], flat[1] if two else None, positions, turns, out_flat[0],
-                      out_flat[1] if two else None, bool(interleaved), factor, sign)
-    return outs
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, turns, factor, interleaved):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions)
-        ctx.meta = (turns, factor, interleaved)
-        if k is None:
-            return _rotary_launch([q], positions, turns, factor, 1.0, interleaved)[0], None
-        return tuple(_rotary_launch([q, k], positions, turns, factor, 1.0, interleaved))
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        positions, = ctx.saved_tensors
-        turns, factor, interleaved = ctx.meta
-        given = [g for g in (gq, gk) if g is not None]
-        outs = iter(_rotary_launch(given, positions, turns, factor, -1.0, interleaved) if given else ())
-        dq = next(outs) if gq is not None else None
-        dk = next(outs) if gk is not None else None
-        return dq, dk, None, None, None, None
-
-
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                      theta: float = 10000.0, rotary_dim: Optional[int] = None, interleaved: bool = False,
                      scaling: Optional[RopeScaling] = None):
@@ -293,4 +260,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
         args = (positions, float(theta), R, interleaved, scaling)
         return rotary_reference(q, *args), None if k is None else rotary_reference(k, *args)
     turns, factor = _rope_turns(R, float(theta), scaling)
-    return _Rotary.apply(q, k, positions.reshape(-1).contiguous(), turns, factor, bool(interleaved))
+    if positions.dim() != 1 or not positions.is_contiguous():
+        positions = positions.reshape(-1).contiguous()
+    out = _ext.ext().rotary_embedding(q, k, positions, turns, bool(interleaved), factor)
+    return (out[0], None) if k is None else (out[0], out[1])
