@@ -21,7 +21,7 @@ void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, 
 void distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, OptTensor targets, at::Tensor rows, at::Tensor sums,
              OptTensor grad, OptTensor loss, int64_t vocab, int64_t ignore_index, double temperature, double alpha);
 void distill_grad(at::Tensor logits, at::Tensor ids, at::Tensor teacher, OptTensor targets, at::Tensor sums, at::Tensor g,
-                  at::Tensor grad, int64_t vocab, int64_t ignore_index, double temperature, double alpha);
+                  at::Tensor grad, int64_t vocab, int64_t ignore_index, double temperature, double alpha, bool mean);
 void scale_by_scalar(at::Tensor x, at::Tensor g);
 
 namespace {
@@ -167,18 +167,22 @@ struct DistillMean : public torch::autograd::Function<DistillMean> {
   }
 };
 
-// The rows' losses; the backward reads the logits again with each row's own upstream
+// The rows' losses, or their mean; the backward reads the logits again with the upstream
 // gradient in 32 bits.
 struct DistillRows : public torch::autograd::Function<DistillRows> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher,
-                            const OptTensor& targets, int64_t vocab, int64_t ignore_index, double temperature, double alpha) {
+                            const OptTensor& targets, int64_t vocab, int64_t ignore_index, double temperature, double alpha,
+                            bool mean) {
     at::AutoDispatchBelowADInplaceOrView below;
     const auto f32 = z.options().dtype(at::kFloat);
     at::Tensor rows = at::empty({z.size(0)}, f32), sums = at::empty({3 * z.size(0)}, f32);
-    distill(z, ids, teacher, targets, rows, sums, c10::nullopt, c10::nullopt, vocab, ignore_index, temperature, alpha);
+    OptTensor loss;
+    if (mean) loss = at::empty({}, f32);
+    distill(z, ids, teacher, targets, rows, sums, c10::nullopt, loss, vocab, ignore_index, temperature, alpha);
+    ctx->saved_data["mean"] = mean;
     ctx->save_for_backward({z, ids, teacher, targets.has_value() ? *targets : at::Tensor(), sums});
     save_args(ctx, {vocab, ignore_index, temperature, alpha});
-    return rows;
+    return mean ? *loss : rows;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "distillation_loss: its backward is not differentiable");
@@ -188,8 +192,10 @@ struct DistillRows : public torch::autograd::Function<DistillRows> {
     if (s[3].defined()) targets = s[3];
     distill_grad(s[0], s[1], s[2], targets, s[4], g[0].to(at::kFloat).contiguous(), grad, ctx->saved_data["vocab"].toInt(),
                  ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["temperature"].toDouble(),
-                 ctx->saved_data["alpha"].toDouble());
-    return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+                 ctx->saved_data["alpha"].toDouble(), ctx->saved_data["mean"].toBool());
+    variable_list out(9);
+    out[0] = grad;
+    return out;
   }
 };
 
@@ -226,7 +232,7 @@ at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan
   return o;
 }
 
-// `fused`: the mean with its gradient in one pass (needs a gradient to be wanted); otherwise the rows
+// The mean (`fused`: with its gradient in the same pass, where one is wanted) or the rows
 at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, OptTensor targets, int64_t vocab,
                         int64_t ignore_index, double temperature, double alpha, bool mean, bool fused) {
   ids = ids.contiguous();
@@ -234,10 +240,7 @@ at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, OptTen
   if (targets.has_value()) targets = targets->to(at::kLong).contiguous();
   if (wants_grad({&z})) {
     if (mean && fused) return DistillMean::apply(z, ids, teacher, targets, vocab, ignore_index, temperature, alpha);
-    at::Tensor rows = DistillRows::apply(z, ids, teacher, targets, vocab, ignore_index, temperature, alpha);
-    if (!mean) return rows;
-    if (!targets.has_value()) return rows.sum() / rows.size(0);
-    return rows.sum() / targets->ge(0).logical_and_(targets->lt(vocab)).sum().clamp_min(1);
+    return DistillRows::apply(z, ids, teacher, targets, vocab, ignore_index, temperature, alpha, mean);
   }
   const auto f32 = z.options().dtype(at::kFloat);
   at::Tensor rows = at::empty({z.size(0)}, f32), sums = at::empty({3 * z.size(0)}, f32);
