@@ -181,10 +181,9 @@ __device__ __forceinline__ float dist_smooth1(float v, float ss, float shift_s, 
   return lo;
 }
 
-// mbar_wait, and where it is over (`cluster`) once more with the acquire of the cluster's
-// writes (a costly one, so not at every look).  The looks hint at a long sleep: the
-// other block of the SM has work to issue meanwhile.
-__device__ __forceinline__ bool dist_wait_cluster(uint64_t* bar, uint32_t parity, bool cluster, DeviceStatus* st) {
+// mbar_wait whose looks hint at a long sleep: the other block of the SM has work to
+// issue meanwhile
+__device__ __forceinline__ bool dist_wait_long(uint64_t* bar, uint32_t parity, DeviceStatus* st) {
   unsigned long long t0 = 0;
   for (;;) {
     uint32_t ok;
@@ -197,7 +196,7 @@ __device__ __forceinline__ bool dist_wait_cluster(uint64_t* bar, uint32_t parity
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
         : "memory");
-    if (ok != 0) break;
+    if (ok != 0) return true;
     if (t0 == 0) {
       t0 = globaltimer();
     } else if (globaltimer() - t0 > kWaitTimeoutNs) {
@@ -205,19 +204,18 @@ __device__ __forceinline__ bool dist_wait_cluster(uint64_t* bar, uint32_t parity
       return false;
     }
   }
-  if (cluster) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        "  .reg .pred p;\n"
-        "  mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        "  selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-  }
-  return true;
+}
+
+// 16 bytes into the shared memory of block `rank` of the cluster, which complete that
+// many bytes of its barrier.  (An arrival with a release at cluster scope would wait
+// for the gradient stores of the row before.)
+__device__ __forceinline__ void dist_send(float* to, uint64_t* bar, int rank, float x, float y, float z) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+          map_to_cta(smem_u32(to), (uint32_t)rank)),
+      "r"(__float_as_uint(x)), "r"(__float_as_uint(y)), "r"(__float_as_uint(z)), "r"(0u),
+      "r"(map_to_cta(smem_u32(bar), (uint32_t)rank))
+      : "memory");
 }
 
 // 16 bytes of a row
@@ -285,19 +283,22 @@ struct DistShape {
   static constexpr int64_t kRing = (int64_t)SLOTS * kBytes;
 };
 using DistSmall = DistShape<128, 2, 8, 5>;      //  32 KB
-using DistMiddle = DistShape<256, 2, 6, 3>;     //  48 KB
-using DistWide = DistShape<512, 2, 6, 2>;       //  96 KB
-using DistWidest = DistShape<512, 2, 12, 1>;    // 192 KB
+using DistWide = DistShape<256, 4, 4, 3>;       //  64 KB
+using DistWidest = DistShape<512, 4, 6, 1>;     // 192 KB
 
 template <typename T, typename S, int MODE>
 __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const __grid_constant__ DistillParams p) {
   constexpr int NT = S::kNT, N = DistVec<T>::N, P = DistVec<T>::P;
   extern __shared__ __align__(128) uint8_t dist_smem[];
   uint8_t* ring = dist_smem;
-  float* s_p2 = reinterpret_cast<float*>(ring + S::kRing);   // [2][K + 1] log2 of the teacher's probability
-  int* s_id2 = reinterpret_cast<int*>(s_p2 + 2 * (p.K + 1)); // [2][K + 1] column, or -1
+  // the teacher's entries of two rows, and the target as the last of each: log2 of the
+  // probability, the column (or -1) and its logit
+  float* s_p2 = reinterpret_cast<float*>(ring + S::kRing);
+  int* s_id2 = reinterpret_cast<int*>(s_p2 + 2 * (p.K + 1));
+  float* s_z2 = reinterpret_cast<float*>(s_id2 + 2 * (p.K + 1));
   __shared__ uint64_t full[S::kSlots], empty[S::kSlots], joined[2];
-  __shared__ float s_part[2][kDistMaxCluster * S::kWarps][3];   // of all the cluster's warps
+  // of all the cluster's compute warps; behind them a token of each teacher warp
+  __shared__ __align__(16) float s_part[2][kDistMaxCluster * (S::kWarps + 1)][4];
   __shared__ float s_some[2];
   __shared__ uint32_t s_seen[kDistSeen / 32], s_twice[kDistSeen / 32];
   __shared__ int s_count;
@@ -316,8 +317,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
     }
     // the compute and teacher warps of the whole cluster: none of them is more than a row
     // ahead of another, so a row's parts are read before the next but one overwrites them
-    mbar_init(&joined[0], (uint32_t)(csize * (S::kWarps + 1)));
-    mbar_init(&joined[1], (uint32_t)(csize * (S::kWarps + 1)));
+    // (in a cluster by the bytes that they send)
+    mbar_init(&joined[0], csize > 1 ? 1u : (uint32_t)(S::kWarps + 1));
+    mbar_init(&joined[1], csize > 1 ? 1u : (uint32_t)(S::kWarps + 1));
     fence_mbar_init();
     s_count = 0;
   }
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
 
   // the end of pass 1: every warp's sums, the teacher's distribution
   auto wait_joined = [&](uint32_t turn) {
-    if (!dead && !dist_wait_cluster(&joined[turn & 1u], (turn >> 1) & 1u, csize > 1, p.status)) dead = true;
+    if (!dead && !dist_wait_long(&joined[turn & 1u], (turn >> 1) & 1u, p.status)) dead = true;
     __syncwarp();
   };
   struct Factors {
@@ -519,11 +521,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
           mbar_arrive(&joined[par]);
         }
       } else if (lane < csize) {
-        const uint32_t to = map_to_cta(smem_u32(s_part[par][crank * S::kWarps + warp]), (uint32_t)lane);
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u), "f"(a.soft) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8u), "f"(a.hard) : "memory");
-        mbar_arrive_cluster(map_to_cta(smem_u32(&joined[par]), (uint32_t)lane));
+        dist_send(s_part[par][crank * S::kWarps + warp], &joined[par], lane, a.m, a.soft, a.hard);
       }
       __syncwarp();
       if (dz != nullptr) {
@@ -587,6 +585,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
       const int par = (int)(turn & 1u);
       float* s_p = s_p2 + par * (p.K + 1);
       int* s_id = s_id2 + par * (p.K + 1);
+      float* s_z = s_z2 + par * (p.K + 1);
+      const T* z = logits_row(row);
       float tm = -INFINITY;
       for (int k0 = lane; k0 < p.K; k0 += 128) {   // four of each lane at once
         int64_t v[4];
@@ -603,6 +603,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
           if (k0 + 32 * u >= p.K) break;
           const bool in = v[u] >= 0 && v[u] < p.vocab;
           const float x = in ? t[u] * (kLog2e / p.tau) : -INFINITY;   // t / τ in log2 units
+          s_z[k0 + 32 * u] = in ? to_f32<T>(z[v[u]]) : 0.0f;
           s_id[k0 + 32 * u] = in ? (int)v[u] : -1;
           s_p[k0 + 32 * u] = x;
           tm = fmaxf(tm, x);
@@ -611,6 +612,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
       if (lane == 0) {
         s_id[p.K] = p.targets != nullptr ? (int)y : -1;
         s_p[p.K] = -INFINITY;
+        s_z[p.K] = p.targets != nullptr ? to_f32<T>(z[y]) : 0.0f;
       }
       __syncwarp();
       tm = -dist_shift(warp_max(tm), 1.0f);
@@ -624,8 +626,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
       __syncwarp();
       if (csize == 1) {
         if (lane == 0) mbar_arrive(&joined[par]);
-      } else if (lane < csize) {
-        mbar_arrive_cluster(map_to_cta(smem_u32(&joined[par]), (uint32_t)lane));
+      } else {
+        if (lane == 0) mbar_arrive_expect_tx(&joined[par], (uint32_t)(csize * (S::kWarps + 1)) * 16u);
+        if (lane < csize) dist_send(s_part[par][csize * S::kWarps + crank], &joined[par], lane, 0.0f, 0.0f, 0.0f);
       }
       __syncwarp();
     };
@@ -640,22 +643,22 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
       if (next < p.M) entries(next, turn + 1);
       const float* s_p = s_p2 + (turn & 1u) * (p.K + 1);
       const int* s_id = s_id2 + (turn & 1u) * (p.K + 1);
-      const T* z = logits_row(row);
-      const Cut c = cut(z);
+      const float* s_z = s_z2 + (turn & 1u) * (p.K + 1);
+      const Cut c = cut(logits_row(row));
       if (!p.grad_only && crank == 0) {
         const float log_s = log2f(f.a.soft);
         float kl = 0.0f;
 #pragma unroll 4
         for (int k = lane; k < p.K; k += 32) {
           const float lp = s_p[k], pk = dist_exp2(lp);
-          if (s_id[k] >= 0 && !(pk == 0.0f)) kl += pk * (lp - (fmaf(to_f32<T>(z[s_id[k]]), ss, f.shift_s) - log_s));
+          if (s_id[k] >= 0 && !(pk == 0.0f)) kl += pk * (lp - (fmaf(s_z[k], ss, f.shift_s) - log_s));
         }
         kl = warp_sum(kl);
         if (lane == 0) {
           float loss = 0.0f;
           if (p.alpha > 0.0f) loss = p.alpha * p.tau * p.tau * kLn2 * kl;
           if (p.alpha < 1.0f) {
-            const float zy = to_f32<T>(z[y_row]);
+            const float zy = s_z[p.K];
             const float at = MODE == 0 ? fmaf(zy, kLog2e, f.shift_h) : (MODE == 1 ? 1.0f : (float)MODE) * fmaf(zy, ss, f.shift_s);
             loss += (1.0f - p.alpha) * kLn2 * (log2f(MODE == 1 ? f.a.soft : f.a.hard) - at);
           }
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
             for (int j = 0; j < p.K; ++j)
               if (s_id[j] == id) pk += dist_exp2(s_p[j]);
           }
-          float d = dist_smooth1<MODE>(to_f32<T>(z[id]), ss, f.shift_s, f.shift_h, f.fs, f.fh) - f.cs * pk;
+          float d = dist_smooth1<MODE>(s_z[k], ss, f.shift_s, f.shift_h, f.fs, f.fh) - f.cs * pk;
           if (p.targets != nullptr && id == (int)y_row) d -= f.ch;
           dz[id] = from_f32<T>(d);
         }
@@ -784,8 +787,8 @@ static void launch_distill(const DistillParams& p, int csize, cudaStream_t strea
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const size_t smem = (size_t)S::kRing + 16 * std::min((size_t)1 << kpow, (size_t)kDistMaxK + 1);
-  const size_t most = (size_t)S::kRing + 16 * (kDistMaxK + 1);
+  const size_t smem = (size_t)S::kRing + 24 * std::min((size_t)1 << kpow, (size_t)kDistMaxK + 1);
+  const size_t most = (size_t)S::kRing + 24 * (kDistMaxK + 1);
   if (!configured[dev]) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     configured[dev] = true;
@@ -823,17 +826,22 @@ static void launch_distill_shape(DistillParams& p, cudaStream_t stream) {
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   const int64_t row = p.vocab * (int64_t)sizeof(T);
   auto slice = [&](int c) { return (row + c - 1) / c + 16; };
-  // as many blocks to a row as its slices need to fit into the rings; more of them where
-  // the rows leave SMs idle, down to 8 KB of logits a block
-  int csize = 1;
-  while (csize < kDistMaxCluster && slice(csize) > DistWide::kRing) csize *= 2;
+  // A row's slices have to fit into the rings.  Three blocks to an SM where that takes at
+  // most two slices (50257 columns of bf16: 187 us against 197 with one block to an SM,
+  // 4096 rows at τ = 2; 16384 x 32003: 546 against 1094), otherwise one (152064 columns,
+  // 8192 rows: 877 us with two slices against 1238 with eight smaller ones; a cluster of
+  // eight leaves SMs without a place for it).
+  int csize = slice(1) <= DistWide::kRing ? 1 : 2;
+  if (slice(2) > DistWide::kRing) {
+    csize = 1;
+    while (csize < kDistMaxCluster && slice(csize) > DistWidest::kRing) csize *= 2;
+  }
   TORCH_CHECK(slice(csize) <= DistWidest::kRing, "distill: a row of logits may have up to ",
               kDistMaxCluster * (DistWidest::kRing - 16), " bytes, got ", row);
+  // more slices where the rows leave SMs idle, down to 8 KB of logits a block
   while (csize < kDistMaxCluster && p.M * csize * 2 <= sms && slice(2 * csize) >= 8192) csize *= 2;
-  // rings that hold a slice twice where they can: the next row loads beside this one
   const int64_t mine = slice(csize);
   if (2 * mine <= DistSmall::kRing) launch_distill_mode<T, DistSmall>(p, csize, stream);
-  else if (2 * mine <= DistMiddle::kRing) launch_distill_mode<T, DistMiddle>(p, csize, stream);
   else if (mine <= DistWide::kRing) launch_distill_mode<T, DistWide>(p, csize, stream);
   else launch_distill_mode<T, DistWidest>(p, csize, stream);
 }
