@@ -34,13 +34,15 @@ import torch.nn as nn
 import torch.utils.checkpoint as ckpt
 
 from ..ops.activations import gelu, swiglu
-from ..ops.attention import flash_attention
+from ..ops.attention import flash_attention, flash_attention_varlen
 from ..ops.cross_entropy import cross_entropy, lm_head_cross_entropy
+from ..ops.distill import distillation_loss
 from ..ops.gemm import LMHeadFunction
 from ..ops.norm import add_rmsnorm
+from ..ops.packed import PackedSequences
 from ..ops.qlinear import Linear4bit
 from ..ops.qkv import qkv_fusable, qkv_projection
-from ..ops.rope import RopeSpec, apply_rope, rope_table
+from ..ops.rope import RopeScaling, RopeSpec, apply_rope, rope_table, rotary_embedding
 from ..utils.metrics import nvtx_range
 
 
@@ -56,6 +58,7 @@ class DecoderConfig:
     ffn_act: str = "swiglu"  # "swiglu" | "gelu"
     qkv_bias: bool = False   # Qwen2-family models carry Q/K/V biases
     rope_theta: float = 10000.0
+    rope_scaling: Optional[RopeScaling] = None   # for contexts longer than trained on
     norm_eps: float = 1e-6
     tie_embeddings: bool = True
     vocab_pad_multiple: int = 128
@@ -183,16 +186,32 @@ class DecoderLayer(nn.Module):
         out += [("up_proj", self.up_proj), ("down_proj", self.down_proj)]
         return out
 
-    def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor]):
+    def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor],
+                seqs: Optional[PackedSequences] = None):
         """``h`` is the residual stream, ``delta`` the previous block's output that
-        still has to be added (fused into this layer's first norm)."""
+        still has to be added (fused into this layer's first norm).  ``seqs``: the
+        sequences that the batch's one row is packed from."""
         cfg = self.cfg
         B, S, d = h.shape
         if delta is None:
             x = self.attn_norm(h)
         else:
             h, x = self.attn_norm(h, delta)
-        if self._fused_rope(x):
+        if seqs is not None:
+            # every sequence has its own positions and sees itself alone
+            q = self.q_proj(x).view(S, cfg.n_heads, cfg.head_dim)
+            k = self.k_proj(x).view(S, cfg.n_kv_heads, cfg.head_dim)
+            v = self.v_proj(x).view(S, cfg.n_kv_heads, cfg.head_dim)
+            q, k = rotary_embedding(q, k, seqs.positions, theta=cfg.rope_theta, scaling=cfg.rope_scaling)
+            o = flash_attention_varlen(q, k, v, seqs, causal=True)
+        elif cfg.rope_scaling is not None:
+            q = self.q_proj(x).view(B, S, cfg.n_heads, cfg.head_dim)
+            k = self.k_proj(x).view(B, S, cfg.n_kv_heads, cfg.head_dim)
+            v = self.v_proj(x).view(B, S, cfg.n_kv_heads, cfg.head_dim)
+            q, k = rotary_embedding(q, k, torch.arange(S, device=x.device), theta=cfg.rope_theta,
+                                    scaling=cfg.rope_scaling)
+            o = flash_attention(q, k, v, causal=True)
+        elif self._fused_rope(x):
             # the q/k projection GEMMs apply the rotary embedding in their epilogue;
             # the attention backward could also rotate dQ/dK back (flash_attention
             # rope=spec) but measured slower than the RoPE kernel it replaces
@@ -217,7 +236,7 @@ class DecoderLayer(nn.Module):
             v = self.v_proj(x).view(B, S, cfg.n_kv_heads, cfg.head_dim)
             q, k = apply_rope(q, k, cfg.rope_theta)
             o = flash_attention(q, k, v, causal=True)
-        a = self.o_proj(o.view(B, S, cfg.n_heads * cfg.head_dim))
+        a = self.o_proj(o.reshape(B, S, cfg.n_heads * cfg.head_dim))
         h, x = self.mlp_norm(h, a)
         if self.gate_proj is not None:
             if self._fused_mlp(with_gate=True):
@@ -340,16 +359,37 @@ class DecoderLM(nn.Module):
         return self
 
     # -- forward -----------------------------------------------------------------
-    def _layer_call(self, layer, h, delta):
+    def _layer_call(self, layer, h, delta, seqs=None):
+        more = () if seqs is None else (seqs,)
         if self.cfg.activation_checkpointing and self.training and torch.is_grad_enabled():
             if delta is None:
-                return ckpt.checkpoint(lambda hh: layer(hh, None), h, use_reentrant=False)
-            return ckpt.checkpoint(layer, h, delta, use_reentrant=False)
-        return layer(h, delta)
+                return ckpt.checkpoint(lambda hh: layer(hh, None, *more), h, use_reentrant=False)
+            return ckpt.checkpoint(layer, h, delta, *more, use_reentrant=False)
+        return layer(h, delta, *more)
 
     def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None,
-                ignore_index: int = -100):
+                ignore_index: int = -100, cu_seqlens=None, teacher=None, temperature: float = 1.0,
+                alpha: float = 0.5):
+        """Logits, or with ``targets`` the mean loss over the rows whose target counts.
+
+        ``cu_seqlens`` (``[n + 1]``, or a :class:`~zeroq_b200.ops.packed.PackedSequences`):
+        the batch is one row ``[1, T]`` of sequences behind one another; each has its own
+        positions and sees itself alone, rows behind the last one are padding (give them
+        ``ignore_index`` as target).  ``teacher``: ``(ids, logits)``, each ``[B, S, K]`` or
+        ``[B * S, K]``, a teacher's top entries for every row; the loss is then
+        :func:`~zeroq_b200.ops.distill.distillation_loss` with ``temperature`` and ``alpha``."""
         B, S = input_ids.shape
+        seqs = None
+        if cu_seqlens is not None:
+            if B != 1:
+                raise ValueError(f"packed sequences are one row [1, T], got a batch of {B}")
+            seqs = cu_seqlens
+            if not isinstance(seqs, PackedSequences):
+                seqs = PackedSequences(seqs, S, device=input_ids.device)
+            if seqs.total != S:
+                raise ValueError(f"the sequences divide {seqs.total} rows, the batch has {S}")
+        if teacher is not None and targets is None:
+            raise ValueError("a teacher's entries need targets")
         h = self.embed_tokens(input_ids)
         delta = None
         cb = getattr(self, "_layer_grad_cb", None)
@@ -359,18 +399,22 @@ class DecoderLM(nn.Module):
                 # that layer's backward (its parameter gradients included) is queued
                 h.register_hook(lambda g, i=i: cb(i))
             with nvtx_range(f"layer{i}"):
-                h, delta = self._layer_call(layer, h, delta)
+                h, delta = self._layer_call(layer, h, delta, seqs)
         x = self.norm(h) if delta is None else self.norm(h, delta)[1]
         W = self.head_weight()
         if W.numel() == 0:
             raise RuntimeError("the LM head weight is sharded and not gathered here; keep "
                                "'embed_tokens' and 'lm_head' in exclude_modules")
-        if targets is not None and self.cfg.ce_chunk > 0:
+        if targets is not None and teacher is None and self.cfg.ce_chunk > 0:
             return lm_head_cross_entropy(x, W, targets.reshape(-1), vocab=self.cfg.vocab_size,
                                          ignore_index=ignore_index, chunk=self.cfg.ce_chunk)
         logits = LMHeadFunction.apply(x, W)
         if targets is None:
             return logits.view(B, S, -1)[..., : self.cfg.vocab_size]
+        if teacher is not None:
+            ids, top = (t.reshape(-1, t.shape[-1]) for t in teacher)
+            return distillation_loss(logits, ids, top, targets.reshape(-1), temperature=temperature, alpha=alpha,
+                                     vocab=self.cfg.vocab_size, ignore_index=ignore_index)
         return cross_entropy(logits, targets.reshape(-1), vocab=self.cfg.vocab_size,
                              ignore_index=ignore_index)
 

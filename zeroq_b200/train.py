@@ -58,8 +58,8 @@ class Trainer:
         self.opt.use_device_clock()
         self._graph_on = True
 
-    def _eager(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
-        loss = self.model(input_ids, targets)
+    def _eager(self, input_ids: torch.Tensor, targets: torch.Tensor, **batch) -> torch.Tensor:
+        loss = self.model(input_ids, targets, **batch)
         if hasattr(self.opt, "arm_overlap"):   # one backward per step: sync buckets may start
             self.opt.arm_overlap()
         loss.backward()
@@ -101,20 +101,25 @@ class Trainer:
             self._tg = torch.empty(shape, dtype=torch.int64, device=self.device)
         return self._in, self._tg
 
-    def step_device(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def step_device(self, input_ids: torch.Tensor, targets: torch.Tensor, **batch) -> torch.Tensor:
+        """``batch``: further arguments of the model for this batch (``cu_seqlens``,
+        ``teacher``, ... of :class:`~zeroq_b200.models.DecoderLM`), on the device; not with
+        CUDA-graph steps, whose inputs are fixed."""
+        if batch and self._graph_on:
+            raise ValueError(f"CUDA-graph steps take input_ids and targets alone, got {sorted(batch)}")
         if self.logger is None:
-            return self._step_device(input_ids, targets)
+            return self._step_device(input_ids, targets, **batch)
         self.logger.begin()
-        loss = self._step_device(input_ids, targets)
+        loss = self._step_device(input_ids, targets, **batch)
         self.logger.end(loss, input_ids.numel())
         return loss
 
-    def _step_device(self, input_ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def _step_device(self, input_ids: torch.Tensor, targets: torch.Tensor, **batch) -> torch.Tensor:
         from .utils.metrics import nvtx_range
 
         if not self._graph_on:
             with nvtx_range("train_step"):
-                return self._eager(input_ids, targets)
+                return self._eager(input_ids, targets, **batch)
         if self._graph is None:
             return self._capture(input_ids, targets)
         if input_ids.data_ptr() != self._gin.data_ptr():
