@@ -98,10 +98,10 @@ __device__ __forceinline__ void vl_load_tile(uint8_t* dst, const CUtensorMap* ma
   for (int a = 0; a < DP / 64; ++a) tma_load_3d(dst + a * ROWS * 128, map, bar, a * 64, head, row);
 }
 
-// zeros to rows [from, ROWS) of such a tile, by 128 threads; then visible to the MMAs
+// zeros to rows [from, ROWS) of such a tile, by 256 threads; then visible to the MMAs
 template <int DP, int ROWS>
 __device__ __forceinline__ void vl_zero_rows(uint8_t* tile, int from, int thread) {
-  for (int i = thread; i < (DP / 64) * ROWS; i += 128) {
+  for (int i = thread; i < (DP / 64) * ROWS; i += 256) {
     const int row = i % ROWS;
     if (row >= from) {
       uint4* r = reinterpret_cast<uint4*>(tile + (i / ROWS) * ROWS * 128 + row * 128);
@@ -155,41 +155,59 @@ __device__ __forceinline__ float vl_with_low(float rounded, uint32_t bytes) {
   return rounded == 0.0f ? 0.0f : __int_as_float(__float_as_int(rounded) + d);   // (below 0's pattern lies NaN)
 }
 
-// N accumulator columns of this lane times f, rounded, to out; columns from D on do not exist
+// A warp's 32 accumulator rows (one a lane) of N columns times f, rounded, to rows `out`
+// (ld elements apart; the first `live` exist, and columns below D).  They go through
+// `stage` (64 N bytes of the warp's own), so that a store covers whole lines of a few
+// rows instead of 16 bytes of 32 rows each.  `low` (optional): the low bytes, likewise.
 template <bool FP16, int N>
-__device__ __forceinline__ void vl_store_row(uint32_t taddr, float f, uint16_t* out, int col0, int D, bool store,
-                                             uint8_t* low = nullptr) {
-#pragma unroll 1
+__device__ __forceinline__ void vl_store_rows(uint32_t taddr, float f, uint8_t* stage, uint16_t* out, int64_t ld, int col0, int D,
+                                              int live, uint8_t* low = nullptr) {
+  const int lane = threadIdx.x & 31;
+  constexpr int per = N / 8;                       // 16-byte chunks of a row, and lanes to a row
+  // a row's chunks, their places turned by the row against bank conflicts
+  auto at = [&](int r, int c) { return stage + r * (N * 2) + ((c ^ (r & (per - 1))) << 4); };
+  uint32_t lb[N / 4];
+#pragma unroll
   for (int c = 0; c < N; c += 32) {
     uint32_t o[32];
     tmem_ld_32x32b_x32(taddr + (uint32_t)c, o);
     tmem_ld_wait();
 #pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint4 v;
-      v.x = vl_pack<FP16>(__uint_as_float(o[8 * i + 0]) * f, __uint_as_float(o[8 * i + 1]) * f);
-      v.y = vl_pack<FP16>(__uint_as_float(o[8 * i + 2]) * f, __uint_as_float(o[8 * i + 3]) * f);
-      v.z = vl_pack<FP16>(__uint_as_float(o[8 * i + 4]) * f, __uint_as_float(o[8 * i + 5]) * f);
-      v.w = vl_pack<FP16>(__uint_as_float(o[8 * i + 6]) * f, __uint_as_float(o[8 * i + 7]) * f);
-      if (store && col0 + c + 8 * i < D) *reinterpret_cast<uint4*>(out + col0 + c + 8 * i) = v;
+      v.x = vl_pack<FP16>(__uint_as_float(o[8 * i + 0]), __uint_as_float(o[8 * i + 1]));
+      v.y = vl_pack<FP16>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+      v.z = vl_pack<FP16>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+      v.w = vl_pack<FP16>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+      *reinterpret_cast<uint4*>(at(lane, c / 8 + i)) = v;
     }
-    if (low != nullptr) {
-      uint32_t b[8];
+    if (low != nullptr)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        b[i] = vl_low_bytes<FP16>(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f,
-                                  __uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
-      uint8_t* to = low + col0 + c;
-      if ((D & 31) == 0) {   // whole 32-byte sectors
-        if (store && col0 + c < D) {
-          reinterpret_cast<uint4*>(to)[0] = make_uint4(b[0], b[1], b[2], b[3]);
-          reinterpret_cast<uint4*>(to)[1] = make_uint4(b[4], b[5], b[6], b[7]);
-        }
-      } else {
+        lb[c / 4 + i] = vl_low_bytes<FP16>(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                           __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+  }
+  __syncwarp();
+  const int chunk = lane % per;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (store && col0 + c + 8 * i < D) reinterpret_cast<uint2*>(to)[i] = make_uint2(b[2 * i], b[2 * i + 1]);
-      }
+  for (int r0 = 0; r0 < 32; r0 += 32 / per) {
+    const int r = r0 + lane / per;
+    const uint4 v = *reinterpret_cast<const uint4*>(at(r, chunk));
+    if (r < live && col0 + 8 * chunk < D) *reinterpret_cast<uint4*>(out + r * ld + col0 + 8 * chunk) = v;
+  }
+  if (low != nullptr) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i)
+      *reinterpret_cast<uint2*>(at(lane, i)) = make_uint2(lb[2 * i], lb[2 * i + 1]);
+    __syncwarp();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 32 / per) {
+      const int r = r0 + lane / per;
+      const uint2 v = *reinterpret_cast<const uint2*>(at(r, chunk));
+      if (r < live && col0 + 8 * chunk < D) *reinterpret_cast<uint2*>(low + r * ld + col0 + 8 * chunk) = v;
     }
   }
 }
@@ -329,17 +347,20 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
 // Forward: two query tiles (256 rows of one sequence and head) per CTA.
 //
 // Tensor memory: S_A 0-127, S_B 128-255, O_A 256.., O_B 384..; P (16-bit pairs)
-// is written over the first 64 columns of its tile's S.  Q_A and Q_B stay in
-// shared memory, K and V tiles of 128 keys stream through two-stage rings read by
-// both query tiles.  320 threads: warps 0-3 / 4-7 are the softmax warpgroup of
-// tile A / B (thread = query row = TMEM lane), warp 8 issues the MMAs in the order
+// is written over S's own columns.  Q_A and Q_B stay in shared memory, K and V tiles
+// of 128 keys stream through two-stage rings read by both query tiles.  576 threads:
+// warps 0-7 / 8-15 are the softmax warps of tile A / B, two threads to a query row (=
+// TMEM lane) with 64 keys each, which exchange their maxima through shared memory;
+// warp 16 issues the MMAs in the order
 //     PV_A(j), S_A(j+1) | PV_B(j), S_B(j+1) | ...
-// so one tile's exponentials run beside the other's products; warp 9 loads.
+// so one tile's exponentials run beside the other's products; warp 17 loads.
+// (The loop of a tile - scores, softmax, P V, next scores - is serial, so the time from
+// scores to P counts in full: that is why a row has two threads.)
 // The running maximum moves only when a row's maximum grows by more than 2^8 (O is
 // rescaled then); O / l and lse use the same one, so the result is exact.
 // When the sequence ends inside tile A, tile B does not exist and is skipped.
 // ============================================================================
-constexpr int kVfThreads = 320;
+constexpr int kVfThreads = 576;   // 16 softmax warps, MMA warp, loader warp
 constexpr int kVfStages = 2;
 constexpr float kVlRescale = 8.0f;
 
@@ -347,7 +368,8 @@ template <int DP>
 struct VfSmem {
   static constexpr int kTile = 128 * DP * 2;
   static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kVfStages * kTile;
-  static constexpr int kBar = kV + kVfStages * kTile;
+  static constexpr int kX = kV + kVfStages * kTile;     // [2 tiles][2 parities][2 halves][128 rows] fp32
+  static constexpr int kBar = kX + 2 * 2 * 2 * 128 * 4;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
 
@@ -373,12 +395,12 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entry = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+  const VlTile w = p.tiles[entry];   // (read beside the count; past it the plan's other words)
   const int count = p.meta[p.count_at];
   if (entry >= count) {
     if (entry == count) vl_zero_outside(O, p.T, p.Hq, h, p.D, p.meta);
     return;
   }
-  const VlTile w = p.tiles[entry];
   const int hk = h / (p.Hq / p.Hk);
   const int row_a = w.tile * 256, row_b = row_a + 128;
   const int nkt = (w.len + 127) / 128;
@@ -396,7 +418,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(drain, 1);
@@ -405,7 +427,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -414,7 +436,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 9) {
+  if (warp == 17) {
     // ------------------------------------------------------------ TMA loader (one thread)
     if (lane == 0) {
       mbar_arrive_expect_tx(q_full, (n_b > 0 ? 2 : 1) * L::kTile);
@@ -442,7 +464,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           mbar_wait(&v_full[j % kVfStages], (j / kVfStages) & 1, nullptr, 0);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------ MMA issuer (whole warp)
     constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 128, false);
     constexpr uint32_t idesc_pv = vl_idesc<FP16>(128, DP, true);
@@ -469,7 +491,8 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (elect_one_sync()) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_f16_ts(tmem + 256u + (uint32_t)(x * 128), tmem + (uint32_t)(x * 128 + kk * 8), vd + (uint64_t)(kk * 128),
+          umma_f16_ts(tmem + 256u + (uint32_t)(x * 128), tmem + (uint32_t)(x * 128 + (kk >> 2) * 64 + (kk & 3) * 8),
+                      vd + (uint64_t)(kk * 128),
                       idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&pv_done[x]);
         if (last) umma_commit(&v_empty[j % kVfStages]);
@@ -511,49 +534,56 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     mbar_wait(drain, 0, nullptr, 0);
   } else {
     // ------------------------------------------------------------ softmax + epilogue
-    const int x = warp >> 2;                        // 0: tile A, 1: tile B
+    const int x = warp >> 3;                        // 0: tile A, 1: tile B
+    const int half = (warp >> 2) & 1;               // keys (and O columns) of this thread's half row
     const int quad = warp & 3;                      // TMEM lane quadrant
     const int row = quad * 32 + lane;               // row in the tile = TMEM lane
+    const int pair_bar = 1 + x * 4 + quad;          // the two warps of these rows
     const int q = (x == 0 ? row_a : row_b) + row;   // row in the sequence
     const int n_kv = x == 0 ? n_a : n_b;
-    const int limit = p.causal ? min(q + 1, w.len) : w.len;   // keys that the row sees
-    const uint32_t t_s = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(x * 128);
-    const uint32_t t_o = t_s + 256u;
+    const int limit = (p.causal ? min(q + 1, w.len) : w.len) - 64 * half;   // keys that the row sees, from this half's first
+    const uint32_t t_s = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(x * 128 + half * 64);
+    const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + 256u + (uint32_t)(x * 128 + half * (DP / 2));
+    float* xs = reinterpret_cast<float*>(smem + L::kX) + x * 512;
     float m_used = -INFINITY;
-    float l = 0.0f;
-    bool ok = n_kv > 0;
+    float l = 0.0f;                                 // this half's share of the row sum
+    bool ok = true;
+    // a wait that ran out makes the later ones return at once: the two warps of a row meet
+    // at their barrier in every step all the same
+    auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && vl_wait(bar, parity, p.status, kErrVlCompute); };
     for (int j = 0; j < n_kv; ++j) {
-      if (!vl_wait(&s_full[x], j & 1, p.status, kErrVlCompute)) { ok = false; break; }
+      wait(&s_full[x], j & 1);
       tc_fence_after();
-      uint32_t r[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        tmem_ld_32x32b_x32(t_s + (uint32_t)(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+      uint32_t r[64];
+      tmem_ld64(t_s, r);
       tmem_ld_wait();
       const int seen = limit - j * 128;
-      if (__any_sync(0xffffffffu, seen < 128)) {
+      if (__any_sync(0xffffffffu, seen < 64)) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
+        for (int c = 0; c < 64; ++c)
           if (c >= seen) r[c] = __float_as_uint(-INFINITY);
       }
-      // row max: 8 independent chains of 3-input maxima over columns 8..119, then the rest
+      // row max: 8 independent chains of 3-input maxima over columns 8..55, then the rest
       float pm[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) pm[i] = __uint_as_float(r[i]);
 #pragma unroll
-      for (int c = 8; c < 120; c += 16)
+      for (int c = 8; c < 56; c += 16)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           pm[i] = fmax3(pm[i], __uint_as_float(r[c + i]), __uint_as_float(r[c + 8 + i]));
-      const float mx = fmax3(fmax3(pm[0], pm[1], __uint_as_float(r[120])),
-                             fmax3(pm[2], pm[3], __uint_as_float(r[121])),
-                             fmax3(fmax3(pm[4], pm[5], __uint_as_float(r[122])),
-                                   fmax3(pm[6], pm[7], __uint_as_float(r[123])),
-                                   fmax3(__uint_as_float(r[124]), __uint_as_float(r[125]),
-                                         fmaxf(__uint_as_float(r[126]), __uint_as_float(r[127]))))) *
-                       p.scale_log2;
+      const float mine = fmax3(fmax3(pm[0], pm[1], __uint_as_float(r[56])),
+                               fmax3(pm[2], pm[3], __uint_as_float(r[57])),
+                               fmax3(fmax3(pm[4], pm[5], __uint_as_float(r[58])),
+                                     fmax3(pm[6], pm[7], __uint_as_float(r[59])),
+                                     fmax3(__uint_as_float(r[60]), __uint_as_float(r[61]),
+                                           fmaxf(__uint_as_float(r[62]), __uint_as_float(r[63])))));
+      float* xm = xs + (j & 1) * 256 + row;
+      xm[half * 128] = mine;
+      named_barrier(pair_bar, 64);
+      const float mx = fmaxf(mine, xm[(half ^ 1) * 128]) * p.scale_log2;
       const bool need = mx > m_used + kVlRescale;
-      const bool rescale = __any_sync(0xffffffffu, need);
+      const bool rescale = __any_sync(0xffffffffu, need);   // (the same in both warps of the rows)
       float factor = 1.0f;
       if (rescale) {
         const float m_new = need ? mx : m_used;
@@ -562,9 +592,8 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       }
       const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-m_used, -m_used);
       uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
-      uint32_t pk[64];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {  // masked keys hold -inf: 2^x gives 0 (the polynomial 2^-120)
+      for (int i = 0; i < 32; ++i) {  // masked keys hold -inf: 2^x gives 0 (the polynomial 2^-120)
         float a0, a1;
         f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, nm2), a0, a1);
         float p0, p1;
@@ -575,20 +604,19 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           p1 = fast_exp2(a1);
         }
         ps2[i & 3] = f2_add(ps2[i & 3], f2_pack(p0, p1));
-        pk[i] = vl_pack<FP16>(p0, p1);
+        r[i] = vl_pack<FP16>(p0, p1);
       }
-      tmem_st_32x32b_x32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
-      tmem_st_32x32b_x32(t_s + 32u, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+      tmem_st_32x32b_x32(t_s, *reinterpret_cast<const uint32_t(*)[32]>(&r[0]));   // over this half's own scores
       float ps[4];
       f2_unpack(f2_add(ps2[0], ps2[1]), ps[0], ps[1]);
       f2_unpack(f2_add(ps2[2], ps2[3]), ps[2], ps[3]);
       l = l * factor + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
       if (rescale && j > 0) {
-        // O holds PV_0..PV_{j-1}: wait for PV_{j-1}, then scale this thread's row
-        if (!vl_wait(&pv_done[x], (j - 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
+        // O holds PV_0..PV_{j-1}: wait for PV_{j-1}, then scale this thread's half row
+        wait(&pv_done[x], (j - 1) & 1);
         tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
+        for (int c = 0; c < DP / 64; ++c) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(t_o + (uint32_t)(c * 32), o);
           tmem_ld_wait();
@@ -600,29 +628,36 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       // the sequence ends inside this key tile: zero V's other rows, by the first
       // query tile that uses it (PV_B(j) is issued after PV_A(j))
       if (w.len - j * 128 < 128 && (x == 0 || j >= n_a)) {
-        if (!vl_wait(&v_full[j % kVfStages], (j / kVfStages) & 1, p.status, kErrVlCompute)) { ok = false; break; }
-        vl_zero_rows<DP, 128>(smem + L::kV + (j % kVfStages) * L::kTile, w.len - j * 128, threadIdx.x & 127);
+        wait(&v_full[j % kVfStages], (j / kVfStages) & 1);
+        vl_zero_rows<DP, 128>(smem + L::kV + (j % kVfStages) * L::kTile, w.len - j * 128, threadIdx.x & 255);
       }
       tmem_st_wait();
       tc_fence_before();          // TMEM loads/stores of this step ordered before the arrive
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[x]);
     }
-    if (ok) {
+    if (n_kv > 0) {
       const int jl = n_kv - 1;
-      if (vl_wait(&pv_done[x], jl & 1, p.status, kErrVlCompute)) {
+      float* xl = xs + (n_kv & 1) * 256 + row;      // (the other parity than the last step's)
+      xl[half * 128] = l;
+      named_barrier(pair_bar, 64);
+      l += xl[(half ^ 1) * 128];
+      wait(&pv_done[x], jl & 1);
+      if (ok) {
         tc_fence_after();
-        const bool store = q < w.len;
-        const int64_t at = (int64_t)(w.start + q) * p.Hq + h;
-        vl_store_row<FP16, DP>(t_o, 1.0f / l, O + at * p.D, 0, p.D, store, low != nullptr ? low + at * p.D : nullptr);
-        if (store) lse[(int64_t)h * p.T + w.start + q] = (m_used + __log2f(l)) * 0.69314718055994531f;
+        // (this tile's Q has given all its scores: its memory stages the output)
+        const int64_t at = ((int64_t)(w.start + q - lane) * p.Hq + h) * p.D;
+        vl_store_rows<FP16, DP / 2>(t_o, 1.0f / l, smem + L::kQ + x * L::kTile + (warp & 7) * (L::kTile / 8), O + at,
+                                    (int64_t)p.Hq * p.D, half * (DP / 2), p.D, w.len - (q - lane),
+                                    low != nullptr ? low + at : nullptr);
+        if (q < w.len && half == 0) lse[(int64_t)h * p.T + w.start + q] = (m_used + __log2f(l)) * 0.69314718055994531f;
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -633,24 +668,24 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 //
 // Q and dO are copied into tensor memory once, so that S = Q Kᵀ and dP = dO Vᵀ
 // (N = 64) read only K and V from shared memory.  S and dP are double-buffered:
-// two warpgroups take alternate key tiles (thread = query row, all 64 columns of
-// it: no exchange between warps), the MMA warp issues the scores of tile t + 1
+// two groups of eight warps take alternate key tiles (two threads to a query row, 32
+// columns each: no exchange between warps), the MMA warp issues the scores of tile t + 1
 // before it waits for dS of tile t.  dS (16-bit pairs, over S's own columns) times
 // K (read MN-major) adds into dQ; dQ is written once: no atomics.
 // Tensor memory: S 64 b, dP 128 + 64 b (b = t & 1), dQ 256.., Q 384.., dO 448...
-// The kernel also forms delta = rowsum(dO ∘ O) and lse·log2(e) of its rows and
+// The kernel also forms delta = rowsum(dO ∘ O) and -lse·log2(e) of its rows and
 // stores them by slots of 128 rows for the dK/dV kernel, which runs after it.
 // ============================================================================
 constexpr int kVlMaxSplit = 4;      // CTAs that share a key tile at most (dK/dV)
-constexpr int kVbThreads = 352;     // two compute warpgroups, MMA warp, two loader warps
+constexpr int kVbThreads = 608;     // two groups of eight compute warps, MMA warp, two loader warps
 
 template <int DP>
 struct VqSmem {
   static constexpr int kKStages = 5, kVStages = 3;
   static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2;
   static constexpr int kQ = 0, kDO = kTile, kK = 2 * kTile, kV = kK + kKStages * kHalf;
-  static constexpr int kX = kV + kVStages * kHalf;       // [2][128] fp32
-  static constexpr int kBar = kX + 1024;
+  static constexpr int kX = kV + kVStages * kHalf;       // [128] fp32
+  static constexpr int kBar = kX + 512;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
 
@@ -659,7 +694,7 @@ __global__ void __launch_bounds__(kVbThreads, 1)
 attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                       const __grid_constant__ VlParams p, const uint16_t* __restrict__ O,
-                      const uint8_t* __restrict__ low, const float* __restrict__ lse, float* __restrict__ delta, float* __restrict__ lse2,
+                      const uint8_t* __restrict__ low, const float* __restrict__ lse, float* __restrict__ delta, float* __restrict__ nlse2,
                       uint16_t* __restrict__ dQ) {
   using L = VqSmem<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -672,18 +707,18 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   uint64_t* v_full = k_empty + L::kKStages;    // [kVStages]
   uint64_t* v_empty = v_full + L::kVStages;
   uint64_t* s_full = v_empty + L::kVStages;    // [2]
-  uint64_t* ds_full = s_full + 2;              // [2], four arrivals
+  uint64_t* ds_full = s_full + 2;              // [2], eight arrivals
   uint64_t* dq_done = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entry = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+  const VlTile w = p.tiles[entry];   // (read beside the count; past it the plan's other words)
   const int count = p.meta[p.count_at];
   if (entry >= count) {
     if (entry == count) vl_zero_outside(dQ, p.T, p.Hq, h, p.D, p.meta);
     return;
   }
-  const VlTile w = p.tiles[entry];
   const int hk = h / (p.Hq / p.Hk);
   const int row0 = w.tile * 128;
   const int keys = p.causal ? min(row0 + 128, w.len) : w.len;
@@ -691,24 +726,24 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(in_tmem, 8);
+    mbar_init(in_tmem, 16);
     for (int i = 0; i < L::kKStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < L::kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&ds_full[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&ds_full[i], 8); }
     mbar_init(dq_done, 1);
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmDO);
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 16) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 9) {
+  if (warp >= 17) {
     // ------------------------------------------------------------ TMA loaders (K with Q and dO; V)
     if (lane == 0) {
-      const bool is_k = warp == 9;
+      const bool is_k = warp == 17;
       if (is_k) {
         mbar_arrive_expect_tx(q_full, 2 * L::kTile);
         vl_load_tile<DP, 128>(smem + L::kQ, &tmQ, q_full, h, w.start + row0);
@@ -733,7 +768,7 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         for (int t = max(issued - nst, 0); t < issued; ++t) mbar_wait(&full[t % nst], (t / nst) & 1, nullptr, 0);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------ MMA issuer (whole warp)
     constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 64, false);
     constexpr uint32_t idesc_q = vl_idesc<FP16>(128, DP, true);
@@ -768,7 +803,7 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       if (elect_one_sync()) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_f16_ts(tmem + 256u, tmem + (uint32_t)(64 * b + kk * 8), kd + (uint64_t)(kk * 128), idesc_q,
+          umma_f16_ts(tmem + 256u, tmem + (uint32_t)(64 * b + (kk >> 1) * 32 + (kk & 1) * 8), kd + (uint64_t)(kk * 128), idesc_q,
                       (t > 0 || kk > 0) ? 1u : 0u);
         umma_commit(&k_empty[ks]);
       }
@@ -779,81 +814,83 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     mbar_wait(dq_done, 0, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
   } else {
     // ------------------------------------------------------------ dS + epilogue
-    const int quad = warp & 3, g = warp >> 2;
+    const int quad = warp & 3, half = (warp >> 2) & 1, g = warp >> 3;
     const int row = quad * 32 + lane, q = row0 + row;
     const bool live = q < w.len;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const int limit = live ? (p.causal ? q + 1 : w.len) : 0;     // keys that the row sees
-    const float l2 = live ? lse[(int64_t)h * p.T + w.start + q] * 1.4426950408889634f : 0.0f;
-    // delta: this warpgroup's half of the columns, O from global (before the wait), dO from the tile
-    constexpr int CH = DP / 16;                                  // 8-column chunks of the half
-    uint4 ov[CH];
-    uint2 lv[CH];
-    {
-      const int64_t at = ((int64_t)(w.start + q) * p.Hq + h) * p.D;
-      const uint16_t* orow = O + at;
+    // keys that the row sees, from this half's first
+    const int limit = (live ? (p.causal ? q + 1 : w.len) : 0) - 32 * half;
+    const float lse_row = live ? lse[(int64_t)h * p.T + w.start + q] : 0.0f;
+    // delta of eight rows a warp: DP / 8 lanes to a row (whole lines), O from global before
+    // the wait, dO from the tile
+    constexpr int LR = DP / 8, RI = 32 / LR, NI = 8 / RI;        // lanes to a row, rows at once, steps
+    uint4 ov[NI];
+    uint2 lv[NI];
+    const int dchunk = lane % LR, drow0 = warp * 8 + lane / LR;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int col = g * (DP / 2) + c * 8;
-        ov[c] = live && col < p.D ? *reinterpret_cast<const uint4*>(orow + col) : make_uint4(0, 0, 0, 0);
-        lv[c] = live && col < p.D ? *reinterpret_cast<const uint2*>(low + at + col) : make_uint2(0, 0);
-      }
+    for (int i = 0; i < NI; ++i) {
+      const int r = drow0 + i * RI;
+      const bool in = row0 + r < w.len && dchunk * 8 < p.D;
+      const int64_t at = ((int64_t)(w.start + row0 + r) * p.Hq + h) * p.D + dchunk * 8;
+      ov[i] = in ? *reinterpret_cast<const uint4*>(O + at) : make_uint4(0, 0, 0, 0);
+      lv[i] = in ? *reinterpret_cast<const uint2*>(low + at) : make_uint2(0, 0);
     }
     bool ok = vl_wait(q_full, 0, p.status, kErrVlCompute);
-    if (ok) {  // warpgroup 0 copies Q, warpgroup 1 dO: the first scores can start
-      const uint8_t* src = smem + (g == 0 ? L::kQ : L::kDO) + row * 128;
-#pragma unroll
-      for (int a = 0; a < DP / 64; ++a)
-        copy_row_to_tmem(src + a * 16384, row, lane_base + 384u + (uint32_t)(64 * g + 32 * a));
+    if (ok) {  // group 0 copies Q, group 1 dO, an atom each half: the first scores can start
+      if (half < DP / 64)
+        copy_row_to_tmem(smem + (g == 0 ? L::kQ : L::kDO) + half * 16384 + row * 128, row,
+                         lane_base + 384u + (uint32_t)(64 * g + 32 * half));
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(in_tmem);
     }
-    float dl = 0.0f;
-    {
+    float* xs = reinterpret_cast<float*>(smem + L::kX);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = drow0 + i * RI;
+      const uint4 du = *reinterpret_cast<const uint4*>(smem + L::kDO + (dchunk >> 3) * 16384 + r * 128 +
+                                                       (((dchunk & 7) ^ (r & 7)) << 4));
+      const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[i].x, ov[i].y, ov[i].z, ov[i].w};
       float acc = 0.0f;
-      const int a0 = DP == 128 ? g : 0;                          // atom of the half's columns
-      const uint8_t* drow = smem + L::kDO + a0 * 16384 + row * 128;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int chunk = (DP == 128 ? 0 : g * CH) + c;
-        const uint4 du = *reinterpret_cast<const uint4*>(drow + ((chunk ^ (row & 7)) << 4));
-        const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[c].x, ov[c].y, ov[c].z, ov[c].w};
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t lw = j == 0 ? lv[i].x : lv[i].y;
+        const float2 a0 = vl_unpack<FP16>(dw[2 * j]), b0 = vl_unpack<FP16>(ow[2 * j]);
+        const float2 a1 = vl_unpack<FP16>(dw[2 * j + 1]), b1 = vl_unpack<FP16>(ow[2 * j + 1]);
+        acc = fmaf(a0.x, vl_with_low<FP16, 0>(b0.x, lw), acc);
+        acc = fmaf(a0.y, vl_with_low<FP16, 1>(b0.y, lw), acc);
+        acc = fmaf(a1.x, vl_with_low<FP16, 2>(b1.x, lw), acc);
+        acc = fmaf(a1.y, vl_with_low<FP16, 3>(b1.y, lw), acc);
+      }
+      // (a row past the sequence's end: whatever its dO holds, O is 0 there, and NaN stays in the row)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t lw = j == 0 ? lv[c].x : lv[c].y;
-          const float2 a0 = vl_unpack<FP16>(dw[2 * j]), b0 = vl_unpack<FP16>(ow[2 * j]);
-          const float2 a1 = vl_unpack<FP16>(dw[2 * j + 1]), b1 = vl_unpack<FP16>(ow[2 * j + 1]);
-          acc = fmaf(a0.x, vl_with_low<FP16, 0>(b0.x, lw), acc);
-          acc = fmaf(a0.y, vl_with_low<FP16, 1>(b0.y, lw), acc);
-          acc = fmaf(a1.x, vl_with_low<FP16, 2>(b1.x, lw), acc);
-          acc = fmaf(a1.y, vl_with_low<FP16, 3>(b1.y, lw), acc);
-        }
-      }
-      float* xs = reinterpret_cast<float*>(smem + L::kX);
-      xs[g * 128 + row] = acc;
-      named_barrier(1, 256);
-      dl = live ? xs[row] + xs[128 + row] : 0.0f;
-      if (g == 0) {
-        const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
-        delta[at] = dl;
-        lse2[at] = l2;
-      }
+      for (int o = LR / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      if (dchunk == 0) xs[r] = acc;
     }
+    named_barrier(1, 512);
+    const float l2 = lse_row * 1.4426950408889634f;
+    const float dl = live ? xs[row] : 0.0f;
+    if (g == 0 && half == 0) {
+      const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
+      delta[at] = dl;
+      nlse2[at] = -l2;
+    }
+    const int part = 2 * g + half;
     const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(-l2, -l2), dl2 = f2_pack(dl, dl);
+    const uint32_t t_s = lane_base + (uint32_t)(64 * g + 32 * half);
     for (int t = g; t < n_kv && ok; t += 2) {
       if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
       tc_fence_after();
-      uint32_t s[64], dp[64];
-      tmem_ld64(lane_base + (uint32_t)(64 * g), s);
-      tmem_ld64(lane_base + 128u + (uint32_t)(64 * g), dp);
+      uint32_t s[32], dp[32];
+      tmem_ld_32x32b_x32(t_s, s);
+      tmem_ld_32x32b_x32(t_s + 128u, dp);
       tmem_ld_wait();
       const int seen = limit - t * 64;
-      const bool cut = __any_sync(0xffffffffu, seen < 64);
-      uint32_t pk[32];
+      const bool cut = __any_sync(0xffffffffu, seen < 32);
+      uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < 16; ++i) {
         const int c = 2 * i;
         float a0, a1, g0, g1;
         f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
@@ -865,9 +902,9 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         pk[i] = vl_pack<FP16>(g0, g1);
       }
-      tmem_st_32x32b_x32(lane_base + (uint32_t)(64 * g), pk);
+      tmem_st_32x32b_x16(t_s, pk);   // over this half's own scores
       if (w.len - t * 64 < 64)   // the sequence ends inside this key tile (K_t has given its scores)
-        vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, w.len - t * 64, threadIdx.x & 127);
+        vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, w.len - t * 64, threadIdx.x & 255);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -875,14 +912,16 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     }
     if (ok && vl_wait(dq_done, 0, p.status, kErrVlCompute)) {
       tc_fence_after();
-      uint16_t* out = dQ + ((int64_t)(w.start + q) * p.Hq + h) * p.D;
-      vl_store_row<FP16, DP / 2>(lane_base + 256u + (uint32_t)(g * (DP / 2)), p.scale, out, g * (DP / 2), p.D, live);
+      uint16_t* out = dQ + ((int64_t)(w.start + q - lane) * p.Hq + h) * p.D;
+      if (part < DP / 32)   // 32 columns a warp, through the memory of Q
+        vl_store_rows<FP16, 32>(lane_base + 256u + (uint32_t)(part * 32), p.scale, smem + L::kQ + (part * 4 + quad) * 2048, out,
+                                (int64_t)p.Hq * p.D, part * 32, p.D, w.len - (q - lane));
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 // ============================================================================
@@ -891,11 +930,12 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 //
 //   Sᵀ_t = K Q_tᵀ, dPᵀ_t = V dO_tᵀ       M = 128 keys, N = 64 queries
 //   dV += Pᵀ_t dO_t, dK += dSᵀ_t Q_t      A = Pᵀ / dSᵀ from tensor memory, B MN-major
-// Two warpgroups take alternate query tiles (thread = key row, its 64 columns);
+// Two groups of eight warps take alternate query tiles (two threads to a key row, 32
+// queries each);
 // the scores of tile t + 1 are issued before the wait for Pᵀ/dSᵀ of tile t.
 // Tensor memory: dV 0.., dK 128.., Sᵀ 256 + 128 b, dPᵀ 320 + 128 b (b = t & 1),
-// Pᵀ and dSᵀ over the first 32 columns of theirs.  Q and dO come through rings of
-// four tiles with the tile's lse·log2(e) and delta.
+// Pᵀ and dSᵀ over the scores that they were formed from.  Q and dO come through rings of
+// four tiles with the tile's -lse·log2(e) and delta.
 //
 // Where there are few key tiles a cluster of S CTAs shares one: CTA r takes every
 // S-th of its query tiles, and at the end each writes its dV and dK (32 bits) into
@@ -907,7 +947,7 @@ struct VkSmem {
   static constexpr int kStages = 4;
   static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2;
   static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kDO = kQ + kStages * kHalf;
-  static constexpr int kLD = kDO + kStages * kHalf;      // per stage: lse2[64], delta[64]
+  static constexpr int kLD = kDO + kStages * kHalf;      // per stage: -lse·log2(e) [64], delta [64]
   static constexpr int kBar = kLD + kStages * 512;
   static constexpr int kBytes = kBar + 256 + 1024;
 };
@@ -916,7 +956,7 @@ template <bool FP16, int DP>
 __global__ void __launch_bounds__(kVbThreads, 1)
 attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
-                       const __grid_constant__ VlParams p, const float* __restrict__ lse2,
+                       const __grid_constant__ VlParams p, const float* __restrict__ nlse2,
                        const float* __restrict__ delta, uint16_t* __restrict__ dK, uint16_t* __restrict__ dV) {
   using L = VkSmem<DP>;
   static_assert(2 * L::kStages * L::kHalf >= 2 * 128 * DP * 4, "the rings hold dV and dK in 32 bits");
@@ -926,16 +966,17 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   uint64_t* kv_full = bars;                          // K and V landed
   uint64_t* q_full = bars + 1;                       // [kStages]
   uint64_t* q_empty = q_full + L::kStages;
-  uint64_t* o_full = q_empty + L::kStages;           // dO with lse2 and delta
+  uint64_t* o_full = q_empty + L::kStages;           // dO with the rows' statistics
   uint64_t* o_empty = o_full + L::kStages;
   uint64_t* s_full = o_empty + L::kStages;           // [2]
-  uint64_t* p_full = s_full + 2;                     // [2], four arrivals
+  uint64_t* p_full = s_full + 2;                     // [2], eight arrivals
   uint64_t* acc_done = p_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = p.split, rank = (int)(blockIdx.x % (unsigned)S);
   const int entry = blockIdx.x / (unsigned)S / p.Hk, hk = blockIdx.x / (unsigned)S % p.Hk;
+  const VlTile w = p.tiles[entry];   // (read beside the count; past it the plan's other words)
   const int count = p.meta[p.count_at];
   if (entry >= count) {   // (all of a cluster)
     if (entry == count && rank == 0) {
@@ -944,7 +985,6 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     }
     return;
   }
-  const VlTile w = p.tiles[entry];
   const int group = p.Hq / p.Hk, key0 = w.tile * 128;
   const int i0 = p.causal ? 2 * w.tile : 0;          // first 64-query tile that sees this key tile
   const int per_head = (w.len + 63) / 64 - i0;
@@ -957,21 +997,21 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
       mbar_init(&o_full[i], 1); mbar_init(&o_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 8); }
     mbar_init(acc_done, 1);
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmDO);
   }
-  if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 16) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 9) {
+  if (warp >= 17) {
     // ------------------------------------------------------------ TMA loaders (Q with K and V; dO)
     if (lane == 0) {
-      const bool is_q = warp == 9;
+      const bool is_q = warp == 17;
       if (is_q) {
         mbar_arrive_expect_tx(kv_full, 2 * L::kTile);
         vl_load_tile<DP, 128>(smem + L::kK, &tmK, kv_full, hk, w.start + key0);
@@ -989,9 +1029,9 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (!mbar_wait(&empty[st], ((t / L::kStages) & 1) ^ 1, p.status, kErrVlLoad)) { ok = false; break; }
         mbar_arrive_expect_tx(&full[st], L::kHalf + (is_q ? 0 : 512));
         vl_load_tile<DP, 64>(ring + st * L::kHalf, map, &full[st], h, w.start + it * 64);
-        if (!is_q) {  // this query tile's lse2 and delta (256 B each)
+        if (!is_q) {  // this query tile's -lse·log2(e) and delta (256 B each)
           const int64_t at = ((int64_t)h * p.slots + slot0) * 128 + it * 64;
-          bulk_load(smem + L::kLD + st * 512, lse2 + at, 256, &full[st]);
+          bulk_load(smem + L::kLD + st * 512, nlse2 + at, 256, &full[st]);
           bulk_load(smem + L::kLD + st * 512 + 256, delta + at, 256, &full[st]);
         }
         issued = t + 1;
@@ -1004,7 +1044,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           mbar_wait(&full[t % L::kStages], (t / L::kStages) & 1, nullptr, 0);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------ MMA issuer (whole warp)
     constexpr uint32_t idesc_s = vl_idesc<FP16>(128, 64, false);
     constexpr uint32_t idesc_g = vl_idesc<FP16>(128, DP, true);
@@ -1042,8 +1082,8 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (elect_one_sync()) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {   // dV += Pᵀ dO and dK += dSᵀ Q
-          umma_f16_ts(tmem, sc + (uint32_t)(kk * 8), od + (uint64_t)(kk * 128), idesc_g, (t > 0 || kk > 0) ? 1u : 0u);
-          umma_f16_ts(tmem + 128u, sc + 64u + (uint32_t)(kk * 8), qd + (uint64_t)(kk * 128), idesc_g,
+          umma_f16_ts(tmem, sc + (uint32_t)((kk >> 1) * 32 + (kk & 1) * 8), od + (uint64_t)(kk * 128), idesc_g, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_f16_ts(tmem + 128u, sc + 64u + (uint32_t)((kk >> 1) * 32 + (kk & 1) * 8), qd + (uint64_t)(kk * 128), idesc_g,
                       (t > 0 || kk > 0) ? 1u : 0u);
         }
         umma_commit(&q_empty[st]);
@@ -1056,53 +1096,65 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     mbar_wait(acc_done, 0, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
   } else {
     // ------------------------------------------------------------ Pᵀ, dSᵀ + epilogue
-    const int quad = warp & 3, g = warp >> 2;
+    const int quad = warp & 3, half = (warp >> 2) & 1, g = warp >> 3;
     const int row = quad * 32 + lane, key = key0 + row;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t sc = lane_base + 256u + 128u * (uint32_t)g;
+    const uint32_t sc = lane_base + 256u + 128u * (uint32_t)g + 32u * (uint32_t)half;
     bool ok = true;
     int it = i0 + (rank + S * g) % per_head;
     for (int t = g; t < n_it; t += 2) {
       const int st = t % L::kStages;
-      const float* sl = reinterpret_cast<const float*>(smem + L::kLD + st * 512);
-      // (o_full has completed by then; waiting on it makes lse2 and delta visible here)
+      const float* sl = reinterpret_cast<const float*>(smem + L::kLD + st * 512) + 32 * half;
+      // (o_full has completed by then; waiting on it makes the row statistics visible here)
       if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute) ||
           !vl_wait(&o_full[st], (t / L::kStages) & 1, p.status, kErrVlCompute)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      uint32_t s[64], dp[64];
-      tmem_ld64(sc, s);
-      tmem_ld64(sc + 64u, dp);
+      uint32_t s[32], dp[32];
+      tmem_ld_32x32b_x32(sc, s);
+      tmem_ld_32x32b_x32(sc + 64u, dp);
       tmem_ld_wait();
-      // queries [from, to) of the tile see this key
-      const int to = w.len - it * 64;
-      const int from = p.causal ? key - it * 64 : 0;
-      const bool cut = to < 64 || __any_sync(0xffffffffu, from > 0);
+      // queries [from, to) of the tile see this key (this half's first is 0)
+      const int to = w.len - it * 64 - 32 * half;
+      const int from = p.causal ? key - it * 64 - 32 * half : 0;
+      const bool cut = to < 32 || __any_sync(0xffffffffu, from > 0);
+      uint32_t pp[16], dsp[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {   // 4 queries per step: shared-memory broadcasts
+      for (int i = 0; i < 8; ++i) {   // 4 queries per step: shared-memory broadcasts
         const float4 l4 = reinterpret_cast<const float4*>(sl)[i];
         const float4 d4 = reinterpret_cast<const float4*>(sl + 64)[i];
-        const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dv4[4] = {d4.x, d4.y, d4.z, d4.w};
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
         float pr[4], ds[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int c = 4 * i + u;
-          pr[u] = fast_exp2(fmaf(__uint_as_float(s[c]), p.scale_log2, -lv[u]));
-          ds[u] = pr[u] * (__uint_as_float(dp[c]) - dv4[u]);
-          if (cut && (c < from || c >= to)) pr[u] = ds[u] = 0.0f;
+        for (int u = 0; u < 2; ++u) {
+          const int c = 4 * i + 2 * u;
+          const uint64_t lv = u == 0 ? f2_pack(l4.x, l4.y) : f2_pack(l4.z, l4.w);
+          const uint64_t dv2 = u == 0 ? f2_pack(d4.x, d4.y) : f2_pack(d4.z, d4.w);
+          float a0, a1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, lv), a0, a1);
+          pr[2 * u] = fast_exp2(a0);
+          pr[2 * u + 1] = fast_exp2(a1);
+          f2_unpack(f2_mul(f2_pack(pr[2 * u], pr[2 * u + 1]),
+                           f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dv2)),
+                    ds[2 * u], ds[2 * u + 1]);
         }
-        s[2 * i] = vl_pack<FP16>(pr[0], pr[1]);
-        s[2 * i + 1] = vl_pack<FP16>(pr[2], pr[3]);
-        dp[2 * i] = vl_pack<FP16>(ds[0], ds[1]);
-        dp[2 * i + 1] = vl_pack<FP16>(ds[2], ds[3]);
+        if (cut) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (4 * i + u < from || 4 * i + u >= to) pr[u] = ds[u] = 0.0f;
+        }
+        pp[2 * i] = vl_pack<FP16>(pr[0], pr[1]);
+        pp[2 * i + 1] = vl_pack<FP16>(pr[2], pr[3]);
+        dsp[2 * i] = vl_pack<FP16>(ds[0], ds[1]);
+        dsp[2 * i + 1] = vl_pack<FP16>(ds[2], ds[3]);
       }
-      tmem_st_32x32b_x32(sc, *reinterpret_cast<const uint32_t(*)[32]>(&s[0]));
-      tmem_st_32x32b_x32(sc + 64u, *reinterpret_cast<const uint32_t(*)[32]>(&dp[0]));
-      if (to < 64) {   // the sequence ends inside this query tile (it has given its scores)
-        vl_zero_rows<DP, 64>(smem + L::kQ + st * L::kHalf, to, threadIdx.x & 127);
-        vl_zero_rows<DP, 64>(smem + L::kDO + st * L::kHalf, to, threadIdx.x & 127);
+      tmem_st_32x32b_x16(sc, pp);
+      tmem_st_32x32b_x16(sc + 64u, dsp);
+      if (w.len - it * 64 < 64) {   // the sequence ends inside this query tile (it has given its scores)
+        vl_zero_rows<DP, 64>(smem + L::kQ + st * L::kHalf, w.len - it * 64, threadIdx.x & 255);
+        vl_zero_rows<DP, 64>(smem + L::kDO + st * L::kHalf, w.len - it * 64, threadIdx.x & 255);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -1113,15 +1165,19 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     }
     ok = ok && vl_wait(acc_done, 0, p.status, kErrVlCompute);
     tc_fence_after();
-    // warpgroup 0 has dV, warpgroup 1 dK
-    const uint32_t acc = lane_base + (uint32_t)(128 * g);
+    // group 0 has dV, group 1 dK; half of the columns a warp
+    const int col0 = half * (DP / 2);
+    const uint32_t acc = lane_base + (uint32_t)(128 * g + col0);
     if (S == 1) {
-      const int64_t at = ((int64_t)(w.start + key) * p.Hk + hk) * p.D;
-      if (ok) vl_store_row<FP16, DP>(acc, g == 0 ? 1.0f : p.scale, (g == 0 ? dV : dK) + at, 0, p.D, key < w.len);
+      // (K and V have given all their products: their memory stages the output)
+      const int64_t at = ((int64_t)(w.start + key - lane) * p.Hk + hk) * p.D;
+      if (ok)
+        vl_store_rows<FP16, DP / 2>(acc, g == 0 ? 1.0f : p.scale, smem + L::kK + warp * (L::kTile / 8), (g == 0 ? dV : dK) + at,
+                                    (int64_t)p.Hk * p.D, col0, p.D, w.len - (key - lane));
     } else {   // [column][row]: the lanes of a warp write one line
-      float* mine = reinterpret_cast<float*>(smem + L::kQ) + g * DP * 128 + row;
+      float* mine = reinterpret_cast<float*>(smem + L::kQ) + g * DP * 128 + col0 * 128 + row;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = 0; c < DP / 2; c += 32) {
         uint32_t o[32];
         if (n_it > 0) {
           tmem_ld_32x32b_x32(acc + (uint32_t)c, o);
@@ -1136,14 +1192,14 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   if (S > 1) {
     __syncwarp();
     cluster_sync_all();   // every CTA's dV and dK are in its shared memory
-    if (warp < 8) {
-      const int g = warp >> 2, row = (warp & 3) * 32 + lane, key = key0 + row;
+    if (warp < 16) {
+      const int g = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, key = key0 + row;
       const float f = g == 0 ? 1.0f : p.scale;
       const uint32_t mine = smem_u32(smem + L::kQ) + (uint32_t)((g * DP * 128 + row) * 4);
       uint16_t* out = (g == 0 ? dV : dK) + ((int64_t)(w.start + key) * p.Hk + hk) * p.D;
-      const int cols = DP / S;
+      const int cols = DP / S / 2;   // of each half
 #pragma unroll 1
-      for (int c = rank * cols; c < (rank + 1) * cols; c += 8) {
+      for (int c = (2 * rank + half) * cols; c < (2 * rank + half + 1) * cols; c += 8) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
@@ -1167,7 +1223,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 }  // namespace zq
@@ -1314,7 +1370,7 @@ struct VlBwd {
   const uint16_t* o;
   const uint8_t* low;
   const float* lse;
-  float *delta, *lse2;
+  float *delta, *nlse2;
   uint16_t *dq, *dk, *dv;
 };
 
@@ -1331,7 +1387,7 @@ static void vl_launch_bwd(VlCall& c, const VlBwd& b, int dev) {
   c.p.tiles = tiles + c.c256;
   kq<<<(unsigned)((c.c128 + 1) * c.p.Hq), kVbThreads, VqSmem<DP>::kBytes, stream>>>(b.q128, b.k64, b.v64, b.do128, c.p, b.o, b.low,
                                                                                    b.lse,
-                                                                                   b.delta, b.lse2, b.dq);
+                                                                                   b.delta, b.nlse2, b.dq);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   c.p.count_at = 2;
   c.p.tiles = tiles + c.c256 + c.c128;
@@ -1353,7 +1409,7 @@ static void vl_launch_bwd(VlCall& c, const VlBwd& b, int dev) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kk, b.q64, b.k128, b.v128, b.do64, c.p, (const float*)b.lse2, (const float*)b.delta,
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kk, b.q64, b.k128, b.v128, b.do64, c.p, (const float*)b.nlse2, (const float*)b.delta,
                                     b.dk, b.dv));
 }
 
