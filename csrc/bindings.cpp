@@ -78,6 +78,7 @@ std::vector<at::Tensor> rotary_embedding(at::Tensor q, c10::optional<at::Tensor>
                                          bool interleaved, double factor);
 std::vector<at::Tensor> packed_sequences(at::Tensor cu, int64_t T);
 at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, bool causal, double scale);
+at::Tensor attn_varlen_cu(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, bool causal, double scale);
 at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, c10::optional<at::Tensor> targets, int64_t vocab,
                         int64_t ignore_index, double temperature, double alpha, bool mean, bool fused);
 // p2p.cu
@@ -171,6 +172,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // the differentiable forms: kernels of the backward are launched from C++
   m.def("rotary_embedding", &rotary_embedding);
   m.def("attn_varlen", &attn_varlen);
+  m.def("attn_varlen_cu", &attn_varlen_cu);
   m.def("distill_loss", &distill_loss);
   m.def("gelu_fwd", &gelu_fwd);
   m.def("gelu_bwd", &gelu_bwd);

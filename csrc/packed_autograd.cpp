@@ -232,6 +232,12 @@ at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan
   return o;
 }
 
+// with the sequences as cu_seqlens (int32, on q's device): the plan is built for this call
+at::Tensor attn_varlen_cu(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, bool causal, double scale) {
+  const at::Tensor plan = packed_sequences(cu, q.size(0))[0];
+  return attn_varlen(q, k, v, plan, cu.numel() - 1, causal, scale);
+}
+
 // The mean (`fused`: with its gradient in the same pass, where one is wanted) or the rows
 at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, OptTensor targets, int64_t vocab,
                         int64_t ignore_index, double temperature, double alpha, bool mean, bool fused) {

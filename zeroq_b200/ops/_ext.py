@@ -40,7 +40,7 @@ def available() -> bool:
 
 # kernels launched per call of each binding (bindings not listed launch one; of the
 # differentiable ones the forward's are counted, their backward runs without a binding)
-_KERNELS_PER_CALL = {"attn_bwd_tc": 3, "packed_plan_words": 0, "gemm_status": 0, "set_gemm_pair_mode": 0,
+_KERNELS_PER_CALL = {"attn_bwd_tc": 3, "packed_plan_words": 0, "attn_varlen_cu": 2, "distill_loss": 2, "gemm_status": 0, "set_gemm_pair_mode": 0,
                      "peer_alloc": 0, "peer_handle": 0, "peer_open": 0, "peer_close": 0,
                      "peer_free": 0, "tensor_from_ptr": 0, "peer_status_read": 0,
                      "peer_flag_words": 0}

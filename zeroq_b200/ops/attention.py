@@ -175,15 +175,23 @@ def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"flash_attention_varlen: scale must be positive, got {scale}")
+    cu = None
     if not isinstance(seqs, PackedSequences):
-        seqs = PackedSequences(seqs, T, device=q.device)
-    if seqs.total != T or seqs.device != q.device:
+        if q.is_cuda and seqs.dtype == torch.int32 and seqs.device == q.device and seqs.dim() == 1 and seqs.numel() and \
+                seqs.is_contiguous():
+            cu = seqs          # its plan is built by the same call
+        else:
+            seqs = PackedSequences(seqs, T, device=q.device)
+    if cu is None and (seqs.total != T or seqs.device != q.device):
         raise ValueError(f"flash_attention_varlen: the sequences divide {seqs.total} rows on {seqs.device}, "
                          f"q has {T} on {q.device}")
     if not q.is_cuda or T == 0:
+        seqs = seqs if cu is None else PackedSequences(cu, T)
         return attention_varlen_reference(q, k, v, seqs, causal, scale)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"flash_attention_varlen: bf16 or fp16 on the GPU, got {q.dtype}")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"flash_attention_varlen: head width a multiple of 8 up to 128 on the GPU, got {D}")
+    if cu is not None:
+        return _ext.ext().attn_varlen_cu(q, k, v, cu, bool(causal), scale)
     return _ext.ext().attn_varlen(q, k, v, seqs.plan, seqs.n, bool(causal), scale)
