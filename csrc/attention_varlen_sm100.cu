@@ -28,6 +28,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "attention_common.cuh"
 
 // defined in gemm_sm100.cu
@@ -889,19 +891,24 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       const int seen = limit - t * 64;
       const bool cut = __any_sync(0xffffffffu, seen < 32);
       uint32_t pk[16];
+      // (with and without the mask apart: a branch in every step would keep the steps apart)
+      auto form = [&](auto masked) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int c = 2 * i;
-        float a0, a1, g0, g1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
-        f2_unpack(f2_mul(f2_pack(fast_exp2(a0), fast_exp2(a1)),
-                         f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl2)), g0, g1);
-        if (cut) {
-          if (c >= seen) g0 = 0.0f;
-          if (c + 1 >= seen) g1 = 0.0f;
+        for (int i = 0; i < 16; ++i) {
+          const int c = 2 * i;
+          float a0, a1, g0, g1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
+          f2_unpack(f2_mul(f2_pack(fast_exp2(a0), fast_exp2(a1)),
+                           f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl2)), g0, g1);
+          if constexpr (decltype(masked)::value) {
+            g0 = c >= seen ? 0.0f : g0;
+            g1 = c + 1 >= seen ? 0.0f : g1;
+          }
+          pk[i] = vl_pack<FP16>(g0, g1);
         }
-        pk[i] = vl_pack<FP16>(g0, g1);
-      }
+      };
+      if (cut) form(std::true_type());
+      else form(std::false_type());
       tmem_st_32x32b_x16(t_s, pk);   // over this half's own scores
       if (w.len - t * 64 < 64)   // the sequence ends inside this key tile (K_t has given its scores)
         vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, w.len - t * 64, threadIdx.x & 255);
