@@ -1032,9 +1032,9 @@ using namespace zq;
 // host side
 // ----------------------------------------------------------------------------
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
-  // The encoder is a driver call and needs the calling thread's context, which only a
-  // runtime call makes current: an autograd thread whose first work is one of this
-  // extension's backwards has made none (the driver then ends in a segmentation fault).
+  // The encoder is a driver call and fails without a context of the calling thread, which
+  // only a runtime call makes current: an autograd thread whose first work is one of this
+  // extension's backwards has made none.
   static thread_local bool bound = false;
   if (!bound) {
     int dev;

@@ -33,6 +33,10 @@ setup(
             sources=SOURCES,
             extra_compile_args={"cxx": ["-O3", "-std=c++17"] + DEFINES, "nvcc": NVCC_FLAGS},
             libraries=["cublas"],
+            # the shared C++ runtime that torch uses, by its own name: a toolchain that only
+            # finds the static one would link a second copy, and an error thrown here would
+            # then end the process where it unwinds past a local object
+            extra_link_args=["-Wl,--no-as-needed", "-l:libstdc++.so.6", "-Wl,--as-needed"],
         )
     ],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
