@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
     t.tile = s - b[lo];
     t.slot = s;
     // a sequence whose tiles do not all fit is left out (its row statistics would not either)
-    if (b[lo + 1] > cap || t.tile * rows >= t.len) return false;
+    if (b[lo + 1] > cap || t.tile < 0 || t.tile * rows >= t.len) return false;
     const int row = t.tile * rows;
     const int work = kind == 2 ? t.len - row : min(row + rows, t.len);
     cls = kPlanClasses - 1 - min(kPlanClasses - 1, (work + 63) / 64 >> shift);   // longest first
@@ -1271,11 +1271,11 @@ void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions
 static CUtensorMap vl_tmap(const at::Tensor& t, int box_rows) {
   CUtensorMap map;
   const int64_t T = t.size(0), H = t.size(1), D = t.size(2);
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(2) == 1 && t.stride(1) % 8 == 0 &&
-                  t.stride(0) % 8 == 0 && t.stride(1) >= 0 && t.stride(0) >= 0,
-              "attention: 16-byte aligned rows with unit stride");
   // the stride of an axis of one is never taken; the map wants a real one all the same
   const int64_t sh = H > 1 ? t.stride(1) : D, st = T > 1 ? t.stride(0) : H * D;
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(2) == 1 && sh % 8 == 0 && st % 8 == 0 && sh > 0 &&
+                  st > 0,
+              "attention: 16-byte aligned rows with unit stride");
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
   cuuint64_t strides[2] = {(cuuint64_t)(sh * 2), (cuuint64_t)(st * 2)};
   cuuint32_t box[3] = {64u, 1u, (cuuint32_t)box_rows};

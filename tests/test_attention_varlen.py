@@ -240,6 +240,44 @@ def test_strides_shared_plan_and_partial_gradients(cuda):
 
 
 @pytest.mark.gpu
+def test_no_sequence_one_head_and_one_row(cuda):
+    q = torch.randn(70, 2, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    o = flash_attention_varlen(q, q, q, torch.zeros(1, dtype=torch.int32, device=cuda))
+    dq, = torch.autograd.grad(o, q, torch.ones_like(o))
+    assert (o == 0).all() and (dq == 0).all()
+    # axes of one with strides that no tensor map could take
+    base = torch.randn(40 * 64, device=cuda, dtype=torch.bfloat16)
+    odd = base.as_strided((40, 1, 64), (64, 3, 1))
+    cu = torch.tensor([0, 40], dtype=torch.int32, device=cuda)
+    assert torch.equal(flash_attention_varlen(odd, odd, odd, cu), flash_attention_varlen(*[base.view(40, 1, 64)] * 3, cu))
+    one = base.as_strided((1, 2, 64), (7, 64, 1))
+    cu1 = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    assert torch.equal(flash_attention_varlen(one, one, one, cu1), one)
+
+
+@pytest.mark.gpu
+def test_sequences_out_of_order_stay_in_bounds(cuda):
+    """The host cannot see such a division: it gives nothing useful, within the buffers."""
+    q = torch.randn(300, 2, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    for cu in ([0, 300, 0, 300, 0, 300, 0, 300], [-50, 7000, 2 ** 31 - 1], [200, 100, -2 ** 31, 150], [300, 0]):
+        o = flash_attention_varlen(q, q, q, torch.tensor(cu, device=cuda).to(torch.int32))
+        torch.autograd.grad(o, q, torch.ones_like(o))
+    torch.cuda.synchronize()
+    from zeroq_b200.ops import _ext
+    assert _ext.ext().gemm_status(0)[0] in (0, 324)   # 324: a division with more tiles than rows could give
+    assert _ext.ext().gemm_status(0)[0] == 0
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(cuda):
+    q, k, v, do, cu = inputs([10], 0, 2, 2, 64, torch.bfloat16, cuda)
+    leaf = q.detach().requires_grad_()
+    o = flash_attention_varlen(leaf, k, v, cu)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(o, leaf, do, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_kernel_refusals(cuda):
     q, k, v, do, cu = inputs([10], 0, 2, 2, 128, torch.bfloat16, cuda)
     with pytest.raises(TypeError):

@@ -89,6 +89,15 @@ def test_reference_matches_definition(T, a, reduction):
     check(*make(9, 50, 7, torch.float32), T, a, 50, reduction)
 
 
+def test_ignore_index_within_the_vocabulary():
+    z, ids, t, y = make(9, 50, 7, torch.float32)
+    y[:] = torch.arange(9) % 4
+    out = torch.where(y == 2, -100, y)
+    for r in ("mean", "none"):
+        assert torch.equal(distillation_loss(z, ids, t, y, alpha=0.5, ignore_index=2, reduction=r),
+                           distillation_loss(z, ids, t, out, alpha=0.5, reduction=r))
+
+
 def test_gradient_against_differences():
     z, ids, t, y = make(5, 11, 4, torch.float64)
     z.requires_grad_()
@@ -98,7 +107,7 @@ def test_gradient_against_differences():
 
 @pytest.mark.parametrize("bad", [
     dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(alpha=1.5), dict(alpha=-0.1),
-    dict(alpha=0.5, targets=None), dict(vocab=0), dict(vocab=51), dict(ignore_index=3), dict(reduction="sum"),
+    dict(alpha=0.5, targets=None), dict(vocab=0), dict(vocab=51), dict(reduction="sum"),
     dict(targets=torch.zeros(3, dtype=torch.int64)), dict(targets=torch.zeros(6)),
     dict(teacher_ids=torch.zeros(6, 4)), dict(teacher_ids=torch.zeros(5, 4, dtype=torch.int64)),
     dict(teacher_logits=torch.zeros(6, 3)), dict(logits=torch.zeros(6, 50, dtype=torch.int64)),
@@ -216,6 +225,23 @@ def test_kernel_strided_logits_second_backward_and_no_grad(cuda):
     with torch.no_grad():
         again = distillation_loss(leaf, ids, t, y, alpha=0.5, vocab=256)
     assert abs(again.item() - loss.item()) <= 2.0 ** -20 * abs(loss.item())
+
+
+@pytest.mark.gpu
+def test_kernel_refuses_rows_that_do_not_fit_and_second_derivatives(cuda):
+    z = torch.zeros(1, 500000, device=cuda)
+    ids, t = torch.zeros(1, 2, dtype=torch.int64, device=cuda), torch.zeros(1, 2, device=cuda)
+    with pytest.raises(RuntimeError, match="bytes"):
+        distillation_loss(z, ids, t)
+    z, ids, t, y = make(4, 50, 3, torch.float32, cuda)
+    for r in ("mean", "none"):
+        leaf = z.detach().requires_grad_()
+        loss = distillation_loss(leaf, ids, t, y, alpha=0.5, reduction=r)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(loss.sum(), leaf, create_graph=True)
+    y[1] = 7
+    assert torch.equal(distillation_loss(z, ids, t, y, alpha=0.5, ignore_index=7),
+                       distillation_loss(z, ids, t, torch.where(y == 7, -100, y), alpha=0.5))
 
 
 @pytest.mark.gpu

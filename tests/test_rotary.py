@@ -147,6 +147,8 @@ def test_kernel_strides_shapes_and_partial_gradients(cuda):
     check(dq, gq, *args, sign=-1.0)
     only, none = rotary_embedding(q.detach(), None, *args)
     assert none is None and torch.equal(only, yq)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(yq, q, gq, create_graph=True)
     with pytest.raises(RuntimeError, match="rotary"):          # the entry's own checks
         from zeroq_b200.ops import _ext
         _ext.ext().rotary(q.detach()[0], None, pos[:5], torch.ones(32, dtype=torch.float64),

@@ -63,7 +63,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     ``reduction="mean"``: the mean over the counted rows (0 if there are none), whose
     backward may run once; ``"none"``: the rows' losses, fp32 ``[M]``.  Differentiable in
-    ``logits``."""
+    ``logits``.  bf16, fp16 or fp32 on the GPU, a row of up to 1.5 MB."""
     if logits.dim() != 2 or teacher_ids.dim() != 2 or teacher_ids.shape[0] != logits.shape[0]:
         raise ValueError(f"distillation_loss: logits [M, V] and teacher_ids [M, K], got {tuple(logits.shape)} "
                          f"and {tuple(teacher_ids.shape)}")
@@ -80,8 +80,6 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         raise ValueError("distillation_loss: alpha below 1 needs targets")
     if targets is not None and targets.shape != (M,):
         raise ValueError(f"distillation_loss: targets must be [{M}], got {tuple(targets.shape)}")
-    if 0 <= ignore_index < vocab:
-        raise ValueError("distillation_loss: ignore_index must be outside the vocabulary")
     if reduction not in ("mean", "none"):
         raise ValueError(f"distillation_loss: reduction is 'mean' or 'none', got {reduction!r}")
     if teacher_ids.dtype not in (torch.int32, torch.int64):
@@ -94,6 +92,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
         raise ValueError("distillation_loss: all tensors on one device")
     if K > MAX_TEACHER_ENTRIES:
         raise ValueError(f"distillation_loss: at most {MAX_TEACHER_ENTRIES} teacher entries a row, got {K}")
+    if targets is not None and 0 <= ignore_index < vocab:   # an id of the vocabulary marks the rows that count nothing
+        targets = targets.masked_fill(targets == ignore_index, -1)
+        ignore_index = -1
     if not logits.is_cuda or logits.dtype == torch.float64 or M == 0:
         return distillation_reference(logits, teacher_ids, teacher_logits.detach(), targets, temperature, alpha,
                                       vocab, ignore_index, reduction)

@@ -24,7 +24,8 @@ class PackedSequences:
     ``cu_seqlens``: int32 or int64 ``[n + 1]``.  On the CPU it is checked here (it starts
     at 0, does not fall and ends within ``total``) and copied to ``device``; on the GPU
     it is not read by the host - values out of order are clamped by the kernel, and the
-    result for such a division is undefined."""
+    result for such a division is undefined.  The tables are those of the values that it
+    had here: make another one for another division."""
 
     def __init__(self, cu_seqlens: torch.Tensor, total: int, device: Optional[torch.device] = None):
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
