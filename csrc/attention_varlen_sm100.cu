@@ -1244,8 +1244,8 @@ int64_t packed_plan_words(int64_t T, int64_t n) {
   return 4 * (vl_cap(T, n, 256) + 2 * vl_cap(T, n, 128)) + kVlMeta + 3 * (n + 1);
 }
 
-// plan: int32 [packed_plan_words(T, n)], 16-byte aligned; positions: int32 [T]
-void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions) {
+// plan: int32 [packed_plan_words(T, n)], 16-byte aligned; positions (optional): int32 [T]
+void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, c10::optional<at::Tensor> positions) {
   TORCH_CHECK(cu.is_cuda() && cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.dim() == 1 && cu.numel() >= 1,
               "packed_plan: cu_seqlens int32 [n + 1] on the GPU");
   const int64_t n = cu.numel() - 1;
@@ -1253,17 +1253,18 @@ void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions
   TORCH_CHECK(plan.is_cuda() && plan.get_device() == cu.get_device() && plan.scalar_type() == at::kInt && plan.is_contiguous() &&
                   plan.numel() == packed_plan_words(T, n) && (reinterpret_cast<uintptr_t>(plan.data_ptr()) & 15) == 0,
               "packed_plan: plan int32 [packed_plan_words]");
-  TORCH_CHECK(positions.is_cuda() && positions.get_device() == cu.get_device() && positions.scalar_type() == at::kInt &&
-                  positions.is_contiguous() && positions.numel() == T,
+  const bool rows = positions.has_value() && T > 0;
+  TORCH_CHECK(!rows || (positions->is_cuda() && positions->get_device() == cu.get_device() &&
+                        positions->scalar_type() == at::kInt && positions->is_contiguous() && positions->numel() == T),
               "packed_plan: positions int32 [T]");
   const c10::cuda::CUDAGuard guard(cu.device());
   const int64_t c256 = vl_cap(T, n, 256), c128 = vl_cap(T, n, 128);
   int* words = plan.data_ptr<int>();
   int* meta = words + 4 * (c256 + 2 * c128);
-  const unsigned grid = 3 + (unsigned)((T + kPlanThreads - 1) / kPlanThreads);
+  const unsigned grid = 3 + (rows ? (unsigned)((T + kPlanThreads - 1) / kPlanThreads) : 0u);
   packed_plan_kernel<<<grid, kPlanThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
       cu.data_ptr<int>(), (int)n, (int)T, (int)c256, (int)c128, reinterpret_cast<VlTile*>(words), meta + kVlMeta, meta,
-      T > 0 ? positions.data_ptr<int>() : nullptr, status_buffer(cu.get_device()));
+      rows ? positions->data_ptr<int>() : nullptr, status_buffer(cu.get_device()));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

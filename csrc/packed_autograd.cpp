@@ -12,7 +12,7 @@ void rotary(at::Tensor q, OptTensor k, at::Tensor positions, at::Tensor turns, a
             double factor, double sign);
 // attention_varlen_sm100.cu
 int64_t packed_plan_words(int64_t T, int64_t n);
-void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, at::Tensor positions);
+void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, OptTensor positions);
 void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, at::Tensor o, at::Tensor lse,
                      OptTensor low, bool causal, double scale);
 void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor lse, at::Tensor low,
@@ -234,7 +234,8 @@ at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan
 
 // with the sequences as cu_seqlens (int32, on q's device): the plan is built for this call
 at::Tensor attn_varlen_cu(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cu, bool causal, double scale) {
-  const at::Tensor plan = packed_sequences(cu, q.size(0))[0];
+  at::Tensor plan = at::empty({packed_plan_words(q.size(0), cu.numel() - 1)}, cu.options());
+  packed_plan(cu, q.size(0), plan, c10::nullopt);
   return attn_varlen(q, k, v, plan, cu.numel() - 1, causal, scale);
 }
 

@@ -24,6 +24,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cstring>
+
 #include "common.cuh"
 
 namespace zq {
@@ -253,7 +255,7 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
   p.rot = (int)R;
   p.factor = (float)factor;
   p.sin_factor = (float)(factor * sign);
-  for (int64_t i = 0; i < turns.numel(); ++i) p.turns[i] = turns.data_ptr<double>()[i];
+  std::memcpy(p.turns, turns.data_ptr<double>(), (size_t)(R / 2) * sizeof(double));
   const c10::cuda::CUDAGuard guard(q.device());
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   auto stream = at::cuda::getCurrentCUDAStream();

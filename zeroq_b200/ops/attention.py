@@ -164,32 +164,32 @@ def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     to ``1/sqrt(D)``.  Rows of no sequence get an output and gradients of zero, whatever
     they hold.  P and dS are rounded to the inputs' type before their products;
     scores, softmax statistics and accumulators are in 32 bits."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError(f"flash_attention_varlen: q [T, Hq, D], k and v [T, Hk, D], got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    T, Hq, D = q.shape
-    if k.shape[1] < 1 or Hq < 1 or Hq % k.shape[1]:
-        raise ValueError(f"flash_attention_varlen: {Hq} query heads do not share {k.shape[1]} kv heads evenly")
-    if not (k.dtype == v.dtype == q.dtype) or not (k.device == v.device == q.device):
+    qs, ks, dtype, device = tuple(q.shape), tuple(k.shape), q.dtype, q.device
+    if len(qs) != 3 or len(ks) != 3 or tuple(v.shape) != ks or ks[0] != qs[0] or ks[2] != qs[2]:
+        raise ValueError(f"flash_attention_varlen: q [T, Hq, D], k and v [T, Hk, D], got {qs}, {ks}, {tuple(v.shape)}")
+    T, Hq, D = qs
+    if ks[1] < 1 or Hq < 1 or Hq % ks[1]:
+        raise ValueError(f"flash_attention_varlen: {Hq} query heads do not share {ks[1]} kv heads evenly")
+    if not (k.dtype == v.dtype == dtype) or not (k.device == v.device == device):
         raise TypeError("flash_attention_varlen: q, k and v of one type on one device")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"flash_attention_varlen: scale must be positive, got {scale}")
     cu = None
     if not isinstance(seqs, PackedSequences):
-        if q.is_cuda and seqs.dtype == torch.int32 and seqs.device == q.device and seqs.dim() == 1 and seqs.numel() and \
-                seqs.is_contiguous():
+        if (device.type == "cuda" and seqs.dtype == torch.int32 and seqs.device == device and seqs.dim() == 1
+                and seqs.numel() and seqs.is_contiguous()):
             cu = seqs          # its plan is built by the same call
         else:
-            seqs = PackedSequences(seqs, T, device=q.device)
-    if cu is None and (seqs.total != T or seqs.device != q.device):
+            seqs = PackedSequences(seqs, T, device=device)
+    if cu is None and (seqs.total != T or seqs.device != device):
         raise ValueError(f"flash_attention_varlen: the sequences divide {seqs.total} rows on {seqs.device}, "
-                         f"q has {T} on {q.device}")
-    if not q.is_cuda or T == 0:
+                         f"q has {T} on {device}")
+    if device.type != "cuda" or T == 0:
         seqs = seqs if cu is None else PackedSequences(cu, T)
         return attention_varlen_reference(q, k, v, seqs, causal, scale)
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"flash_attention_varlen: bf16 or fp16 on the GPU, got {q.dtype}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"flash_attention_varlen: bf16 or fp16 on the GPU, got {dtype}")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"flash_attention_varlen: head width a multiple of 8 up to 128 on the GPU, got {D}")
     if cu is not None:

@@ -224,6 +224,9 @@ def rotary_reference(x: torch.Tensor, positions: torch.Tensor, theta: float = 10
     return torch.cat([y, xf[..., R:]], dim=-1).to(x.dtype)
 
 
+_ROTARY_TYPES = frozenset((torch.bfloat16, torch.float16, torch.float32, torch.float64))
+
+
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                      theta: float = 10000.0, rotary_dim: Optional[int] = None, interleaved: bool = False,
                      scaling: Optional[RopeScaling] = None):
@@ -236,31 +239,33 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     pairs are columns ``(i, i + rotary_dim/2)``, or ``(2i, 2i + 1)`` with ``interleaved``.
     The other columns pass through.  Angles are formed in 64 bits, so positions may be
     far; the products are in 32 bits with one rounding.  bf16, fp16 or fp32, any strides."""
-    if q.dim() < 3:
-        raise ValueError(f"rotary_embedding: q must be [..., S, H, D], got {tuple(q.shape)}")
-    D = q.shape[-1]
+    qs, dtype, device = tuple(q.shape), q.dtype, q.device
+    if len(qs) < 3:
+        raise ValueError(f"rotary_embedding: q must be [..., S, H, D], got {qs}")
+    D, rows = qs[-1], qs[:-2]
     R = D if rotary_dim is None else int(rotary_dim)
     if R < 2 or R % 2 or R > D or R > 256:
         raise ValueError(f"rotary_embedding: rotary_dim must be even, at most the head's {D} and at most 256, got {R}")
-    if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != D or k.dtype != q.dtype
-                          or k.device != q.device):
-        raise ValueError(f"rotary_embedding: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float64):
-        raise TypeError(f"rotary_embedding: bf16, fp16 or fp32 tensors, got {q.dtype}")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if k is not None:
+        ks = tuple(k.shape)
+        if ks[:-2] != rows or ks[-1] != D or k.dtype != dtype or k.device != device:
+            raise ValueError(f"rotary_embedding: k {ks} {k.dtype} does not go with q {qs} {dtype}")
+    if dtype not in _ROTARY_TYPES:
+        raise TypeError(f"rotary_embedding: bf16, fp16 or fp32 tensors, got {dtype}")
+    if positions.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"rotary_embedding: positions must be int32 or int64, got {positions.dtype}")
-    if positions.device != q.device:
+    if positions.device != device:
         raise ValueError("rotary_embedding: positions must be on q's device")
-    if positions.shape != q.shape[:-2] and positions.shape != q.shape[-3:-2]:
-        raise ValueError(f"rotary_embedding: positions {tuple(positions.shape)} must be {tuple(q.shape[:-2])} "
-                         f"or {tuple(q.shape[-3:-2])}")
+    ps = tuple(positions.shape)
+    if ps != rows and ps != rows[-1:]:
+        raise ValueError(f"rotary_embedding: positions {ps} must be {rows} or {rows[-1:]}")
     if not theta > 1.0:
         raise ValueError(f"rotary_embedding: theta must be above 1, got {theta}")
-    if not q.is_cuda or q.dtype == torch.float64:
+    if device.type != "cuda" or dtype == torch.float64:
         args = (positions, float(theta), R, interleaved, scaling)
         return rotary_reference(q, *args), None if k is None else rotary_reference(k, *args)
     turns, factor = _rope_turns(R, float(theta), scaling)
-    if positions.dim() != 1 or not positions.is_contiguous():
+    if len(ps) != 1 or not positions.is_contiguous():
         positions = positions.reshape(-1).contiguous()
     out = _ext.ext().rotary_embedding(q, k, positions, turns, bool(interleaved), factor)
     return (out[0], None) if k is None else (out[0], out[1])
