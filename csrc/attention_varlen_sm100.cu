@@ -27,8 +27,8 @@
 // shared memory (N = 128: 74 and 107, N = 64: 42 and 75) against N / 2 of arithmetic.
 //
 // Measured (bf16, D = 128, causal; the multiply rate counts the visible pairs):
-//   9 sequences, 8080 rows, 28/4 heads    forward 124 us, dQ 184, dK/dV 205
-//   7 sequences, 6004 rows, 24/24 heads   forward 73 us, dQ 100, dK/dV 122
+//   9 sequences, 8080 rows, 28/4 heads    forward 124 us, dQ 157, dK/dV 205
+//   7 sequences, 6004 rows, 24/24 heads   forward 73 us, dQ 87, dK/dV 122
 //   8191 + 1037 rows, 8/2 heads           forward 127 us (1.1 PFLOP/s), dQ 181, dK/dV 267
 // Short sequences are bound by what a block does around its loop (launch, first loads,
 // pipeline fill, output: 7-8 us of a block's 15-20 us, with one block to an SM, which
@@ -679,8 +679,17 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 }
 
 // ============================================================================
-// dQ: one CTA per (128-query tile, head), key tiles of 64.
+// dQ: an item is a 128-query tile of a head, its steps are key tiles of 64.
 //
+// A CTA does one item after another: when the loader comes to the last key tiles of one it
+// asks the hardware for a block of the grid that has not started, and takes that block's
+// item over (no counter in memory, and the longest-first order of the grid still evens
+// out; asked for at the item's start, the items of 8191 + 1037 rows took 201 us, not
+// 192).  So Q, dO and the first K and V of the next item are on their way during the
+// last steps of this one, its O comes to L2, its first scores are formed while dQ of
+// this one leaves, and tensor memory and barriers are set up once.  One item to a CTA,
+// which paid for all this between any two: 184 us against 157 (8080 rows, 28/4 heads),
+// 100 against 87 (6004 rows, 24/24 heads), 181 both at 8191 + 1037 rows.
 // Q and dO are copied into tensor memory once, so that S = Q Kᵀ and dP = dO Vᵀ
 // (N = 64) read only K and V from shared memory.  S and dP are double-buffered:
 // two groups of eight warps take alternate key tiles (two threads to a query row, 32
@@ -695,14 +704,62 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 constexpr int kVlMaxSplit = 4;      // CTAs that share a key tile at most (dK/dV)
 constexpr int kVbThreads = 608;     // two groups of eight compute warps, MMA warp, two loader warps
 
+// Asks for a block of this grid that has not started: it then never starts, and its
+// index comes to `answer` (16 bytes; -1 in vl_answered_block: none was left, and no
+// further request may be made).
+__device__ __forceinline__ void vl_request_block(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int vl_answered_block(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+      "ld.shared.b128 a, [%1];\n\t"
+      "mov.u32 %0, -1;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
+// threadIdx.x, read where it is written
+__device__ __forceinline__ int vl_tid() {
+  int t;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ void vl_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// loads that stay where they are written
+__device__ __forceinline__ float vl_ld_f32(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 vl_ld_u2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 vl_ld_u4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 template <int DP>
 struct VqSmem {
   static constexpr int kKStages = 5, kVStages = 3;
   static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2;
   static constexpr int kQ = 0, kDO = kTile, kK = 2 * kTile, kV = kK + kKStages * kHalf;
-  static constexpr int kX = kV + kVStages * kHalf;       // [128] fp32
-  static constexpr int kBar = kX + 512;
-  static constexpr int kBytes = kBar + 256 + 1024;
+  static constexpr int kStage = kV + kVStages * kHalf;   // dQ on its way out, 2 KB a warp
+  static constexpr int kX = kStage + 256 * DP;           // [2][128] fp32
+  static constexpr int kBar = kX + 1024;
+  static constexpr int kBytes = kBar + 288 + 1024;
+  static_assert(kBytes <= 232448, "shared memory of a block");
 };
 
 template <bool FP16, int DP>
@@ -725,20 +782,24 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   uint64_t* s_full = v_empty + L::kVStages;    // [2]
   uint64_t* ds_full = s_full + 2;              // [2], eight arrivals
   uint64_t* dq_done = ds_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
+  uint64_t* q_empty = dq_done + 1;             // the tile of Q and dO may be loaded over
+  uint64_t* dq_read = dq_done + 2;             // dQ left tensor memory
+  uint64_t* next_full = dq_done + 3;           // the answer to a request for another block's item
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 4);
+  // the loader's note of an item, for the other warps (two: an item's epilogue comes under the next)
+  VlTile* s_tile = reinterpret_cast<VlTile*>(smem + L::kBar + 224);
+  int* s_head = reinterpret_cast<int*>(s_tile + 2);                  // [2], -1: no more
+  int* s_zero = s_head + 2;                                          // head whose outside rows are left, or -1
+  uint8_t* answer = smem + L::kBar + 272;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int entry = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
-  const VlTile w = p.tiles[entry];   // (read beside the count; past it the plan's other words)
   const int count = p.meta[p.count_at];
-  if (entry >= count) {
-    if (entry == count) vl_zero_outside(dQ, p.T, p.Hq, h, p.D, p.meta);
+  const int own = blockIdx.x;   // item (entry, head)
+  if (own / p.Hq >= count) {
+    if (own / p.Hq == count) vl_zero_outside(dQ, p.T, p.Hq, own % p.Hq, p.D, p.meta);
     return;
   }
-  const int hk = h / (p.Hq / p.Hk);
-  const int row0 = w.tile * 128;
-  const int keys = p.causal ? min(row0 + 128, w.len) : w.len;
-  const int n_kv = (keys + 63) / 64;
+  auto key_tiles = [&](const VlTile& w) { return ((p.causal ? min(w.tile * 128 + 128, w.len) : w.len) + 63) / 64; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -747,6 +808,10 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     for (int i = 0; i < L::kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&ds_full[i], 8); }
     mbar_init(dq_done, 1);
+    mbar_init(q_empty, 16);
+    mbar_init(dq_read, 16);
+    mbar_init(next_full, 1);
+    *s_zero = -1;
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmDO);
   }
@@ -756,33 +821,83 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 17) {
-    // ------------------------------------------------------------ TMA loaders (K with Q and dO; V)
-    if (lane == 0) {
-      const bool is_k = warp == 17;
-      if (is_k) {
-        mbar_arrive_expect_tx(q_full, 2 * L::kTile);
+  if (warp == 17) {
+    // ------------------------------------------------------------ TMA loader of Q, dO and K; items
+    int t = 0, it = 0, i = own, asked = -1;   // key tiles of all items so far; items; this one; requests
+    bool ok = true;
+    for (;; ++it) {
+      if (it > 0 && !vl_wait(q_empty, (it - 1) & 1, p.status, kErrVlLoad)) { ok = false; break; }
+      if (i < 0) {
+        if (lane == 0) {
+          s_head[it & 1] = -1;
+          mbar_arrive(q_full);
+        }
+        break;
+      }
+      const VlTile w = p.tiles[i / p.Hq];
+      const int h = i % p.Hq, hk = h / (p.Hq / p.Hk), n_kv = key_tiles(w), row0 = w.tile * 128;
+      if (lane == 0) {
+        s_tile[it & 1] = w;
+        s_head[it & 1] = h;
+        mbar_arrive_expect_tx(q_full, 2 * L::kTile);   // (releases the note)
         vl_load_tile<DP, 128>(smem + L::kQ, &tmQ, q_full, h, w.start + row0);
         vl_load_tile<DP, 128>(smem + L::kDO, &tmDO, q_full, h, w.start + row0);
       }
-      const CUtensorMap* map = is_k ? &tmK : &tmV;
-      uint64_t* empty = is_k ? k_empty : v_empty;
-      uint64_t* full = is_k ? k_full : v_full;
-      uint8_t* ring = smem + (is_k ? L::kK : L::kV);
-      const int nst = is_k ? L::kKStages : L::kVStages;
-      int issued = 0;
+      for (int r = lane; r < min(128, w.len - row0); r += 32) {   // O, read between two items, to L2
+        const int64_t at = ((int64_t)(w.start + row0 + r) * p.Hq + h) * p.D;
+        vl_prefetch(O + at);
+        vl_prefetch(O + at + p.D - 8);
+        vl_prefetch(low + at);
+      }
+      __syncwarp();
+      if (lane == 0)
+        for (int j = 0; j < n_kv; ++j, ++t) {
+          const int st = t % L::kKStages;
+          ok = mbar_wait(&k_empty[st], ((t / L::kKStages) & 1) ^ 1, p.status, kErrVlLoad);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[st], L::kHalf);
+          vl_load_tile<DP, 64>(smem + L::kK + st * L::kHalf, &tmK, &k_full[st], hk, w.start + j * 64);
+          if (j == max(n_kv - 2, 0)) {   // (not sooner: the items then even out over the SMs)
+            asked = it;
+            mbar_arrive_expect_tx(next_full, 16);
+            vl_request_block(answer, next_full);
+          }
+        }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok || !vl_wait(next_full, it & 1, p.status, kErrVlLoad)) { ok = false; ++it; break; }
+      i = vl_answered_block(answer);
+      if (i >= 0 && i / p.Hq >= count) {   // a block with no tile: no more requests after it
+        if (lane == 0 && i / p.Hq == count) *s_zero = i % p.Hq;
+        i = -1;
+      }
+      fence_proxy_async_smem();            // the answer is read before the next is written
+      __syncwarp();
+    }
+    if (!ok && lane == 0) {  // let every copy this thread issued land before the CTA can exit
+      if (asked >= 0) mbar_wait(next_full, asked & 1, nullptr, 0);
+      if (it > 0) mbar_wait(q_full, (it - 1) & 1, nullptr, 0);
+      for (int u = max(t - L::kKStages, 0); u < t; ++u) mbar_wait(&k_full[u % L::kKStages], (u / L::kKStages) & 1, nullptr, 0);
+    }
+  } else if (warp == 18) {
+    // ------------------------------------------------------------ TMA loader of V, by the other's notes
+    if (lane == 0) {
+      int t = 0;
       bool ok = true;
-      for (int t = 0; t < n_kv; ++t) {
-        const int st = t % nst;
-        if (!mbar_wait(&empty[st], ((t / nst) & 1) ^ 1, p.status, kErrVlLoad)) { ok = false; break; }
-        mbar_arrive_expect_tx(&full[st], L::kHalf);
-        vl_load_tile<DP, 64>(ring + st * L::kHalf, map, &full[st], hk, w.start + t * 64);
-        issued = t + 1;
+      for (int it = 0; ok; ++it) {
+        if (!mbar_wait(q_full, it & 1, p.status, kErrVlLoad)) { ok = false; break; }
+        if (s_head[it & 1] < 0) break;
+        const VlTile w = s_tile[it & 1];
+        const int hk = s_head[it & 1] / (p.Hq / p.Hk), n_kv = key_tiles(w);
+        for (int j = 0; j < n_kv; ++j, ++t) {
+          const int st = t % L::kVStages;
+          ok = mbar_wait(&v_empty[st], ((t / L::kVStages) & 1) ^ 1, p.status, kErrVlLoad);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&v_full[st], L::kHalf);
+          vl_load_tile<DP, 64>(smem + L::kV + st * L::kHalf, &tmV, &v_full[st], hk, w.start + j * 64);
+        }
       }
-      if (!ok) {  // let every copy this thread issued land before the CTA can exit
-        if (is_k) mbar_wait(q_full, 0, nullptr, 0);
-        for (int t = max(issued - nst, 0); t < issued; ++t) mbar_wait(&full[t % nst], (t / nst) & 1, nullptr, 0);
-      }
+      if (!ok)
+        for (int u = max(t - L::kVStages, 0); u < t; ++u) mbar_wait(&v_full[u % L::kVStages], (u / L::kVStages) & 1, nullptr, 0);
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------ MMA issuer (whole warp)
@@ -809,140 +924,187 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       __syncwarp();
       return true;
     };
-    bool ok = vl_wait(in_tmem, 0, p.status, kErrVlMma) && issue_scores(0);
-    for (int t = 0; t < n_kv && ok; ++t) {
-      if (t + 1 < n_kv && !issue_scores(t + 1)) { ok = false; break; }
-      const int b = t & 1, ks = t % L::kKStages;
-      if (!vl_wait(&ds_full[b], (t >> 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
-      tc_fence_after();
-      const uint64_t kd = umma_desc_sw128_mnmajor(k_base + ks * L::kHalf, 8192u);
-      if (elect_one_sync()) {
+    bool ok = true;
+    int base = 0, it = 0;   // key tiles of the items before, items
+    for (; ok; ++it) {
+      if (!vl_wait(in_tmem, it & 1, p.status, kErrVlMma)) break;
+      // (reduced over the warp: with it the descriptors below are known to be warp-uniform)
+      const int n_kv = (int)__reduce_max_sync(0xffffffffu, s_head[it & 1] < 0 ? 0u : (unsigned)key_tiles(s_tile[it & 1]));
+      if (n_kv == 0) break;
+      const int end = base + n_kv;
+      ok = issue_scores(base);
+      for (int t = base; t < end && ok; ++t) {
+        if (t + 1 < end && !issue_scores(t + 1)) { ok = false; break; }
+        const int b = t & 1, ks = t % L::kKStages;
+        if (!vl_wait(&ds_full[b], (t >> 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
+        if (t == base && it > 0 && !vl_wait(dq_read, (it - 1) & 1, p.status, kErrVlMma)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t kd = umma_desc_sw128_mnmajor(k_base + ks * L::kHalf, 8192u);
+        if (elect_one_sync()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_f16_ts(tmem + 256u, tmem + (uint32_t)(64 * b + (kk >> 1) * 32 + (kk & 1) * 8), kd + (uint64_t)(kk * 128), idesc_q,
-                      (t > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&k_empty[ks]);
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16_ts(tmem + 256u, tmem + (uint32_t)(64 * b + (kk >> 1) * 32 + (kk & 1) * 8), kd + (uint64_t)(kk * 128), idesc_q,
+                        (t > base || kk > 0) ? 1u : 0u);
+          umma_commit(&k_empty[ks]);
+        }
+        __syncwarp();
       }
+      if (elect_one_sync()) umma_commit(dq_done);
       __syncwarp();
+      base = end;
     }
-    if (elect_one_sync()) umma_commit(dq_done);
-    __syncwarp();
-    mbar_wait(dq_done, 0, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
+    if (it > 0) mbar_wait(dq_done, (it - 1) & 1, nullptr, 0);   // every MMA issued has completed before TMEM can be freed
   } else {
     // ------------------------------------------------------------ dS + epilogue
-    const int quad = warp & 3, half = (warp >> 2) & 1, g = warp >> 3;
-    const int row = quad * 32 + lane, q = row0 + row;
-    const bool live = q < w.len;
-    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    // keys that the row sees, from this half's first
-    const int limit = (live ? (p.causal ? q + 1 : w.len) : 0) - 32 * half;
-    const float lse_row = live ? lse[(int64_t)h * p.T + w.start + q] : 0.0f;
-    // delta of eight rows a warp: DP / 8 lanes to a row (whole lines), O from global before
-    // the wait, dO from the tile
-    constexpr int LR = DP / 8, RI = 32 / LR, NI = 8 / RI;        // lanes to a row, rows at once, steps
-    uint4 ov[NI];
-    uint2 lv[NI];
-    const int dchunk = lane % LR, drow0 = warp * 8 + lane / LR;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = drow0 + i * RI;
-      const bool in = row0 + r < w.len && dchunk * 8 < p.D;
-      const int64_t at = ((int64_t)(w.start + row0 + r) * p.Hq + h) * p.D + dchunk * 8;
-      ov[i] = in ? *reinterpret_cast<const uint4*>(O + at) : make_uint4(0, 0, 0, 0);
-      lv[i] = in ? *reinterpret_cast<const uint2*>(low + at) : make_uint2(0, 0);
-    }
-    bool ok = vl_wait(q_full, 0, p.status, kErrVlCompute);
-    if (ok) {  // group 0 copies Q, group 1 dO, an atom each half: the first scores can start
-      if (half < DP / 64)
-        copy_row_to_tmem(smem + (g == 0 ? L::kQ : L::kDO) + half * 16384 + row * 128, row,
-                         lane_base + 384u + (uint32_t)(64 * g + 32 * half));
-      tmem_st_wait();
-      tc_fence_before();
+    constexpr int LR = DP / 8, RI = 32 / LR, NI = 8 / RI;        // delta: lanes to a row, rows at once, steps
+    int base = 0;              // key tiles of the items before
+    for (int it = 0;; ++it) {
+      // (the thread's places are formed again for each item: over the loop below they would
+      // not fit beside its scores)
+      const int tid = vl_tid(), wp = tid >> 5, lane = tid & 31;
+      const int quad = wp & 3, half = (wp >> 2) & 1, g = wp >> 3, part = wp >> 2;
+      const int row = quad * 32 + lane;
+      const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+      const VlTile& w = s_tile[it & 1];
+      float* xs = reinterpret_cast<float*>(smem + L::kX) + 128 * (it & 1);
+      float lse_row = 0.0f;
+      // eight rows of delta a warp: DP / 8 lanes to a row (whole lines), O from global, dO from the tile
+      const int dchunk = lane % LR, drow0 = wp * 8 + lane / LR;
+      // with the last scores of the item before, Q and dO may leave tensor memory
+      if (it > 0 && !vl_wait(&s_full[(base - 1) & 1], ((base - 1) >> 1) & 1, p.status, kErrVlCompute)) break;
+      if (!vl_wait(q_full, it & 1, p.status, kErrVlCompute)) break;
+      const int h = s_head[it & 1];
+      const bool more = h >= 0;
+      if (more) {   // group 0 copies Q, group 1 dO, an atom each half: the first scores can start
+        tc_fence_after();
+        if (half < DP / 64)
+          copy_row_to_tmem(smem + (g == 0 ? L::kQ : L::kDO) + half * 16384 + row * 128, row,
+                           lane_base + 384u + (uint32_t)(64 * g + 32 * half));
+        tmem_st_wait();
+        tc_fence_before();
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(in_tmem);
-    }
-    float* xs = reinterpret_cast<float*>(smem + L::kX);
+      if (more) {
+        const int row0 = w.tile * 128;
+        if (row0 + row < w.len) lse_row = vl_ld_f32(lse + (int64_t)h * p.T + w.start + row0 + row);
+        uint4 ov[NI];
+        uint2 lv[NI];
+        const int left = dchunk * 8 < p.D ? w.len - row0 - drow0 : 0;   // rows from this lane's first
+        int64_t at = ((int64_t)(w.start + row0 + drow0) * p.Hq + h) * p.D + dchunk * 8;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = drow0 + i * RI;
-      const uint4 du = *reinterpret_cast<const uint4*>(smem + L::kDO + (dchunk >> 3) * 16384 + r * 128 +
-                                                       (((dchunk & 7) ^ (r & 7)) << 4));
-      const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[i].x, ov[i].y, ov[i].z, ov[i].w};
-      float acc = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t lw = j == 0 ? lv[i].x : lv[i].y;
-        const float2 a0 = vl_unpack<FP16>(dw[2 * j]), b0 = vl_unpack<FP16>(ow[2 * j]);
-        const float2 a1 = vl_unpack<FP16>(dw[2 * j + 1]), b1 = vl_unpack<FP16>(ow[2 * j + 1]);
-        acc = fmaf(a0.x, vl_with_low<FP16, 0>(b0.x, lw), acc);
-        acc = fmaf(a0.y, vl_with_low<FP16, 1>(b0.y, lw), acc);
-        acc = fmaf(a1.x, vl_with_low<FP16, 2>(b1.x, lw), acc);
-        acc = fmaf(a1.y, vl_with_low<FP16, 3>(b1.y, lw), acc);
-      }
-      // (a row past the sequence's end: whatever its dO holds, O is 0 there, and NaN stays in the row)
-#pragma unroll
-      for (int o = LR / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      if (dchunk == 0) xs[r] = acc;
-    }
-    named_barrier(1, 512);
-    const float l2 = lse_row * 1.4426950408889634f;
-    const float dl = live ? xs[row] : 0.0f;
-    if (g == 0 && half == 0) {
-      const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
-      delta[at] = dl;
-      nlse2[at] = -l2;
-    }
-    const int part = 2 * g + half;
-    const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(-l2, -l2), dl2 = f2_pack(dl, dl);
-    const uint32_t t_s = lane_base + (uint32_t)(64 * g + 32 * half);
-    for (int t = g; t < n_kv && ok; t += 2) {
-      if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t s[32], dp[32];
-      tmem_ld_32x32b_x32(t_s, s);
-      tmem_ld_32x32b_x32(t_s + 128u, dp);
-      tmem_ld_wait();
-      const int seen = limit - t * 64;
-      const bool cut = __any_sync(0xffffffffu, seen < 32);
-      uint32_t pk[16];
-      // (with and without the mask apart: a branch in every step would keep the steps apart)
-      auto form = [&](auto masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int c = 2 * i;
-          float a0, a1, g0, g1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
-          f2_unpack(f2_mul(f2_pack(fast_exp2(a0), fast_exp2(a1)),
-                           f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl2)), g0, g1);
-          if constexpr (decltype(masked)::value) {
-            g0 = c >= seen ? 0.0f : g0;
-            g1 = c + 1 >= seen ? 0.0f : g1;
+        for (int i = 0; i < NI; ++i) {
+          ov[i] = make_uint4(0, 0, 0, 0);
+          lv[i] = make_uint2(0, 0);
+          if (i * RI < left) {
+            ov[i] = vl_ld_u4(O + at);
+            lv[i] = vl_ld_u2(low + at);
           }
-          pk[i] = vl_pack<FP16>(g0, g1);
+          at += (int64_t)RI * p.Hq * p.D;
         }
-      };
-      if (cut) form(std::true_type());
-      else form(std::false_type());
-      tmem_st_32x32b_x16(t_s, pk);   // over this half's own scores
-      if (w.len - t * 64 < 64)   // the sequence ends inside this key tile (K_t has given its scores)
-        vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, w.len - t * 64, threadIdx.x & 255);
-      tmem_st_wait();
-      tc_fence_before();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int r = drow0 + i * RI;
+          const uint4 du = *reinterpret_cast<const uint4*>(smem + L::kDO + (dchunk >> 3) * 16384 + r * 128 +
+                                                           (((dchunk & 7) ^ (r & 7)) << 4));
+          const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ov[i].x, ov[i].y, ov[i].z, ov[i].w};
+          float acc = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t lw = j == 0 ? lv[i].x : lv[i].y;
+            const float2 a0 = vl_unpack<FP16>(dw[2 * j]), b0 = vl_unpack<FP16>(ow[2 * j]);
+            const float2 a1 = vl_unpack<FP16>(dw[2 * j + 1]), b1 = vl_unpack<FP16>(ow[2 * j + 1]);
+            acc = fmaf(a0.x, vl_with_low<FP16, 0>(b0.x, lw), acc);
+            acc = fmaf(a0.y, vl_with_low<FP16, 1>(b0.y, lw), acc);
+            acc = fmaf(a1.x, vl_with_low<FP16, 2>(b1.x, lw), acc);
+            acc = fmaf(a1.y, vl_with_low<FP16, 3>(b1.y, lw), acc);
+          }
+          // (a row past the sequence's end: whatever its dO holds, O is 0 there, and NaN stays in the row)
+#pragma unroll
+          for (int o = LR / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+          if (dchunk == 0) xs[r] = acc;
+        }
+      }
+      if (it > 0) {   // dQ of the item before, while the first scores of this one are formed
+        if (!vl_wait(dq_done, (it - 1) & 1, p.status, kErrVlCompute)) break;
+        tc_fence_after();
+        const VlTile& b = s_tile[(it - 1) & 1];
+        const int first = b.tile * 128 + quad * 32;
+        uint16_t* out = dQ + ((int64_t)(b.start + first) * p.Hq + s_head[(it - 1) & 1]) * p.D;
+        if (part < DP / 32)   // 32 columns a warp
+          vl_store_rows<FP16, 32>(lane_base + 256u + (uint32_t)(part * 32), p.scale,
+                                  smem + L::kStage + (part * 4 + quad) * 2048, out, (int64_t)p.Hq * p.D, part * 32, p.D,
+                                  b.len - first);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_read);
+      }
+      if (!more) break;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[g]);
-    }
-    if (ok && vl_wait(dq_done, 0, p.status, kErrVlCompute)) {
-      tc_fence_after();
-      uint16_t* out = dQ + ((int64_t)(w.start + q - lane) * p.Hq + h) * p.D;
-      if (part < DP / 32)   // 32 columns a warp, through the memory of Q
-        vl_store_rows<FP16, 32>(lane_base + 256u + (uint32_t)(part * 32), p.scale, smem + L::kQ + (part * 4 + quad) * 2048, out,
-                                (int64_t)p.Hq * p.D, part * 32, p.D, w.len - (q - lane));
+      if (lane == 0) mbar_arrive(q_empty);   // (with the note of the item before read)
+      if (!vl_wait(q_empty, it & 1, p.status, kErrVlCompute)) break;   // the other warps' delta
+      const int len = w.len;
+      const bool live = w.tile * 128 + row < len;
+      const float l2 = lse_row * 1.4426950408889634f;
+      const float dl = live ? xs[row] : 0.0f;
+      if (g == 0 && half == 0) {
+        const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
+        delta[at] = dl;
+        nlse2[at] = -l2;
+      }
+      const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(-l2, -l2), dl2 = f2_pack(dl, dl);
+      const uint32_t t_s = lane_base + (uint32_t)(64 * g + 32 * half);
+      // keys that the row sees, from this half's first, and the sequence's end, both counted
+      // from the CTA's first key tile
+      const uint32_t limit = (live ? (p.causal ? w.tile * 128 + row + 1 : len) : 0) - 32 * half + base * 64u;
+      const uint32_t keys = len + base * 64u;
+      const int first = base;
+      base += key_tiles(w);
+      bool ok = true;
+      for (int t = first + (g ^ (first & 1)); t < base; t += 2) {
+        if (!vl_wait(&s_full[g], (t >> 1) & 1, p.status, kErrVlCompute)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t s[32], dp[32];
+        tmem_ld_32x32b_x32(t_s, s);
+        tmem_ld_32x32b_x32(t_s + 128u, dp);
+        tmem_ld_wait();
+        const int seen = (int)(limit - t * 64u);
+        const bool cut = __any_sync(0xffffffffu, seen < 32);
+        uint32_t pk[16];
+        // (with and without the mask apart: a branch in every step would keep the steps apart)
+        auto form = [&](auto masked) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int c = 2 * i;
+            float a0, a1, g0, g1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nl2), a0, a1);
+            f2_unpack(f2_mul(f2_pack(fast_exp2(a0), fast_exp2(a1)),
+                             f2_sub(f2_pack(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), dl2)), g0, g1);
+            if constexpr (decltype(masked)::value) {
+              g0 = c >= seen ? 0.0f : g0;
+              g1 = c + 1 >= seen ? 0.0f : g1;
+            }
+            pk[i] = vl_pack<FP16>(g0, g1);
+          }
+        };
+        if (cut) form(std::true_type());
+        else form(std::false_type());
+        tmem_st_32x32b_x16(t_s, pk);   // over this half's own scores
+        if (keys - t * 64u < 64u)   // the sequence ends inside this key tile (K_t has given its scores)
+          vl_zero_rows<DP, 64>(smem + L::kK + (t % L::kKStages) * L::kHalf, (int)(keys - t * 64u), tid & 255);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[g]);
+      }
+      if (!ok) break;
     }
   }
 
   tc_fence_before();
   __syncthreads();
   if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (*s_zero >= 0) vl_zero_outside(dQ, p.T, p.Hq, *s_zero, p.D, p.meta);
 }
 
 // ============================================================================
