@@ -32,7 +32,7 @@
 //   8191 + 1037 rows, 8/2 heads           forward 127 us (1.1 PFLOP/s), dQ 181, dK/dV 267
 // Short sequences are bound by what a block does around its loop (launch, first loads,
 // pipeline fill, output: 7-8 us of a block's 15-20 us, with one block to an SM, which
-// tensor and shared memory allow), long ones by the chain of MMAs and exponentials.
+// tensor and shared memory allow; dQ runs part of it under the block before), long ones by the chain of MMAs and exponentials.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
