@@ -782,7 +782,7 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   uint64_t* s_full = v_empty + L::kVStages;    // [2]
   uint64_t* ds_full = s_full + 2;              // [2], eight arrivals
   uint64_t* dq_done = ds_full + 2;
-  uint64_t* q_empty = dq_done + 1;             // the tile of Q and dO may be loaded over
+  uint64_t* q_empty = dq_done + 1;             // the tile of Q and dO may be loaded over, the note is copied
   uint64_t* dq_read = dq_done + 2;             // dQ left tensor memory
   uint64_t* next_full = dq_done + 3;           // the answer to a request for another block's item
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 4);
@@ -808,7 +808,7 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     for (int i = 0; i < L::kVStages; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&ds_full[i], 8); }
     mbar_init(dq_done, 1);
-    mbar_init(q_empty, 16);
+    mbar_init(q_empty, 17);
     mbar_init(dq_read, 16);
     mbar_init(next_full, 1);
     *s_zero = -1;
@@ -888,6 +888,9 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (s_head[it & 1] < 0) break;
         const VlTile w = s_tile[it & 1];
         const int hk = s_head[it & 1] / (p.Hq / p.Hk), n_kv = key_tiles(w);
+        // (an item whose K fits the ring needs no V for the next one's Q and dO to come: without
+        // this arrival q_full could complete twice before this thread has looked at it once)
+        mbar_arrive(q_empty);
         for (int j = 0; j < n_kv; ++j, ++t) {
           const int st = t % L::kVStages;
           ok = mbar_wait(&v_empty[st], ((t / L::kVStages) & 1) ^ 1, p.status, kErrVlLoad);

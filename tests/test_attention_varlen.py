@@ -321,3 +321,31 @@ def test_repeatable_in_a_graph_with_changing_sequences(cuda):
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
     from zeroq_b200.ops import _ext
     assert _ext.ext().gemm_status(0)[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_blocks_that_take_over_items(cuda, dtype, causal, D):
+    """Several dQ items (128 queries of a head) to each SM: documents of one to three key
+    tiles between longer ones, so that items start on odd and even key tiles."""
+    lengths = [60, 100, 190, 700, 30, 129, 400, 64, 65, 0, 1, 1000, 130, 20, 150, 63]
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    per_head = sum((n + 127) // 128 for n in lengths)
+    hk = 3 * sms // (2 * per_head) + 1
+    hq = 2 * hk
+    assert per_head * hq > 3 * sms
+    check(lengths, 77, hq, hk, D, dtype, cuda, causal, seed=D)
+    q, k, v, do, cu = inputs(lengths, 77, hq, hk, D, dtype, cuda, seed=D)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = flash_attention_varlen(*leaves, cu, causal=causal)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+
+    first = step()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    from zeroq_b200.ops import _ext
+    assert _ext.ext().gemm_status(0)[0] == 0
