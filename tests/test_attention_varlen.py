@@ -108,6 +108,23 @@ def test_positions_and_bounds():
     assert s.bounds() == [(0, 3), (3, 3), (3, 7)]
 
 
+def test_a_device_by_another_spelling():
+    """"cpu:0" for "cpu", as "cuda" for "cuda:0": the device is the one that the rows are on."""
+    q = torch.randn(8, 2, 16)
+    s = PackedSequences(torch.tensor([0, 3, 8]), 8, device="cpu:0")
+    assert s.device == q.device == s.cu_seqlens.device
+    assert torch.equal(flash_attention_varlen(q, q, q, s), flash_attention_varlen(q, q, q, torch.tensor([0, 3, 8])))
+
+
+@pytest.mark.gpu
+def test_a_device_without_an_index(cuda):
+    q = torch.randn(8, 2, 64, device=cuda, dtype=torch.bfloat16)
+    for cu in (torch.tensor([0, 3, 8]), torch.tensor([0, 3, 8], dtype=torch.int32, device=cuda)):
+        s = PackedSequences(cu, 8, device="cuda")
+        assert s.device == q.device == s.positions.device
+        assert torch.equal(flash_attention_varlen(q, q, q, s), flash_attention_varlen(q, q, q, cu))
+
+
 @pytest.mark.parametrize("cu,total", [
     (torch.tensor([1, 3]), 5), (torch.tensor([0, 4, 3]), 5), (torch.tensor([0, 6]), 5), (torch.tensor([[0, 3]]), 5),
     (torch.tensor([0.0, 3.0]), 5), (torch.tensor([], dtype=torch.int32), 5), (torch.tensor([0]), -1)])

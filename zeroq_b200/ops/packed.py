@@ -41,12 +41,12 @@ class PackedSequences:
                 raise ValueError(f"PackedSequences: cu_seqlens must rise from 0 to at most total={total}")
         self.total = int(total)
         self.n = cu_seqlens.numel() - 1
-        self.device = device
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.device != device or not cu_seqlens.is_contiguous():
             cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
         self.cu_seqlens = cu_seqlens
+        self.device = cu_seqlens.device   # with its index: "cuda" is the current device
         self.plan = None
-        if device.type == "cuda":
+        if cu_seqlens.is_cuda:
             self.plan, self.positions = _ext.ext().packed_sequences(self.cu_seqlens, self.total)
         else:
             self.positions = torch.zeros(self.total, dtype=torch.int32)
