@@ -108,6 +108,16 @@ def test_positions_and_bounds():
     assert s.bounds() == [(0, 3), (3, 3), (3, 7)]
 
 
+def test_a_division_is_the_one_it_was_made_with():
+    cu = torch.tensor([0, 3, 8], dtype=torch.int32)
+    q = torch.randn(8, 2, 16)
+    s = PackedSequences(cu, 8)
+    want = flash_attention_varlen(q, q, q, s)
+    cu[1] = 6                       # the caller's tensor goes on to the next batch
+    assert s.bounds() == [(0, 3), (3, 8)] and s.positions.tolist() == [0, 1, 2, 0, 1, 2, 3, 4]
+    assert torch.equal(flash_attention_varlen(q, q, q, s), want)
+
+
 def test_a_device_by_another_spelling():
     """"cpu:0" for "cpu", as "cuda" for "cuda:0": the device is the one that the rows are on."""
     q = torch.randn(8, 2, 16)

@@ -43,6 +43,8 @@ class PackedSequences:
         self.n = cu_seqlens.numel() - 1
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.device != device or not cu_seqlens.is_contiguous():
             cu_seqlens = cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+        elif not cu_seqlens.is_cuda:
+            cu_seqlens = cu_seqlens.clone()   # bounds() goes on reading it
         self.cu_seqlens = cu_seqlens
         self.device = cu_seqlens.device   # with its index: "cuda" is the current device
         self.plan = None
@@ -54,6 +56,7 @@ class PackedSequences:
                 self.positions[a:b] = torch.arange(b - a, dtype=torch.int32)
 
     def bounds(self):
-        """``[(first row, end row)]`` of the sequences (read from the device where they are there)."""
+        """``[(first row, end row)]`` of the sequences (on the GPU read from there, int32
+        ``cu_seqlens`` from the caller's own tensor as it is by now)."""
         c = self.cu_seqlens.tolist()
         return list(zip(c, c[1:]))
