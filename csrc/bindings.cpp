@@ -74,7 +74,7 @@ void attn_varlen_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, 
 void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
             c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign);
 // packed_autograd.cpp
-std::vector<at::Tensor> rotary_embedding(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns,
+std::vector<at::Tensor> rotary_embedding(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, std::string turns,
                                          bool interleaved, double factor);
 std::vector<at::Tensor> packed_sequences(at::Tensor cu, int64_t T);
 at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, bool causal, double scale);

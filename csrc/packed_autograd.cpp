@@ -8,8 +8,8 @@ using torch::autograd::variable_list;
 using OptTensor = c10::optional<at::Tensor>;
 
 // rotary.cu
-void rotary(at::Tensor q, OptTensor k, at::Tensor positions, at::Tensor turns, at::Tensor qo, OptTensor ko, bool interleaved,
-            double factor, double sign);
+void rotary_turns(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions, const void* turns, int64_t pairs,
+                  const at::Tensor& qo, const OptTensor& ko, bool interleaved, double factor, double sign);
 // attention_varlen_sm100.cu
 int64_t packed_plan_words(int64_t T, int64_t n);
 void packed_plan(at::Tensor cu, int64_t T, at::Tensor plan, OptTensor positions);
@@ -43,21 +43,24 @@ at::Tensor rows3(const at::Tensor& x) {   // [..., H, D] as [T, H, D], unit stri
   return r.stride(2) == 1 ? r : r.contiguous();
 }
 
-variable_list rotary_call(const at::Tensor& a, const at::Tensor& b, const at::Tensor& positions, const at::Tensor& turns,
+// turns: the bytes of 64-bit numbers
+variable_list rotary_call(const at::Tensor& a, const at::Tensor& b, const at::Tensor& positions, const std::string& turns,
                           bool interleaved, double factor, double sign) {
+  TORCH_CHECK(turns.size() % sizeof(double) == 0, "rotary: turns are 64-bit numbers");
   at::Tensor ya = fresh(a), yb = b.defined() ? fresh(b) : at::Tensor();
   OptTensor rb, ryb;
   if (b.defined()) {
     rb = rows3(b);
     ryb = yb.dim() == 3 ? yb : yb.flatten(0, -3);
   }
-  rotary(rows3(a), rb, positions, turns, ya.dim() == 3 ? ya : ya.flatten(0, -3), ryb, interleaved, factor, sign);
+  rotary_turns(rows3(a), rb, positions, turns.data(), (int64_t)(turns.size() / sizeof(double)),
+               ya.dim() == 3 ? ya : ya.flatten(0, -3), ryb, interleaved, factor, sign);
   return {ya, yb};
 }
 
 struct Rotary : public torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const at::Tensor& positions,
-                               const at::Tensor& turns, bool interleaved, double factor) {
+                               const std::string& turns, bool interleaved, double factor) {
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({positions});
@@ -75,7 +78,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
     if (!gq.defined() && !gk.defined()) return out;
     const bool first = gq.defined();
     variable_list d = rotary_call(first ? gq : gk, first ? gk : at::Tensor(), ctx->get_saved_variables()[0],
-                                  ctx->saved_data["turns"].toTensor(), ctx->saved_data["interleaved"].toBool(),
+                                  ctx->saved_data["turns"].toStringRef(), ctx->saved_data["interleaved"].toBool(),
                                   ctx->saved_data["factor"].toDouble(), -1.0);
     out[first ? 0 : 1] = d[0];
     if (first && gk.defined()) out[1] = d[1];
@@ -202,7 +205,7 @@ struct DistillRows : public torch::autograd::Function<DistillRows> {
 }  // namespace
 
 // (q', k') for [..., H, D] tensors; positions 1-D
-std::vector<at::Tensor> rotary_embedding(at::Tensor q, OptTensor k, at::Tensor positions, at::Tensor turns, bool interleaved,
+std::vector<at::Tensor> rotary_embedding(at::Tensor q, OptTensor k, at::Tensor positions, std::string turns, bool interleaved,
                                          double factor) {
   const at::Tensor kt = k.has_value() ? *k : at::Tensor();
   variable_list y;

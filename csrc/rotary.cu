@@ -210,15 +210,15 @@ static void launch_rotary(RotaryParams& p, bool wide, bool inter, int sms, cudaS
 using namespace zq;
 
 // q [T, Hq, D] and (optional) k [T, Hk, D], unit stride inside a head; qo, ko
-// contiguous; positions int32 / int64 (1-D); turns: fp64 CPU tensor [R/2] of
-// turns per position; factor scales cos and sin, sign = -1 turns back.
-void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
-            c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign) {
+// contiguous; positions int32 / int64 (1-D); turns: `pairs` 64-bit turns per
+// position, on the host; factor scales cos and sin, sign = -1 turns back.
+void rotary_turns(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& positions, const void* turns,
+                  int64_t pairs, const at::Tensor& qo, const c10::optional<at::Tensor>& ko, bool interleaved, double factor,
+                  double sign) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && (!k.has_value() || (k->is_cuda() && k->dim() == 3 && ko.has_value())),
               "rotary: q and k are [T, H, D] CUDA tensors");
-  TORCH_CHECK(turns.device().is_cpu() && turns.scalar_type() == at::kDouble && turns.is_contiguous() &&
-                  turns.numel() >= 1 && turns.numel() <= kRotMaxPairs && 2 * turns.numel() <= q.size(2),
-              "rotary: turns must be 1 to ", kRotMaxPairs, " fp64 values on the CPU, two columns of the head each");
+  TORCH_CHECK(pairs >= 1 && pairs <= kRotMaxPairs && 2 * pairs <= q.size(2),
+              "rotary: turns must be 1 to ", kRotMaxPairs, " values, two columns of the head each");
   TORCH_CHECK(positions.is_cuda() && positions.get_device() == q.get_device() && positions.is_contiguous() &&
                   (positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt),
               "rotary: positions must be contiguous int32 or int64 on q's device");
@@ -227,7 +227,7 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
   TORCH_CHECK(positions.numel() > 0 && T % positions.numel() == 0, "rotary: one position per token");
   RotaryParams p;
   const int64_t esize = q.element_size();
-  const int64_t W = 16 / esize, R = 2 * turns.numel();
+  const int64_t W = 16 / esize, R = 2 * pairs;
   bool wide = D % W == 0 && (D - R) % W == 0 && (interleaved ? R : R / 2) % W == 0;
   const at::Tensor* xs[2] = {&q, k.has_value() ? &*k : nullptr};
   const at::Tensor* ys[2] = {&qo, k.has_value() ? &*ko : nullptr};
@@ -257,7 +257,7 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
   p.rot = (int)R;
   p.factor = (float)factor;
   p.sin_factor = (float)(factor * sign);
-  std::memcpy(p.turns, turns.data_ptr<double>(), (size_t)(R / 2) * sizeof(double));
+  std::memcpy(p.turns, turns, (size_t)pairs * sizeof(double));
   const c10::cuda::CUDAGuard guard(q.device());
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   auto stream = at::cuda::getCurrentCUDAStream();
@@ -268,4 +268,12 @@ void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at:
     default: TORCH_CHECK(false, "rotary: bf16, fp16 or fp32");
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// the same with the turns as an fp64 CPU tensor [R/2]
+void rotary(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor positions, at::Tensor turns, at::Tensor qo,
+            c10::optional<at::Tensor> ko, bool interleaved, double factor, double sign) {
+  TORCH_CHECK(turns.device().is_cpu() && turns.scalar_type() == at::kDouble && turns.is_contiguous(),
+              "rotary: turns must be fp64 values on the CPU");
+  rotary_turns(q, k, positions, turns.data_ptr(), turns.numel(), qo, ko, interleaved, factor, sign);
 }

@@ -95,6 +95,21 @@ def test_scaling_limits():
     assert y[0] == f[0] and math.isclose(y[-1], f[-1] / 8.0, rel_tol=1e-12) and m == 0.1 * math.log(8.0) + 1.0
 
 
+def test_a_fake_call_leaves_nothing_to_the_real_ones():
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    from zeroq_b200.ops.rope import _rope_turns
+
+    with FakeTensorMode():   # as a trace of a model makes it: the first call with these parameters
+        _rope_turns(64, 4321.0, None)
+        rotary_embedding(torch.empty(3, 1, 64), None, torch.arange(3), theta=4321.0)
+    kept, factor = _rope_turns(64, 4321.0, None)
+    assert not isinstance(kept, FakeTensor) and factor == 1.0
+    turns = torch.frombuffer(bytearray(kept), dtype=torch.float64)
+    freq, _ = _rope_frequencies(64, 4321.0, None)
+    assert turns.tolist() == [f / (2 * math.pi) for f in freq]
+
+
 @pytest.mark.parametrize("bad", [
     dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=66), dict(theta=0.5),
     dict(positions=torch.arange(5)), dict(positions=torch.arange(8.0)), dict(k=torch.randn(8, 2, 32)),

@@ -13,6 +13,7 @@ the model was trained on.  CUDA tensors run ``csrc/rotary.cu``.
 
 from __future__ import annotations
 
+import array
 import functools
 import math
 from dataclasses import dataclass
@@ -198,11 +199,11 @@ def _rope_frequencies(rotary_dim: int, theta: float, scaling: Optional[RopeScali
 
 
 @functools.lru_cache(maxsize=256)
-def _rope_turns(rotary_dim: int, theta: float, scaling: Optional[RopeScaling]) -> Tuple[torch.Tensor, float]:
-    """The frequencies in turns per position, as the CPU tensor that the kernel's
-    parameters are filled from (nothing of it is kept on a device)."""
+def _rope_turns(rotary_dim: int, theta: float, scaling: Optional[RopeScaling]) -> Tuple[bytes, float]:
+    """The frequencies in turns per position, as the bytes (64-bit numbers) that the
+    kernel's parameters are filled from.  (No tensor: a cached one could be a tracer's.)"""
     freq, factor = _rope_frequencies(rotary_dim, theta, scaling)
-    return torch.tensor([f / (2 * math.pi) for f in freq], dtype=torch.float64, device="cpu"), factor
+    return array.array("d", [f / (2 * math.pi) for f in freq]).tobytes(), factor
 
 
 def rotary_reference(x: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0,
