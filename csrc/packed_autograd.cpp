@@ -26,7 +26,11 @@ void scale_by_scalar(at::Tensor x, at::Tensor g);
 
 namespace {
 
-bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+// Whether a call goes through its autograd node.  A forward-mode tangent is refused here: a
+// call past the node would give a result without one, and no error.
+bool wants_grad(std::initializer_list<const at::Tensor*> ts, const char* name) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, ": no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -209,7 +213,7 @@ std::vector<at::Tensor> rotary_embedding(at::Tensor q, OptTensor k, at::Tensor p
                                          double factor) {
   const at::Tensor kt = k.has_value() ? *k : at::Tensor();
   variable_list y;
-  if (wants_grad({&q, &kt})) {
+  if (wants_grad({&q, &kt}, "rotary_embedding")) {
     y = Rotary::apply(q, k, positions, turns, interleaved, factor);
   } else {
     y = rotary_call(q, kt, positions, turns, interleaved, factor, 1.0);
@@ -228,7 +232,7 @@ std::vector<at::Tensor> packed_sequences(at::Tensor cu, int64_t T) {
 }
 
 at::Tensor attn_varlen(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor plan, int64_t n, bool causal, double scale) {
-  if (wants_grad({&q, &k, &v})) return VarlenAttention::apply(q, k, v, plan, n, causal, scale);
+  if (wants_grad({&q, &k, &v}, "flash_attention_varlen")) return VarlenAttention::apply(q, k, v, plan, n, causal, scale);
   q = mapped(q);
   at::Tensor o = fresh(q), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   attn_varlen_fwd(q, mapped(k), mapped(v), plan, n, o, lse, c10::nullopt, causal, scale);
@@ -248,7 +252,7 @@ at::Tensor distill_loss(at::Tensor z, at::Tensor ids, at::Tensor teacher, OptTen
   ids = ids.contiguous();
   teacher = teacher.contiguous();
   if (targets.has_value()) targets = targets->to(at::kLong).contiguous();
-  if (wants_grad({&z})) {
+  if (wants_grad({&z}, "distillation_loss")) {
     if (mean && fused) return DistillMean::apply(z, ids, teacher, targets, vocab, ignore_index, temperature, alpha);
     return DistillRows::apply(z, ids, teacher, targets, vocab, ignore_index, temperature, alpha, mean);
   }

@@ -141,3 +141,24 @@ def test_gpu_trainer_steps_on_changing_divisions(cuda):
     assert torch.isfinite(t.step_device(ids, y))   # unpacked, with the scaled positions
     from zeroq_b200.ops import _ext
     assert _ext.ext().gemm_status(0)[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_gpu_forward_mode_is_refused(cuda, grad):
+    """A tangent is not dropped without a word, with the backward's graph or without."""
+    from torch.autograd import forward_ad
+
+    from zeroq_b200.ops import distillation_loss, flash_attention_varlen, rotary_embedding
+
+    q = torch.randn(8, 2, 64, device=cuda, dtype=torch.bfloat16)
+    z = torch.randn(8, 50, device=cuda)
+    pos, cu = torch.arange(8, device=cuda), torch.tensor([0, 8], dtype=torch.int32, device=cuda)
+    top = torch.zeros(8, 2, dtype=torch.int64, device=cuda), torch.zeros(8, 2, device=cuda)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual, dz = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (q, z))
+        for call in (lambda: rotary_embedding(dual, None, pos), lambda: rotary_embedding(q, dual, pos),
+                     lambda: flash_attention_varlen(q, q, dual, cu), lambda: flash_attention_varlen(dual, q, q, cu),
+                     lambda: distillation_loss(dz, *top), lambda: distillation_loss(dz, *top, reduction="none")):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
