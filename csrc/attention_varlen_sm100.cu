@@ -267,7 +267,9 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
     begin = plan_bound(cu, i, T);
     len = max(plan_bound(cu, i + 1, T) - begin, 0);
   };
-  // b[i] = tiles of the sequences before i
+  // b[i] = tiles of the sequences before i, or cap + 1 where these are more (a rising
+  // division has no more than cap; one out of order can ask for more than 2^31, so every
+  // sum is cut off there: cap < 2^25, 32 of them fit)
   if (tid == 0) s_run = 0;
   for (int i = tid; i < kPlanClasses; i += kPlanThreads) s_class[i] = 0;
   __syncthreads();
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
     if (i < n) {
       int begin, len;
       bounds(i, begin, len);
-      c = (len + rows - 1) / rows;
+      c = min((len + rows - 1) / rows, cap + 1);
     }
     int x = c;
 #pragma unroll
@@ -285,13 +287,13 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if ((tid & 31) >= o) x += y;
     }
-    if ((tid & 31) == 31) s_warp[tid >> 5] = x;
+    if ((tid & 31) == 31) s_warp[tid >> 5] = min(x, cap + 1);
     __syncthreads();
     int before = s_run;
-    for (int w = 0; w < (tid >> 5); ++w) before += s_warp[w];
-    if (i < n) b[i] = before + x - c;
+    for (int w = 0; w < (tid >> 5); ++w) before = min(before + s_warp[w], cap + 1);
+    if (i < n) b[i] = min(before + x - c, cap + 1);
     __syncthreads();
-    if (tid == kPlanThreads - 1) s_run = before + x;
+    if (tid == kPlanThreads - 1) s_run = min(before + x, cap + 1);
     __syncthreads();
   }
   const int want = s_run, total = min(want, cap);

@@ -191,6 +191,30 @@ def test_plan_tables(cuda, lengths, tail):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 2])
+def test_plan_of_more_tiles_than_32_bits_count(cuda, extra):
+    """2^18 sequences over all of 2^20 rows, which fall back to 0 in between: 2^31 tiles of
+    128 rows.  The tables keep the sequences that fit, and nothing else."""
+    T, pairs = 1 << 20, (1 << 18) + extra
+    cu = torch.tensor([0, T], dtype=torch.int32, device=cuda).repeat(pairs)
+    n = cu.numel() - 1
+    s = PackedSequences(cu, T)
+    words, at = s.plan.cpu(), 0
+    caps = [T // 256 + n] + [T // 128 + n] * 2
+    meta = words[4 * sum(caps):][:3].tolist()
+    for cap, count, rows in zip(caps, meta, (256, 128, 128)):
+        fit = cap // (T // rows)                         # whole sequences
+        assert count == fit * (T // rows)
+        start, length, tile, slot = words[at: at + 4 * count].view(count, 4).unbind(1)
+        at += 4 * cap
+        assert (start == 0).all() and (length == T).all()
+        assert torch.equal(slot.sort().values, torch.arange(count, dtype=torch.int32))
+        assert torch.equal(tile, slot % (T // rows))
+    from zeroq_b200.ops import _ext
+    assert _ext.ext().gemm_status(0)[0] == 324
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lengths,tail,hq,hk,D", [
