@@ -380,6 +380,9 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* __
 constexpr int kVfThreads = 576;   // 16 softmax warps, MMA warp, loader warp
 constexpr int kVfStages = 2;
 constexpr float kVlRescale = 8.0f;
+// exp2_poly3_x2 of anything up to -120, to the bit: taken off its results, a masked key weighs
+// 0 (a value behind the mask is weighed by it), and what exceeds 2^-96 does not change
+constexpr float kVlPolyFloor = 0.9999289512634277f * 0x1p-120f;
 
 template <int DP>
 struct VfSmem {
@@ -610,12 +613,13 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-m_used, -m_used);
       uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {  // masked keys hold -inf: 2^x gives 0 (the polynomial 2^-120)
+      for (int i = 0; i < 32; ++i) {  // masked keys hold -inf: 2^x gives 0
         float a0, a1;
         f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc2, nm2), a0, a1);
         float p0, p1;
         if (i % 4 == 3) {
           exp2_poly3_x2(a0, a1, p0, p1);
+          f2_unpack(f2_sub(f2_pack(p0, p1), f2_pack(kVlPolyFloor, kVlPolyFloor)), p0, p1);
         } else {
           p0 = fast_exp2(a0);
           p1 = fast_exp2(a1);

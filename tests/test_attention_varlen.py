@@ -264,6 +264,21 @@ def test_a_neighbour_does_not_enter(cuda, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_later_value_does_not_enter_however_large(cuda, D):
+    """A masked key's weight is 0, not merely small: values near the type's largest behind
+    the mask change no row before them."""
+    q, k, v, do, cu = inputs([300, 60], 9, 4, 2, D, torch.bfloat16, cuda)
+    v = v.contiguous()
+    clean = flash_attention_varlen(q, k, v, cu)
+    for first in (1, 64, 150, 257):
+        large = v.clone()
+        large[first:300] = 2.0 ** 127
+        o = flash_attention_varlen(q, k, large, cu)
+        assert torch.equal(o[:first], clean[:first]) and torch.equal(o[300:], clean[300:])
+
+
+@pytest.mark.gpu
 def test_large_scores_move_the_running_maximum(cuda):
     check([600, 300], 0, 2, 1, 128, torch.bfloat16, cuda, seed=3, std=1.0, scale=1.0)
     check([600, 300], 0, 2, 1, 64, torch.bfloat16, cuda, causal=False, seed=4, scale=0.01)
