@@ -610,7 +610,9 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         factor = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
         m_used = m_new;
       }
-      const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-m_used, -m_used);
+      // (a row whose scores so far are all -inf: shifted by nothing they weigh 0, not NaN)
+      const float shift = m_used == -INFINITY ? 0.0f : -m_used;
+      const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(shift, shift);
       uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
       for (int i = 0; i < 32; ++i) {  // masked keys hold -inf: 2^x gives 0

@@ -279,6 +279,24 @@ def test_a_later_value_does_not_enter_however_large(cuda, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_that_overflow_downwards_weigh_nothing(cuda, D):
+    """The first 150 keys, a whole key tile among them, score -2^140 scale: -inf in 32 bits."""
+    q, k, v, do, cu = inputs([300], 0, 2, 1, D, torch.bfloat16, cuda)
+    q, k = torch.zeros_like(q), k.clone()
+    q[..., 0] = 2.0 ** 70
+    k[..., 0] = 0
+    k[:150, :, 0] = -2.0 ** 70
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = flash_attention_varlen(*leaves, cu)
+    got = (o.detach(),) + torch.autograd.grad(o, leaves, do)
+    want = exact(q, k, v, do, [300], True, 1 / math.sqrt(D))
+    for x, (value, tol) in zip(got, want.values()):   # the rows before see nothing else
+        assert ((x[150:].double() - value[150:]).abs() <= tol[150:]).all()
+    assert torch.isnan(got[0][:150]).all()
+
+
+@pytest.mark.gpu
 def test_large_scores_move_the_running_maximum(cuda):
     check([600, 300], 0, 2, 1, 128, torch.bfloat16, cuda, seed=3, std=1.0, scale=1.0)
     check([600, 300], 0, 2, 1, 64, torch.bfloat16, cuda, causal=False, seed=4, scale=0.01)
