@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
         for (int u = 0; u < 4; ++u) {
           if (k0 + 32 * u >= p.K) break;
           const bool in = v[u] >= 0 && v[u] < p.vocab;
-          const float x = in ? t[u] * (kLog2e / p.tau) : -INFINITY;   // t / τ in log2 units
+          const float x = in ? t[u] : -INFINITY;
           s_z[k0 + 32 * u] = in ? to_f32<T>(z[v[u]]) : 0.0f;
           s_id[k0 + 32 * u] = in ? (int)v[u] : -1;
           s_p[k0 + 32 * u] = x;
@@ -620,12 +620,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
       }
       __syncwarp();
       tm = -dist_shift(warp_max(tm), 1.0f);
+      // (the largest taken off before the scale: entries near the type's lowest value stay finite)
+      const float c = kLog2e / p.tau;
       float mass = 0.0f;
-      for (int k = lane; k < p.K; k += 32) mass += dist_exp2(s_p[k] - tm);
+      for (int k = lane; k < p.K; k += 32) mass += dist_exp2((s_p[k] - tm) * c);
       mass = warp_sum(mass);
       const bool some = !(mass == 0.0f);
       const float lm = log2f(mass);
-      for (int k = lane; k < p.K; k += 32) s_p[k] = some ? (s_p[k] - tm) - lm : -INFINITY;
+      for (int k = lane; k < p.K; k += 32) s_p[k] = some ? (s_p[k] - tm) * c - lm : -INFINITY;
       if (lane == 0) s_some[par] = some ? 1.0f : 0.0f;
       __syncwarp();
       if (csize == 1) {

@@ -1,0 +1,86 @@
+"""distillation_loss on rows at the ends of their type's range, against its formula in 64 bits.
+
+Tolerances as for ordinary rows: every term of a loss row is formed in 32 bits from exp2 and
+log2 of relative error 2^-22, so 2^-17 (tau^2 + |loss|) bounds a row, and 2^-17 g (a tau + 1 - a)
+with one rounding of the type a gradient entry.  Differences from the row's largest value are
+exact here or so large that their exponential is 0."""
+
+import pytest
+import torch
+
+from zeroq_b200.ops import distillation_loss
+
+
+def exact(z, ids, t, y, T, a, V, g):
+    """(loss rows, gradient) of sum(g * rows) in 64 bits."""
+    z64, ids, t64 = z.detach().double().cpu()[:, :V], ids.cpu().long(), t.double().cpu()
+    on = (y.cpu() >= 0) & (y.cpu() < V)
+    w = torch.softmax((t64 / T).masked_fill((ids < 0) | (ids >= V), -float("inf")), -1)
+    p = torch.zeros_like(z64).scatter_add_(1, ids.clamp(0, V - 1), w)
+    lq, lr = torch.log_softmax(z64 / T, -1), torch.log_softmax(z64, -1)
+    label = y.cpu().clamp(0, V - 1)[:, None]
+    cross = torch.where(p > 0, p * lq, torch.zeros_like(p)).sum(-1)
+    rows = a * T * T * (torch.xlogy(w, w).sum(-1) - cross) - (1 - a) * lr.gather(1, label)[:, 0]
+    d = a * T * (lq.exp() - p) + (1 - a) * lr.exp()
+    d.scatter_add_(1, label, torch.full_like(label, a - 1, dtype=torch.float64))
+    return torch.where(on, rows, 0.0), torch.where(on, g, 0.0)[:, None] * d
+
+
+def check(z, ids, t, y, T, a, V):
+    """Rows with a gradient each, and their mean."""
+    u, sub = torch.finfo(z.dtype).eps / 2, 2.0 ** -25 if z.dtype == torch.float16 else 0.0
+    n = int(((y >= 0) & (y < V)).sum())
+    for reduction, g in (("none", torch.linspace(0.5, 1.5, len(y), dtype=torch.float64)),
+                         ("mean", torch.full((len(y),), 1.0 / n, dtype=torch.float64))):
+        leaf = z.detach().requires_grad_()
+        loss = distillation_loss(leaf, ids, t, y, temperature=T, alpha=a, vocab=V, reduction=reduction)
+        up = g.float().to(z.device) if reduction == "none" else torch.ones((), device=z.device)
+        grad, = torch.autograd.grad(loss, leaf, up)
+        rows, want = exact(z, ids, t, y, T, a, V, g)
+        tol = 2.0 ** -17 * (T * T + rows.abs())
+        if reduction == "mean":
+            rows, tol = rows.sum() / n, tol.sum() / n
+        assert ((loss.detach().double().cpu() - rows).abs() <= tol).all(), (loss, rows)
+        tol = u * want.abs() + 2.0 ** -17 * (a * T + 1 - a) * g[:, None] + sub
+        assert ((grad.double().cpu()[:, :V] - want).abs() <= tol).all()
+        assert (grad[:, V:] == 0).all()
+
+
+def make(M, V, K, dtype, teacher, device, wide=None):
+    g = torch.Generator().manual_seed(M + V)
+    z = (torch.randn(M, wide or V, generator=g) * 3).to(dtype).to(device)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(M)]).to(device)
+    t = (torch.randn(M, K, generator=g) * 3).to(teacher).to(device)
+    y = torch.randint(0, V, (M,), generator=g)
+    y[::5] = -100
+    return z, ids, t, y.to(device)
+
+
+def lowest_teacher(dtype, teacher, device="cpu"):
+    """Entries at and near the type's lowest value are entries, not none."""
+    z, ids, t, y = make(12, 300, 6, dtype, teacher, device)
+    low = torch.finfo(teacher).min
+    t[1] = low                    # all alike: uniform
+    t[2, :3] = low                # next to ordinary ones: nothing of the mass
+    t[3, 1:] = low
+    t[4] = low
+    t[4, 4] = 0.75 * low          # all of the mass
+    t[6] = -low
+    ids[7, 2:], t[7] = -1, low    # two entries
+    return z, ids, t, y
+
+
+TEMPERATURES = [(1.0, 1.0), (1.0, 0.4), (2.0, 0.5), (0.5, 1.0), (1.5, 0.3), (4.0, 0.5), (3.0, 0.0)]
+
+
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+def test_reference_teacher_at_the_lowest_value(T, a):
+    check(*lowest_teacher(torch.float32, torch.float32), T, a, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("teacher", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+def test_kernel_teacher_at_the_lowest_value(cuda, teacher, T, a):
+    check(*lowest_teacher(torch.float32, teacher, cuda), T, a, 300)
+    check(*lowest_teacher(torch.bfloat16, teacher, cuda), T, a, 300)

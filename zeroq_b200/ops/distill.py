@@ -28,8 +28,10 @@ def distillation_reference(logits, teacher_ids, teacher_logits, targets=None, te
     z = z if z.dtype == torch.float64 else z.float()
     ids = teacher_ids.long()
     there = (ids >= 0) & (ids < vocab)
-    t = (teacher_logits.to(z.dtype) / temperature).masked_fill(~there, float("-inf"))
+    t = teacher_logits.to(z.dtype).masked_fill(~there, float("-inf"))
     some = (t > float("-inf")).any(-1, keepdim=True)
+    if t.shape[-1]:   # (the largest taken off before the scale: entries near the type's lowest value stay finite)
+        t = (t - t.amax(-1, keepdim=True)) / temperature
     p = torch.softmax(torch.where(some, t, torch.zeros_like(t)), -1)
     p = torch.where(some & (p != 0), p, torch.zeros_like(p))
     at = torch.where(there, ids, torch.zeros_like(ids))
