@@ -84,8 +84,10 @@ struct RowSums {
   float m, soft, hard;
 };
 
-// (a maximum of -inf shifts by nothing: sums of 0, not NaN)
-__device__ __forceinline__ float dist_shift(float m, float s) { return m == -INFINITY ? 0.0f : -m * s; }
+// (a maximum of -inf shifts by nothing: sums of 0, not NaN.  The product is kept from the
+// compiler's own fma, which would round one of two shifts and not the other: a maximum
+// that stays would raise its sum by 2^(|m·s| 2^-25))
+__device__ __forceinline__ float dist_shift(float m, float s) { return m == -INFINITY ? 0.0f : -__fmul_rn(m, s); }
 
 // factor of a sum when the maximum goes from `from` up to `to`
 __device__ __forceinline__ float dist_raise(float from, float to, float s) {

@@ -84,3 +84,17 @@ def test_reference_teacher_at_the_lowest_value(T, a):
 def test_kernel_teacher_at_the_lowest_value(cuda, teacher, T, a):
     check(*lowest_teacher(torch.float32, teacher, cuda), T, a, 300)
     check(*lowest_teacher(torch.bfloat16, teacher, cuda), T, a, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,offset", [
+    (torch.float32, 30001.0), (torch.float32, -1e6), (torch.bfloat16, -999.0), (torch.float16, -6e4), (torch.float16, 3e4)])
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+def test_kernel_logits_with_an_offset(cuda, dtype, offset, T, a):
+    """A shift of a row's logits drops out, as far as their type holds their differences."""
+    for V in (300, 5000):
+        z, ids, t, y = make(12, V, 6, torch.float32, torch.float32, cuda)
+        z = z.round() + offset
+        z[1] = offset                      # all alike
+        z[2, V // 2:] = offset + 5
+        check(z.to(dtype), ids, t, y, T, a, V)
