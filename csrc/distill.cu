@@ -79,7 +79,9 @@ __device__ __forceinline__ float dist_exp2(float x) {
 // A row's reference m (its maximum or somewhat less, in the logits' own units) and the sums of
 // 2^(x·s + shift(m, s)) at the softmaxes' scales s.  The shift is the ROUNDED product
 // -m·s, everywhere the same one: x·s + shift is then one exact product and one
-// rounding of a small number, and no error of the size of m·s enters.
+// rounding of a small number, and no error of the size of m·s enters.  It is rounded down:
+// where m is a mask's value so far (-1e9, the type's lowest) what the rounding leaves may
+// be any power of two, but none above 1, and sums of 0 go when the maximum moves up.
 struct RowSums {
   float m, soft, hard;
 };
@@ -87,7 +89,7 @@ struct RowSums {
 // (a maximum of -inf shifts by nothing: sums of 0, not NaN.  The product is kept from the
 // compiler's own fma, which would round one of two shifts and not the other: a maximum
 // that stays would raise its sum by 2^(|m·s| 2^-25))
-__device__ __forceinline__ float dist_shift(float m, float s) { return m == -INFINITY ? 0.0f : -__fmul_rn(m, s); }
+__device__ __forceinline__ float dist_shift(float m, float s) { return m == -INFINITY ? 0.0f : __fmul_rd(-m, s); }
 
 // factor of a sum when the maximum goes from `from` up to `to`
 __device__ __forceinline__ float dist_raise(float from, float to, float s) {

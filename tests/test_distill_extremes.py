@@ -98,3 +98,41 @@ def test_kernel_logits_with_an_offset(cuda, dtype, offset, T, a):
         z[1] = offset                      # all alike
         z[2, V // 2:] = offset + 5
         check(z.to(dtype), ids, t, y, T, a, V)
+
+
+def masked_logits(V, dtype, device="cpu", wide=None):
+    """Rows with a part of the vocabulary masked out: whole blocks of columns, all but the
+    teacher's entries and the target, single columns."""
+    z, ids, t, y = make(20, V, 6, dtype, torch.float32, device, wide)
+    low = torch.finfo(dtype).min
+    values = (low, -1e10, -1e9, -3e38, -1e30) if low < -1e5 else (low, -6e4, -3e4, -65504.0, -5e4)
+    for r in range(20):
+        value = values[r % 5]
+        keep = torch.cat([ids[r], y[r: r + 1].clamp_min(0)])
+        row = z[r].clone()
+        if r < 5:
+            z[r] = value                       # everything
+        elif r < 10:
+            z[r, : V // 2] = value             # the first half: whole threads, warps and blocks begin with it
+        elif r < 15:
+            z[r, V // 2:] = value
+        else:
+            z[r, ::3] = value
+        z[r, keep] = row[keep]                 # but these
+    y[y < 0] = 1
+    y[3], y[8] = -100, V
+    z[torch.arange(20, device=device), y.clamp(0, V - 1)] = 0.5
+    return z, ids, t, y
+
+
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+def test_reference_masked_vocabulary(T, a):
+    check(*masked_logits(300, torch.float32), T, a, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+@pytest.mark.parametrize("V,wide", [(7, 7), (300, 300), (1003, 1024), (50257, 50304), (152064, 152064)])
+def test_kernel_masked_vocabulary(cuda, V, wide, T, a, dtype):
+    check(*masked_logits(V, dtype, cuda, wide), T, a, V)
