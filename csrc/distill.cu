@@ -66,7 +66,7 @@ struct DistillParams {
   int K, ids64, teacher_type;
   float soft_scale;         // log2(e) / τ; with one softmax, its scale
   float alpha, tau;
-  bool grad_only, g_mean;
+  bool grad_only, g_mean, two;   // two: two softmaxes
   DeviceStatus* status;
 };
 
@@ -728,27 +728,150 @@ __global__ void __launch_bounds__(S::kThreads, S::kBlocks) distill_kernel(const 
   }
 }
 
-// loss = sum of the rows over the number of counted ones, in 64 bits and a fixed order
-__global__ void __launch_bounds__(1024) distill_mean_kernel(const float* __restrict__ rows,
-                                                            const int64_t* __restrict__ targets,
-                                                            float* __restrict__ loss, int64_t M, int64_t vocab) {
+// ============================================================================
+// After the rows: those whose mask left nothing, and the mean.
+//
+// Where a row's largest logit is a mask's value (-1e9, the type's lowest), so that m·s is
+// beyond 2^26, the rounded shift is off by more than the sums' range allows for.  Such a
+// row, which the kernel above leaves unusable, is formed again here from (x - m)·s, a row
+// at a time by the whole block.  The mean (`loss`, one block) is the sum of the rows over
+// the number of counted ones, in 64 bits and a fixed order.
+// ============================================================================
+constexpr int kDistFinish = 1024;
+
+__device__ __forceinline__ float dist_block(float v, bool max, float* part) {   // over the block, in every thread
+  v = max ? warp_max(v) : warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[threadIdx.x & 31];
+  return max ? warp_max(v) : warp_sum(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDistFinish) distill_finish_kernel(const __grid_constant__ DistillParams p,
+                                                                     float* __restrict__ loss) {
   __shared__ double s_sum[32];
-  __shared__ int s_n[32];
+  __shared__ int s_n[32], s_row;
+  __shared__ float s_part[32], s_p[kDistMaxK + 1], s_z[kDistMaxK + 1];
+  __shared__ int s_id[kDistMaxK + 1];
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const float ss = p.soft_scale, fast = fmaxf(ss, kLog2e);
+  auto far = [&](int64_t row) {   // (rows that count nothing have m = 0)
+    const float m = p.sums[3 * row];
+    return (m != -INFINITY) & (fabsf(m) * fast > 67108864.0f);
+  };
+  const float* rows = loss != nullptr ? p.rows : p.sums;   // (any readable floats)
   double s = 0.0;
   int n = 0;
-  for (int64_t i = threadIdx.x; i < M; i += 1024) {
+  bool some_far = false;
+#pragma unroll 4
+  for (int64_t i = tid; i < p.M; i += kDistFinish) {   // (nothing here waits for a load before the next one)
     s += rows[i];
-    n += (targets == nullptr || (targets[i] >= 0 && targets[i] < vocab)) ? 1 : 0;
+    const int64_t y = p.targets != nullptr ? p.targets[i] : 0;
+    n += ((y >= 0) & (y < p.vocab)) ? 1 : 0;
+    some_far |= far(i);
   }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((tid & 31) == 0) s_n[warp] = n;
+  if (__syncthreads_or(some_far)) {
+    n = 0;
+    for (int w = 0; w < 32; ++w) n += s_n[w];
+    const float inv_n = 1.0f / fmaxf((float)n, 1.0f);
+    auto redo = [&](int64_t row) {
+      const T* z = reinterpret_cast<const T*>(p.logits) + row * p.stride;
+      const float m = p.sums[3 * row];
+      auto near = [&](int64_t j) { return to_f32<T>(z[j]) - m; };
+      float soft = 0.0f, hard = 0.0f;
+      for (int64_t j = tid; j < p.vocab; j += kDistFinish) {
+        const float x = near(j);
+        soft += dist_exp2(x * ss);
+        hard += p.two ? dist_exp2(x * kLog2e) : 0.0f;
+      }
+      soft = dist_block(soft, false, s_part);
+      hard = p.two ? dist_block(hard, false, s_part) : soft;
+      // the entries as columns, log2 p and logits; the target behind them
+      const int y = p.targets != nullptr ? (int)p.targets[row] : -1;
+      float tm = -INFINITY;
+      for (int k = tid; k <= p.K; k += kDistFinish) {
+        const int64_t e = row * p.K + k;
+        int64_t id = y;
+        float t = -INFINITY;
+        if (k < p.K) {
+          id = p.ids64 ? reinterpret_cast<const int64_t*>(p.ids)[e] : (int64_t)reinterpret_cast<const int32_t*>(p.ids)[e];
+          if (id < 0 || id >= p.vocab) id = -1;
+          if (id >= 0) t = dist_teacher(p, e);
+        }
+        s_id[k] = (int)id;
+        s_p[k] = t;
+        s_z[k] = id >= 0 ? near(id) : 0.0f;
+        tm = fmaxf(tm, t);
+      }
+      tm = -dist_shift(dist_block(tm, true, s_part), 1.0f);
+      const float c = kLog2e / p.tau;
+      float mass = 0.0f;
+      for (int k = tid; k < p.K; k += kDistFinish) mass += dist_exp2((s_p[k] - tm) * c);
+      mass = dist_block(mass, false, s_part);
+      const bool some = !(mass == 0.0f);
+      const float lm = log2f(mass), log_s = log2f(soft);
+      float kl = 0.0f;
+      for (int k = tid; k < p.K; k += kDistFinish) {
+        const float lp = some ? (s_p[k] - tm) * c - lm : -INFINITY, pk = dist_exp2(lp);
+        s_p[k] = lp;
+        if (s_id[k] >= 0 && !(pk == 0.0f)) kl += pk * (lp - (s_z[k] * ss - log_s));
+      }
+      kl = dist_block(kl, false, s_part);
+      if (tid == 0 && !p.grad_only) {
+        float v = 0.0f;
+        if (p.alpha > 0.0f) v = p.alpha * p.tau * p.tau * kLn2 * kl;
+        if (p.alpha < 1.0f) v += (1.0f - p.alpha) * kLn2 * (log2f(hard) - s_z[p.K] * (p.two ? kLog2e : ss));
+        p.rows[row] = v;
+      }
+      if (p.grad != nullptr) {
+        const float g = !p.grad_only ? inv_n : p.g_mean ? p.g[0] * inv_n : p.g[row];
+        const float cs = p.alpha * p.tau * (some ? 1.0f : 0.0f) * g, ch = (1.0f - p.alpha) * g;
+        const float fs = (p.two ? cs : cs + ch) / soft, fh = p.two ? ch / hard : 0.0f;
+        auto smooth = [&](float x) { return fs * dist_exp2(x * ss) + (p.two ? fh * dist_exp2(x * kLog2e) : 0.0f); };
+        T* dz = reinterpret_cast<T*>(p.grad) + row * p.grad_stride;
+        for (int64_t j = tid; j < p.vocab; j += kDistFinish) dz[j] = from_f32<T>(smooth(near(j)));
+        __syncthreads();
+        for (int k = tid; k <= p.K; k += kDistFinish) {
+          const int id = s_id[k];
+          if (id < 0) continue;
+          float pk = 0.0f;
+          for (int j = 0; j < p.K; ++j)
+            if (s_id[j] == id) pk += dist_exp2(s_p[j]);
+          dz[id] = from_f32<T>(smooth(s_z[k]) - cs * pk - (id == y ? ch : 0.0f));
+        }
+      }
+      __syncthreads();
+    };
+    for (int64_t base = blockIdx.x; base < p.M; base += (int64_t)gridDim.x * kDistFinish) {
+      const int64_t row = base + (int64_t)tid * gridDim.x;
+      bool left = row < p.M && far(row);
+      for (;;) {   // the block's far rows, lowest first
+        if (tid == 0) s_row = kDistFinish;
+        __syncthreads();
+        if (left) atomicMin(&s_row, tid);
+        __syncthreads();
+        const int t = s_row;
+        __syncthreads();
+        if (t == kDistFinish) break;
+        redo(base + (int64_t)t * gridDim.x);
+        left = left && t != tid;
+      }
+    }
+    if (loss != nullptr) {
+      s = 0.0;
+      for (int64_t i = tid; i < p.M; i += kDistFinish) s += p.rows[i];
+    }
+  }
+  if (loss == nullptr) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) {
-    s_sum[threadIdx.x >> 5] = s;
-    s_n[threadIdx.x >> 5] = n;
-  }
+  if ((tid & 31) == 0) s_sum[warp] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     s = 0.0;
     n = 0;
     for (int w = 0; w < 32; ++w) {
@@ -819,6 +942,7 @@ static void launch_distill(const DistillParams& p, int csize, cudaStream_t strea
 template <typename T, typename S>
 static void launch_distill_mode(DistillParams& p, int csize, cudaStream_t stream) {
   const bool both = p.alpha > 0.0f && p.alpha < 1.0f && p.tau != 1.0f;
+  p.two = both;
   if (!both) {
     if (p.alpha == 0.0f) p.soft_scale = kLog2e;   // the hard softmax alone
     launch_distill<T, S, 1>(p, csize, stream);
@@ -918,12 +1042,22 @@ static DistillParams distill_params(const at::Tensor& logits, const at::Tensor& 
   return p;
 }
 
-static void launch_distill_typed(const at::Tensor& logits, DistillParams& p) {
+template <typename T>
+static void launch_distill_rows(DistillParams& p, float* loss, cudaStream_t stream) {
+  launch_distill_shape<T>(p, stream);
+  // (without a mean the rows are divided over a few blocks)
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const unsigned grid = loss != nullptr ? 1u : (unsigned)std::min<int64_t>(sms, (p.M + 31) / 32);
+  distill_finish_kernel<T><<<grid, kDistFinish, 0, stream>>>(p, loss);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+static void launch_distill_typed(const at::Tensor& logits, DistillParams& p, float* loss) {
   auto stream = at::cuda::getCurrentCUDAStream();
   switch (logits.scalar_type()) {
-    case at::kBFloat16: launch_distill_shape<__nv_bfloat16>(p, stream); break;
-    case at::kHalf: launch_distill_shape<__half>(p, stream); break;
-    case at::kFloat: launch_distill_shape<float>(p, stream); break;
+    case at::kBFloat16: launch_distill_rows<__nv_bfloat16>(p, loss, stream); break;
+    case at::kHalf: launch_distill_rows<__half>(p, loss, stream); break;
+    case at::kFloat: launch_distill_rows<float>(p, loss, stream); break;
     default: TORCH_CHECK(false, "distill: bf16, fp16 or fp32 logits");
   }
 }
@@ -940,16 +1074,15 @@ void distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::optiona
                   rows.scalar_type() == at::kFloat && rows.numel() == p.M,
               "distill: rows [M] fp32");
   p.rows = rows.data_ptr<float>();
-  const c10::cuda::CUDAGuard guard(logits.device());
-  launch_distill_typed(logits, p);
+  float* mean = nullptr;
   if (loss.has_value() && loss->defined()) {
     TORCH_CHECK(loss->is_cuda() && loss->get_device() == logits.get_device() && loss->scalar_type() == at::kFloat &&
                     loss->numel() == 1,
                 "distill: loss is one fp32 value");
-    distill_mean_kernel<<<1, 1024, 0, at::cuda::getCurrentCUDAStream()>>>(p.rows, p.targets, loss->data_ptr<float>(), p.M,
-                                                                          p.vocab);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    mean = loss->data_ptr<float>();
   }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  launch_distill_typed(logits, p, mean);
 }
 
 // The gradient of the loss rows times g [M], or of their mean times g [1] (`mean`),
@@ -965,7 +1098,7 @@ void distill_grad(at::Tensor logits, at::Tensor ids, at::Tensor teacher, c10::op
   p.grad_only = true;
   p.g_mean = mean;
   const c10::cuda::CUDAGuard guard(logits.device());
-  launch_distill_typed(logits, p);
+  launch_distill_typed(logits, p, nullptr);
 }
 
 // x *= g[0] in place (one more rounding); where g[0] is 1 the kernel returns at once

@@ -136,3 +136,62 @@ def test_reference_masked_vocabulary(T, a):
 @pytest.mark.parametrize("V,wide", [(7, 7), (300, 300), (1003, 1024), (50257, 50304), (152064, 152064)])
 def test_kernel_masked_vocabulary(cuda, V, wide, T, a, dtype):
     check(*masked_logits(V, dtype, cuda, wide), T, a, V)
+
+
+def far_logits(V, dtype, teacher=torch.float32, device="cpu", wide=None):
+    """Rows whose largest logit lies far from 0: masks that left nothing, and others."""
+    z, ids, t, y = make(20, V, 6, dtype, teacher, device, wide)
+    g = torch.Generator().manual_seed(V)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    rows = [r for r in range(20) if r % 5]      # (every fifth counts nothing)
+    z[rows[0]] = low                            # a mask by the lowest value over everything
+    for r, value in zip(rows[1:6], (-1e9, -1e10, -1e30, 3e9, 1e37) if high > 1e5 else (-6e4, -3e4, -65504.0, 6e4, 5e4)):
+        z[r] = value
+    z[rows[6]] = high
+    r = rows[7]                                 # a mask over everything but the teacher's entries and the target
+    keep = torch.cat([ids[r], y[r: r + 1]])
+    z[r], z[r, keep] = low, z[r, keep].clone()
+    r = rows[8]                                 # lowest values, and -inf behind them
+    z[r] = low
+    z[r, torch.randperm(V, generator=g)[: V // 2].to(device)] = -float("inf")
+    z[r, ids[r]] = z[r, y[r]] = low
+    for r, base in zip(rows[9:15], (-2.0 ** 26, -2.0 ** 25, -4.66e7, 4.66e7, 2.0 ** 24, -1.2e7)):
+        steps = torch.randint(0, 9, z[r].shape, generator=g).to(device)   # next to where the kernel's forms meet
+        z[r] = base + 4 * steps if high > 1e5 else steps.to(dtype)
+    z[rows[15], : V // 2] = -1e9 if high > 1e5 else low       # ordinary rows with a part masked out
+    ids[rows[15]] = V // 2 + torch.arange(6, device=device)
+    y[rows[15]] = V - 1
+    return z, ids, t, y
+
+
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+def test_reference_logits_far_from_zero(T, a):
+    check(*far_logits(300, torch.float32), T, a, 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,a", TEMPERATURES)
+@pytest.mark.parametrize("V,wide", [(300, 300), (1003, 1024), (50257, 50304), (152064, 152064)])
+def test_kernel_logits_far_from_zero(cuda, V, wide, T, a, dtype):
+    check(*far_logits(V, dtype, device=cuda, wide=wide), T, a, V)
+
+
+@pytest.mark.gpu
+def test_kernel_low_temperatures(cuda):
+    """Ordinary logits over a small temperature are far from 0 as well."""
+    for dtype in (torch.float32, torch.float16):
+        check(*far_logits(777, dtype, device=cuda), 0.01, 0.5, 777)
+        check(*far_logits(777, dtype, device=cuda), 0.001, 1.0, 777)
+
+
+@pytest.mark.gpu
+def test_kernel_a_batch_of_rows_far_from_zero(cuda):
+    """More of them than a block looks at together, repeated ids and a target among them."""
+    z, ids, t, y = make(2500, 200, 40, torch.bfloat16, torch.float32, cuda)
+    z[::2] = torch.finfo(z.dtype).min
+    z[1] = 0.5
+    ids[::4, 20:] = ids[::4, :1]
+    y[::6] = ids[::6, 3]
+    check(z, ids, t, y, 2.0, 0.5, 200)
+    check(z, ids, t, y, 1.0, 0.5, 200)

@@ -26,6 +26,7 @@ def distillation_reference(logits, teacher_ids, teacher_logits, targets=None, te
     vocab = logits.shape[-1] if vocab is None else vocab
     z = logits[:, :vocab]
     z = z if z.dtype == torch.float64 else z.float()
+    z = z - z.detach().amax(-1, keepdim=True)   # before the scale too: logits far from 0 keep their differences
     ids = teacher_ids.long()
     there = (ids >= 0) & (ids < vocab)
     t = teacher_logits.to(z.dtype).masked_fill(~there, float("-inf"))
