@@ -108,6 +108,25 @@ def test_positions_and_bounds():
     assert s.bounds() == [(0, 3), (3, 3), (3, 7)]
 
 
+@pytest.mark.parametrize("cu,total", [([0, 8], 8), (None, 8), (torch.tensor([0, 8]), 8.5), (torch.tensor([0, 8]), None)])
+def test_packed_refuses_other_kinds_of_arguments(cu, total):
+    with pytest.raises(TypeError, match="PackedSequences"):
+        PackedSequences(cu, total)
+
+
+@pytest.mark.parametrize("seqs", [[0, 8], None, 8])
+def test_attention_refuses_other_kinds_of_divisions(seqs):
+    q = torch.zeros(8, 2, 16)
+    with pytest.raises(TypeError, match="flash_attention_varlen"):
+        flash_attention_varlen(q, q, q, seqs)
+
+
+def test_attention_refuses_heads_of_no_width():
+    q = torch.zeros(8, 2, 0)
+    with pytest.raises(ValueError, match="flash_attention_varlen"):
+        flash_attention_varlen(q, q, q, torch.tensor([0, 8]))
+
+
 def test_a_division_is_the_one_it_was_made_with():
     cu = torch.tensor([0, 3, 8], dtype=torch.int32)
     q = torch.randn(8, 2, 16)

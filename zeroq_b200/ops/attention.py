@@ -172,6 +172,10 @@ def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"flash_attention_varlen: {Hq} query heads do not share {ks[1]} kv heads evenly")
     if not (k.dtype == v.dtype == dtype) or not (k.device == v.device == device):
         raise TypeError("flash_attention_varlen: q, k and v of one type on one device")
+    if D < 1:
+        raise ValueError("flash_attention_varlen: heads of no width")
+    if not isinstance(seqs, (PackedSequences, torch.Tensor)):
+        raise TypeError(f"flash_attention_varlen: seqs are PackedSequences or a cu_seqlens tensor, got {type(seqs).__name__}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"flash_attention_varlen: scale must be positive, got {scale}")

@@ -28,6 +28,9 @@ class PackedSequences:
     had here: make another one for another division."""
 
     def __init__(self, cu_seqlens: torch.Tensor, total: int, device: Optional[torch.device] = None):
+        if not isinstance(cu_seqlens, torch.Tensor) or not hasattr(total, "__index__"):
+            raise TypeError(f"PackedSequences: cu_seqlens a tensor and total a whole number, got {type(cu_seqlens).__name__} "
+                            f"and {type(total).__name__}")
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
             raise ValueError(f"PackedSequences: cu_seqlens must be [n + 1], got {tuple(cu_seqlens.shape)}")
         if cu_seqlens.dtype not in (torch.int32, torch.int64):
