@@ -1118,6 +1118,7 @@ DeviceStatus* status_buffer(int device) {
   static std::mutex mu;
   std::lock_guard<std::mutex> g(mu);
   if (bufs[device] == nullptr) {
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));   // (callers ask before they make it current)
     C10_CUDA_CHECK(cudaMalloc(&bufs[device], sizeof(DeviceStatus)));
     C10_CUDA_CHECK(cudaMemset(bufs[device], 0, sizeof(DeviceStatus)));
   }

@@ -452,3 +452,13 @@ def test_blocks_that_take_over_items(cuda, dtype, causal, D):
         assert all(torch.equal(a, b) for a, b in zip(first, step()))
     from zeroq_b200.ops import _ext
     assert _ext.ext().gemm_status(0)[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_tensors_on_another_device_than_the_current_one(cuda):
+    other = torch.device("cuda", 1)
+    with torch.cuda.device(0):   # (the first work of this device: its status words are set up there)
+        check([130, 1, 60], 5, 4, 2, 128, torch.bfloat16, other)
+        from zeroq_b200.ops import _ext
+        assert _ext.ext().gemm_status(1)[0] == 0
