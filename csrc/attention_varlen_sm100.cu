@@ -668,9 +668,12 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       wait(&pv_done[x], jl & 1);
       if (ok) {
         tc_fence_after();
+        // 1 / l, a last bit up: where few keys have equal weights O would often lie at a tie of
+        // its rounding, which its byte cannot tell apart; with the bit it lies above it
+        const float inv = __uint_as_float(__float_as_uint(1.0f / l) + 1u);
         // (this tile's Q has given all its scores: its memory stages the output)
         const int64_t at = ((int64_t)(w.start + q - lane) * p.Hq + h) * p.D;
-        vl_store_rows<FP16, DP / 2>(t_o, 1.0f / l, smem + L::kQ + x * L::kTile + (warp & 7) * (L::kTile / 8), O + at,
+        vl_store_rows<FP16, DP / 2>(t_o, inv, smem + L::kQ + x * L::kTile + (warp & 7) * (L::kTile / 8), O + at,
                                     (int64_t)p.Hq * p.D, half * (DP / 2), p.D, w.len - (q - lane),
                                     low != nullptr ? low + at : nullptr);
         if (q < w.len && half == 0) lse[(int64_t)h * p.T + w.start + q] = (m_used + __log2f(l)) * 0.69314718055994531f;

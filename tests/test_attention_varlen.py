@@ -462,3 +462,57 @@ def test_tensors_on_another_device_than_the_current_one(cuda):
         check([130, 1, 60], 5, 4, 2, 128, torch.bfloat16, other)
         from zeroq_b200.ops import _ext
         assert _ext.ext().gemm_status(1)[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,lost", [(torch.bfloat16, 8), (torch.float16, 5)])
+def test_the_forward_keeps_eight_more_bits_of_o(cuda, dtype, lost):
+    """Equal scores: every weight is 1 and the sum of a row's is in its lse, so the 32-bit O
+    is sum(v) exp(-lse).  With its byte O lacks the pattern's last `lost` bits, 2^(lost - 23)
+    of it; lse's logarithm adds 2^-20, and sums of up to 40 values 40 steps of 2^-23 of their
+    mean size.  A value of 32 bits lies at a tie that is rounded down (the kept bits even, those
+    behind them 100..0) with probability 2^-(lost + 9); its byte reads the other way.  Rows of
+    two and three keys must not do so more often.  Heads share their values in pairs here, so
+    of N values at most N 2^-(lost + 9) and six deviations, of pairs, are such."""
+    from zeroq_b200.ops import _ext
+
+    lengths = list(range(1, 41))
+    q, k, v, do, cu = inputs(lengths, 0, 4, 2, 64, dtype, cuda)
+    q = torch.zeros_like(q)
+    seqs = PackedSequences(cu, q.shape[0])
+    o, low = torch.empty_like(q), torch.empty(q.shape, dtype=torch.int8, device=cuda)
+    lse = torch.empty(4, q.shape[0], device=cuda)
+    _ext.ext().attn_varlen_fwd(q, k, v, seqs.plan, seqs.n, o, lse, low, True, 0.125)
+    got = (o.float().view(torch.int32) + (low.int() << lost)).view(torch.float32).double()
+    got = torch.where(o == 0, 0.0, got)
+    total, size, a = torch.zeros_like(got), torch.zeros_like(got), 0
+    for n in lengths:
+        r = slice(a, a + n)
+        a += n
+        both = v[r].double().repeat_interleave(2, 1)
+        total[r], size[r] = both.cumsum(0), both.abs().cumsum(0)
+    down = torch.exp(-lse.double()).T[:, :, None]
+    want, size = total * down, size * down
+    off = (got - want).abs()
+    tol = (2.0 ** (lost - 23) + 2.0 ** -20) * want.abs() + 40 * 2.0 ** -23 * size
+    if dtype == torch.float16:   # below the normal range the byte counts 2^-11 of the value
+        tol = tol + torch.where(want.abs() < 2.0 ** -14, 2.0 ** -11 * want.abs() + 2.0 ** -25, 0.0)
+    ties = off.numel() * 2.0 ** -(lost + 9)
+    wrong = off > tol
+    assert wrong.sum() <= ties + 6 * math.sqrt(2 * ties) and (low[wrong] == -128).all()
+    assert ((o.double() - want).abs() > tol).float().mean() > 0.5    # (what the byte is for)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_delta_is_formed_from_them(cuda, dtype):
+    """Two tokens with one key: dS of the second is +d and -d, whose sum is twice what delta
+    is off by, so dQ = 0 unless the two round apart.  Off by 2^-16 of O, at steps of 2^-8 of
+    d, a few rows in a hundred do; from the rounded O half of them would."""
+    q, k, v, do, cu = inputs([2] * 400, 0, 4, 4, 64, dtype, cuda)
+    k = k.clone()
+    k[1::2] = k[::2]
+    leaf = q.detach().requires_grad_()
+    o = flash_attention_varlen(leaf, k, v, cu)
+    dq, = torch.autograd.grad(o, leaf, do)
+    assert (dq[1::2] != 0).any(-1).float().mean() < 0.1
