@@ -162,3 +162,43 @@ def test_gpu_forward_mode_is_refused(cuda, grad):
                      lambda: distillation_loss(dz, *top), lambda: distillation_loss(dz, *top, reduction="none")):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_gpu_gradients_of_rows_stay_within_their_document(cuda, head_dim):
+    """The loss's gradient with respect to the tokens' embeddings: 0 for every row of a
+    document without targets and of the padding, and for the other rows the same to the bit
+    whatever tokens that document holds.  (The weights' gradients are sums over the rows by
+    atomics, in any order.)"""
+    cfg = dict(head_dim=head_dim, d_model=256, n_heads=4, n_kv_heads=2, ffn_dim=512, vocab_size=1000, lora_r=16)
+    m = model(cuda, torch.bfloat16, **cfg)
+    zq.initialize(m, zq.ZeroQConfig(compute_dtype=torch.bfloat16, compute_in_4bit=True, gather_once=True,
+                                    exclude_modules=["lm_head", "embed_tokens"]), trainable_patterns=("lora_", "norm"))
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if "lora_B" in n:
+                p.normal_(0, 0.02, generator=torch.Generator(device=cuda).manual_seed(1))
+    ids, y, cu, teacher = batch(cuda, [130, 77, 300], tail=5, k=8, vocab=1000)
+    y[0, 130:207] = -100
+    leaves = []
+
+    def leaf(module, args, out):
+        leaves.append(out.detach().requires_grad_())
+        return leaves[-1]
+
+    m.embed_tokens.register_forward_hook(leaf)
+
+    def gradient(ids):
+        m.zero_grad()
+        m(ids, y, cu_seqlens=cu, teacher=teacher, temperature=2.0, alpha=0.5).backward()
+        return leaves[-1].grad[0]
+
+    first = gradient(ids)
+    other = ids.clone()
+    other[0, 130:207] = (other[0, 130:207] + 17) % 1000
+    second = gradient(other)
+    for g in (first, second):
+        assert torch.isfinite(g).all() and (g[:130] != 0).any(-1).float().mean() > 0.9
+        assert (g[130:207] == 0).all() and (g[507:] == 0).all()
+    assert torch.equal(first[:130], second[:130]) and torch.equal(first[207:], second[207:])
