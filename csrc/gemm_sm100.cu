@@ -1119,8 +1119,20 @@ DeviceStatus* status_buffer(int device) {
   std::lock_guard<std::mutex> g(mu);
   if (bufs[device] == nullptr) {
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));   // (callers ask before they make it current)
-    C10_CUDA_CHECK(cudaMalloc(&bufs[device], sizeof(DeviceStatus)));
-    C10_CUDA_CHECK(cudaMemset(bufs[device], 0, sizeof(DeviceStatus)));
+    // (a process' first call may be one that is captured: outside of the capture, on a stream
+    // that the capture does not wait for)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaStream_t side = nullptr;
+    DeviceStatus* fresh = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMalloc(&fresh, sizeof(DeviceStatus));
+    if (e == cudaSuccess) e = cudaMemsetAsync(fresh, 0, sizeof(DeviceStatus), side);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(side);
+    if (side != nullptr) cudaStreamDestroy(side);
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    C10_CUDA_CHECK(e);
+    bufs[device] = fresh;
   }
   return bufs[device];
 }

@@ -202,3 +202,38 @@ def test_gpu_gradients_of_rows_stay_within_their_document(cuda, head_dim):
         assert torch.isfinite(g).all() and (g[:130] != 0).any(-1).float().mean() > 0.9
         assert (g[130:207] == 0).all() and (g[507:] == 0).all()
     assert torch.equal(first[:130], second[:130]) and torch.equal(first[207:], second[207:])
+
+
+_FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, {root!r})
+from zeroq_b200.ops import _ext, distillation_loss, flash_attention_varlen, rotary_embedding
+dev = torch.device("cuda", 0)
+q = torch.randn(100, 2, 64, device=dev, dtype=torch.bfloat16)
+cu = torch.tensor([0, 60, 100], dtype=torch.int32, device=dev)
+z, pos = torch.randn(8, 50, device=dev), torch.arange(100, device=dev)
+top = torch.zeros(8, 2, dtype=torch.int64, device=dev), torch.zeros(8, 2, device=dev)
+calls = dict(attention=lambda: flash_attention_varlen(q, q, q, cu), rotary=lambda: rotary_embedding(q, None, pos)[0],
+             distill=lambda: distillation_loss(z, *top))
+call = calls[{name!r}]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = call()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, call()) and _ext.ext().gemm_status(0)[0] == 0
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attention", "rotary", "distill"])
+def test_gpu_first_call_of_a_process_may_be_captured(cuda, name):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", _FIRST_CALL.format(root=root, name=name)], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
