@@ -51,11 +51,15 @@ namespace zq {
 constexpr int kVlRows = 128;
 enum VlErr { kErrVlLoad = 321, kErrVlMma = 322, kErrVlCompute = 323, kErrVlPlan = 324 };
 
-// One tile of a sequence.  slot: number of this 128-row tile over all sequences
-// (row statistics of the backward live in slots of 128 rows).
+// One tile of a sequence.  slot: number of this tile over all sequences.
 struct __align__(16) VlTile {
   int start, len, tile, slot;
 };
+// Where a sequence's row statistics begin in a head's row of them: at its first row and four
+// more for every 128-row tile before it, rounded down to 16 bytes (they are loaded in bulk).
+// A sequence with rows has a tile, so the next one begins behind its last row.
+__device__ __forceinline__ int vl_stats_at(const VlTile& w) { return (w.start + 4 * (w.slot - w.tile)) & ~3; }
+static int64_t vl_stats_row(int64_t T, int64_t tiles) { return (T + 4 * tiles + 64 + 3) / 4 * 4; }   // (a whole load behind the last)
 // meta words: [0] 256-row tiles, [1] 128-row query tiles, [2] 128-row key tiles,
 // [3] first row of a sequence, [4] row behind the last sequence
 constexpr int kVlMeta = 8;
@@ -64,7 +68,7 @@ struct VlParams {
   const VlTile* tiles;
   const int* meta;        // the plan's meta words
   int count_at;           // which of them counts these tiles
-  int T, Hq, Hk, D, causal, slots;
+  int T, Hq, Hk, D, causal, stats_row;
   int split;              // CTAs of a cluster that share a key tile (dK/dV)
   float scale, scale_log2;
   DeviceStatus* status;
@@ -710,7 +714,7 @@ attn_varlen_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 // Tensor memory: S 64 b, dP 128 + 64 b (b = t & 1), dQ 256.., Q 384.., dO 448...
 // A key tile takes about 1400 cycles, of which its MMAs need 970.
 // The kernel also forms delta = rowsum(dO ∘ O) and -lse·log2(e) of its rows and
-// stores them by slots of 128 rows for the dK/dV kernel, which runs after it.
+// stores them for the dK/dV kernel, which runs after it.
 // ============================================================================
 constexpr int kVlMaxSplit = 4;      // CTAs that share a key tile at most (dK/dV)
 constexpr int kVbThreads = 608;     // two groups of eight compute warps, MMA warp, two loader warps
@@ -1061,8 +1065,8 @@ attn_varlen_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       const bool live = w.tile * 128 + row < len;
       const float l2 = lse_row * 1.4426950408889634f;
       const float dl = live ? xs[row] : 0.0f;
-      if (g == 0 && half == 0) {
-        const int64_t at = ((int64_t)h * p.slots + w.slot) * 128 + row;
+      if (g == 0 && half == 0 && live) {
+        const int64_t at = (int64_t)h * p.stats_row + vl_stats_at(w) + w.tile * 128 + row;
         delta[at] = dl;
         nlse2[at] = -l2;
       }
@@ -1191,7 +1195,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   const int i0 = p.causal ? 2 * w.tile : 0;          // first 64-query tile that sees this key tile
   const int per_head = (w.len + 63) / 64 - i0;
   const int n_it = (group * per_head - rank + S - 1) / S;   // this CTA's; 0 where there are fewer tiles than CTAs
-  const int slot0 = w.slot - w.tile;                 // the sequence's first slot
+  const int stats_at = vl_stats_at(w);
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -1232,7 +1236,7 @@ attn_varlen_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         mbar_arrive_expect_tx(&full[st], L::kHalf + (is_q ? 0 : 512));
         vl_load_tile<DP, 64>(ring + st * L::kHalf, map, &full[st], h, w.start + it * 64);
         if (!is_q) {  // this query tile's -lse·log2(e) and delta (256 B each)
-          const int64_t at = ((int64_t)h * p.slots + slot0) * 128 + it * 64;
+          const int64_t at = (int64_t)h * p.stats_row + stats_at + it * 64;
           bulk_load(smem + L::kLD + st * 512, nlse2 + at, 256, &full[st]);
           bulk_load(smem + L::kLD + st * 512 + 256, delta + at, 256, &full[st]);
         }
@@ -1512,7 +1516,7 @@ static VlCall vl_check(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   TORCH_CHECK((c.c128 + 1) * Hq * kVlMaxSplit < (1LL << 31), "attention: grid too large");
   const int* words = plan.data_ptr<int>();
   c.p = VlParams{reinterpret_cast<const VlTile*>(words), words + 4 * (c.c256 + 2 * c.c128), 0, (int)T, (int)Hq, (int)Hk,
-                 (int)D, causal ? 1 : 0, (int)c.c128, 1, (float)scale, (float)(scale * 1.4426950408889634),
+                 (int)D, causal ? 1 : 0, (int)vl_stats_row(T, c.c128), 1, (float)scale, (float)(scale * 1.4426950408889634),
                  status_buffer(q.get_device())};
   c.fp16 = q.scalar_type() == at::kHalf;
   c.narrow = D <= 64;
@@ -1627,7 +1631,7 @@ void attn_varlen_bwd(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v, 
                   lse.numel() == q.size(0) * q.size(1),
               "attention: lse [Hq, T] fp32");
   const c10::cuda::CUDAGuard guard(q.device());
-  auto stats = at::empty({2, q.size(1), c.c128 * 128}, lse.options());
+  auto stats = at::empty({2, q.size(1), c.p.stats_row}, lse.options());
   VlBwd b{vl_tmap(q, 128), vl_tmap(dout, 128), vl_tmap(k, 64), vl_tmap(v, 64), vl_tmap(q, 64), vl_tmap(dout, 64), vl_tmap(k, 128),
           vl_tmap(v, 128), vl_out(o, q), vl_low(low, q), lse.data_ptr<float>(), stats.data_ptr<float>(),
           stats.data_ptr<float>() + stats.numel() / 2, vl_out(dq, q), vl_out(dk, k), vl_out(dv, v)};
