@@ -26,13 +26,15 @@
 // one SM, back to back: N / 2 + 10 cycles with A in tensor memory, N / 2 + 43 with A in
 // shared memory (N = 128: 74 and 107, N = 64: 42 and 75) against N / 2 of arithmetic.
 //
-// Measured (bf16, D = 128, causal; the multiply rate counts the visible pairs):
-//   9 sequences, 8080 rows, 28/4 heads    forward 124 us, dQ 157, dK/dV 205
-//   7 sequences, 6004 rows, 24/24 heads   forward 73 us, dQ 87, dK/dV 122
-//   8191 + 1037 rows, 8/2 heads           forward 127 us (1.1 PFLOP/s), dQ 181, dK/dV 267
+// Measured (bf16, D = 128, causal, inputs not in L2; the multiply rate counts the visible pairs):
+//   9 sequences, 8080 rows, 28/4 heads    forward 127 us, dQ 161, dK/dV 207
+//   7 sequences, 6004 rows, 24/24 heads   forward 77 us, dQ 89, dK/dV 123
+//   8191 + 1037 rows, 8/2 heads           forward 130 us (1.1 PFLOP/s), dQ 192, dK/dV 268
+// and fp16, D = 64, bidirectional, 8 sequences, 2393 rows, 12/12 heads: 18.5, 22, 32.6.
 // Short sequences are bound by what a block does around its loop (launch, first loads,
-// pipeline fill, output: 7-8 us of a block's 15-20 us, with one block to an SM, which
-// tensor and shared memory allow; dQ runs part of it under the block before), long ones by the chain of MMAs and exponentials.
+// pipeline fill, output: 7-8 us of a block's 15-20 us, with one block to an SM by its
+// registers and tensor memory; dQ runs part of it under the block before), long ones by
+// the chain of MMAs and exponentials.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -28,11 +28,11 @@
 // What bounds it: memory, next to the special-function unit's 16 exponentials a cycle
 // and SM: two a logit at τ = 1 (0.57 ms of 8192 x 152064 against 0.76 ms of memory).  At
 // τ = 2 and 4 the hard softmax's exponential is the soft one's square or fourth power;
-// other τ take four a logit and are bound by them.  Measured with a fifth of the rows not
-// counted: 8192 x 152064 bf16 890 us (5.6 TB/s of logits and gradient, 0.86 of a copy),
-// 4096 x 50257 at τ = 2 194 us (0.65; a row's joins, about 4000 cycles next to 8000 of its
-// passes, are what is left).  One block a row that read it twice, the second time from L2,
-// took 1130 and 350 us.
+// other τ take four a logit.  Measured with a fifth of the rows not counted, which are not
+// read (so 0.9 of the bytes of all logits and gradients move): 8192 x 152064 bf16 870 us,
+// 5.2 TB/s, 0.79 of a copy; 4096 x 50257 at τ = 2 178 us, 4.2 TB/s, 0.64 (a row's joins,
+// about 4000 cycles next to 8000 of its passes, are what is left), at τ = 1.5 250 us.  One
+// block a row that read it twice, the second time from L2, took 1130 and 350 us.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

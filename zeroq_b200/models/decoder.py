@@ -377,7 +377,9 @@ class DecoderLM(nn.Module):
         positions and sees itself alone, rows behind the last one are padding (give them
         ``ignore_index`` as target).  ``teacher``: ``(ids, logits)``, each ``[B, S, K]`` or
         ``[B * S, K]``, a teacher's top entries for every row; the loss is then
-        :func:`~zeroq_b200.ops.distill.distillation_loss` with ``temperature`` and ``alpha``."""
+        :func:`~zeroq_b200.ops.distill.distillation_loss` with ``temperature`` and ``alpha``,
+        over whole logits and with a gradient of their size beside them (``ce_chunk`` holds for
+        the hard targets alone)."""
         B, S = input_ids.shape
         seqs = None
         if cu_seqlens is not None:

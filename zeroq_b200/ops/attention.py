@@ -162,7 +162,9 @@ def flash_attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``cu_seqlens`` (then its tables are built for this call).  ``causal``: a row sees its
     sequence's rows up to itself, otherwise all of them.  ``scale`` (positive) defaults
     to ``1/sqrt(D)``.  Rows of no sequence get an output and gradients of zero, whatever
-    they hold.  P and dS are rounded to the inputs' type before their products;
+    they hold, and another sequence's rows do not enter.  Within a sequence a key behind the
+    mask weighs 0 (which times an infinite or NaN value is NaN, as in any product of P and V).
+    P and dS are rounded to the inputs' type before their products;
     scores, softmax statistics and accumulators are in 32 bits."""
     qs, ks, dtype, device = tuple(q.shape), tuple(k.shape), q.dtype, q.device
     if len(qs) != 3 or len(ks) != 3 or tuple(v.shape) != ks or ks[0] != qs[0] or ks[2] != qs[2]:

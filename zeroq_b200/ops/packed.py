@@ -25,7 +25,9 @@ class PackedSequences:
     at 0, does not fall and ends within ``total``) and copied to ``device``; on the GPU
     it is not read by the host - values out of order are clamped by the kernel, and the
     result for such a division is undefined.  The tables are those of the values that it
-    had here: make another one for another division."""
+    had here: make another one for another division.  A fixed ``n`` with empty sequences
+    at the end is fine (a graph's static ``cu_seqlens``); each costs 60 bytes of tables, a few
+    rows' worth of the attention backward's statistics and empty blocks in its launches."""
 
     def __init__(self, cu_seqlens: torch.Tensor, total: int, device: Optional[torch.device] = None):
         if not isinstance(cu_seqlens, torch.Tensor) or not hasattr(total, "__index__"):
