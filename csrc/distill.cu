@@ -761,20 +761,34 @@ __global__ void __launch_bounds__(kDistFinish) distill_finish_kernel(const __gri
     const float m = p.sums[3 * row];
     return (m != -INFINITY) & (fabsf(m) * fast > 67108864.0f);
   };
-  const float* rows = loss != nullptr ? p.rows : p.sums;   // (any readable floats)
+  auto counted = [&](int64_t row) {
+    const int64_t y = p.targets != nullptr ? p.targets[row] : 0;
+    return ((y >= 0) & (y < p.vocab)) ? 1 : 0;
+  };
   double s = 0.0;
   int n = 0;
   bool some_far = false;
+  if (loss != nullptr) {
 #pragma unroll 4
-  for (int64_t i = tid; i < p.M; i += kDistFinish) {   // (nothing here waits for a load before the next one)
-    s += rows[i];
-    const int64_t y = p.targets != nullptr ? p.targets[i] : 0;
-    n += ((y >= 0) & (y < p.vocab)) ? 1 : 0;
-    some_far |= far(i);
+    for (int64_t i = tid; i < p.M; i += kDistFinish) {   // (nothing here waits for a load before the next one)
+      s += p.rows[i];
+      n += counted(i);
+      some_far |= far(i);
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0) s_n[warp] = n;
+  } else {
+#pragma unroll 1
+    for (int64_t i = blockIdx.x + (int64_t)tid * gridDim.x; i < p.M; i += (int64_t)gridDim.x * kDistFinish) some_far |= far(i);
   }
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((tid & 31) == 0) s_n[warp] = n;
   if (__syncthreads_or(some_far)) {
+    if (loss == nullptr) {   // (wanted by the gradient of a mean alone)
+#pragma unroll 1
+      for (int64_t i = tid; p.g_mean && i < p.M; i += kDistFinish) n += counted(i);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if ((tid & 31) == 0) s_n[warp] = n;
+      __syncthreads();
+    }
     n = 0;
     for (int w = 0; w < 32; ++w) n += s_n[w];
     const float inv_n = 1.0f / fmaxf((float)n, 1.0f);
