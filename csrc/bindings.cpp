@@ -124,6 +124,17 @@ void plan_gather_dequant(std::vector<int64_t> psrc, std::vector<int64_t> pstarts
                          int64_t cols, int64_t row0, int64_t blocksize, int64_t qtype, bool transpose,
                          at::Tensor out);
 
+// row_autograd.cpp (embedding.cu, layernorm.cu, act8.cu, logprobs.cu)
+at::Tensor embedding_lookup(at::Tensor ids, at::Tensor w, double scale);
+std::vector<at::Tensor> layer_norm(at::Tensor x, c10::optional<at::Tensor> delta, c10::optional<at::Tensor> w,
+                                   c10::optional<at::Tensor> b, double eps, bool keep8);
+std::vector<at::Tensor> act8_quantize(at::Tensor x);
+at::Tensor act8_dequantize(at::Tensor codes, at::Tensor steps, std::vector<int64_t> shape, at::ScalarType dtype);
+at::Tensor gelu8(at::Tensor x);
+at::Tensor swiglu8(at::Tensor gate, at::Tensor up);
+std::vector<at::Tensor> token_logprobs(at::Tensor z, c10::optional<at::Tensor> targets, int64_t K, int64_t vocab,
+                                       double temperature);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "zeroq_b200 sm_100a kernels";
   m.def("nf4_quantize", &nf4_quantize);
@@ -174,6 +185,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_varlen", &attn_varlen);
   m.def("attn_varlen_cu", &attn_varlen_cu);
   m.def("distill_loss", &distill_loss);
+  m.def("embedding_lookup", &embedding_lookup, "scaled table rows; gradient by sorted tokens");
+  m.def("layer_norm", &layer_norm, "(h, y) of a residual addition and layer norm, or (y)");
+  m.def("act8_quantize", &act8_quantize, "(codes, steps) of rows in groups of 128 columns");
+  m.def("act8_dequantize", &act8_dequantize);
+  m.def("gelu8", &gelu8, "GELU whose input is kept in 8 bits");
+  m.def("swiglu8", &swiglu8, "SwiGLU whose inputs are kept in 8 bits");
+  m.def("token_logprobs", &token_logprobs);
   m.def("gelu_fwd", &gelu_fwd);
   m.def("gelu_bwd", &gelu_bwd);
   m.def("gelu_cdf_pdf", &gelu_cdf_pdf);

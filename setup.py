@@ -11,7 +11,8 @@ from setuptools import setup
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
-SOURCES = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/bindings.cpp", "csrc/packed_autograd.cpp"]
+SOURCES = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/bindings.cpp", "csrc/packed_autograd.cpp",
+                                                           "csrc/row_autograd.cpp"]
 DEFINES = []
 
 NVCC_FLAGS = [
