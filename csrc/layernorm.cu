@@ -7,9 +7,9 @@
 //   dx = r (a - mean a - n mean(a n)) (+ dh);  dw = sum over rows dy n;  db = sum over rows dy
 //
 // A team of W warps takes one row at a time and holds it in registers, K tiles of 256 columns
-// a warp, with w (and b, and the sums of dw and db) of the same columns beside it; teams go
-// over the rows with a fixed stride, and the loads of the next row are under way while this
-// one is reduced.  The variance is the joined sum of squares about each warp's own mean
+// a warp (the backward with its sums of dw and db beside it; w and b are in shared memory);
+// teams go over the rows with a fixed stride, and the loads of the next row are under way while
+// this one is reduced.  The variance is the joined sum of squares about each warp's own mean
 // (columns n_i, mean m_i, squares q_i: q = sum q_i + n_i (m_i - mu)^2), so one exchange gives
 // both and nothing cancels.  dw and db: a block's teams add up in team order in shared memory,
 // the blocks' rows of partial sums are added in block order by a second kernel: no atomics.
@@ -29,7 +29,7 @@ constexpr int kLnMaxWarps = 16;   // of a team
 constexpr int kLnMaxTeams = 8;    // of a block
 
 struct LnParams {
-  const void *x, *delta, *dy, *dh;   // rows of pitch xs, deltas, dys, dhs
+  const void *x, *delta, *dy, *dh;   // rows of pitch xs, ds, dys, dhs
   int64_t xs, ds, dys, dhs;
   void *h, *y, *dx;                  // dense
   const void *w, *b;                 // type wt: 0 fp32, 1 bf16, 2 fp16
@@ -39,6 +39,7 @@ struct LnParams {
   float* part;                       // [grid, 2, D]
   int64_t M, P, G;
   int D, wt, W, R;                   // warps of a team, teams of a block
+  int slots, slots_at;               // rows under way in shared memory, where they begin
   float eps;
 };
 
@@ -48,20 +49,47 @@ __device__ __forceinline__ float ln_param(const void* p, int type, int i) {
   return reinterpret_cast<const float*>(p)[i];
 }
 
-template <bool VEC, int K>
-__device__ __forceinline__ void ln_params(const void* p, int type, float absent, int wt, int W, int lane, int D,
-                                          float (&v)[K][8]) {
+// w or b in shared memory, in 32 bits and in the lanes' order (a lane's 8 columns of a tile in
+// two runs of 4, so that a warp's 16-byte reads fall on different banks)
+template <bool VEC>
+__device__ __forceinline__ int ln_place(int c) {   // of column c
+  const int i = c & (kTile - 1);
+  return VEC ? (c - i) + ((i >> 2) & 1) * 128 + (i >> 3) * 4 + (i & 3) : c;
+}
+template <bool VEC>
+__device__ __forceinline__ void ln_stage(float* s, const void* p, int type, float absent, int D) {
+  const int whole = (D + kTile - 1) / kTile * kTile;
+  for (int c = threadIdx.x; c < whole; c += blockDim.x)
+    s[ln_place<VEC>(c)] = c >= D ? 0.0f : p == nullptr ? absent : ln_param(p, type, c);
+}
+template <bool VEC>
+__device__ __forceinline__ void ln_staged(const float* s, int base, int lane, uint64_t (&v)[4]) {
+  if constexpr (VEC) {
+    const float4 a = *reinterpret_cast<const float4*>(s + base + lane * 4);
+    const float4 b = *reinterpret_cast<const float4*>(s + base + 128 + lane * 4);
+    v[0] = f2_pack(a.x, a.y), v[1] = f2_pack(a.z, a.w), v[2] = f2_pack(b.x, b.y), v[3] = f2_pack(b.z, b.w);
+  } else {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = (wt + k * W) * kTile + tile_col<VEC>(lane, i);
-      v[k][i] = c >= D ? 0.0f : p == nullptr ? absent : ln_param(p, type, c);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = f2_pack(s[base + 64 * i + lane], s[base + 64 * i + 32 + lane]);
   }
 }
 
-// Every warp's pair of numbers, in every thread of the team.  Buffers alternate from row to
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+// A lane's mask of values that are columns of the row.
+template <bool VEC>
+__device__ __forceinline__ uint32_t ln_mask(int base, int lane, int D) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m |= (base + tile_col<VEC>(lane, i) < D ? 1u : 0u) << i;
+  return m;
+}
+
+// Every warp's pair of numbers, for every thread of the team.  Buffers alternate from row to
 // row: a thread that writes one again has passed the other's barrier, to which its readers
 // came after they had read.
 __device__ __forceinline__ void ln_exchange(float2 (&buf)[kLnMaxWarps], float2 mine, int wt, int lane, int team, int W) {
@@ -69,18 +97,14 @@ __device__ __forceinline__ void ln_exchange(float2 (&buf)[kLnMaxWarps], float2 m
   named_barrier(1 + team, W * 32);
 }
 
-template <typename T, bool VEC, int K, bool RES>
+template <typename T, bool VEC, int K, bool RES, bool KEEP>
 __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_constant__ LnParams p) {
   __shared__ float2 s_red[kLnMaxTeams][2][kLnMaxWarps];
+  __shared__ float s_cols[kLnMaxWarps];   // columns of a team's warps
+  extern __shared__ __align__(16) float s_wb[];   // w and b
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D;
-  float w[K][8], b[K][8];
-  ln_params<VEC, K>(p.w, p.wt, 1.0f, wt, W, lane, D, w);
-  ln_params<VEC, K>(p.b, p.wt, 0.0f, wt, W, lane, D, b);
-  float cols = 0.0f;   // of this warp
-#pragma unroll
-  for (int k = 0; k < K; ++k) cols += (float)max(0, min(kTile, D - (wt + k * W) * kTile));
-  const float inv_cols = cols > 0.0f ? 1.0f / cols : 0.0f, inv_d = 1.0f / (float)D;
+  const int whole = (D + kTile - 1) / kTile * kTile;
 
   const int64_t step = (int64_t)gridDim.x * p.R;
   RawTile<T, VEC> rx[K], rd[RES ? K : 1];
@@ -96,167 +120,326 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   };
   int64_t row = (int64_t)blockIdx.x * p.R + team;
   if (row < p.M) load(row);
+  ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
+  ln_stage<VEC>(s_wb + whole, p.b, p.wt, 0.0f, D);
+  float cols = 0.0f;   // of this warp
+#pragma unroll
+  for (int k = 0; k < K; ++k) cols += (float)max(0, min(kTile, D - (wt + k * W) * kTile));
+  const float inv_cols = cols > 0.0f ? 1.0f / cols : 0.0f, inv_d = 1.0f / (float)D;
+  if (team == 0 && lane == 0) s_cols[wt] = cols;
+  __syncthreads();
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
-    float v[K][8];
+    uint64_t v[K][4];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      rx[k].values(v[k]);
+      const int base = (wt + k * W) * kTile;
+      rx[k].pairs(v[k]);
       if constexpr (RES) {
-        float d[8];
-        rd[k].values(d);
+        uint64_t d[4];
+        rd[k].pairs(d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] += d[i];
+        for (int i = 0; i < 4; ++i) v[k][i] = f2_add(v[k][i], d[i]);
         RawTile<T, VEC> h;
         h.set(v[k]);
-        h.store(reinterpret_cast<T*>(p.h) + row * D, (wt + k * W) * kTile, lane, D);
-        h.values(v[k]);   // as the next layer and the backward see it
+        h.store(reinterpret_cast<T*>(p.h) + row * D, base, lane, D);
+        h.pairs(v[k]);   // as the next layer and the backward see it
       }
     }
     if (row + step < p.M) load(row + step);
-    float s = 0.0f;
+    uint64_t s = 0ull;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[k][i];
-    float mu = warp_sum(s) * inv_cols;
+      for (int i = 0; i < 4; ++i) s = f2_add(s, v[k][i]);
+    float mu = warp_sum(f2_sum(s)) * inv_cols;
     float q = 0.0f;
+    {
+      const uint64_t away = f2_pack(-mu, -mu);
+      uint64_t q2 = 0ull;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k) {
+        const int base = (wt + k * W) * kTile;
+        if (base + kTile <= D) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[k][i] - mu;
-        if ((wt + k * W) * kTile + tile_col<VEC>(lane, i) < D) q = fmaf(d, d, q);
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t d = f2_add(v[k][i], away);
+            q2 = f2_fma(d, d, q2);
+          }
+        } else {   // the row ends in this tile
+          const uint32_t mask = ln_mask<VEC>(base, lane, D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a, b;
+            f2_unpack(f2_add(v[k][i], away), a, b);
+            if (mask >> (2 * i) & 1u) q = fmaf(a, a, q);
+            if (mask >> (2 * i + 1) & 1u) q = fmaf(b, b, q);
+          }
+        }
       }
-    q = warp_sum(q);
+      q = warp_sum(q + f2_sum(q2));
+    }
     if (W > 1) {
       float2(&buf)[kLnMaxWarps] = s_red[team][turn];
       ln_exchange(buf, make_float2(mu, q), wt, lane, team, W);
-      // columns of a warp: as above
       float m = 0.0f;
-      auto columns = [&](int i) {
-        float n = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) n += (float)max(0, min(kTile, D - (i + k * W) * kTile));
-        return n;
-      };
-      for (int i = 0; i < W; ++i) m = fmaf(columns(i), buf[i].x, m);
+      for (int i = 0; i < W; ++i) m = fmaf(s_cols[i], buf[i].x, m);
       m *= inv_d;
       q = 0.0f;
       for (int i = 0; i < W; ++i) {
         const float d = buf[i].x - m;
-        q += buf[i].y + columns(i) * d * d;
+        q += fmaf(s_cols[i] * d, d, buf[i].y);
       }
       mu = m;
     }
     const float r = 1.0f / sqrtf(q * inv_d + p.eps);
     if (wt == 0 && lane == 0 && p.mean != nullptr) p.mean[row] = mu, p.rstd[row] = r;
+    const uint64_t away = f2_pack(-mu, -mu), r2 = f2_pack(r, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
-      if (p.codes != nullptr && base < D) keep_tile<VEC>(v[k], p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
+      if (base >= D) continue;
+      if constexpr (KEEP) {
+        float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = fmaf((v[k][i] - mu) * r, w[k][i], b[k][i]);
-      store_tile<T, VEC>(reinterpret_cast<T*>(p.y) + row * D, base, lane, D, v[k]);
+        for (int i = 0; i < 4; ++i) f2_unpack(v[k][i], f[2 * i], f[2 * i + 1]);
+        keep_tile<VEC>(f, p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
+      }
+      uint64_t w[4], b[4];
+      ln_staged<VEC>(s_wb, base, lane, w);
+      ln_staged<VEC>(s_wb + whole, base, lane, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[k][i] = f2_fma(f2_mul(f2_add(v[k][i], away), r2), w[i], b[i]);
+      RawTile<T, VEC> y;
+      y.set(v[k]);
+      y.store(reinterpret_cast<T*>(p.y) + row * D, base, lane, D);
     }
   }
 }
 
+// The backward's rows on their way: every thread copies its own columns into its own places of
+// shared memory, S rows ahead, and reads them back itself (twice: for the row's sums, and for
+// dx once they are known), so no barrier belongs to it and nothing is held in registers.  Rows
+// that cannot be copied that way (PIPE false: not on 16-byte boundaries, or too wide) are read
+// where they are.
+template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE>
+struct LnRows {
+  static constexpr int kVecs = (int)sizeof(T) / 2;   // 16-byte vectors of a lane's 8 elements
+  static constexpr int kSlot = K * (16 * kVecs * (1 + (KEPT ? 0 : 1) + (RES ? 1 : 0)) + (KEPT ? 12 : 0));   // bytes a thread
+
+  RawTile<T, VEC> g[PIPE ? 1 : K], x[PIPE || KEPT ? 1 : K], h[PIPE || !RES ? 1 : K];
+  RawCodes<VEC> c[PIPE || !KEPT ? 1 : K];
+
+  static __device__ __forceinline__ void copy(void* to, const void* from, int bytes, bool there) {
+    const uint32_t n = there ? bytes : 0;   // (0: zeros)
+    if (bytes == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
+    else if (bytes == 8)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
+  }
+  // places of a slot: [stream][tile][vector][thread] of 16 bytes, then codes (8) and steps (4)
+  static __device__ __forceinline__ uint8_t* place(uint8_t* slot, int stream, int k, int v) {
+    return slot + (((stream * K + k) * kVecs + v) * (int)blockDim.x + (int)threadIdx.x) * 16;
+  }
+  static __device__ __forceinline__ uint8_t* place_codes(uint8_t* slot, int k) {
+    return slot + ((1 + (RES ? 1 : 0)) * K * kVecs * 16 + k * 8) * (int)blockDim.x + threadIdx.x * 8;
+  }
+  static __device__ __forceinline__ uint8_t* place_step(uint8_t* slot, int k) {
+    return slot + ((1 + (RES ? 1 : 0)) * K * kVecs * 16 + K * 8 + k * 4) * (int)blockDim.x + threadIdx.x * 4;
+  }
+  // streams of 16-byte vectors: dy, then dh, then the input
+  static constexpr int kH = 1, kX = RES ? 2 : 1;
+
+  static __device__ __forceinline__ void fetch(const LnParams& p, uint8_t* slot, int64_t row, int wt, int lane) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int at = (wt + k * p.W) * kTile + lane * 8;
+      const bool there = at < p.D;
+      const int from = there ? at : 0;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int e = from + v * (16 / (int)sizeof(T));
+        copy(place(slot, 0, k, v), reinterpret_cast<const T*>(p.dy) + row * p.dys + e, 16, there);
+        if constexpr (RES) copy(place(slot, kH, k, v), reinterpret_cast<const T*>(p.dh) + row * p.dhs + e, 16, there);
+        if constexpr (!KEPT) copy(place(slot, kX, k, v), reinterpret_cast<const T*>(p.x) + row * p.xs + e, 16, there);
+      }
+      if constexpr (KEPT) {
+        copy(place_codes(slot, k), p.codes + row * p.P + from, 8, there);
+        copy(place_step(slot, k), p.steps + row * p.G + from / kGroup, 4, there);
+      }
+    }
+  }
+  __device__ __forceinline__ void read(const LnParams& p, int64_t row, int wt, int lane) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int base = (wt + k * p.W) * kTile;
+      g[k].load(reinterpret_cast<const T*>(p.dy) + row * p.dys, base, lane, p.D);
+      if constexpr (KEPT) c[k].load(p.codes + row * p.P, p.steps + row * p.G, base, lane, p.D);
+      else x[k].load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, p.D);
+      if constexpr (RES) h[k].load(reinterpret_cast<const T*>(p.dh) + row * p.dhs, base, lane, p.D);
+    }
+  }
+  static __device__ __forceinline__ void from_slot(const uint8_t* slot, int stream, int k, uint64_t (&v)[4]) {
+    RawTile<T, VEC> t;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(place(const_cast<uint8_t*>(slot), stream, k, i));
+      t.w[4 * i] = u.x, t.w[4 * i + 1] = u.y, t.w[4 * i + 2] = u.z, t.w[4 * i + 3] = u.w;
+    }
+    t.pairs(v);
+  }
+  __device__ __forceinline__ void dy(const uint8_t* slot, int k, uint64_t (&v)[4]) const {
+    if constexpr (PIPE) from_slot(slot, 0, k, v);
+    else g[k].pairs(v);
+  }
+  __device__ __forceinline__ void dh(const uint8_t* slot, int k, uint64_t (&v)[4]) const {
+    if constexpr (PIPE) from_slot(slot, kH, k, v);
+    else h[k].pairs(v);
+  }
+  __device__ __forceinline__ void centred(const uint8_t* slot, int k, float mu, uint64_t (&v)[4]) const {   // h - mu
+    const uint64_t away = f2_pack(-mu, -mu);
+    if constexpr (KEPT) {
+      RawCodes<VEC> q;
+      if constexpr (PIPE) {
+        q.w = *reinterpret_cast<const uint2*>(place_codes(const_cast<uint8_t*>(slot), k));
+        q.step[0] = *reinterpret_cast<const float*>(place_step(const_cast<uint8_t*>(slot), k));
+      } else {
+        q = c[k];
+      }
+      float f[8];
+      q.values(f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+    } else if constexpr (PIPE) {
+      from_slot(slot, kX, k, v);
+    } else {
+      x[k].pairs(v);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f2_add(v[i], away);
+  }
+};
+
 // KEPT: h in 8 bits; RES: dh is added
-template <typename T, bool VEC, int K, bool KEPT, bool RES>
-__global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_constant__ LnParams p) {
+template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bwd_kernel(const __grid_constant__ LnParams p) {
+  using Rows = LnRows<T, VEC, K, KEPT, RES, PIPE>;
   __shared__ float2 s_red[kLnMaxTeams][2][kLnMaxWarps];
-  extern __shared__ float s_part[];   // [2, D], teams add up
+  extern __shared__ __align__(16) float s_wb[];   // w, at the end [2, D]: teams add up; the slots
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D;
-  float w[K][8], dw[K][8], db[K][8];
-  ln_params<VEC, K>(p.w, p.wt, 1.0f, wt, W, lane, D, w);
+  const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D, S = p.slots;
+  const int64_t step = (int64_t)gridDim.x * p.R;
+  int64_t row = (int64_t)blockIdx.x * p.R + team;
+  uint8_t* slots = reinterpret_cast<uint8_t*>(s_wb) + p.slots_at;
+  const int slot_bytes = Rows::kSlot * (int)blockDim.x;
+  float mu_next = 0.0f, r_next = 0.0f;
+  if (row < p.M) mu_next = p.mean[row], r_next = p.rstd[row];
+  if constexpr (PIPE) {
+    for (int i = 0; i < S; ++i) {
+      if (row + i * step < p.M) Rows::fetch(p, slots + i * slot_bytes, row + i * step, wt, lane);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
+  uint64_t dw[K][4], db[K][4];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[k][i] = db[k][i] = 0.0f;
+    for (int i = 0; i < 4; ++i) dw[k][i] = db[k][i] = 0ull;
   const float inv_d = 1.0f / (float)D;
+  __syncthreads();
 
-  const int64_t step = (int64_t)gridDim.x * p.R;
-  RawTile<T, VEC> rg[K], rx[KEPT ? 1 : K], rh[RES ? K : 1];
-  RawCodes<VEC> rc[KEPT ? K : 1];
-  float mu_next = 0.0f, r_next = 0.0f;
-  auto load = [&](int64_t row) {
-    const T* g = reinterpret_cast<const T*>(p.dy) + row * p.dys;
+  int at = 0;   // the row's slot
+  for (int turn = 0; row < p.M; row += step, turn ^= 1) {
+    const float mu = mu_next, r = r_next;
+    if (row + step < p.M) mu_next = p.mean[row + step], r_next = p.rstd[row + step];
+    uint8_t* slot = slots + at * slot_bytes;
+    Rows t;
+    if constexpr (PIPE) {   // all but the S - 1 rows behind this one
+      if (S == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (S == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    } else {
+      t.read(p, row, wt, lane);
+    }
+    const uint64_t r2 = f2_pack(r, r);
+    uint64_t t1 = 0ull, t2 = 0ull;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
-      rg[k].load(g, base, lane, D);
-      if constexpr (KEPT) rc[k].load(p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
-      else rx[k].load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
-      if constexpr (RES) rh[k].load(reinterpret_cast<const T*>(p.dh) + row * p.dhs, base, lane, D);
-    }
-    mu_next = p.mean[row];
-    r_next = p.rstd[row];
-  };
-  int64_t row = (int64_t)blockIdx.x * p.R + team;
-  if (row < p.M) load(row);
-  for (int turn = 0; row < p.M; row += step, turn ^= 1) {
-    const float mu = mu_next, r = r_next;
-    float a[K][8], n[K][8];
-    RawTile<T, VEC> h[RES ? K : 1];
-    float s1 = 0.0f, s2 = 0.0f;
+      if (base >= D) continue;
+      uint64_t g[4], n[4], w[4];
+      t.dy(slot, k, g);
+      t.centred(slot, k, mu, n);
+      ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      rg[k].values(a[k]);
-      if constexpr (KEPT) rc[k].values(n[k]);
-      else rx[k].values(n[k]);
-      if constexpr (RES) h[k] = rh[k];
-    }
-    if (row + step < p.M) load(row + step);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {   // (past the row's end dy and w are 0)
-        n[k][i] = (n[k][i] - mu) * r;
-        dw[k][i] = fmaf(a[k][i], n[k][i], dw[k][i]);
-        db[k][i] += a[k][i];
-        a[k][i] *= w[k][i];
-        s1 += a[k][i];
-        s2 = fmaf(a[k][i], n[k][i], s2);
+      for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
+        n[i] = f2_mul(n[i], r2);
+        dw[k][i] = f2_fma(g[i], n[i], dw[k][i]);
+        db[k][i] = f2_add(db[k][i], g[i]);
+        g[i] = f2_mul(g[i], w[i]);
+        t1 = f2_add(t1, g[i]);
+        t2 = f2_fma(g[i], n[i], t2);
       }
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
+    float s1 = warp_sum(f2_sum(t1)), s2 = warp_sum(f2_sum(t2));
     if (W > 1) {
       float2(&buf)[kLnMaxWarps] = s_red[team][turn];
       ln_exchange(buf, make_float2(s1, s2), wt, lane, team, W);
       s1 = s2 = 0.0f;
       for (int i = 0; i < W; ++i) s1 += buf[i].x, s2 += buf[i].y;
+    } else {
+      __syncwarp();
     }
-    s1 *= inv_d;
-    s2 *= inv_d;
+    // dx = r a - r mean a - (h - mu) r^2 mean(a n)
+    const float c0 = -r * (s1 * inv_d), c1 = -r * r * (s2 * inv_d);
+    const uint64_t c02 = f2_pack(c0, c0), c12 = f2_pack(c1, c1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float add[8];
-      if constexpr (RES) h[k].values(add);
+      const int base = (wt + k * W) * kTile;
+      if (base >= D) continue;
+      uint64_t g[4], d[4], w[4];
+      t.dy(slot, k, g);
+      t.centred(slot, k, mu, d);
+      ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = r * (a[k][i] - s1 - n[k][i] * s2);
-        a[k][i] = RES ? d + add[i] : d;
+      for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(d[i], c12, c02));
+      if constexpr (RES) {
+        uint64_t h[4];
+        t.dh(slot, k, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = f2_add(g[i], h[i]);
       }
-      store_tile<T, VEC>(reinterpret_cast<T*>(p.dx) + row * D, (wt + k * W) * kTile, lane, D, a[k]);
+      RawTile<T, VEC> o;
+      o.set(g);
+      o.store(reinterpret_cast<T*>(p.dx) + row * D, base, lane, D);
+    }
+    if constexpr (PIPE) {   // the slot is read: the row S behind this one
+      if (row + S * step < p.M) Rows::fetch(p, slot, row + S * step, wt, lane);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      at = at + 1 == S ? 0 : at + 1;
     }
   }
   if (p.part == nullptr) return;
   float* out = p.part + (int64_t)blockIdx.x * 2 * D;
-  for (int t = 0; t < p.R; ++t) {
-    if (t > 0) __syncthreads();
-    if (team != t) continue;
+  for (int j = 0; j < p.R; ++j) {
+    __syncthreads();
+    if (team != j) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int c = (wt + k * W) * kTile + tile_col<VEC>(lane, i);
         if (c < D) {
-          const float u = t > 0 ? s_part[c] + dw[k][i] : dw[k][i];
-          const float v = t > 0 ? s_part[D + c] + db[k][i] : db[k][i];
-          if (t == p.R - 1) out[c] = u, out[D + c] = v;
-          else s_part[c] = u, s_part[D + c] = v;
+          float a, b, u, v;
+          f2_unpack(dw[k][i / 2], a, b);
+          u = i & 1 ? b : a;
+          f2_unpack(db[k][i / 2], a, b);
+          v = i & 1 ? b : a;
+          if (j > 0) u += s_wb[c], v += s_wb[D + c];
+          if (j == p.R - 1) out[c] = u, out[D + c] = v;
+          else s_wb[c] = u, s_wb[D + c] = v;
         }
       }
     }
@@ -366,6 +549,7 @@ int ln_shape(LnParams& p) {
 template <typename F>
 unsigned ln_grid(F kern, const LnParams& p, size_t smem) {
   int n = 0;
+  if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, p.W * p.R * 32, smem));
   TORCH_CHECK(n > 0, "layer_norm: a block does not fit the device");
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
@@ -384,12 +568,19 @@ unsigned ln_grid(F kern, const LnParams& p, size_t smem) {
 
 template <typename T, bool VEC, int K>
 static void ln_fwd_launch(const LnParams& p, cudaStream_t stream) {
+  const size_t smem = (size_t)2 * ((p.D + kTile - 1) / kTile * kTile) * 4;
   auto go = [&](auto kern) {
-    kern<<<ln_grid(kern, p, 0), p.W * p.R * 32, 0, stream>>>(p);
+    const unsigned grid = ln_grid(kern, p, smem);
+    kern<<<grid, p.W * p.R * 32, smem, stream>>>(p);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   };
-  if (p.delta != nullptr) go(ln_fwd_kernel<T, VEC, K, true>);
-  else go(ln_fwd_kernel<T, VEC, K, false>);
+  if (p.codes != nullptr) {
+    if (p.delta != nullptr) go(ln_fwd_kernel<T, VEC, K, true, true>);
+    else go(ln_fwd_kernel<T, VEC, K, false, true>);
+  } else {
+    if (p.delta != nullptr) go(ln_fwd_kernel<T, VEC, K, true, false>);
+    else go(ln_fwd_kernel<T, VEC, K, false, false>);
+  }
 }
 
 // h and y [M, D]; stats [2, M] (mean, 1 / deviation), codes and steps where a backward follows
@@ -436,8 +627,9 @@ template <typename T, bool VEC, int K>
 static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::Tensor>& dw, c10::optional<at::Tensor>& db,
                           cudaStream_t stream) {
   const bool sums = dw.has_value() || db.has_value();
-  const size_t smem = sums && p.R > 1 ? (size_t)2 * p.D * 4 : 0;
-  auto go = [&](auto kern) {
+  // w; [2, D] where several teams' sums are added
+  const size_t row = (size_t)((p.D + kTile - 1) / kTile * kTile) * 4, front = sums && p.R > 1 ? 2 * row : row;
+  auto go = [&](auto kern, size_t smem) {
     const unsigned grid = ln_grid(kern, p, smem);
     at::Tensor part;
     if (sums) {
@@ -460,12 +652,32 @@ static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::T
     else if (type == at::kBFloat16) finish(__nv_bfloat16{});
     else finish(__half{});
   };
+  auto shape = [&](auto kept, auto res) {
+    constexpr bool KEPT = decltype(kept)::value, RES = decltype(res)::value;
+    if constexpr (VEC) {
+      // Rows under way: as many of 2 to 4 as leave two blocks to an SM, or one where that
+      // takes the most of them.
+      const size_t slot = (size_t)LnRows<T, VEC, K, KEPT, RES, true>::kSlot * p.W * p.R * 32;
+      constexpr size_t most = 227 * 1024 - 4096, half = 113 * 1024 - 4096;   // (static arrays and 1 KB a block)
+      const size_t room = front + 2 * slot <= half ? half : most;
+      p.slots = (int)std::min<size_t>(4, front < room ? (room - front) / slot : 0);
+      p.slots_at = (int)front;
+      if (p.slots >= 2) {
+        // (up to 10 warps the registers leave two blocks to an SM)
+        if (K <= 2 && p.W * p.R <= 10) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, K <= 2 ? 10 : kLnMaxWarps>, front + p.slots * slot);
+        return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, kLnMaxWarps>, front + p.slots * slot);
+      }
+    }
+    go(ln_bwd_kernel<T, VEC, K, KEPT, RES, false, kLnMaxWarps>, front);
+  };
+  const std::true_type yes;
+  const std::false_type no;
   if (p.codes != nullptr) {
-    if (p.dh != nullptr) go(ln_bwd_kernel<T, VEC, K, true, true>);
-    else go(ln_bwd_kernel<T, VEC, K, true, false>);
+    if (p.dh != nullptr) shape(yes, yes);
+    else shape(yes, no);
   } else {
-    if (p.dh != nullptr) go(ln_bwd_kernel<T, VEC, K, false, true>);
-    else go(ln_bwd_kernel<T, VEC, K, false, false>);
+    if (p.dh != nullptr) shape(no, yes);
+    else shape(no, no);
   }
 }
 

@@ -9,9 +9,12 @@
 // are not read) or where no logit is above -inf: zeros, ids -1, a gradient of 0.  NaN or +inf
 // make the row's numbers NaN (NaN is the largest value for the top alternatives).
 //
-// Forward: one pass over a row with a running maximum m and S = Σ 2^t, A = Σ t 2^t,
-// t = (z - m) log2(e) / τ; H = ln2 (log2 S - A / S).  Where m rises by d powers of two,
-// A' = (A - d S) 2^-d, S' = S 2^-d.  The top alternatives cost that pass the maximum of every
+// Forward: one pass over a row with a running reference m (the maximum, or up to 12 powers of
+// two less) and S = Σ 2^t, A = Σ t 2^t, t = z s - m s, s = log2(e) / τ; H = ln2 (log2 S - A / S).
+// Where m rises by d powers of two, A' = (A - d S) 2^-d, S' = S 2^-d.  The shift m s is rounded
+// and the same one wherever it enters, so t carries one rounding of a small number and no
+// error of the size of m s.  Rows whose maximum is far from 0 (all masked by the type's lowest
+// value) are summed again from differences.  The top alternatives cost that pass the maximum of every
 // chunk of columns (8 of them, or a warp's tile where the row is long): the k best of the row
 // lie in the k chunks with the best maxima, so the k-th best of those is a bound, and only
 // chunks above it are looked at again.
@@ -57,9 +60,20 @@ __device__ __forceinline__ float lp_exp2(float x) {
   return y;
 }
 
-// t of a logit: exact difference first, so nothing overflows that is finite in the end, and a
-// bound from below, under which 2^t is 0 (t 2^t would be 0 · -inf).  NaN stays.
+// t of a logit for any row: exact difference first, so nothing overflows that is finite in the
+// end, and a bound from below, under which 2^t is 0 (t 2^t would be 0 · -inf).  NaN stays.
 __device__ __forceinline__ float lp_t(float z, float m, float scale) { return max_nan((z - m) * scale, -1000.0f); }
+
+// The shift of a reference m, the rounded product -m s.  It is rounded down: where m is a mask's
+// value so far (-1e9, the type's lowest) what the rounding leaves may be any power of two, but
+// none above 1, and sums of 0 go when the reference moves up.
+__device__ __forceinline__ float lp_shift(float m, float scale) { return __fmul_rd(-m, scale); }
+
+// Logits from here down are taken as this: they weigh 0 in a row whose reference is in the range
+// where what the shift's rounding leaves is small (temperatures of 1e-6 to 1e6), and t stays
+// finite.  Other rows take the form above.
+constexpr float kLpFloor = -1e30f;
+__device__ __forceinline__ bool lp_plain(float m, float scale) { return fabsf(m * scale) < 1e6f; }
 
 // 16 bytes of a row
 template <typename T>
@@ -80,6 +94,45 @@ struct LpVec {
         v[2 * i] = f.x, v[2 * i + 1] = f.y;
       }
     }
+  }
+  // the largest; NaN where there is one
+  __device__ __forceinline__ float largest() const {
+    if constexpr (sizeof(T) == 4) {
+      return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2 a = __hmax2_nan(*reinterpret_cast<const T2*>(&u.x), *reinterpret_cast<const T2*>(&u.y));
+      const T2 b = __hmax2_nan(*reinterpret_cast<const T2*>(&u.z), *reinterpret_cast<const T2*>(&u.w));
+      const T2 c = __hmax2_nan(a, b);
+      return max_nan(to_f32<T>(c.x), to_f32<T>(c.y));
+    }
+  }
+  // bounded from below by the floor (bf16 has it: before the values are spread); NaN stays
+  __device__ __forceinline__ void floored_pairs(uint64_t (&p)[N / 2]) const {
+    float v[N];
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      __nv_bfloat162 low;
+      low.x = low.y = __float2bfloat16_rn(kLpFloor);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), low);
+        const float2 f = bf16x2_to_f2(*reinterpret_cast<const uint32_t*>(&m));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      }
+    } else {
+      values(v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = max_nan(v[i], kLpFloor);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) p[i] = f2_pack(v[2 * i], v[2 * i + 1]);
+  }
+  __device__ __forceinline__ void set_pairs(const uint64_t (&p)[N / 2]) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) f2_unpack(p[i], v[2 * i], v[2 * i + 1]);
+    set(v);
   }
   __device__ __forceinline__ void set(const float (&v)[N]) {
     uint32_t w[4];
@@ -104,28 +157,31 @@ template <typename T>
 struct LpRow {
   static constexpr int N = LpVec<T>::N;
   const T* z;
-  int lead;
-  int64_t V, vecs;
-  __device__ __forceinline__ LpRow(const void* base, int64_t row, int64_t stride, int64_t V_) : V(V_) {
+  int lead, V, vecs;
+  __device__ __forceinline__ LpRow(const void* base, int64_t row, int64_t stride, int V_) : V(V_) {
     z = reinterpret_cast<const T*>(base) + row * stride;
     lead = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
     vecs = (lead + V + N - 1) / N;
   }
-  __device__ __forceinline__ int64_t col(int64_t i) const { return i * N - lead; }
-  __device__ __forceinline__ bool whole(int64_t i) const { return col(i) >= 0 && col(i) + N <= V; }
-  __device__ __forceinline__ LpVec<T> load(int64_t i) const {
+  __device__ __forceinline__ int col(int i) const { return i * N - lead; }
+  __device__ __forceinline__ bool whole(int i) const { return col(i) >= 0 && col(i) + N <= V; }
+  // vectors [i, i + n) are whole
+  __device__ __forceinline__ bool inside(int i, int n) const { return col(i) >= 0 && col(i + n) <= V; }
+  __device__ __forceinline__ LpVec<T> load_whole(int i) const {
     LpVec<T> r;
-    if (whole(i)) {
-      r.u = __ldg(reinterpret_cast<const uint4*>(z + col(i)));
-    } else {
-      float v[N];
+    r.u = __ldg(reinterpret_cast<const uint4*>(z - lead) + i);
+    return r;
+  }
+  __device__ __forceinline__ LpVec<T> load(int i) const {   // (-inf behind the row's last, too)
+    if (whole(i)) return load_whole(i);
+    LpVec<T> r;
+    float v[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int64_t c = col(i) + j;
-        v[j] = c >= 0 && c < V ? to_f32<T>(z[c]) : -INFINITY;
-      }
-      r.set(v);
+    for (int j = 0; j < N; ++j) {
+      const int c = col(i) + j;
+      v[j] = c >= 0 && c < V ? to_f32<T>(z[c]) : -INFINITY;
     }
+    r.set(v);
     return r;
   }
 };
@@ -134,29 +190,34 @@ struct LpSums {
   float m, s, a;
 };
 
-// the sums when the maximum goes to `to` (above m)
+// How far the largest may leave the reference behind, in powers of two: 2^t stays below 2^12
+// (S and A are relative to m in any case), and the rescaling, which one of a warp's lanes
+// would nearly always want, becomes rare.
+constexpr float kLpBehind = 12.0f;
+
+// Factors of S and A where the reference goes up from m to `to`: PLAIN as their shifts differ
+template <bool PLAIN>
 __device__ __forceinline__ void lp_raise(LpSums& x, float to, float scale) {
-  if (x.m == -INFINITY) {   // nothing yet
-    x.m = to;
-    return;
+  if (x.m != -INFINITY) {   // (otherwise nothing yet, or a NaN, which stays)
+    const float d = PLAIN ? lp_shift(to, scale) - lp_shift(x.m, scale) : lp_t(x.m, to, scale);   // <= 0
+    const float f = lp_exp2(d);
+    x.a = f * fmaf(d, x.s, x.a);
+    x.s *= f;
   }
-  const float d = lp_t(x.m, to, scale);   // <= 0
-  const float f = lp_exp2(d);
-  x.a = f * fmaf(d, x.s, x.a);
-  x.s *= f;
   x.m = to;
 }
 
+template <bool PLAIN>
 __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float scale) {
-  // (a NaN is in the sums of its lane; maxima that are NaN there are not compared)
   const float to = fmaxf(a.m, b.m);
-  if (to > a.m) lp_raise(a, to, scale);
-  if (to > b.m) lp_raise(b, to, scale);
+  if (to > a.m) lp_raise<PLAIN>(a, to, scale);
+  if (to > b.m) lp_raise<PLAIN>(b, to, scale);
   a.s += b.s;
   a.a += b.a;
   return a;
 }
 
+template <bool PLAIN>
 __device__ __forceinline__ LpSums lp_warp_join(LpSums x, float scale) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -164,15 +225,17 @@ __device__ __forceinline__ LpSums lp_warp_join(LpSums x, float scale) {
     y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
     y.s = __shfl_xor_sync(0xffffffffu, x.s, o);
     y.a = __shfl_xor_sync(0xffffffffu, x.a, o);
-    x = lp_join(x, y, scale);
+    x = lp_join<PLAIN>(x, y, scale);
   }
   return x;
 }
 
-// (z - m) / τ - log S, in 64 bits for a row's few numbers
-__device__ __forceinline__ float lp_log(float z, float m, double tau, double log_s) {
-  return (float)(((double)z - (double)m) / tau - log_s);
-}
+// A row's sums for its few numbers in 64 bits: l = (z - m) / τ - log S.  (PLAIN sums are
+// relative to the rounded shift: m is what it stands for.)
+struct LpLog {
+  double m, log_s, tau;
+  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) / tau - log_s); }
+};
 
 // Whole numbers in the values' order (0 and -0 equal, NaN above all), without the places that
 // are the same for all values of the type.
@@ -199,8 +262,8 @@ __device__ __forceinline__ uint32_t lp_block_sum(uint32_t v, uint32_t* s_n, int 
 
 // The top alternatives of a row, by the block that has all chunks' maxima.
 template <typename T, int NT, bool FINE>
-__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const float* s_max, int chunks, float high,
-                       double log_s, bool nan, uint32_t* s_n, uint64_t* s_list, uint32_t* s_count) {
+__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const float* s_max, int chunks, const LpLog& log,
+                       bool nan, uint32_t* s_n, uint64_t* s_list, uint32_t* s_count) {
   constexpr int N = LpVec<T>::N, kVecs = FINE ? 1 : 32;   // vectors of a chunk
   using Key = LpKey<T>;
   const int tid = threadIdx.x, lane = tid & 31;
@@ -222,17 +285,24 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
   }
   // Elements above the bound, in any order (they are ranked below).  Where they do not fit the
   // list (a row whose best lie side by side), the bound rises to the K-th best element.
-  auto each = [&](uint32_t at_least, auto&& f) {   // elements of chunks whose maximum reaches it
-    for (int c = tid / kVecs; c < chunks; c += NT / kVecs) {
-      if (Key::of(s_max[c]) < at_least) continue;
-      const int64_t i = (int64_t)c * kVecs + tid % kVecs;
-      if (i >= row.vecs) continue;
-      float v[N];
-      row.load(i).values(v);
+  auto vector = [&](int i, auto&& f) {
+    if (i >= row.vecs) return;
+    float v[N];
+    row.load(i).values(v);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int64_t col = row.col(i) + j;
-        if (col >= 0 && col < row.V) f(Key::of(v[j]), (uint32_t)col);
+    for (int j = 0; j < N; ++j) {
+      const int col = row.col(i) + j;
+      if (col >= 0 && col < row.V) f(Key::of(v[j]), (uint32_t)col);
+    }
+  };
+  auto each = [&](uint32_t at_least, auto&& f) {   // elements of chunks whose maximum reaches it
+    for (int c0 = tid - lane; c0 < chunks; c0 += NT) {
+      const bool look = c0 + lane < chunks && Key::of(s_max[min(c0 + lane, chunks - 1)]) >= at_least;
+      if constexpr (FINE) {
+        if (look) vector(c0 + lane, f);
+      } else {
+        for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0; in &= in - 1)
+          vector((c0 + __ffs(in) - 1) * kVecs + lane, f);
       }
     }
   };
@@ -265,36 +335,25 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
   // elements at the bound, in the order of their columns, until there are K
   uint32_t n = above;
   if (tid < 32 && n < K) {
-    constexpr int kStep = 32 / kVecs;   // chunks that a warp looks at at once
-    for (int c0 = 0; c0 < chunks && n < K; c0 += kStep) {
-      const int c = c0 + lane / kVecs;
-      const bool look = c < chunks && Key::of(s_max[c]) >= bound;
-      if (!__any_sync(0xffffffffu, look)) continue;
-      const int64_t i = (int64_t)c * kVecs + lane % kVecs;
-      uint32_t ties = 0;
-      float v[N];
-      if (look && i < row.vecs) {
-        row.load(i).values(v);
+    for (int c0 = 0; c0 < chunks && n < K; c0 += 32) {
+      const bool look = c0 + lane < chunks && Key::of(s_max[min(c0 + lane, chunks - 1)]) >= bound;
+      // a step of the warp: a vector a lane, of 32 chunks (FINE) or of one
+      for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0 && n < K; in = FINE ? 0u : in & (in - 1)) {
+        const int i = FINE ? c0 + lane : (c0 + __ffs(in) - 1) * kVecs + lane;
+        uint32_t ties = 0;
+        if (!FINE || look) vector(i, [&](uint32_t key, uint32_t col) { ties |= (key == bound ? 1u : 0u) << (int)(col - row.col(i)); });
+        uint32_t before = __popc(ties);   // of lower lanes
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const int64_t col = row.col(i) + j;
-          if (col >= 0 && col < row.V && Key::of(v[j]) == bound) ties |= 1u << j;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += up;
         }
+        const uint32_t all = __shfl_sync(0xffffffffu, before, 31);
+        uint32_t at = n + before - __popc(ties);
+        for (; ties != 0 && at < K; ties &= ties - 1, ++at)
+          s_list[at] = ((uint64_t)bound << 32) | (uint32_t)~(uint32_t)(row.col(i) + __ffs(ties) - 1);
+        n = min(K, n + all);
       }
-      uint32_t before = __popc(ties);   // of lower lanes
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += up;
-      }
-      const uint32_t all = __shfl_sync(0xffffffffu, before, 31);
-      uint32_t at = n + before - __popc(ties);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if ((ties >> j & 1u) && at < K) s_list[at] = ((uint64_t)bound << 32) | (uint32_t)~(uint32_t)(row.col(i) + j);
-        at += ties >> j & 1u;
-      }
-      n = min(K, n + all);
     }
   }
   if (tid == 0) *s_count = max(n, above);   // (above K only where the list holds it)
@@ -308,16 +367,137 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
     if (rank < K) {
       const uint32_t col = ~(uint32_t)mine;
       p.ids[m * p.K + rank] = col;
-      p.top[m * p.K + rank] = nan ? NAN : lp_log(to_f32<T>(row.z[col]), high, p.tau, log_s);
+      p.top[m * p.K + rank] = nan ? NAN : log.of(to_f32<T>(row.z[col]));
     }
   }
+}
+
+// A slice of a row, tiles [t0, t1) of 32 vectors: its sums, and its chunks' maxima.  Tiles that
+// lie inside the row go in groups of U a warp, the next group's loads ahead of this one's
+// arithmetic, in packed pairs.
+template <typename T, int NT, bool TOP, bool FINE>
+__device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, float* s_max) {
+  constexpr int N = LpVec<T>::N, P = N / 2, U = 4, kStep = NT / 32 * U;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float behind = kLpBehind / scale;
+  float m = -INFINITY;
+  uint64_t s2 = 0ull, a2 = 0ull;
+  auto chunk = [&](const LpVec<T>& v, int tile, float top) {
+    if constexpr (TOP && FINE) {
+      if (tile * 32 + lane < row.vecs) s_max[tile * 32 + lane] = top;
+    } else if constexpr (TOP) {
+      float all;
+      asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
+      if (lane == 0) s_max[tile] = all;
+    }
+  };
+  auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
+    float top[U], cm = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (j < n) {
+        top[j] = r[j].largest();
+        chunk(r[j], tile + j, top[j]);
+        cm = fmaxf(cm, top[j]);
+      }
+    }
+    cm = fmaxf(cm, kLpFloor);
+    if (cm > m + behind || m == -INFINITY) {
+      float s, a, lo, hi;
+      f2_unpack(s2, lo, hi), s = lo + hi;
+      f2_unpack(a2, lo, hi), a = lo + hi;
+      LpSums x{m, s, a};
+      lp_raise<true>(x, cm, scale);
+      m = x.m, s2 = f2_pack(x.s, 0.0f), a2 = f2_pack(x.a, 0.0f);
+    }
+    const float shift = lp_shift(m, scale);
+    const uint64_t sc = f2_pack(scale, scale), sh = f2_pack(shift, shift);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (j < n) {
+        uint64_t z[P];
+        r[j].floored_pairs(z);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const uint64_t t = f2_fma(z[i], sc, sh);
+          float lo, hi;
+          f2_unpack(t, lo, hi);
+          const uint64_t w = f2_pack(lp_exp2(lo), lp_exp2(hi));
+          s2 = f2_add(s2, w);
+          a2 = f2_fma(w, t, a2);
+        }
+      }
+    }
+  };
+  int t = t0 + warp * U;
+  auto inside = [&](int t) { return t + U <= t1 && row.inside(t * 32, 32 * U); };
+  auto fetch = [&](LpVec<T> (&r)[U], int t) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) r[j] = row.load_whole((t + j) * 32 + lane);
+  };
+  while (t < t1) {
+    if (inside(t)) {
+      LpVec<T> next[U];
+      fetch(next, t);
+      for (;;) {
+        LpVec<T> r[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) r[j] = next[j];
+        const int here = t;
+        t += kStep;
+        const bool more = inside(t);
+        if (more) fetch(next, t);
+        add(r, here, U);
+        if (!more) break;
+      }
+    } else {
+      LpVec<T> r[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) r[j] = row.load((t + j) * 32 + lane);
+      add(r, t, min(U, t1 - t));
+      t += kStep;
+    }
+  }
+  float lo, hi;
+  LpSums x{m, 0.0f, 0.0f};
+  f2_unpack(s2, lo, hi), x.s = lo + hi;
+  f2_unpack(a2, lo, hi), x.a = lo + hi;
+  return x;
+}
+
+// The sums of a whole row from differences, for rows whose maximum is far from 0.
+template <typename T, int NT>
+__device__ LpSums lp_far(const LpRow<T>& row, float scale, LpSums* s_part) {
+  constexpr int N = LpVec<T>::N;
+  LpSums x{-INFINITY, 0.0f, 0.0f};
+  for (int i = threadIdx.x; i < row.vecs; i += NT) {
+    const LpVec<T> r = row.load(i);
+    float v[N];
+    r.values(v);
+    const float top = r.largest();
+    if (top > x.m) lp_raise<false>(x, top, scale);
+    const float from = x.m == -INFINITY ? 0.0f : x.m;   // nothing but -inf so far: weights of 0
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float t = lp_t(v[e], from, scale), w = lp_exp2(t);
+      x.s += w;
+      x.a = fmaf(w, t, x.a);
+    }
+  }
+  x = lp_warp_join<false>(x, scale);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = s_part[0];
+  for (int i = 1; i < NT / 32; ++i) x = lp_join<false>(x, s_part[i], scale);
+  return x;
 }
 
 // A block (a cluster of them, each with a slice of the columns, where there are fewer rows
 // than places) works on one row.
 template <typename T, int NT, bool TOP, bool FINE>
 __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__ LogprobParams p) {
-  constexpr int N = LpVec<T>::N, U = 4, kWarps = NT / 32;
+  constexpr int kWarps = NT / 32;
   namespace cg = cooperative_groups;
   auto cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
@@ -327,97 +507,48 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.x / (unsigned)csize;
   const int64_t y = p.targets != nullptr ? p.targets[m] : 0;
-  const bool counted = y >= 0 && y < p.V;
-  if (!counted) {   // (all blocks of the cluster)
-    if (crank == 0) {
-      for (int i = tid; i < p.K; i += NT) p.ids[m * p.K + i] = -1, p.top[m * p.K + i] = 0.0f;
-      if (tid == 0) {
-        if (p.targets != nullptr) p.logp[m] = 0.0f;
-        p.entropy[m] = 0.0f;
-        p.stats[3 * m] = 0.0f, p.stats[3 * m + 1] = INFINITY, p.stats[3 * m + 2] = 0.0f;
-      }
-    }
-    return;
-  }
-  const LpRow<T> row(p.z, m, p.stride, p.V);
-  float* s_max = lp_smem;
-  if (csize > 1) {
-    if constexpr (TOP) s_max = cluster.map_shared_rank(lp_smem, 0);
-    cluster.sync();   // rank 0, to which the others write, is there
-  }
-  // tiles of 32 vectors; a warp takes U of them at a time
-  const int64_t tiles = (row.vecs + 31) / 32, per = (tiles + csize - 1) / csize;
-  const int64_t t0 = min(tiles, per * crank), t1 = min(tiles, t0 + per);
-  LpSums x{-INFINITY, 0.0f, 0.0f};
-  const float scale = p.scale;
-  for (int64_t t = t0 + warp * U; t < t1; t += kWarps * U) {
-    LpVec<T> r[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int64_t i = (t + j) * 32 + lane;
-      if (t + j < t1 && i < row.vecs) r[j] = row.load(i);
-      else {
-        float none[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) none[e] = -INFINITY;
-        r[j].set(none);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      float v[N];
-      r[j].values(v);
-      float top = v[0];
-#pragma unroll
-      for (int e = 1; e < N; ++e) top = max_nan(top, v[e]);
-      if constexpr (TOP) {
-        if constexpr (FINE) {
-          if (t + j < t1 && (t + j) * 32 + lane < row.vecs) s_max[(t + j) * 32 + lane] = top;
-        } else {
-          float all;
-          asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
-          if (lane == 0 && t + j < t1) s_max[t + j] = all;
-        }
-      }
-      if (top > x.m) lp_raise(x, top, scale);
-      const float from = x.m == -INFINITY ? 0.0f : x.m;   // nothing but -inf so far: weights of 0
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float tt = lp_t(v[e], from, scale), w = lp_exp2(tt);
-        x.s += w;
-        x.a = fmaf(w, tt, x.a);
-      }
-    }
-  }
-  x = lp_warp_join(x, scale);
-  if (lane == 0) {
-    LpSums* to = s_part;
-    if (csize > 1) to = cluster.map_shared_rank(s_part, 0);
-    to[crank * kWarps + warp] = x;
-  }
-  if (csize > 1) {
-    cluster.sync();
-    if (crank > 0) return;
-  } else {
-    __syncthreads();
-  }
-  x = LpSums{-INFINITY, 0.0f, 0.0f};
-  for (int i = 0; i < csize * kWarps; ++i) x = lp_join(x, s_part[i], scale);   // the same in every thread
-  if (x.m == -INFINITY && !(x.s != x.s)) {   // no logit above -inf
+  auto nothing = [&] {   // the row does not count
     for (int i = tid; i < p.K; i += NT) p.ids[m * p.K + i] = -1, p.top[m * p.K + i] = 0.0f;
     if (tid == 0) {
       if (p.targets != nullptr) p.logp[m] = 0.0f;
       p.entropy[m] = 0.0f;
       p.stats[3 * m] = 0.0f, p.stats[3 * m + 1] = INFINITY, p.stats[3 * m + 2] = 0.0f;
     }
+  };
+  if (y < 0 || y >= p.V) {   // (all blocks of the cluster)
+    if (crank == 0) nothing();
     return;
   }
-  const bool nan = !(x.s < INFINITY) || x.m == INFINITY;
-  const double log_s = log((double)x.s);
+  const LpRow<T> row(p.z, m, p.stride, (int)p.V);
+  float* s_max = lp_smem;
+  LpSums* to = s_part;
+  if (csize > 1) {
+    s_max = cluster.map_shared_rank(lp_smem, 0);
+    to = cluster.map_shared_rank(s_part, 0);
+    cluster.sync();   // rank 0, to which the others write, is there
+  }
+  const int tiles = (row.vecs + 31) / 32, per = (tiles + csize - 1) / csize;
+  const int t0 = min(tiles, per * crank), t1 = min(tiles, t0 + per);
+  const float scale = p.scale;
+  LpSums x = lp_warp_join<true>(lp_slice<T, NT, TOP, FINE>(row, t0, t1, scale, s_max), scale);
+  if (lane == 0) to[crank * kWarps + warp] = x;
+  if (csize > 1) {
+    cluster.sync();
+    if (crank > 0) return;
+  } else {
+    __syncthreads();
+  }
+  x = s_part[0];
+  for (int i = 1; i < csize * kWarps; ++i) x = lp_join<true>(x, s_part[i], scale);   // the same in every thread
+  const bool plain = lp_plain(x.m, scale);
+  if (!plain) x = lp_far<T, NT>(row, scale, s_part);
+  if (x.m == -INFINITY && x.s == x.s) return nothing();   // no logit above -inf
+  const bool nan = !(x.s < INFINITY) || !(x.m < INFINITY);
+  const LpLog log{plain ? -(double)lp_shift(x.m, scale) / (double)scale : (double)x.m, ::log((double)x.s), p.tau};
   if (tid == 0) {
     const double l2 = log2((double)x.s);
     const float h = nan ? NAN : fmaxf(0.0f, (float)((l2 - (double)x.a / (double)x.s) * 0.6931471805599453));
-    if (p.targets != nullptr) p.logp[m] = nan ? NAN : lp_log(to_f32<T>(row.z[y]), x.m, p.tau, log_s);
+    if (p.targets != nullptr) p.logp[m] = nan ? NAN : log.of(to_f32<T>(row.z[y]));
     p.entropy[m] = h;
     p.stats[3 * m] = nan ? NAN : x.m;
     p.stats[3 * m + 1] = nan ? NAN : (float)l2;
@@ -425,89 +556,102 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__
   }
   if constexpr (TOP) {
     uint64_t* s_list = reinterpret_cast<uint64_t*>(lp_smem + (p.chunks + 1) / 2 * 2);
-    lp_top<T, NT, FINE>(p, row, m, lp_smem, (int)(FINE ? row.vecs : tiles), x.m, log_s, nan, s_n, s_list, &s_count);
+    lp_top<T, NT, FINE>(p, row, m, lp_smem, FINE ? row.vecs : tiles, log, nan, s_n, s_list, &s_count);
   }
 }
 
-// Gradient: a block takes kLpSeg vectors of a row.
-constexpr int kLpBwdThreads = 256, kLpBwdVecs = 4;
-constexpr int kLpSeg = kLpBwdThreads * kLpBwdVecs;
+// Gradient: a warp takes U tiles of 32 vectors of a row and needs no other: it sums the row's
+// entries of g itself, and the columns of its tiles with a g term it writes a second time.
+constexpr int kLpBwdWarps = 8, kLpBwdTiles = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(kLpBwdThreads) logprob_bwd_kernel(const __grid_constant__ LogprobParams p, int segs) {
-  constexpr int N = LpVec<T>::N;
-  __shared__ float s_g[kLpBwdThreads / 32];
-  __shared__ int s_hit;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t m = blockIdx.x / (unsigned)segs, seg = blockIdx.x - m * segs;
+__global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __grid_constant__ LogprobParams p, uint32_t segs) {
+  constexpr int N = LpVec<T>::N, P = N / 2, U = kLpBwdTiles;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * kLpBwdWarps + (threadIdx.x >> 5);
+  const int64_t m = (uint32_t)unit / segs;   // (checked: below 2^32)
+  if (m >= p.M) return;
+  const int i0 = (int)((uint32_t)unit - (uint32_t)m * segs) * 32 * U;   // first vector
   // the gradient's row has the logits' alignment; its vectors, the columns behind V among them
-  const LpRow<T> row(p.z, m, p.stride, p.V);
+  const LpRow<T> row(p.z, m, p.stride, (int)p.V);
   T* out = reinterpret_cast<T*>(p.dz) + m * p.gstride;
   const float high = p.stats[3 * m], l2 = p.stats[3 * m + 1], h = p.stats[3 * m + 2];
   const bool counted = !(l2 == INFINITY);
-  const int64_t i0 = seg * kLpSeg + tid;
-  LpVec<T> r[kLpBwdVecs];
+  LpVec<T> r[U];
+  const bool inside = row.inside(i0, 32 * U);
+  if (counted) {
 #pragma unroll
-  for (int j = 0; j < kLpBwdVecs; ++j) {
-    const int64_t i = i0 + j * kLpBwdThreads;
-    r[j].u = make_uint4(0u, 0u, 0u, 0u);
-    if (counted && i < row.vecs) r[j] = row.load(i);
+    for (int j = 0; j < U; ++j) r[j] = inside ? row.load_whole(i0 + j * 32 + lane) : row.load(i0 + j * 32 + lane);
   }
-  const float gh = p.gh != nullptr && counted ? p.gh[m] : 0.0f;
-  const float gy = p.gp != nullptr && counted ? p.gp[m] : 0.0f;
+  const int64_t y = p.gp != nullptr && p.targets != nullptr ? p.targets[m] : -1;
+  const float gh = p.gh != nullptr ? p.gh[m] : 0.0f, gy = p.gp != nullptr ? p.gp[m] : 0.0f;
   float g = 0.0f;   // of all entries
-  if (p.gt != nullptr && counted) {
-    for (int i = tid; i < p.K; i += kLpBwdThreads) g += p.gt[m * p.K + i];
+  if (p.gt != nullptr) {
+    for (int i = lane; i < p.K; i += 32) g += p.gt[m * p.K + i];
     g = warp_sum(g);
-    if (lane == 0) s_g[warp] = g;
-    __syncthreads();
-    g = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kLpBwdThreads / 32; ++i) g += s_g[i];
   }
   // dz = p (c0 + c1 log2 p) + g terms
   const float inv = (float)(1.0 / p.tau);
   const float c0 = -(g + gy + gh * h) * inv, c1 = -gh * kLpLn2 * inv;
+  const bool plain = lp_plain(high, p.scale);
+  const float shift = lp_shift(high, p.scale);
   auto smooth = [&](float z) {
-    const float t = max_nan((z - high) * p.scale - l2, -1000.0f);
+    const float t = plain ? fmaf(max_nan(z, kLpFloor), p.scale, shift) - l2 : max_nan((z - high) * p.scale - l2, -1000.0f);
     return lp_exp2(t) * fmaf(c1, t, c0);
   };
+  if (inside && counted && plain) {
+    const uint64_t sc = f2_pack(p.scale, p.scale), sh = f2_pack(shift, shift), l = f2_pack(-l2, -l2);
+    const uint64_t d0 = f2_pack(c0, c0), d1 = f2_pack(c1, c1);
 #pragma unroll
-  for (int j = 0; j < kLpBwdVecs; ++j) {
-    const int64_t i = i0 + j * kLpBwdThreads, col = row.col(i);
-    if (col >= p.width) continue;
-    float v[N];
-    r[j].values(v);
+    for (int j = 0; j < U; ++j) {
+      uint64_t z[P];
+      r[j].floored_pairs(z);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = counted && col + e < p.V ? smooth(v[e]) : 0.0f;
-    if (col >= 0 && col + N <= p.width) {
+      for (int i = 0; i < P; ++i) {
+        const uint64_t t = f2_add(f2_fma(z[i], sc, sh), l);
+        float lo, hi;
+        f2_unpack(t, lo, hi);
+        z[i] = f2_mul(f2_pack(lp_exp2(lo), lp_exp2(hi)), f2_fma(d1, t, d0));
+      }
       LpVec<T> o;
-      o.set(v);
-      *reinterpret_cast<uint4*>(out + col) = o.u;
-    } else {
+      o.set_pairs(z);
+      reinterpret_cast<uint4*>(out - row.lead)[i0 + j * 32 + lane] = o.u;
+    }
+  } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (col + e >= 0 && col + e < p.width) out[col + e] = from_f32<T>(v[e]);
+    for (int j = 0; j < U; ++j) {
+      const int col = row.col(i0 + j * 32 + lane);
+      if (col >= p.width) continue;
+      float v[N];
+      if (counted) r[j].values(v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = counted && col + e < p.V ? smooth(v[e]) : 0.0f;
+      if (col >= 0 && col + N <= p.width) {
+        LpVec<T> o;
+        o.set(v);
+        *reinterpret_cast<uint4*>(out + col) = o.u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (col + e >= 0 && col + e < p.width) out[col + e] = from_f32<T>(v[e]);
+      }
     }
   }
   if (!counted) return;
-  // columns with g terms
-  const int64_t y = p.targets != nullptr && p.gp != nullptr ? p.targets[m] : -1;
-  const int64_t c_begin = row.col(seg * kLpSeg), c_end = row.col((seg + 1) * kLpSeg);
-  if (tid == 0) s_hit = 0;
-  __syncthreads();   // the vectors are written
+  // columns with g terms: this warp's, once its vectors are written
+  const int c_begin = max(0, row.col(i0)), c_end = row.col(i0 + 32 * U);
+  bool hit = false;
+  __syncwarp();
   if (p.gt != nullptr) {
-    for (int i = tid; i < p.K; i += kLpBwdThreads) {
+    for (int i = lane; i < p.K; i += 32) {
       const int64_t c = p.ids[m * p.K + i];
-      if (c == y) s_hit = 1;
-      if (c < c_begin || c >= c_end || c < 0) continue;
-      const float more = p.gt[m * p.K + i] + (c == y ? gy : 0.0f);
-      out[c] = from_f32<T>(smooth(to_f32<T>(row.z[c])) + more * inv);
+      hit = hit || c == y;
+      if (c < c_begin || c >= c_end) continue;
+      out[c] = from_f32<T>(smooth(to_f32<T>(row.z[c])) + (p.gt[m * p.K + i] + (c == y ? gy : 0.0f)) * inv);
     }
-    __syncthreads();
+    hit = __any_sync(0xffffffffu, hit);
   }
-  if (tid == 0 && y >= c_begin && y < c_end && y >= 0 && s_hit == 0)
-    out[y] = from_f32<T>(smooth(to_f32<T>(row.z[y])) + gy * inv);
+  if (lane == 0 && !hit && y >= c_begin && y < c_end) out[y] = from_f32<T>(smooth(to_f32<T>(row.z[y])) + gy * inv);
 }
 
 }  // namespace zq
@@ -635,12 +779,13 @@ void logprob_bwd(at::Tensor z, c10::optional<at::Tensor> targets, at::Tensor top
   TORCH_CHECK(((reinterpret_cast<uintptr_t>(p.z) ^ reinterpret_cast<uintptr_t>(p.dz)) & 15) == 0 &&
                   (p.M == 1 || ((p.stride - p.gstride) * es) % 16 == 0),
               "token_logprobs: logits rows must be aligned as the gradient's");
-  const int64_t N = 16 / es, vecs = (p.width + 2 * N - 2) / N, segs = (vecs + kLpSeg - 1) / kLpSeg;
-  TORCH_CHECK(p.M * segs < (1LL << 31), "token_logprobs: too many rows");
+  const int64_t N = 16 / es, vecs = (p.width + 2 * N - 2) / N, segs = (vecs + 32 * kLpBwdTiles - 1) / (32 * kLpBwdTiles);
+  TORCH_CHECK(p.M * segs < (1LL << 32) - kLpBwdWarps && p.width < (1LL << 30), "token_logprobs: too many rows or columns");
   const c10::cuda::CUDAGuard guard(z.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   ZQ_LP_TYPES(z.scalar_type(), {
-    logprob_bwd_kernel<T><<<(unsigned)(p.M * segs), kLpBwdThreads, 0, stream>>>(p, (int)segs);
+    logprob_bwd_kernel<T><<<(unsigned)((p.M * segs + kLpBwdWarps - 1) / kLpBwdWarps), kLpBwdWarps * 32, 0, stream>>>(
+        p, (uint32_t)segs);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }

@@ -62,6 +62,19 @@ struct RawTile {
       }
     }
   }
+  // the same as packed pairs (2i, 2i + 1)
+  __device__ __forceinline__ void pairs(uint64_t (&v)[4]) const {
+    float f[8];
+    values(f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+  }
+  __device__ __forceinline__ void set(const uint64_t (&v)[4]) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f2_unpack(v[i], f[2 * i], f[2 * i + 1]);
+    set(f);
+  }
   // rounds to the type, once
   __device__ __forceinline__ void set(const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {

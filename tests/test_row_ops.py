@@ -31,8 +31,11 @@ def near(got, want, more):
     tol = torch.finfo(got.dtype).eps / 2 * want.abs() + more.double().cpu()
     if got.dtype == torch.float16:
         tol = tol + 2.0 ** -25
-    off = (got.detach().double().cpu() - want).abs()
     assert got.shape == want.shape
+    beyond = want.abs() > torch.finfo(got.dtype).max * (1 + torch.finfo(got.dtype).eps)   # of the type's range
+    got = got.detach().double().cpu()
+    assert (got.isinf() & (got.sign() == want.sign()))[beyond].all()
+    off = torch.where(beyond, 0.0, (got - want).abs())
     assert (off <= tol).all(), (float((off - tol).max()), int((off > tol).sum()))
 
 
@@ -565,6 +568,9 @@ def test_token_logprobs_masks(device, V, k, dtype):
     z[9, 7] = torch.finfo(dtype).max / 4
     targets = torch.tensor([1, V - 2, 1, V - 1, 5, 0, 2, V - 1, 0, 7], device=device)
     logprob_case(device, z, None, k, targets=targets)
+    z[2:4, 1] = 60000.0                     # masks and temperatures at the ends of their range
+    for tau in (1e-6, 0.01, 300.0, 1e6):
+        logprob_case(device, z, None, k, tau, targets=targets)
 
 
 @pytest.mark.parametrize("V", [300, pytest.param(70000, marks=pytest.mark.gpu)])

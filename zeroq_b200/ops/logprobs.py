@@ -74,7 +74,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     above -inf is taken the same way.  Without ``targets`` every row counts and ``logprobs``
     is None.  NaN or +inf make a row's numbers NaN; for the alternatives NaN is the largest.
 
-    Differentiable in ``logits`` through all three outputs.  bf16, fp16 or fp32 on the GPU, a
+    Differentiable in ``logits`` through all three outputs.  Temperatures of 1e-6 to 1e6; bf16, fp16 or fp32 on the GPU, a
     vocabulary of up to 2^22 and up to 256 alternatives."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError("token_logprobs: logits must be floating-point [M, V], got "
@@ -83,8 +83,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     vocab = logits.shape[-1] if vocab is None else int(vocab)
     if not 0 < vocab <= logits.shape[-1]:
         raise ValueError(f"token_logprobs: vocab must be 1 to {logits.shape[-1]}, got {vocab}")
-    if not (temperature > 0 and temperature < float("inf")):
-        raise ValueError(f"token_logprobs: temperature above 0, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"token_logprobs: temperature must be 1e-6 to 1e6, got {temperature}")
     if not 0 <= top_k <= min(vocab, MAX_TOP):
         raise ValueError(f"token_logprobs: top_k must be 0 to {min(vocab, MAX_TOP)}, got {top_k}")
     if targets is not None:
