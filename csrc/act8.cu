@@ -39,16 +39,31 @@ struct ActUnit {
 template <int U>
 __device__ __forceinline__ int act_units(const ActShape& s, ActUnit (&out)[U]) {
   const uint64_t first = ((uint64_t)blockIdx.x * kActWarps + (threadIdx.x >> 5)) * U;
-  if (first >= s.units) return 0;
+  if (first >= s.units) {   // a warp behind the last unit: tiles past every row's end
+#pragma unroll
+    for (int j = 0; j < U; ++j) out[j].row = 0, out[j].base = (int)s.D;
+    return 0;
+  }
   uint32_t row = (uint32_t)first / (uint32_t)s.tiles, tile = (uint32_t)first - row * (uint32_t)s.tiles;
   const int n = (int)min((uint64_t)U, s.units - first);
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     out[j].row = row;
-    out[j].base = (int)tile * kTile;
+    out[j].base = j < n ? (int)tile * kTile : (int)s.D;
     if (++tile == (uint32_t)s.tiles) tile = 0, ++row;
   }
   return n;
+}
+
+template <bool VEC, int U>
+__device__ __forceinline__ void keep_units(const uint64_t (&v)[U][4], const ActUnit (&u)[U], int8_t* codes, float* steps,
+                                           int lane, const ActShape& s) {
+  int8_t* c[U];
+  float* t[U];
+  int base[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j) c[j] = codes + u[j].row * s.P, t[j] = steps + u[j].row * s.G, base[j] = u[j].base;
+  keep_tiles<VEC, U>(v, c, t, base, lane, (int)s.D);
 }
 
 // fp32 activations take CUDA's accurate functions; 16-bit ones those of the kernels that
@@ -70,19 +85,15 @@ __global__ void __launch_bounds__(kActWarps * 32) act8_keep_kernel(const T* __re
                                                                    const ActShape s) {
   const int lane = threadIdx.x & 31;
   ActUnit u[U];
-  const int n = act_units<U>(s, u);
+  if (act_units<U>(s, u) == 0) return;
   RawTile<T, VEC> t[U];
 #pragma unroll
   for (int j = 0; j < U; ++j)
-    if (j < n) t[j].load(x + u[j].row * xs, u[j].base, lane, (int)s.D);
+    if (u[j].base < s.D) t[j].load(x + u[j].row * xs, u[j].base, lane, (int)s.D);
+  uint64_t v[U][4];
 #pragma unroll
-  for (int j = 0; j < U; ++j) {
-    if (j < n) {
-      float v[8];
-      t[j].values(v);
-      keep_tile<VEC>(v, codes + u[j].row * s.P, steps + u[j].row * s.G, u[j].base, lane, (int)s.D);
-    }
-  }
+  for (int j = 0; j < U; ++j) t[j].pairs(v[j]);
+  keep_units<VEC, U>(v, u, codes, steps, lane, s);
 }
 
 template <typename T, bool VEC, int U>
@@ -117,12 +128,17 @@ __global__ void __launch_bounds__(kActWarps * 32) gelu8_fwd_kernel(const T* __re
 #pragma unroll
   for (int j = 0; j < U; ++j)
     if (j < n) t[j].load(x + u[j].row * xs, u[j].base, lane, (int)s.D);
+  {
+    uint64_t v[U][4];
+#pragma unroll
+    for (int j = 0; j < U; ++j) t[j].pairs(v[j]);
+    keep_units<VEC, U>(v, u, codes, steps, lane, s);
+  }
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     if (j < n) {
       float v[8], o[8];
       t[j].values(v);
-      keep_tile<VEC>(v, codes + u[j].row * s.P, steps + u[j].row * s.G, u[j].base, lane, (int)s.D);
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = v[i] * act_gelu<T>(v[i]).cdf;
       store_tile<T, VEC>(y + u[j].row * s.D, u[j].base, lane, (int)s.D, o);
@@ -180,14 +196,27 @@ __global__ void __launch_bounds__(kActWarps * 32) swiglu8_fwd_kernel(const T* __
       b[j].load(up + u[j].row * us, u[j].base, lane, (int)s.D);
     }
   }
+  {   // both inputs' tiles at once
+    uint64_t v[2 * U][4];
+    int8_t* c[2 * U];
+    float* t[2 * U];
+    int base[2 * U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      a[j].pairs(v[2 * j]);
+      b[j].pairs(v[2 * j + 1]);
+      c[2 * j] = gcodes + u[j].row * s.P, t[2 * j] = gsteps + u[j].row * s.G;
+      c[2 * j + 1] = ucodes + u[j].row * s.P, t[2 * j + 1] = usteps + u[j].row * s.G;
+      base[2 * j] = base[2 * j + 1] = u[j].base;
+    }
+    keep_tiles<VEC, 2 * U>(v, c, t, base, lane, (int)s.D);
+  }
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     if (j < n) {
       float v[8], w[8];
       a[j].values(v);
       b[j].values(w);
-      keep_tile<VEC>(v, gcodes + u[j].row * s.P, gsteps + u[j].row * s.G, u[j].base, lane, (int)s.D);
-      keep_tile<VEC>(w, ucodes + u[j].row * s.P, usteps + u[j].row * s.G, u[j].base, lane, (int)s.D);
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] *= v[i] * act_sigmoid<T>(v[i]);
       store_tile<T, VEC>(y + u[j].row * s.D, u[j].base, lane, (int)s.D, w);

@@ -59,6 +59,17 @@ __device__ __forceinline__ int ln_place(int c) {   // of column c
 template <bool VEC>
 __device__ __forceinline__ void ln_stage(float* s, const void* p, int type, float absent, int D) {
   const int whole = (D + kTile - 1) / kTile * kTile;
+  // four columns at a time; a run of four stays one
+  if (p != nullptr && type == 0 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const float4* v = reinterpret_cast<const float4*>(p);
+#pragma unroll 4
+    for (int c = threadIdx.x * 4; c < whole; c += blockDim.x * 4) {
+      const float4 f = c < D ? __ldg(v + c / 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      *reinterpret_cast<float4*>(s + ln_place<VEC>(c)) = f;
+    }
+    return;
+  }
+#pragma unroll 4
   for (int c = threadIdx.x; c < whole; c += blockDim.x)
     s[ln_place<VEC>(c)] = c >= D ? 0.0f : p == nullptr ? absent : ln_param(p, type, c);
 }
@@ -89,70 +100,186 @@ __device__ __forceinline__ uint32_t ln_mask(int base, int lane, int D) {
   return m;
 }
 
-// Every warp's pair of numbers, for every thread of the team.  Buffers alternate from row to
-// row: a thread that writes one again has passed the other's barrier, to which its readers
-// came after they had read.
-__device__ __forceinline__ void ln_exchange(float2 (&buf)[kLnMaxWarps], float2 mine, int wt, int lane, int team, int W) {
+// Every warp's pair of numbers, lane i getting warp i's (0 past the last).  Buffers alternate
+// from row to row: a thread that writes one again has passed the other's barrier, to which its
+// readers came after they had read.
+__device__ __forceinline__ float2 ln_exchange(float2 (&buf)[kLnMaxWarps], float2 mine, int wt, int lane, int team, int W) {
   if (lane == 0) buf[wt] = mine;
   named_barrier(1 + team, W * 32);
+  return lane < W ? buf[lane] : make_float2(0.0f, 0.0f);
+}
+// the sum of the first 16 lanes' values, in every lane
+__device__ __forceinline__ float ln_sum16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
-template <typename T, bool VEC, int K, bool RES, bool KEEP>
+// Rows on their way: every thread copies its own columns of NS tensors of T (and, CODES, of the
+// 8-bit input) into its own places of shared memory, S rows ahead, and reads them back itself,
+// so no barrier belongs to it and nothing waits in registers.
+template <typename T, int K, int NS, bool CODES>
+struct LnSlots {
+  static constexpr int kVecs = (int)sizeof(T) / 2;   // 16-byte vectors of a lane's 8 elements
+  static constexpr int kBytes = K * (16 * kVecs * NS + (CODES ? 12 : 0));   // of a thread
+  const T* from[NS];   // this thread's columns of tile 0 in the row to be fetched next
+  int64_t pitch[NS];
+  const int8_t* codes;
+  const float* steps;
+  int64_t cpitch, spitch;
+  uint32_t slots, slot_bytes, vec, eight, four;   // shared addresses: begin, of a slot, this thread's places in one
+  int tile;            // columns from tile k to k + 1
+  uint32_t there;      // bit k: tile k has columns here
+
+  __device__ __forceinline__ void init(uint8_t* smem, int W, int col, int D, int S) {
+    tile = W * kTile;
+    there = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) there |= (col + k * tile < D ? 1u : 0u) << k;
+    slots = smem_u32(smem);
+    slot_bytes = (uint32_t)kBytes * blockDim.x;
+    vec = threadIdx.x * 16;
+    eight = 16u * K * kVecs * NS * blockDim.x + threadIdx.x * 8;
+    four = (16u * K * kVecs * NS + 8u * K) * blockDim.x + threadIdx.x * 4;
+    if (there + 1 != 1u << K) {   // places that are never filled hold zeros
+      for (int s = 0; s < S; ++s) {
+        const uint32_t at = slots + s * slot_bytes;
+#pragma unroll
+        for (int i = 0; i < NS * K * kVecs; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + vec + 16u * i * blockDim.x), "r"(0) : "memory");
+        if constexpr (CODES) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + eight + 8u * k * blockDim.x), "r"(0) : "memory");
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + four + 4u * k * blockDim.x), "r"(0) : "memory");
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void stream(int i, const void* base, int64_t p, int64_t row, int64_t step, int col) {
+    from[i] = reinterpret_cast<const T*>(base) + row * p + col;
+    pitch[i] = step * p;
+  }
+  __device__ __forceinline__ void kept(const LnParams& p, int64_t row, int64_t step, int col) {
+    codes = p.codes + row * p.P + col;
+    steps = p.steps + row * p.G + col / kGroup;
+    cpitch = step * p.P;
+    spitch = step * p.G;
+  }
+  // fetches a row (where there is one) and goes on to the next
+  __device__ __forceinline__ void fetch(int slot, bool any) {
+    const uint32_t at = slots + slot * slot_bytes;
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (there >> k & 1u) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + vec + 16u * ((i * K + k) * kVecs + v) * blockDim.x),
+                           "l"(from[i] + k * tile + v * (16 / (int)sizeof(T)))
+                           : "memory");
+          if constexpr (CODES) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at + eight + 8u * k * blockDim.x), "l"(codes + k * tile)
+                         : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + four + 4u * k * blockDim.x),
+                         "l"(steps + k * (tile / kGroup))
+                         : "memory");
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < NS; ++i) from[i] += pitch[i];
+    if constexpr (CODES) codes += cpitch, steps += spitch;
+  }
+  // until all but the last S - 1 fetches are there
+  static __device__ __forceinline__ void wait(int S) {
+    if (S == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (S == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  }
+  __device__ __forceinline__ void get(int slot, int i, int k, RawTile<T, true>& t) const {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(t.w[4 * v]), "=r"(t.w[4 * v + 1]), "=r"(t.w[4 * v + 2]), "=r"(t.w[4 * v + 3])
+                   : "r"(slots + slot * slot_bytes + vec + 16u * ((i * K + k) * kVecs + v) * blockDim.x)
+                   : "memory");
+  }
+  __device__ __forceinline__ void get(int slot, int k, RawCodes<true>& c) const {
+    const uint32_t at = slots + slot * slot_bytes;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(c.w.x), "=r"(c.w.y) : "r"(at + eight + 8u * k * blockDim.x) : "memory");
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c.step[0]) : "r"(at + four + 4u * k * blockDim.x) : "memory");
+  }
+};
+
+// PIPE: rows come through shared memory; otherwise (not on 16-byte boundaries, or too wide for
+// two of them) they are read where they are.  KEEP: h is kept in 8 bits.
+template <typename T, bool VEC, int K, bool RES, bool KEEP, bool PIPE>
 __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_constant__ LnParams p) {
   __shared__ float2 s_red[kLnMaxTeams][2][kLnMaxWarps];
-  __shared__ float s_cols[kLnMaxWarps];   // columns of a team's warps
-  extern __shared__ __align__(16) float s_wb[];   // w and b
+  extern __shared__ __align__(16) float s_wb[];   // w and b; the slots
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D;
+  const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D, S = p.slots;
   const int whole = (D + kTile - 1) / kTile * kTile;
-
   const int64_t step = (int64_t)gridDim.x * p.R;
-  RawTile<T, VEC> rx[K], rd[RES ? K : 1];
-  auto load = [&](int64_t row) {
-    const T* x = reinterpret_cast<const T*>(p.x) + row * p.xs;
-#pragma unroll
-    for (int k = 0; k < K; ++k) rx[k].load(x, (wt + k * W) * kTile, lane, D);
-    if constexpr (RES) {
-      const T* d = reinterpret_cast<const T*>(p.delta) + row * p.ds;
-#pragma unroll
-      for (int k = 0; k < K; ++k) rd[k].load(d, (wt + k * W) * kTile, lane, D);
-    }
-  };
   int64_t row = (int64_t)blockIdx.x * p.R + team;
-  if (row < p.M) load(row);
+  LnSlots<T, K, RES ? 2 : 1, false> rows;
+  if constexpr (PIPE) {
+    const int col = wt * kTile + lane * 8;
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, W, col, D, S);
+    rows.stream(0, p.x, p.xs, row, step, col);
+    if constexpr (RES) rows.stream(1, p.delta, p.ds, row, step, col);
+    for (int i = 0; i < S; ++i) rows.fetch(i, row + i * step < p.M);
+  }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
   ln_stage<VEC>(s_wb + whole, p.b, p.wt, 0.0f, D);
-  float cols = 0.0f;   // of this warp
+  // columns of warp i of a team, in lane i; of this warp
+  auto columns = [&](int i) {
+    int n = 0;
 #pragma unroll
-  for (int k = 0; k < K; ++k) cols += (float)max(0, min(kTile, D - (wt + k * W) * kTile));
-  const float inv_cols = cols > 0.0f ? 1.0f / cols : 0.0f, inv_d = 1.0f / (float)D;
-  if (team == 0 && lane == 0) s_cols[wt] = cols;
+    for (int k = 0; k < K; ++k) n += max(0, min(kTile, D - (i + k * W) * kTile));
+    return (float)n;
+  };
+  const float cols = columns(wt), cols_of = columns(lane), inv_cols = cols > 0.0f ? 1.0f / cols : 0.0f, inv_d = 1.0f / (float)D;
   __syncthreads();
+  int at = 0;
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
     uint64_t v[K][4];
+    if constexpr (PIPE) rows.wait(S);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
-      rx[k].pairs(v[k]);
+      RawTile<T, VEC> t;
+      if constexpr (PIPE) rows.get(at, 0, k, t);
+      else t.load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
+      t.pairs(v[k]);
       if constexpr (RES) {
         uint64_t d[4];
-        rd[k].pairs(d);
+        if constexpr (PIPE) rows.get(at, 1, k, t);
+        else t.load(reinterpret_cast<const T*>(p.delta) + row * p.ds, base, lane, D);
+        t.pairs(d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[k][i] = f2_add(v[k][i], d[i]);
-        RawTile<T, VEC> h;
-        h.set(v[k]);
-        h.store(reinterpret_cast<T*>(p.h) + row * D, base, lane, D);
-        h.pairs(v[k]);   // as the next layer and the backward see it
+        t.set(v[k]);
+        if (base < D) t.store(reinterpret_cast<T*>(p.h) + row * D, base, lane, D);
+        t.pairs(v[k]);   // as the next layer and the backward see it
       }
     }
-    if (row + step < p.M) load(row + step);
     uint64_t s = 0ull;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = f2_add(s, v[k][i]);
-    float mu = warp_sum(f2_sum(s)) * inv_cols;
-    float q = 0.0f;
+    float mu = warp_sum(f2_sum(s)) * inv_cols, q = 0.0f;
+    if constexpr (PIPE) {   // the slot is read
+      rows.fetch(at, row + S * step < p.M);
+      at = at + 1 == S ? 0 : at + 1;
+    }
     {
       const uint64_t away = f2_pack(-mu, -mu);
       uint64_t q2 = 0ull;
@@ -165,7 +292,7 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
             const uint64_t d = f2_add(v[k][i], away);
             q2 = f2_fma(d, d, q2);
           }
-        } else {   // the row ends in this tile
+        } else if (base < D) {   // the row ends in this tile
           const uint32_t mask = ln_mask<VEC>(base, lane, D);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -179,31 +306,26 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       q = warp_sum(q + f2_sum(q2));
     }
     if (W > 1) {
-      float2(&buf)[kLnMaxWarps] = s_red[team][turn];
-      ln_exchange(buf, make_float2(mu, q), wt, lane, team, W);
-      float m = 0.0f;
-      for (int i = 0; i < W; ++i) m = fmaf(s_cols[i], buf[i].x, m);
-      m *= inv_d;
-      q = 0.0f;
-      for (int i = 0; i < W; ++i) {
-        const float d = buf[i].x - m;
-        q += fmaf(s_cols[i] * d, d, buf[i].y);
-      }
-      mu = m;
+      const float2 o = ln_exchange(s_red[team][turn], make_float2(mu, q), wt, lane, team, W);
+      mu = ln_sum16(cols_of * o.x) * inv_d;
+      const float d = o.x - mu;
+      q = ln_sum16(lane < W ? fmaf(cols_of * d, d, o.y) : 0.0f);
     }
-    const float r = 1.0f / sqrtf(q * inv_d + p.eps);
+    const float r = rsqrtf(fmaf(q, inv_d, p.eps));
     if (wt == 0 && lane == 0 && p.mean != nullptr) p.mean[row] = mu, p.rstd[row] = r;
+    if constexpr (KEEP) {
+      int8_t* c[K];
+      float* t[K];
+      int base[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) c[k] = p.codes + row * p.P, t[k] = p.steps + row * p.G, base[k] = (wt + k * W) * kTile;
+      keep_tiles<VEC, K>(v, c, t, base, lane, D);
+    }
     const uint64_t away = f2_pack(-mu, -mu), r2 = f2_pack(r, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
       if (base >= D) continue;
-      if constexpr (KEEP) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f2_unpack(v[k][i], f[2 * i], f[2 * i + 1]);
-        keep_tile<VEC>(f, p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
-      }
       uint64_t w[4], b[4];
       ln_staged<VEC>(s_wb, base, lane, w);
       ln_staged<VEC>(s_wb + whole, base, lane, b);
@@ -216,130 +338,28 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   }
 }
 
-// The backward's rows on their way: every thread copies its own columns into its own places of
-// shared memory, S rows ahead, and reads them back itself (twice: for the row's sums, and for
-// dx once they are known), so no barrier belongs to it and nothing is held in registers.  Rows
-// that cannot be copied that way (PIPE false: not on 16-byte boundaries, or too wide) are read
-// where they are.
+// KEPT: h in 8 bits; RES: dh is added.  A row is read twice (through shared memory, or from the
+// caches): for its sums, and for dx once they are known.
 template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE>
-struct LnRows {
-  static constexpr int kVecs = (int)sizeof(T) / 2;   // 16-byte vectors of a lane's 8 elements
-  static constexpr int kSlot = K * (16 * kVecs * (1 + (KEPT ? 0 : 1) + (RES ? 1 : 0)) + (KEPT ? 12 : 0));   // bytes a thread
-
-  RawTile<T, VEC> g[PIPE ? 1 : K], x[PIPE || KEPT ? 1 : K], h[PIPE || !RES ? 1 : K];
-  RawCodes<VEC> c[PIPE || !KEPT ? 1 : K];
-
-  static __device__ __forceinline__ void copy(void* to, const void* from, int bytes, bool there) {
-    const uint32_t n = there ? bytes : 0;   // (0: zeros)
-    if (bytes == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
-    else if (bytes == 8)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
-    else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(n) : "memory");
-  }
-  // places of a slot: [stream][tile][vector][thread] of 16 bytes, then codes (8) and steps (4)
-  static __device__ __forceinline__ uint8_t* place(uint8_t* slot, int stream, int k, int v) {
-    return slot + (((stream * K + k) * kVecs + v) * (int)blockDim.x + (int)threadIdx.x) * 16;
-  }
-  static __device__ __forceinline__ uint8_t* place_codes(uint8_t* slot, int k) {
-    return slot + ((1 + (RES ? 1 : 0)) * K * kVecs * 16 + k * 8) * (int)blockDim.x + threadIdx.x * 8;
-  }
-  static __device__ __forceinline__ uint8_t* place_step(uint8_t* slot, int k) {
-    return slot + ((1 + (RES ? 1 : 0)) * K * kVecs * 16 + K * 8 + k * 4) * (int)blockDim.x + threadIdx.x * 4;
-  }
-  // streams of 16-byte vectors: dy, then dh, then the input
-  static constexpr int kH = 1, kX = RES ? 2 : 1;
-
-  static __device__ __forceinline__ void fetch(const LnParams& p, uint8_t* slot, int64_t row, int wt, int lane) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int at = (wt + k * p.W) * kTile + lane * 8;
-      const bool there = at < p.D;
-      const int from = there ? at : 0;
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const int e = from + v * (16 / (int)sizeof(T));
-        copy(place(slot, 0, k, v), reinterpret_cast<const T*>(p.dy) + row * p.dys + e, 16, there);
-        if constexpr (RES) copy(place(slot, kH, k, v), reinterpret_cast<const T*>(p.dh) + row * p.dhs + e, 16, there);
-        if constexpr (!KEPT) copy(place(slot, kX, k, v), reinterpret_cast<const T*>(p.x) + row * p.xs + e, 16, there);
-      }
-      if constexpr (KEPT) {
-        copy(place_codes(slot, k), p.codes + row * p.P + from, 8, there);
-        copy(place_step(slot, k), p.steps + row * p.G + from / kGroup, 4, there);
-      }
-    }
-  }
-  __device__ __forceinline__ void read(const LnParams& p, int64_t row, int wt, int lane) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int base = (wt + k * p.W) * kTile;
-      g[k].load(reinterpret_cast<const T*>(p.dy) + row * p.dys, base, lane, p.D);
-      if constexpr (KEPT) c[k].load(p.codes + row * p.P, p.steps + row * p.G, base, lane, p.D);
-      else x[k].load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, p.D);
-      if constexpr (RES) h[k].load(reinterpret_cast<const T*>(p.dh) + row * p.dhs, base, lane, p.D);
-    }
-  }
-  static __device__ __forceinline__ void from_slot(const uint8_t* slot, int stream, int k, uint64_t (&v)[4]) {
-    RawTile<T, VEC> t;
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const uint4 u = *reinterpret_cast<const uint4*>(place(const_cast<uint8_t*>(slot), stream, k, i));
-      t.w[4 * i] = u.x, t.w[4 * i + 1] = u.y, t.w[4 * i + 2] = u.z, t.w[4 * i + 3] = u.w;
-    }
-    t.pairs(v);
-  }
-  __device__ __forceinline__ void dy(const uint8_t* slot, int k, uint64_t (&v)[4]) const {
-    if constexpr (PIPE) from_slot(slot, 0, k, v);
-    else g[k].pairs(v);
-  }
-  __device__ __forceinline__ void dh(const uint8_t* slot, int k, uint64_t (&v)[4]) const {
-    if constexpr (PIPE) from_slot(slot, kH, k, v);
-    else h[k].pairs(v);
-  }
-  __device__ __forceinline__ void centred(const uint8_t* slot, int k, float mu, uint64_t (&v)[4]) const {   // h - mu
-    const uint64_t away = f2_pack(-mu, -mu);
-    if constexpr (KEPT) {
-      RawCodes<VEC> q;
-      if constexpr (PIPE) {
-        q.w = *reinterpret_cast<const uint2*>(place_codes(const_cast<uint8_t*>(slot), k));
-        q.step[0] = *reinterpret_cast<const float*>(place_step(const_cast<uint8_t*>(slot), k));
-      } else {
-        q = c[k];
-      }
-      float f[8];
-      q.values(f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
-    } else if constexpr (PIPE) {
-      from_slot(slot, kX, k, v);
-    } else {
-      x[k].pairs(v);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = f2_add(v[i], away);
-  }
-};
-
-// KEPT: h in 8 bits; RES: dh is added
-template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bwd_kernel(const __grid_constant__ LnParams p) {
-  using Rows = LnRows<T, VEC, K, KEPT, RES, PIPE>;
+__global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_constant__ LnParams p) {
   __shared__ float2 s_red[kLnMaxTeams][2][kLnMaxWarps];
   extern __shared__ __align__(16) float s_wb[];   // w, at the end [2, D]: teams add up; the slots
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D, S = p.slots;
   const int64_t step = (int64_t)gridDim.x * p.R;
   int64_t row = (int64_t)blockIdx.x * p.R + team;
-  uint8_t* slots = reinterpret_cast<uint8_t*>(s_wb) + p.slots_at;
-  const int slot_bytes = Rows::kSlot * (int)blockDim.x;
+  constexpr int kH = 1, kX = RES ? 2 : 1;   // streams behind dy
+  LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT> rows;
   float mu_next = 0.0f, r_next = 0.0f;
   if (row < p.M) mu_next = p.mean[row], r_next = p.rstd[row];
   if constexpr (PIPE) {
-    for (int i = 0; i < S; ++i) {
-      if (row + i * step < p.M) Rows::fetch(p, slots + i * slot_bytes, row + i * step, wt, lane);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    const int col = wt * kTile + lane * 8;
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, W, col, D, S);
+    rows.stream(0, p.dy, p.dys, row, step, col);
+    if constexpr (RES) rows.stream(kH, p.dh, p.dhs, row, step, col);
+    if constexpr (KEPT) rows.kept(p, row, step, col);
+    else rows.stream(kX, p.x, p.xs, row, step, col);
+    for (int i = 0; i < S; ++i) rows.fetch(i, row + i * step < p.M);
   }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
   uint64_t dw[K][4], db[K][4];
@@ -354,24 +374,38 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bw
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
     const float mu = mu_next, r = r_next;
     if (row + step < p.M) mu_next = p.mean[row + step], r_next = p.rstd[row + step];
-    uint8_t* slot = slots + at * slot_bytes;
-    Rows t;
-    if constexpr (PIPE) {   // all but the S - 1 rows behind this one
-      if (S == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else if (S == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else asm volatile("cp.async.wait_group 3;" ::: "memory");
-    } else {
-      t.read(p, row, wt, lane);
-    }
-    const uint64_t r2 = f2_pack(r, r);
+    const uint64_t away = f2_pack(-mu, -mu), r2 = f2_pack(r, r);
+    auto gradient = [&](const void* from, int64_t pitch, int stream, int k, uint64_t (&g)[4]) {
+      RawTile<T, VEC> t;
+      if constexpr (PIPE) rows.get(at, stream, k, t);
+      else t.load(reinterpret_cast<const T*>(from) + row * pitch, (wt + k * W) * kTile, lane, D);
+      t.pairs(g);
+    };
+    auto centred = [&](int k, uint64_t (&d)[4]) {   // h - mu
+      const int base = (wt + k * W) * kTile;
+      if constexpr (KEPT) {
+        RawCodes<VEC> c;
+        if constexpr (PIPE) rows.get(at, k, c);
+        else c.load(p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
+        c.pairs(d);
+      } else {
+        RawTile<T, VEC> t;
+        if constexpr (PIPE) rows.get(at, kX, k, t);
+        else t.load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
+        t.pairs(d);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = f2_add(d[i], away);
+    };
+    if constexpr (PIPE) rows.wait(S);
     uint64_t t1 = 0ull, t2 = 0ull;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
       if (base >= D) continue;
       uint64_t g[4], n[4], w[4];
-      t.dy(slot, k, g);
-      t.centred(slot, k, mu, n);
+      gradient(p.dy, p.dys, 0, k, g);
+      centred(k, n);
       ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
@@ -385,12 +419,9 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bw
     }
     float s1 = warp_sum(f2_sum(t1)), s2 = warp_sum(f2_sum(t2));
     if (W > 1) {
-      float2(&buf)[kLnMaxWarps] = s_red[team][turn];
-      ln_exchange(buf, make_float2(s1, s2), wt, lane, team, W);
-      s1 = s2 = 0.0f;
-      for (int i = 0; i < W; ++i) s1 += buf[i].x, s2 += buf[i].y;
-    } else {
-      __syncwarp();
+      const float2 o = ln_exchange(s_red[team][turn], make_float2(s1, s2), wt, lane, team, W);
+      s1 = ln_sum16(o.x);
+      s2 = ln_sum16(o.y);
     }
     // dx = r a - r mean a - (h - mu) r^2 mean(a n)
     const float c0 = -r * (s1 * inv_d), c1 = -r * r * (s2 * inv_d);
@@ -400,14 +431,14 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bw
       const int base = (wt + k * W) * kTile;
       if (base >= D) continue;
       uint64_t g[4], d[4], w[4];
-      t.dy(slot, k, g);
-      t.centred(slot, k, mu, d);
+      gradient(p.dy, p.dys, 0, k, g);
+      centred(k, d);
       ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(d[i], c12, c02));
       if constexpr (RES) {
         uint64_t h[4];
-        t.dh(slot, k, h);
+        gradient(p.dh, p.dhs, kH, k, h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] = f2_add(g[i], h[i]);
       }
@@ -416,8 +447,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS < kLnMaxWarps ? 2 : 1) ln_bw
       o.store(reinterpret_cast<T*>(p.dx) + row * D, base, lane, D);
     }
     if constexpr (PIPE) {   // the slot is read: the row S behind this one
-      if (row + S * step < p.M) Rows::fetch(p, slot, row + S * step, wt, lane);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      rows.fetch(at, row + S * step < p.M);
       at = at + 1 == S ? 0 : at + 1;
     }
   }
@@ -534,15 +564,30 @@ void ln_stats(LnParams& p, const at::Tensor& x, const at::Tensor& stats) {
   p.rstd = p.mean + p.M;
 }
 
-// Tiles of a warp, warps of a team, teams of a block: two tiles a warp where 16 warps reach
-// (more columns in flight per barrier than one, and the sums of the backward fit beside them),
-// about 8 warps a block.
+// Tiles of a warp, warps of a team, teams of a block: up to four tiles a warp (what a row costs
+// beside its columns - reductions, a barrier, addresses - is shared by them; 16384 x 5120 with
+// two: forward 136, backward 146 us), about 8 warps a block.
 int ln_shape(LnParams& p) {
   const int tiles = (p.D + kTile - 1) / kTile;
-  const int K = tiles == 1 ? 1 : tiles <= 2 * kLnMaxWarps ? 2 : 4;
+  const int K = tiles <= 2 ? tiles : 4;
   p.W = (tiles + K - 1) / K;
   p.R = std::max(1, kLnMaxTeams / p.W);
   return K;
+}
+
+// Rows under way in shared memory behind `front` bytes: as many of 2 to 4 as leave `blocks`
+// blocks to an SM, fewer blocks where two rows do not fit.  Returns the bytes in all, 0 where
+// not even one block has room for two rows.
+size_t ln_slots(LnParams& p, size_t front, size_t thread_bytes, int blocks) {
+  const size_t slot = thread_bytes * p.W * p.R * 32;
+  for (; blocks > 0; --blocks) {
+    const size_t room = (size_t)(228 * 1024) / blocks - 1024 - 2048;   // (1 KB of the system's, the static arrays)
+    if (front + 2 * slot > std::min<size_t>(room, 224 * 1024)) continue;
+    p.slots = (int)std::min<size_t>(4, (std::min<size_t>(room, 224 * 1024) - front) / slot);
+    p.slots_at = (int)front;
+    return front + p.slots * slot;
+  }
+  return 0;
 }
 
 // Blocks that are resident at once (a kernel's, by its shape), no more than there are rows for
@@ -566,21 +611,32 @@ unsigned ln_grid(F kern, const LnParams& p, size_t smem) {
     default: TORCH_CHECK(false, "layer_norm: bf16, fp16 or fp32");             \
   }
 
+template <typename F>
+static void ln_flags(bool a, bool b, F f) {
+  const std::true_type yes;
+  const std::false_type no;
+  if (a && b) f(yes, yes);
+  else if (a) f(yes, no);
+  else if (b) f(no, yes);
+  else f(no, no);
+}
+
 template <typename T, bool VEC, int K>
-static void ln_fwd_launch(const LnParams& p, cudaStream_t stream) {
-  const size_t smem = (size_t)2 * ((p.D + kTile - 1) / kTile * kTile) * 4;
-  auto go = [&](auto kern) {
+static void ln_fwd_launch(LnParams& p, cudaStream_t stream) {
+  const size_t front = (size_t)2 * ((p.D + kTile - 1) / kTile * kTile) * 4;   // w and b
+  auto go = [&](auto kern, size_t smem) {
     const unsigned grid = ln_grid(kern, p, smem);
     kern<<<grid, p.W * p.R * 32, smem, stream>>>(p);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   };
-  if (p.codes != nullptr) {
-    if (p.delta != nullptr) go(ln_fwd_kernel<T, VEC, K, true, true>);
-    else go(ln_fwd_kernel<T, VEC, K, false, true>);
-  } else {
-    if (p.delta != nullptr) go(ln_fwd_kernel<T, VEC, K, true, false>);
-    else go(ln_fwd_kernel<T, VEC, K, false, false>);
-  }
+  ln_flags(p.delta != nullptr, p.codes != nullptr, [&](auto res, auto keep) {
+    constexpr bool RES = decltype(res)::value, KEEP = decltype(keep)::value;
+    if constexpr (VEC) {
+      const size_t smem = ln_slots(p, front, LnSlots<T, K, RES ? 2 : 1, false>::kBytes, 4);
+      if (smem > 0) return go(ln_fwd_kernel<T, VEC, K, RES, KEEP, true>, smem);
+    }
+    if constexpr (!VEC || K == 4) go(ln_fwd_kernel<T, VEC, K, RES, KEEP, false>, front);
+  });
 }
 
 // h and y [M, D]; stats [2, M] (mean, 1 / deviation), codes and steps where a backward follows
@@ -652,33 +708,14 @@ static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::T
     else if (type == at::kBFloat16) finish(__nv_bfloat16{});
     else finish(__half{});
   };
-  auto shape = [&](auto kept, auto res) {
+  ln_flags(p.codes != nullptr, p.dh != nullptr, [&](auto kept, auto res) {
     constexpr bool KEPT = decltype(kept)::value, RES = decltype(res)::value;
     if constexpr (VEC) {
-      // Rows under way: as many of 2 to 4 as leave two blocks to an SM, or one where that
-      // takes the most of them.
-      const size_t slot = (size_t)LnRows<T, VEC, K, KEPT, RES, true>::kSlot * p.W * p.R * 32;
-      constexpr size_t most = 227 * 1024 - 4096, half = 113 * 1024 - 4096;   // (static arrays and 1 KB a block)
-      const size_t room = front + 2 * slot <= half ? half : most;
-      p.slots = (int)std::min<size_t>(4, front < room ? (room - front) / slot : 0);
-      p.slots_at = (int)front;
-      if (p.slots >= 2) {
-        // (up to 10 warps the registers leave two blocks to an SM)
-        if (K <= 2 && p.W * p.R <= 10) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, K <= 2 ? 10 : kLnMaxWarps>, front + p.slots * slot);
-        return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, kLnMaxWarps>, front + p.slots * slot);
-      }
+      const size_t smem = ln_slots(p, front, LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT>::kBytes, 3);
+      if (smem > 0) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true>, smem);
     }
-    go(ln_bwd_kernel<T, VEC, K, KEPT, RES, false, kLnMaxWarps>, front);
-  };
-  const std::true_type yes;
-  const std::false_type no;
-  if (p.codes != nullptr) {
-    if (p.dh != nullptr) shape(yes, yes);
-    else shape(yes, no);
-  } else {
-    if (p.dh != nullptr) shape(no, yes);
-    else shape(no, no);
-  }
+    if constexpr (!VEC || K == 4) go(ln_bwd_kernel<T, VEC, K, KEPT, RES, false>, front);
+  });
 }
 
 // dx [M, D], dw and db [D] from dy, the kept input (x, or codes and steps) and stats

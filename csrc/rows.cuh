@@ -140,61 +140,81 @@ __device__ __forceinline__ GroupScale group_scale(float a) {
   return g;
 }
 
-// The groups' scales of a tile, for a lane's values: g[0] (VEC: all of them), g[1].
-template <bool VEC>
-__device__ __forceinline__ void tile_scales(const float (&v)[8], GroupScale (&g)[VEC ? 1 : 2]) {
-  if constexpr (VEC) {
-    float a = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(v[i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-    g[0] = group_scale(a);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float a = fabsf(v[4 * h]);
-#pragma unroll
-      for (int i = 1; i < 4; ++i) a = max_nan(a, fabsf(v[4 * h + i]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-      g[h] = group_scale(a);
-    }
-  }
-}
-
 // The nearest whole number to v * inv, ties to even, in the low byte: one fma onto a number
 // whose last place is 1 (the product is not rounded before).
 __device__ __forceinline__ uint32_t code_of(float v, float inv) {
   return __float_as_uint(__fmaf_rn(v, inv, 12582912.0f));
 }
 
-// Writes a tile's codes and steps.
-template <bool VEC>
-__device__ __forceinline__ void keep_tile(const float (&v)[8], int8_t* codes, float* steps, int base, int lane, int D) {
-  GroupScale g[VEC ? 1 : 2];
-  tile_scales<VEC>(v, g);
+// Writes the codes and steps of K tiles of one warp: tile k holds columns [base[k], base[k] + 256)
+// of row `codes[k]`, `steps[k]`; tiles with base[k] >= D are none.  A group's scale is formed
+// by one lane of it (a division and its checks cost as much as the codes of eight elements)
+// and handed to the others.
+template <bool VEC, int K>
+__device__ __forceinline__ void keep_tiles(const uint64_t (&v)[K][4], int8_t* const (&codes)[K], float* const (&steps)[K],
+                                           const int (&base)[K], int lane, int D) {
+  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
   if constexpr (VEC) {
-    uint32_t c[8];
+    float a[K];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code_of(v[i], g[0].inv);
-    const int at = base + lane * 8;
-    if (at < D) {
-      uint2 w;
-      w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-      w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
-      *reinterpret_cast<uint2*>(codes + at) = w;
-      if ((lane & 15) == 0) steps[at / kGroup] = g[0].step;
+    for (int k = 0; k < K; ++k) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f2_unpack(v[k][i], f[2 * i], f[2 * i + 1]);
+      a[k] = max_nan(max_nan(max_nan(fabsf(f[0]), fabsf(f[1])), max_nan(fabsf(f[2]), fabsf(f[3]))),
+                     max_nan(max_nan(fabsf(f[4]), fabsf(f[5])), max_nan(fabsf(f[6]), fabsf(f[7]))));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) a[k] = max_nan(a[k], __shfl_xor_sync(0xffffffffu, a[k], o));
+    }
+    static_assert(K <= 16, "a lane of a group for each tile");
+    float mine = a[0];
+    int at = base[0];
+    float* to = steps[0];
+#pragma unroll
+    for (int k = 1; k < K; ++k)
+      if ((lane & 15) == k) mine = a[k], at = base[k], to = steps[k];
+    const GroupScale g = group_scale(mine);
+    at += (lane & 16) * 8;   // this half's group
+    if ((lane & 15) < K && at < D) to[at / kGroup] = g.step;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float inv = __shfl_sync(0xffffffffu, g.inv, (lane & 16) | k);
+      const uint64_t inv2 = f2_pack(inv, inv);
+      uint32_t c[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        f2_unpack(f2_fma(v[k][i], inv2, magic), lo, hi);
+        c[2 * i] = __float_as_uint(lo), c[2 * i + 1] = __float_as_uint(hi);
+      }
+      const int col = base[k] + lane * 8;
+      if (col < D) {
+        uint2 w;
+        w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+        *reinterpret_cast<uint2*>(codes[k] + col) = w;
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = base + i * 32 + lane;
-      if (at < D) codes[at] = (int8_t)(code_of(v[i], g[i / 4].inv) & 0xffu);
-    }
-    if (lane == 0) {
-      steps[base / kGroup] = g[0].step;
-      if (base + kGroup < D) steps[base / kGroup + 1] = g[1].step;
+    for (int k = 0; k < K; ++k) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f2_unpack(v[k][i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float a = max_nan(max_nan(fabsf(f[4 * h]), fabsf(f[4 * h + 1])), max_nan(fabsf(f[4 * h + 2]), fabsf(f[4 * h + 3])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const GroupScale g = group_scale(a);
+        const int first = base[k] + h * kGroup;
+        if (lane == 0 && first < D) steps[k][first / kGroup] = g.step;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = first + i * 32 + lane;
+          if (col < D) codes[k][col] = (int8_t)(code_of(f[4 * h + i], g.inv) & 0xffu);
+        }
+      }
     }
   }
 }
@@ -228,6 +248,18 @@ struct RawCodes {
     for (int i = 0; i < 8; ++i) {
       const float f = __uint_as_float(__byte_perm(i < 4 ? x : y, 0x4b000000u, 0x7540u + (i & 3)));
       v[i] = __fmul_rn(__fadd_rn(f, -8388736.0f), step[VEC ? 0 : i / 4]);
+    }
+  }
+  __device__ __forceinline__ void pairs(uint64_t (&v)[4]) const {
+    const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+    const uint64_t away = f2_pack(-8388736.0f, -8388736.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t s = i < 2 ? x : y;
+      const float lo = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + (2 * i & 3)));
+      const float hi = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + (2 * i + 1 & 3)));
+      const float t = step[VEC ? 0 : i / 2];
+      v[i] = f2_mul(f2_add(f2_pack(lo, hi), away), f2_pack(t, t));
     }
   }
 };
