@@ -374,28 +374,29 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_c
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
     const float mu = mu_next, r = r_next;
     if (row + step < p.M) mu_next = p.mean[row + step], r_next = p.rstd[row + step];
-    const uint64_t away = f2_pack(-mu, -mu), r2 = f2_pack(r, r);
+    const float off = -mu * r;
+    const uint64_t off2 = f2_pack(off, off), r2 = f2_pack(r, r);
     auto gradient = [&](const void* from, int64_t pitch, int stream, int k, uint64_t (&g)[4]) {
       RawTile<T, VEC> t;
       if constexpr (PIPE) rows.get(at, stream, k, t);
       else t.load(reinterpret_cast<const T*>(from) + row * pitch, (wt + k * W) * kTile, lane, D);
       t.pairs(g);
     };
-    auto centred = [&](int k, uint64_t (&d)[4]) {   // h - mu
+    auto normal = [&](int k, uint64_t (&n)[4]) {   // (h - mu) r
       const int base = (wt + k * W) * kTile;
       if constexpr (KEPT) {
         RawCodes<VEC> c;
         if constexpr (PIPE) rows.get(at, k, c);
         else c.load(p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
-        c.pairs(d);
+        c.scaled(r, off, n);
       } else {
         RawTile<T, VEC> t;
         if constexpr (PIPE) rows.get(at, kX, k, t);
         else t.load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
-        t.pairs(d);
-      }
+        t.pairs(n);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = f2_add(d[i], away);
+        for (int i = 0; i < 4; ++i) n[i] = f2_fma(n[i], r2, off2);
+      }
     };
     if constexpr (PIPE) rows.wait(S);
     uint64_t t1 = 0ull, t2 = 0ull;
@@ -405,11 +406,10 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_c
       if (base >= D) continue;
       uint64_t g[4], n[4], w[4];
       gradient(p.dy, p.dys, 0, k, g);
-      centred(k, n);
+      normal(k, n);
       ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
-        n[i] = f2_mul(n[i], r2);
         dw[k][i] = f2_fma(g[i], n[i], dw[k][i]);
         db[k][i] = f2_add(db[k][i], g[i]);
         g[i] = f2_mul(g[i], w[i]);
@@ -423,19 +423,19 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_c
       s1 = ln_sum16(o.x);
       s2 = ln_sum16(o.y);
     }
-    // dx = r a - r mean a - (h - mu) r^2 mean(a n)
-    const float c0 = -r * (s1 * inv_d), c1 = -r * r * (s2 * inv_d);
+    // dx = r a - r mean a - n r mean(a n)
+    const float c0 = -r * (s1 * inv_d), c1 = -r * (s2 * inv_d);
     const uint64_t c02 = f2_pack(c0, c0), c12 = f2_pack(c1, c1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
       if (base >= D) continue;
-      uint64_t g[4], d[4], w[4];
+      uint64_t g[4], n[4], w[4];
       gradient(p.dy, p.dys, 0, k, g);
-      centred(k, d);
+      normal(k, n);
       ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(d[i], c12, c02));
+      for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(n[i], c12, c02));
       if constexpr (RES) {
         uint64_t h[4];
         gradient(p.dh, p.dhs, kH, k, h);

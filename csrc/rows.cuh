@@ -250,16 +250,17 @@ struct RawCodes {
       v[i] = __fmul_rn(__fadd_rn(f, -8388736.0f), step[VEC ? 0 : i / 4]);
     }
   }
-  __device__ __forceinline__ void pairs(uint64_t (&v)[4]) const {
+  // code * (step * a) + b, in packed pairs
+  __device__ __forceinline__ void scaled(float a, float b, uint64_t (&v)[4]) const {
     const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
-    const uint64_t away = f2_pack(-8388736.0f, -8388736.0f);
+    const uint64_t away = f2_pack(-8388736.0f, -8388736.0f), b2 = f2_pack(b, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t s = i < 2 ? x : y;
       const float lo = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + (2 * i & 3)));
-      const float hi = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + (2 * i + 1 & 3)));
-      const float t = step[VEC ? 0 : i / 2];
-      v[i] = f2_mul(f2_add(f2_pack(lo, hi), away), f2_pack(t, t));
+      const float hi = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + ((2 * i + 1) & 3)));
+      const float t = step[VEC ? 0 : i / 2] * a;
+      v[i] = f2_fma(f2_add(f2_pack(lo, hi), away), f2_pack(t, t), b2);
     }
   }
 };

@@ -1,3 +1,3 @@
-from .decoder import DecoderConfig, DecoderLM, DecoderLayer, RMSNorm, PRESETS, get_config
+from .decoder import DecoderConfig, DecoderLM, DecoderLayer, LayerNorm, RMSNorm, PRESETS, get_config
 
-__all__ = ["DecoderConfig", "DecoderLM", "DecoderLayer", "RMSNorm", "PRESETS", "get_config"]
+__all__ = ["DecoderConfig", "DecoderLM", "DecoderLayer", "LayerNorm", "RMSNorm", "PRESETS", "get_config"]

@@ -33,12 +33,15 @@ import torch
 import torch.nn as nn
 import torch.utils.checkpoint as ckpt
 
+from ..ops.act8 import check_saved, checkpoint_8bit
 from ..ops.activations import gelu, swiglu
 from ..ops.attention import flash_attention, flash_attention_varlen
 from ..ops.cross_entropy import cross_entropy, lm_head_cross_entropy
 from ..ops.distill import distillation_loss
+from ..ops.embedding import embedding
 from ..ops.gemm import LMHeadFunction
-from ..ops.norm import add_rmsnorm
+from ..ops.logprobs import TokenLogprobs, token_logprobs
+from ..ops.norm import add_layer_norm, add_rmsnorm
 from ..ops.packed import PackedSequences
 from ..ops.qlinear import Linear4bit
 from ..ops.qkv import qkv_fusable, qkv_projection
@@ -60,6 +63,10 @@ class DecoderConfig:
     rope_theta: float = 10000.0
     rope_scaling: Optional[RopeScaling] = None   # for contexts longer than trained on
     norm_eps: float = 1e-6
+    norm: str = "rmsnorm"    # "rmsnorm" | "layernorm" (with a bias)
+    # factor on the embedding's rows (the embedding operator, whose gradient is summed by
+    # sorted tokens); None: torch's lookup
+    embed_scale: Optional[float] = None
     tie_embeddings: bool = True
     vocab_pad_multiple: int = 128
     # LoRA (PEFT naming); targets are projection names
@@ -71,6 +78,10 @@ class DecoderConfig:
     quant_type: str = "nf4"
     # memory
     activation_checkpointing: bool = False
+    # "8bit": what a layer keeps for the backward is held in 8 bits - the inputs of checkpointed
+    # layers; without checkpoints those of the activation function and of layer norms (the
+    # activation then runs apart from the projections' GEMMs)
+    saved_activations: str = "full"
     # > 0: LM head + cross-entropy over vocabulary chunks of this many columns
     # (the [tokens, vocab] logits are never materialised; frozen head only).
     # Off by default: it trades one extra head GEMM for the logits' memory
@@ -91,7 +102,8 @@ class DecoderConfig:
             attn += (self.n_heads + 2 * self.n_kv_heads) * self.head_dim
         mlp = d * self.ffn_dim * (3 if self.ffn_act == "swiglu" else 2)
         emb = self.vocab_size * d * (1 if self.tie_embeddings else 2)
-        return L * (attn + mlp + 2 * d) + emb + d
+        norm = d * (2 if self.norm == "layernorm" else 1)
+        return L * (attn + mlp + 2 * norm) + emb + norm
 
     def to_dict(self) -> dict:
         return asdict(self)
@@ -142,6 +154,43 @@ class RMSNorm(nn.Module):
         return add_rmsnorm(h, delta, self.weight, self.eps)
 
 
+class LayerNorm(nn.Module):
+    """Layer norm with the call of :class:`RMSNorm`; ``saved="8bit"`` keeps its input in 8 bits
+    for the backward."""
+
+    def __init__(self, d: int, eps: float, device=None, trainable: bool = True, saved: str = "full"):
+        super().__init__()
+        self.eps = eps
+        self.saved = saved
+        self.weight = nn.Parameter(torch.ones(d, device=device, dtype=torch.float32), requires_grad=trainable)
+        self.bias = nn.Parameter(torch.zeros(d, device=device, dtype=torch.float32), requires_grad=trainable)
+
+    def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor] = None):
+        out = add_layer_norm(h, delta, self.weight, self.bias, self.eps, self.saved)
+        return out[1] if delta is None else out
+
+
+class Embedding(nn.Embedding):
+    """A table whose rows are looked up times ``scale`` (ids outside it give rows of zeros)."""
+
+    def __init__(self, rows: int, d: int, scale: float, device=None, dtype=None):
+        super().__init__(rows, d, device=device, dtype=dtype)
+        self.scale = scale
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return embedding(ids, self.weight, self.scale)
+
+
+def make_norm(cfg: "DecoderConfig", device=None) -> nn.Module:
+    if cfg.norm == "rmsnorm":
+        return RMSNorm(cfg.d_model, cfg.norm_eps, device, cfg.train_norms)
+    if cfg.norm != "layernorm":
+        raise ValueError(f"norm is 'rmsnorm' or 'layernorm', got {cfg.norm!r}")
+    # (a checkpointed layer keeps its inputs alone)
+    saved = "full" if cfg.activation_checkpointing else cfg.saved_activations
+    return LayerNorm(cfg.d_model, cfg.norm_eps, device, cfg.train_norms, saved)
+
+
 # ZEROQ_FUSED_MLP=0 keeps the activation kernels between the MLP projections
 # (the split forms with GEMM-epilogue activations are the default)
 _FUSED_MLP = os.environ.get("ZEROQ_FUSED_MLP", "1") != "0"
@@ -157,6 +206,8 @@ class DecoderLayer(nn.Module):
         super().__init__()
         self.cfg = cfg
         d, hd = cfg.d_model, cfg.head_dim
+        # the activation's inputs in 8 bits (a checkpointed layer keeps its inputs alone)
+        self.act_saved = "full" if cfg.activation_checkpointing else cfg.saved_activations
 
         def lin(name, i, o):
             r = cfg.lora_r if name in cfg.lora_targets else 0
@@ -165,12 +216,12 @@ class DecoderLayer(nn.Module):
                               quant_type=cfg.quant_type, lora_r=r, lora_alpha=cfg.lora_alpha,
                               device=device, dtype=dtype)
 
-        self.attn_norm = RMSNorm(d, cfg.norm_eps, device, cfg.train_norms)
+        self.attn_norm = make_norm(cfg, device)
         self.q_proj = lin("q_proj", d, cfg.n_heads * hd)
         self.k_proj = lin("k_proj", d, cfg.n_kv_heads * hd)
         self.v_proj = lin("v_proj", d, cfg.n_kv_heads * hd)
         self.o_proj = lin("o_proj", cfg.n_heads * hd, d)
-        self.mlp_norm = RMSNorm(d, cfg.norm_eps, device, cfg.train_norms)
+        self.mlp_norm = make_norm(cfg, device)
         if cfg.ffn_act == "swiglu":
             self.gate_proj = lin("gate_proj", d, cfg.ffn_dim)
         else:
@@ -245,14 +296,14 @@ class DecoderLayer(nn.Module):
                 g = self.gate_proj(x)
                 u, f = self.up_proj(x, act_out="swiglu", gate=g)
                 return h, self.down_proj(f, pre=(g, u))
-            f = swiglu(self.gate_proj(x), self.up_proj(x))
+            f = swiglu(self.gate_proj(x), self.up_proj(x), saved=self.act_saved)
         elif self._fused_gelu_mlp():
             # up-projection epilogue writes h and gelu(h); the down-projection's
             # input-gradient epilogue applies gelu'(h): no GELU kernels
             pre, f = self.up_proj(x, act_out="gelu")
             return h, self.down_proj(f, pre=pre)
         else:
-            f = gelu(self.up_proj(x))
+            f = gelu(self.up_proj(x), saved=self.act_saved)
         return h, self.down_proj(f)
 
     def _fused_rope(self, x: torch.Tensor) -> bool:
@@ -270,7 +321,7 @@ class DecoderLayer(nn.Module):
         from ..ops.qlinear import Linear4bit
 
         mods = (self.up_proj, self.down_proj) + ((self.gate_proj,) if with_gate else ())
-        return (_FUSED_MLP and all(isinstance(m, Linear4bit) for m in mods)
+        return (_FUSED_MLP and self.act_saved == "full" and all(isinstance(m, Linear4bit) for m in mods)
                 and not any(_hooked(m) for m in mods))
 
     def _fused_gelu_mlp(self) -> bool:
@@ -282,11 +333,15 @@ class DecoderLM(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.dtype = dtype
+        check_saved("saved_activations", cfg.saved_activations)
         V = cfg.vocab_padded
-        self.embed_tokens = nn.Embedding(V, cfg.d_model, device=device, dtype=dtype)
+        if cfg.embed_scale is None:
+            self.embed_tokens = nn.Embedding(V, cfg.d_model, device=device, dtype=dtype)
+        else:
+            self.embed_tokens = Embedding(V, cfg.d_model, cfg.embed_scale, device=device, dtype=dtype)
         self.embed_tokens.weight.requires_grad_(cfg.train_embeddings)
         self.layers = nn.ModuleList([DecoderLayer(cfg, device, dtype) for _ in range(cfg.n_layers)])
-        self.norm = RMSNorm(cfg.d_model, cfg.norm_eps, device, cfg.train_norms)
+        self.norm = make_norm(cfg, device)
         if cfg.tie_embeddings:
             self.lm_head = None
         else:
@@ -362,6 +417,8 @@ class DecoderLM(nn.Module):
     def _layer_call(self, layer, h, delta, seqs=None):
         more = () if seqs is None else (seqs,)
         if self.cfg.activation_checkpointing and self.training and torch.is_grad_enabled():
+            if self.cfg.saved_activations == "8bit":
+                return checkpoint_8bit(layer, h, delta, *more)
             if delta is None:
                 return ckpt.checkpoint(lambda hh: layer(hh, None, *more), h, use_reentrant=False)
             return ckpt.checkpoint(layer, h, delta, *more, use_reentrant=False)
@@ -381,6 +438,37 @@ class DecoderLM(nn.Module):
         over whole logits and with a gradient of their size beside them (``ce_chunk`` holds for
         the hard targets alone)."""
         B, S = input_ids.shape
+        if teacher is not None and targets is None:
+            raise ValueError("a teacher's entries need targets")
+        x, W = self._hidden(input_ids, cu_seqlens)
+        if targets is not None and teacher is None and self.cfg.ce_chunk > 0:
+            return lm_head_cross_entropy(x, W, targets.reshape(-1), vocab=self.cfg.vocab_size,
+                                         ignore_index=ignore_index, chunk=self.cfg.ce_chunk)
+        logits = LMHeadFunction.apply(x, W)
+        if targets is None:
+            return logits.view(B, S, -1)[..., : self.cfg.vocab_size]
+        if teacher is not None:
+            ids, top = (t.reshape(-1, t.shape[-1]) for t in teacher)
+            return distillation_loss(logits, ids, top, targets.reshape(-1), temperature=temperature, alpha=alpha,
+                                     vocab=self.cfg.vocab_size, ignore_index=ignore_index)
+        return cross_entropy(logits, targets.reshape(-1), vocab=self.cfg.vocab_size,
+                             ignore_index=ignore_index)
+
+    def logprobs(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0,
+                 temperature: float = 1.0, ignore_index: int = -100, cu_seqlens=None) -> TokenLogprobs:
+        """:func:`~zeroq_b200.ops.logprobs.token_logprobs` of every position, ``[B, S]`` and
+        ``[B, S, top_k]``: the log probability of its target, the entropy and the top
+        alternatives, all with gradients (policy training); ``(top_ids, top_logprobs)`` is a
+        ``teacher`` of :meth:`forward`."""
+        B, S = input_ids.shape
+        x, W = self._hidden(input_ids, cu_seqlens)
+        out = token_logprobs(LMHeadFunction.apply(x, W), None if targets is None else targets.reshape(-1), top_k,
+                             temperature, vocab=self.cfg.vocab_size, ignore_index=ignore_index)
+        return TokenLogprobs(*(None if t is None else t.view(B, S, *t.shape[1:]) for t in out))
+
+    def _hidden(self, input_ids: torch.Tensor, cu_seqlens=None):
+        """The last norm's output and the head's weight."""
+        B, S = input_ids.shape
         seqs = None
         if cu_seqlens is not None:
             if B != 1:
@@ -390,8 +478,6 @@ class DecoderLM(nn.Module):
                 seqs = PackedSequences(seqs, S, device=input_ids.device)
             if seqs.total != S:
                 raise ValueError(f"the sequences divide {seqs.total} rows, the batch has {S}")
-        if teacher is not None and targets is None:
-            raise ValueError("a teacher's entries need targets")
         h = self.embed_tokens(input_ids)
         delta = None
         cb = getattr(self, "_layer_grad_cb", None)
@@ -407,18 +493,7 @@ class DecoderLM(nn.Module):
         if W.numel() == 0:
             raise RuntimeError("the LM head weight is sharded and not gathered here; keep "
                                "'embed_tokens' and 'lm_head' in exclude_modules")
-        if targets is not None and teacher is None and self.cfg.ce_chunk > 0:
-            return lm_head_cross_entropy(x, W, targets.reshape(-1), vocab=self.cfg.vocab_size,
-                                         ignore_index=ignore_index, chunk=self.cfg.ce_chunk)
-        logits = LMHeadFunction.apply(x, W)
-        if targets is None:
-            return logits.view(B, S, -1)[..., : self.cfg.vocab_size]
-        if teacher is not None:
-            ids, top = (t.reshape(-1, t.shape[-1]) for t in teacher)
-            return distillation_loss(logits, ids, top, targets.reshape(-1), temperature=temperature, alpha=alpha,
-                                     vocab=self.cfg.vocab_size, ignore_index=ignore_index)
-        return cross_entropy(logits, targets.reshape(-1), vocab=self.cfg.vocab_size,
-                             ignore_index=ignore_index)
+        return x, W
 
     # -- bookkeeping ---------------------------------------------------------------
     def trainable_parameters(self):

@@ -29,6 +29,8 @@ import torch
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
+from ..ops.act8 import check_saved, checkpoint_8bit
+
 _LAYER_PATTERNS = ["model.layers", "transformer.h", "encoder.layer", "decoder.layers", "layers"]
 
 
@@ -58,13 +60,15 @@ def _get_layer_by_name(model: nn.Module, name: str) -> Optional[nn.Module]:
     return cur
 
 
-def _wrap_layer_with_checkpoint(layer: nn.Module, use_reentrant: bool):
+def _wrap_layer_with_checkpoint(layer: nn.Module, use_reentrant: bool, saved: str = "full"):
     if getattr(layer, "_zq_ckpt_wrapped", False):
         return
     original = layer.forward
 
     def checkpointed_forward(*args, **kwargs):
         if torch.is_grad_enabled():
+            if saved == "8bit":
+                return checkpoint_8bit(original, *args, **kwargs)
             return checkpoint(original, *args, use_reentrant=use_reentrant, **kwargs)
         return original(*args, **kwargs)
 
@@ -73,10 +77,17 @@ def _wrap_layer_with_checkpoint(layer: nn.Module, use_reentrant: bool):
 
 
 def enable_gradient_checkpointing(model: nn.Module, checkpoint_layers: Optional[List[str]] = None,
-                                  use_reentrant: bool = False):
+                                  use_reentrant: bool = False, saved: str = "full"):
+    """``saved="8bit"``: the wrapped layers keep their inputs in 8 bits
+    (:func:`~zeroq_b200.ops.act8.checkpoint_8bit`, without reentrance)."""
+    keep8 = check_saved("enable_gradient_checkpointing", saved)
+    if keep8 and use_reentrant:
+        raise ValueError("enable_gradient_checkpointing: saved='8bit' goes without reentrance")
     if checkpoint_layers is None:
         checkpoint_layers = _auto_detect_layers(model)
     if not checkpoint_layers:
+        if keep8:
+            raise ValueError("enable_gradient_checkpointing: saved='8bit' needs layers to wrap, found none")
         if hasattr(model, "gradient_checkpointing_enable"):
             model.gradient_checkpointing_enable(
                 gradient_checkpointing_kwargs={"use_reentrant": use_reentrant})
@@ -84,7 +95,7 @@ def enable_gradient_checkpointing(model: nn.Module, checkpoint_layers: Optional[
     for name in checkpoint_layers:
         layer = _get_layer_by_name(model, name)
         if layer is not None:
-            _wrap_layer_with_checkpoint(layer, use_reentrant)
+            _wrap_layer_with_checkpoint(layer, use_reentrant, saved)
 
 
 class ZeroQCheckpointedModule(nn.Module):
