@@ -25,8 +25,9 @@
 
 namespace zq {
 
-constexpr int kLnMaxWarps = 16;   // of a team
-constexpr int kLnMaxTeams = 8;    // of a block
+constexpr int kLnMaxWarps = 16;     // of a team
+constexpr int kLnBlockWarps = 24;   // of a block: 80 registers a thread
+constexpr int kLnMaxTeams = kLnBlockWarps / 2;   // of several warps
 
 struct LnParams {
   const void *x, *delta, *dy, *dh;   // rows of pitch xs, ds, dys, dhs
@@ -39,7 +40,9 @@ struct LnParams {
   float* part;                       // [grid, 2, D]
   int64_t M, P, G;
   int D, wt, W, R;                   // warps of a team, teams of a block
-  int slots, slots_at;               // rows under way in shared memory, where they begin
+  int slots, slots_at;               // groups of rows under way in shared memory, where they begin
+  const void* src[3];                // the tensors that go through it, in the kernel's order
+  int64_t pitch[3];
   float eps;
 };
 
@@ -122,79 +125,74 @@ template <typename T, int K, int NS, bool CODES>
 struct LnSlots {
   static constexpr int kVecs = (int)sizeof(T) / 2;   // 16-byte vectors of a lane's 8 elements
   static constexpr int kBytes = K * (16 * kVecs * NS + (CODES ? 12 : 0));   // of a thread
-  const T* from[NS];   // this thread's columns of tile 0 in the row to be fetched next
-  int64_t pitch[NS];
-  const int8_t* codes;
-  const float* steps;
-  int64_t cpitch, spitch;
-  uint32_t slots, slot_bytes, vec, eight, four;   // shared addresses: begin, of a slot, this thread's places in one
-  int tile;            // columns from tile k to k + 1
+  uint32_t mine;       // shared address of this thread's vectors in the first slot
+  uint32_t slot_bytes; // from slot to slot
   uint32_t there;      // bit k: tile k has columns here
+  int col;             // this thread's first column
 
-  __device__ __forceinline__ void init(uint8_t* smem, int W, int col, int D, int S) {
-    tile = W * kTile;
+  // A warp's places in a slot: [tensor][tile][vector][lane] of 16 bytes, codes (8), steps (4).
+  static constexpr int kEight = 512 * K * kVecs * NS, kFour = kEight + 256 * K;
+  static __device__ __forceinline__ uint32_t vec(int i) { return 512u * i; }
+  __device__ __forceinline__ uint32_t eight(int k) const { return kEight + 256u * k - 8u * (threadIdx.x & 31); }
+  __device__ __forceinline__ uint32_t four(int k) const { return kFour + 128u * k - 12u * (threadIdx.x & 31); }
+
+  __device__ __forceinline__ void init(uint8_t* smem, const LnParams& p, int first, int n) {
+    col = first;
     there = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) there |= (col + k * tile < D ? 1u : 0u) << k;
-    slots = smem_u32(smem);
+    for (int k = 0; k < K; ++k) there |= (col + k * p.W * kTile < p.D ? 1u : 0u) << k;
+    mine = smem_u32(smem) + (threadIdx.x >> 5) * (32u * kBytes) + 16u * (threadIdx.x & 31);
     slot_bytes = (uint32_t)kBytes * blockDim.x;
-    vec = threadIdx.x * 16;
-    eight = 16u * K * kVecs * NS * blockDim.x + threadIdx.x * 8;
-    four = (16u * K * kVecs * NS + 8u * K) * blockDim.x + threadIdx.x * 4;
     if (there + 1 != 1u << K) {   // places that are never filled hold zeros
-      for (int s = 0; s < S; ++s) {
-        const uint32_t at = slots + s * slot_bytes;
+      for (int s = 0; s < n; ++s) {
+        const uint32_t at = mine + s * slot_bytes;
 #pragma unroll
         for (int i = 0; i < NS * K * kVecs; ++i)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + vec + 16u * i * blockDim.x), "r"(0) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + vec(i)), "r"(0) : "memory");
         if constexpr (CODES) {
 #pragma unroll
           for (int k = 0; k < K; ++k) {
-            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + eight + 8u * k * blockDim.x), "r"(0) : "memory");
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + four + 4u * k * blockDim.x), "r"(0) : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + eight(k)), "r"(0) : "memory");
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + four(k)), "r"(0) : "memory");
           }
         }
       }
     }
   }
-  __device__ __forceinline__ void stream(int i, const void* base, int64_t p, int64_t row, int64_t step, int col) {
-    from[i] = reinterpret_cast<const T*>(base) + row * p + col;
-    pitch[i] = step * p;
-  }
-  __device__ __forceinline__ void kept(const LnParams& p, int64_t row, int64_t step, int col) {
-    codes = p.codes + row * p.P + col;
-    steps = p.steps + row * p.G + col / kGroup;
-    cpitch = step * p.P;
-    spitch = step * p.G;
-  }
-  // fetches a row (where there is one) and goes on to the next
-  __device__ __forceinline__ void fetch(int slot, bool any) {
-    const uint32_t at = slots + slot * slot_bytes;
-    if (any) {
+  // fetches rows [row, row + B) of M into slots [group B, group B + B), as one group of copies
+  template <int B>
+  __device__ __forceinline__ void fetch(const LnParams& p, int group, int64_t first) const {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (there >> k & 1u) {
+    for (int b = 0; b < B; ++b) {
+      const uint32_t at = mine + (group * B + b) * slot_bytes;
+      const int64_t row = first + b;
+      if (row >= p.M) continue;
 #pragma unroll
-          for (int i = 0; i < NS; ++i)
+      for (int i = 0; i < NS; ++i) {
+        const T* from = reinterpret_cast<const T*>(p.src[i]) + row * p.pitch[i] + col;
 #pragma unroll
-            for (int v = 0; v < kVecs; ++v)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + vec + 16u * ((i * K + k) * kVecs + v) * blockDim.x),
-                           "l"(from[i] + k * tile + v * (16 / (int)sizeof(T)))
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v)
+            if (there >> k & 1u)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + vec((i * K + k) * kVecs + v)),
+                           "l"(from + k * p.W * kTile + v * (16 / (int)sizeof(T)))
                            : "memory");
-          if constexpr (CODES) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at + eight + 8u * k * blockDim.x), "l"(codes + k * tile)
-                         : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + four + 4u * k * blockDim.x),
-                         "l"(steps + k * (tile / kGroup))
+      }
+      if constexpr (CODES) {
+        const int8_t* codes = p.codes + row * p.P + col;
+        const float* steps = p.steps + row * p.G + col / kGroup;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (there >> k & 1u) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at + eight(k)), "l"(codes + k * p.W * kTile) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + four(k)), "l"(steps + k * p.W * (kTile / kGroup))
                          : "memory");
           }
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < NS; ++i) from[i] += pitch[i];
-    if constexpr (CODES) codes += cpitch, steps += spitch;
   }
   // until all but the last S - 1 fetches are there
   static __device__ __forceinline__ void wait(int S) {
@@ -207,13 +205,13 @@ struct LnSlots {
     for (int v = 0; v < kVecs; ++v)
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(t.w[4 * v]), "=r"(t.w[4 * v + 1]), "=r"(t.w[4 * v + 2]), "=r"(t.w[4 * v + 3])
-                   : "r"(slots + slot * slot_bytes + vec + 16u * ((i * K + k) * kVecs + v) * blockDim.x)
+                   : "r"(mine + slot * slot_bytes + vec((i * K + k) * kVecs + v))
                    : "memory");
   }
   __device__ __forceinline__ void get(int slot, int k, RawCodes<true>& c) const {
-    const uint32_t at = slots + slot * slot_bytes;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(c.w.x), "=r"(c.w.y) : "r"(at + eight + 8u * k * blockDim.x) : "memory");
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c.step[0]) : "r"(at + four + 4u * k * blockDim.x) : "memory");
+    const uint32_t at = mine + slot * slot_bytes;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(c.w.x), "=r"(c.w.y) : "r"(at + eight(k)) : "memory");
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c.step[0]) : "r"(at + four(k)) : "memory");
   }
 };
 
@@ -230,11 +228,8 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   int64_t row = (int64_t)blockIdx.x * p.R + team;
   LnSlots<T, K, RES ? 2 : 1, false> rows;
   if constexpr (PIPE) {
-    const int col = wt * kTile + lane * 8;
-    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, W, col, D, S);
-    rows.stream(0, p.x, p.xs, row, step, col);
-    if constexpr (RES) rows.stream(1, p.delta, p.ds, row, step, col);
-    for (int i = 0; i < S; ++i) rows.fetch(i, row + i * step < p.M);
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile + lane * 8, S);
+    for (int i = 0; i < S; ++i) rows.template fetch<1>(p, i, row + i * step);
   }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
   ln_stage<VEC>(s_wb + whole, p.b, p.wt, 0.0f, D);
@@ -277,7 +272,7 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       for (int i = 0; i < 4; ++i) s = f2_add(s, v[k][i]);
     float mu = warp_sum(f2_sum(s)) * inv_cols, q = 0.0f;
     if constexpr (PIPE) {   // the slot is read
-      rows.fetch(at, row + S * step < p.M);
+      rows.template fetch<1>(p, at, row + S * step);
       at = at + 1 == S ? 0 : at + 1;
     }
     {
@@ -321,7 +316,8 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       for (int k = 0; k < K; ++k) c[k] = p.codes + row * p.P, t[k] = p.steps + row * p.G, base[k] = (wt + k * W) * kTile;
       keep_tiles<VEC, K>(v, c, t, base, lane, D);
     }
-    const uint64_t away = f2_pack(-mu, -mu), r2 = f2_pack(r, r);
+    const float off = -mu * r;
+    const uint64_t off2 = f2_pack(off, off), r2 = f2_pack(r, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
@@ -330,7 +326,7 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       ln_staged<VEC>(s_wb, base, lane, w);
       ln_staged<VEC>(s_wb + whole, base, lane, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[k][i] = f2_fma(f2_mul(f2_add(v[k][i], away), r2), w[i], b[i]);
+      for (int i = 0; i < 4; ++i) v[k][i] = f2_fma(f2_fma(v[k][i], r2, off2), w[i], b[i]);
       RawTile<T, VEC> y;
       y.set(v[k]);
       y.store(reinterpret_cast<T*>(p.y) + row * D, base, lane, D);
@@ -338,28 +334,24 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   }
 }
 
-// KEPT: h in 8 bits; RES: dh is added.  A row is read twice (through shared memory, or from the
-// caches): for its sums, and for dx once they are known.
-template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE>
-__global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_constant__ LnParams p) {
-  __shared__ float2 s_red[kLnMaxTeams][2][kLnMaxWarps];
+// KEPT: h in 8 bits; RES: dh is added.  A team takes two consecutive rows at a time, which share
+// the reductions' barrier and latencies.  A row is read twice (through shared memory, or from the
+// caches): for its sums, and for dx once they are known; there are no registers to hold it.
+constexpr int kLnRows = 2;
+template <typename T, bool VEC, int K, bool KEPT, bool RES, bool PIPE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constant__ LnParams p) {
+  constexpr int B = kLnRows;
+  __shared__ float s_red[kLnMaxTeams][2][kLnMaxWarps][2 * B];
   extern __shared__ __align__(16) float s_wb[];   // w, at the end [2, D]: teams add up; the slots
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int W = p.W, team = warp / W, wt = warp - team * W, D = p.D, S = p.slots;
-  const int64_t step = (int64_t)gridDim.x * p.R;
-  int64_t row = (int64_t)blockIdx.x * p.R + team;
-  constexpr int kH = 1, kX = RES ? 2 : 1;   // streams behind dy
+  const int64_t step = (int64_t)gridDim.x * p.R * B;
+  int64_t row = ((int64_t)blockIdx.x * p.R + team) * B;
+  constexpr int kH = 1, kX = RES ? 2 : 1;   // tensors behind dy
   LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT> rows;
-  float mu_next = 0.0f, r_next = 0.0f;
-  if (row < p.M) mu_next = p.mean[row], r_next = p.rstd[row];
   if constexpr (PIPE) {
-    const int col = wt * kTile + lane * 8;
-    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, W, col, D, S);
-    rows.stream(0, p.dy, p.dys, row, step, col);
-    if constexpr (RES) rows.stream(kH, p.dh, p.dhs, row, step, col);
-    if constexpr (KEPT) rows.kept(p, row, step, col);
-    else rows.stream(kX, p.x, p.xs, row, step, col);
-    for (int i = 0; i < S; ++i) rows.fetch(i, row + i * step < p.M);
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile + lane * 8, S * B);
+    for (int i = 0; i < S; ++i) rows.template fetch<B>(p, i, row + i * step);
   }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
   uint64_t dw[K][4], db[K][4];
@@ -370,84 +362,123 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_bwd_kernel(const __grid_c
   const float inv_d = 1.0f / (float)D;
   __syncthreads();
 
-  int at = 0;   // the row's slot
+  int at = 0;   // the rows' group of slots
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
-    const float mu = mu_next, r = r_next;
-    if (row + step < p.M) mu_next = p.mean[row + step], r_next = p.rstd[row + step];
-    const float off = -mu * r;
-    const uint64_t off2 = f2_pack(off, off), r2 = f2_pack(r, r);
-    auto gradient = [&](const void* from, int64_t pitch, int stream, int k, uint64_t (&g)[4]) {
+    const bool second = row + 1 < p.M;
+    float mu[B], r[B];
+    mu[0] = p.mean[row], r[0] = p.rstd[row];
+    mu[1] = second ? p.mean[row + 1] : 0.0f, r[1] = second ? p.rstd[row + 1] : 0.0f;
+    auto gradient = [&](const void* from, int64_t pitch, int stream, int b, int k, uint64_t (&g)[4]) {
       RawTile<T, VEC> t;
-      if constexpr (PIPE) rows.get(at, stream, k, t);
-      else t.load(reinterpret_cast<const T*>(from) + row * pitch, (wt + k * W) * kTile, lane, D);
+      if constexpr (PIPE) rows.get(at * B + b, stream, k, t);
+      else t.load(reinterpret_cast<const T*>(from) + (row + b) * pitch, (wt + k * W) * kTile, lane, D);
       t.pairs(g);
     };
-    auto normal = [&](int k, uint64_t (&n)[4]) {   // (h - mu) r
+    auto normal = [&](int b, int k, uint64_t (&n)[4]) {   // (h - mu) r
       const int base = (wt + k * W) * kTile;
+      const float off = -mu[b] * r[b];
       if constexpr (KEPT) {
         RawCodes<VEC> c;
-        if constexpr (PIPE) rows.get(at, k, c);
-        else c.load(p.codes + row * p.P, p.steps + row * p.G, base, lane, D);
-        c.scaled(r, off, n);
+        if constexpr (PIPE) rows.get(at * B + b, k, c);
+        else c.load(p.codes + (row + b) * p.P, p.steps + (row + b) * p.G, base, lane, D);
+        c.scaled(r[b], off, n);
       } else {
         RawTile<T, VEC> t;
-        if constexpr (PIPE) rows.get(at, kX, k, t);
-        else t.load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
+        if constexpr (PIPE) rows.get(at * B + b, kX, k, t);
+        else t.load(reinterpret_cast<const T*>(p.x) + (row + b) * p.xs, base, lane, D);
         t.pairs(n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = f2_fma(n[i], r2, off2);
+        for (int i = 0; i < 4; ++i) n[i] = f2_fma(n[i], f2_pack(r[b], r[b]), f2_pack(off, off));
       }
     };
     if constexpr (PIPE) rows.wait(S);
-    uint64_t t1 = 0ull, t2 = 0ull;
+    float s[2 * B];   // sums of a and a n of each row
+    {
+      uint64_t t[2 * B];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int base = (wt + k * W) * kTile;
-      if (base >= D) continue;
-      uint64_t g[4], n[4], w[4];
-      gradient(p.dy, p.dys, 0, k, g);
-      normal(k, n);
-      ln_staged<VEC>(s_wb, base, lane, w);
+      for (int i = 0; i < 2 * B; ++i) t[i] = 0ull;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
-        dw[k][i] = f2_fma(g[i], n[i], dw[k][i]);
-        db[k][i] = f2_add(db[k][i], g[i]);
-        g[i] = f2_mul(g[i], w[i]);
-        t1 = f2_add(t1, g[i]);
-        t2 = f2_fma(g[i], n[i], t2);
+      for (int k = 0; k < K; ++k) {
+        const int base = (wt + k * W) * kTile;
+        if (base >= D) continue;
+        uint64_t w[4];
+        ln_staged<VEC>(s_wb, base, lane, w);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          if (b > 0 && !second) continue;
+          uint64_t g[4], n[4];
+          gradient(p.dy, p.dys, 0, b, k, g);
+          normal(b, k, n);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
+            dw[k][i] = f2_fma(g[i], n[i], dw[k][i]);
+            db[k][i] = f2_add(db[k][i], g[i]);
+            g[i] = f2_mul(g[i], w[i]);
+            t[2 * b] = f2_add(t[2 * b], g[i]);
+            t[2 * b + 1] = f2_fma(g[i], n[i], t[2 * b + 1]);
+          }
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 2 * B; ++i) s[i] = f2_sum(t[i]);
     }
-    float s1 = warp_sum(f2_sum(t1)), s2 = warp_sum(f2_sum(t2));
-    if (W > 1) {
-      const float2 o = ln_exchange(s_red[team][turn], make_float2(s1, s2), wt, lane, team, W);
-      s1 = ln_sum16(o.x);
-      s2 = ln_sum16(o.y);
+    // Four sums over a warp: lanes swap what they do not go on with, so that lane i ends with
+    // number i & 3; then over the team.
+    static_assert(B == 2, "four sums");
+    float v;
+    {
+      const bool odd = lane & 1, high = lane & 2;
+      const float a = (odd ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, odd ? s[0] : s[1], 1);
+      const float c = (odd ? s[3] : s[2]) + __shfl_xor_sync(0xffffffffu, odd ? s[2] : s[3], 1);
+      v = (high ? c : a) + __shfl_xor_sync(0xffffffffu, high ? a : c, 2);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
+    if (W > 1) {   // (buffers in turn: see ln_exchange)
+      float(&buf)[kLnMaxWarps][2 * B] = s_red[team][turn];
+      if (lane < 2 * B) buf[wt][lane] = v;
+      named_barrier(1 + team, W * 32);
+      v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kLnMaxWarps; i += 8) {
+        const int from = i + (lane >> 2);
+        if (from < W) v += buf[from][lane & 3];
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * B; ++i) s[i] = __shfl_sync(0xffffffffu, v, i) * inv_d;
     // dx = r a - r mean a - n r mean(a n)
-    const float c0 = -r * (s1 * inv_d), c1 = -r * (s2 * inv_d);
-    const uint64_t c02 = f2_pack(c0, c0), c12 = f2_pack(c1, c1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
       if (base >= D) continue;
-      uint64_t g[4], n[4], w[4];
-      gradient(p.dy, p.dys, 0, k, g);
-      normal(k, n);
+      uint64_t w[4];
       ln_staged<VEC>(s_wb, base, lane, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(n[i], c12, c02));
-      if constexpr (RES) {
-        uint64_t h[4];
-        gradient(p.dh, p.dhs, kH, k, h);
+      for (int b = 0; b < B; ++b) {
+        if (b > 0 && !second) continue;
+        const float c0 = -r[b] * s[2 * b], c1 = -r[b] * s[2 * b + 1];
+        const uint64_t c02 = f2_pack(c0, c0), c12 = f2_pack(c1, c1), r2 = f2_pack(r[b], r[b]);
+        uint64_t g[4], n[4];
+        gradient(p.dy, p.dys, 0, b, k, g);
+        normal(b, k, n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) g[i] = f2_add(g[i], h[i]);
+        for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(n[i], c12, c02));
+        if constexpr (RES) {
+          uint64_t h[4];
+          gradient(p.dh, p.dhs, kH, b, k, h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[i] = f2_add(g[i], h[i]);
+        }
+        RawTile<T, VEC> o;
+        o.set(g);
+        o.store(reinterpret_cast<T*>(p.dx) + (row + b) * D, base, lane, D);
       }
-      RawTile<T, VEC> o;
-      o.set(g);
-      o.store(reinterpret_cast<T*>(p.dx) + row * D, base, lane, D);
     }
-    if constexpr (PIPE) {   // the slot is read: the row S behind this one
-      rows.fetch(at, row + S * step < p.M);
+    if constexpr (PIPE) {   // the slots are read: the rows S groups behind these
+      rows.template fetch<B>(p, at, row + S * step);
       at = at + 1 == S ? 0 : at + 1;
     }
   }
@@ -564,41 +595,58 @@ void ln_stats(LnParams& p, const at::Tensor& x, const at::Tensor& stats) {
   p.rstd = p.mean + p.M;
 }
 
-// Tiles of a warp, warps of a team, teams of a block: up to four tiles a warp (what a row costs
-// beside its columns - reductions, a barrier, addresses - is shared by them; 16384 x 5120 with
-// two: forward 136, backward 146 us), about 8 warps a block.
-int ln_shape(LnParams& p) {
+// Tiles of a warp, warps of a team.  What a row costs beside its columns - reductions, a
+// barrier, addresses - is shared by a warp's tiles: four in the forward (16384 x 5120 kept in 8
+// bits with two: 136 us); in the backward, whose sums of dw and db take the registers, two and
+// two rows, and four where 16 warps do not reach.
+int ln_shape(LnParams& p, int most) {
   const int tiles = (p.D + kTile - 1) / kTile;
-  const int K = tiles <= 2 ? tiles : 4;
+  const int K = tiles <= 2 ? tiles : tiles <= most * kLnMaxWarps ? most : 4;
   p.W = (tiles + K - 1) / K;
-  p.R = std::max(1, kLnMaxTeams / p.W);
   return K;
 }
 
-// Rows under way in shared memory behind `front` bytes: as many of 2 to 4 as leave `blocks`
-// blocks to an SM, fewer blocks where two rows do not fit.  Returns the bytes in all, 0 where
-// not even one block has room for two rows.
-size_t ln_slots(LnParams& p, size_t front, size_t thread_bytes, int blocks) {
-  const size_t slot = thread_bytes * p.W * p.R * 32;
-  for (; blocks > 0; --blocks) {
-    const size_t room = (size_t)(228 * 1024) / blocks - 1024 - 2048;   // (1 KB of the system's, the static arrays)
-    if (front + 2 * slot > std::min<size_t>(room, 224 * 1024)) continue;
-    p.slots = (int)std::min<size_t>(4, (std::min<size_t>(room, 224 * 1024) - front) / slot);
-    p.slots_at = (int)front;
-    return front + p.slots * slot;
+// Teams of a block, as many as `warps` hold, fewer where there are no rows for them, and groups of
+// `rows` rows under way in shared memory behind `front` bytes: 2 to 4, as many as leave `blocks`
+// blocks to an SM; fewer blocks, then fewer teams, where two do not fit.  Returns the bytes in
+// all, 0 where not even one team has room for two groups.
+//   The backward has one block of many teams to an SM (w and a block's row of partial sums are
+// there once), the forward three small ones (its warps have more registers that way: 8192 x 3584
+// with residual 38 us against 46).
+size_t ln_block(LnParams& p, size_t front, size_t thread_bytes, int warps, int rows, int blocks) {
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, groups = (p.M + rows - 1) / rows;
+  const size_t fixed = 1024 + sizeof(float) * kLnMaxTeams * 2 * kLnMaxWarps * 4;   // (the system's, the static arrays)
+  p.slots_at = (int)front;
+  p.slots = 0;
+  for (p.R = (int)std::max<int64_t>(1, std::min<int64_t>(warps / p.W, (groups + sms - 1) / sms)); p.R > 0; --p.R) {
+    const size_t slot = thread_bytes * p.W * p.R * 32 * rows;
+    for (int n = blocks; n > 0; --n) {
+      const size_t room = (size_t)(228 * 1024) / n - fixed;
+      if (front + 2 * slot > room) continue;
+      p.slots = (int)std::min<size_t>(4, (room - front) / slot);
+      return front + p.slots * slot;
+    }
   }
+  p.R = 1;
   return 0;
+}
+
+// Teams of a block without slots: as many as 16 warps hold, and rows are there for
+int ln_teams(const LnParams& p, int rows) {
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, groups = (p.M + rows - 1) / rows;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kLnMaxWarps / p.W, (groups + sms - 1) / sms));
 }
 
 // Blocks that are resident at once (a kernel's, by its shape), no more than there are rows for
 template <typename F>
-unsigned ln_grid(F kern, const LnParams& p, size_t smem) {
+unsigned ln_grid(F kern, const LnParams& p, size_t smem, int rows) {
   int n = 0;
-  if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > 32 * 1024)   // (48 KB with the static arrays go without)
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, p.W * p.R * 32, smem));
   TORCH_CHECK(n > 0, "layer_norm: a block does not fit the device");
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  return (unsigned)std::min<int64_t>((p.M + p.R - 1) / p.R, n * sms);
+  return (unsigned)std::min<int64_t>((p.M + p.R * rows - 1) / (p.R * rows), n * sms);
 }
 
 }  // namespace
@@ -625,17 +673,22 @@ template <typename T, bool VEC, int K>
 static void ln_fwd_launch(LnParams& p, cudaStream_t stream) {
   const size_t front = (size_t)2 * ((p.D + kTile - 1) / kTile * kTile) * 4;   // w and b
   auto go = [&](auto kern, size_t smem) {
-    const unsigned grid = ln_grid(kern, p, smem);
+    const unsigned grid = ln_grid(kern, p, smem, 1);
     kern<<<grid, p.W * p.R * 32, smem, stream>>>(p);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   };
   ln_flags(p.delta != nullptr, p.codes != nullptr, [&](auto res, auto keep) {
     constexpr bool RES = decltype(res)::value, KEEP = decltype(keep)::value;
     if constexpr (VEC) {
-      const size_t smem = ln_slots(p, front, LnSlots<T, K, RES ? 2 : 1, false>::kBytes, 4);
+      p.src[0] = p.x, p.pitch[0] = p.xs;
+      p.src[1] = p.delta, p.pitch[1] = p.ds;
+      const size_t smem = ln_block(p, front, LnSlots<T, K, RES ? 2 : 1, false>::kBytes, 8, 1, 3);
       if (smem > 0) return go(ln_fwd_kernel<T, VEC, K, RES, KEEP, true>, smem);
     }
-    if constexpr (!VEC || K == 4) go(ln_fwd_kernel<T, VEC, K, RES, KEEP, false>, front);
+    if constexpr (!VEC || K == 4) {
+      p.R = VEC ? 1 : ln_teams(p, 1);
+      go(ln_fwd_kernel<T, VEC, K, RES, KEEP, false>, front);
+    }
   });
 }
 
@@ -665,7 +718,7 @@ void layernorm_fwd(at::Tensor x, c10::optional<at::Tensor> delta, c10::optional<
   if (codes.has_value()) ln_kept(p, x, *codes, *steps);
   const c10::cuda::CUDAGuard guard(x.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const int K = ln_shape(p);
+  const int K = ln_shape(p, 4);
   ZQ_LN_TYPES(x.scalar_type(), {
     if (vec) {
       if (K == 1) ln_fwd_launch<T, true, 1>(p, stream);
@@ -683,10 +736,10 @@ template <typename T, bool VEC, int K>
 static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::Tensor>& dw, c10::optional<at::Tensor>& db,
                           cudaStream_t stream) {
   const bool sums = dw.has_value() || db.has_value();
-  // w; [2, D] where several teams' sums are added
-  const size_t row = (size_t)((p.D + kTile - 1) / kTile * kTile) * 4, front = sums && p.R > 1 ? 2 * row : row;
+  // w; [2, D] where teams' sums are added
+  const size_t row = (size_t)((p.D + kTile - 1) / kTile * kTile) * 4, front = sums && p.W <= kLnBlockWarps / 2 ? 2 * row : row;
   auto go = [&](auto kern, size_t smem) {
-    const unsigned grid = ln_grid(kern, p, smem);
+    const unsigned grid = ln_grid(kern, p, smem, kLnRows);
     at::Tensor part;
     if (sums) {
       part = at::empty({(int64_t)grid * 2 * p.D}, dy.options().dtype(at::kFloat));
@@ -711,10 +764,16 @@ static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::T
   ln_flags(p.codes != nullptr, p.dh != nullptr, [&](auto kept, auto res) {
     constexpr bool KEPT = decltype(kept)::value, RES = decltype(res)::value;
     if constexpr (VEC) {
-      const size_t smem = ln_slots(p, front, LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT>::kBytes, 3);
-      if (smem > 0) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true>, smem);
+      p.src[0] = p.dy, p.pitch[0] = p.dys;
+      p.src[1] = RES ? p.dh : p.x, p.pitch[1] = RES ? p.dhs : p.xs;
+      p.src[2] = p.x, p.pitch[2] = p.xs;
+      constexpr int kBytes = LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT>::kBytes;
+      constexpr int kWarps = K <= 2 ? kLnBlockWarps : kLnMaxWarps;
+      const size_t smem = ln_block(p, front, kBytes, kWarps, kLnRows, 1);
+      if (smem > 0) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, kWarps>, smem);
     }
-    if constexpr (!VEC || K == 4) go(ln_bwd_kernel<T, VEC, K, KEPT, RES, false>, front);
+    p.R = VEC ? 1 : ln_teams(p, kLnRows);
+    go(ln_bwd_kernel<T, VEC, K, KEPT, RES, false, kLnMaxWarps>, front);
   });
 }
 
@@ -750,7 +809,7 @@ void layernorm_bwd(at::Tensor dy, c10::optional<at::Tensor> dh, c10::optional<at
   if (db.has_value()) ln_vector(*db, dy, wt, "db");
   const c10::cuda::CUDAGuard guard(dy.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  const int K = ln_shape(p);
+  const int K = ln_shape(p, 2);
   ZQ_LN_TYPES(dy.scalar_type(), {
     if (vec) {
       if (K == 1) ln_bwd_launch<T, true, 1>(p, dy, dw, db, stream);

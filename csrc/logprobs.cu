@@ -34,7 +34,7 @@
 namespace zq {
 
 constexpr int kLpMaxTop = 256;
-constexpr int kLpCandidates = 1024;      // of the list in shared memory, besides k ties
+constexpr int kLpCandidates = 512;      // of the list in shared memory, besides k ties
 constexpr int kLpFine = 65536;           // rows of at most this many columns: chunks of 8
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpLn2 = 0.6931471805599453f;
@@ -50,7 +50,7 @@ struct LogprobParams {
   void* dz;
   int64_t M, stride, gstride, width, V;
   int K, chunks;            // chunks of a row at most
-  float scale;              // log2(e) / τ
+  float scale, inv_tau;     // log2(e) / τ, 1 / τ
   double tau;
 };
 
@@ -172,6 +172,9 @@ struct LpRow {
     r.u = __ldg(reinterpret_cast<const uint4*>(z - lead) + i);
     return r;
   }
+  __device__ __forceinline__ void ahead(int i) const {
+    if (whole(i)) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint4*>(z - lead) + i));
+  }
   __device__ __forceinline__ LpVec<T> load(int i) const {   // (-inf behind the row's last, too)
     if (whole(i)) return load_whole(i);
     LpVec<T> r;
@@ -262,7 +265,7 @@ __device__ __forceinline__ uint32_t lp_block_sum(uint32_t v, uint32_t* s_n, int 
 
 // The top alternatives of a row, by the block that has all chunks' maxima.
 template <typename T, int NT, bool FINE>
-__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const float* s_max, int chunks, const LpLog& log,
+__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const T* s_max, int chunks, const LpLog& log,
                        bool nan, uint32_t* s_n, uint64_t* s_list, uint32_t* s_count) {
   constexpr int N = LpVec<T>::N, kVecs = FINE ? 1 : 32;   // vectors of a chunk
   using Key = LpKey<T>;
@@ -279,64 +282,90 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
     for (int bit = Key::kBits - 1; bit >= 0; --bit) {
       const uint32_t up = bound | (1u << bit);
       uint32_t n = 0;
-      for (int i = tid; i < chunks; i += NT) n += Key::of(s_max[i]) >= up ? 1u : 0u;
+      for (int i = tid; i < chunks; i += NT) n += Key::of(to_f32<T>(s_max[i])) >= up ? 1u : 0u;
       if (lp_block_sum<NT>(n, s_n, turn++) >= K) bound = up;
     }
   }
-  // Elements above the bound, in any order (they are ranked below).  Where they do not fit the
-  // list (a row whose best lie side by side), the bound rises to the K-th best element.
-  auto vector = [&](int i, auto&& f) {
-    if (i >= row.vecs) return;
+  // Elements that reach the bound, in any order (they are ranked below).  Where they do not fit
+  // the list, those above it, and then those at it in the order of their columns as far as they
+  // are wanted (a row of many equal ones); where the former do not fit either (a row whose best
+  // lie side by side), the bound rises to the K-th best element before.
+  auto elements = [&](int i, const LpVec<T>& r, auto&& f) {
     float v[N];
-    row.load(i).values(v);
+    r.values(v);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int col = row.col(i) + j;
       if (col >= 0 && col < row.V) f(Key::of(v[j]), (uint32_t)col);
     }
   };
+  auto vector = [&](int i, auto&& f) {
+    if (i < row.vecs) elements(i, row.load(i), f);
+  };
   auto each = [&](uint32_t at_least, auto&& f) {   // elements of chunks whose maximum reaches it
     for (int c0 = tid - lane; c0 < chunks; c0 += NT) {
-      const bool look = c0 + lane < chunks && Key::of(s_max[min(c0 + lane, chunks - 1)]) >= at_least;
+      const bool look = c0 + lane < chunks && Key::of(to_f32<T>(s_max[min(c0 + lane, chunks - 1)])) >= at_least;
       if constexpr (FINE) {
         if (look) vector(c0 + lane, f);
       } else {
-        for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0; in &= in - 1)
-          vector((c0 + __ffs(in) - 1) * kVecs + lane, f);
+        constexpr int A = 4;   // chunks under way
+        for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0;) {
+          LpVec<T> r[A];
+          int i[A];
+#pragma unroll
+          for (int j = 0; j < A; ++j) {
+            i[j] = in != 0 ? (c0 + __ffs(in) - 1) * kVecs + lane : row.vecs;
+            in &= in - 1;   // (0 stays 0)
+            if (i[j] < row.vecs) r[j] = row.load(i[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < A; ++j)
+            if (i[j] < row.vecs) elements(i[j], r[j], f);
+        }
       }
     }
   };
-  auto collect = [&] {
-    each(bound + 1, [&](uint32_t key, uint32_t col) {
-      if (key > bound) {
+  auto collect = [&](uint32_t from) {
+    each(from, [&](uint32_t key, uint32_t col) {
+      if (key >= from) {
         const uint32_t at = atomicAdd(s_count, 1u);
         if (at < kLpCandidates) s_list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
       }
     });
     __syncthreads();
   };
-  collect();
-  if (*s_count > kLpCandidates) {
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = Key::kBits - 1; bit >= 0; --bit) {
-      const uint32_t up = t | (1u << bit);
-      uint32_t n = 0;
-      each(up, [&](uint32_t key, uint32_t) { n += key >= up ? 1u : 0u; });
-      if (lp_block_sum<NT>(n, s_n, turn++) >= K) t = up;
-    }
-    bound = t;
+  auto clear = [&] {
     __syncthreads();
     if (tid == 0) *s_count = 0u;
     __syncthreads();
-    collect();   // fewer than K
+  };
+  collect(bound);
+  const bool all = *s_count <= kLpCandidates;
+  if (!all && bound < 0xffffffffu) {
+    clear();
+    collect(bound + 1);
+    if (*s_count > kLpCandidates) {
+      uint32_t t = 0;
+#pragma unroll 1
+      for (int bit = Key::kBits - 1; bit >= 0; --bit) {
+        const uint32_t up = t | (1u << bit);
+        uint32_t n = 0;
+        each(up, [&](uint32_t key, uint32_t) { n += key >= up ? 1u : 0u; });
+        if (lp_block_sum<NT>(n, s_n, turn++) >= K) t = up;
+      }
+      bound = t;
+      clear();
+      if (bound < 0xffffffffu) collect(bound + 1);   // fewer than K
+    }
+  } else if (!all) {   // (nothing is above the largest key)
+    clear();
   }
   const uint32_t above = *s_count;
   // elements at the bound, in the order of their columns, until there are K
   uint32_t n = above;
-  if (tid < 32 && n < K) {
+  if (!all && tid < 32 && n < K) {
     for (int c0 = 0; c0 < chunks && n < K; c0 += 32) {
-      const bool look = c0 + lane < chunks && Key::of(s_max[min(c0 + lane, chunks - 1)]) >= bound;
+      const bool look = c0 + lane < chunks && Key::of(to_f32<T>(s_max[min(c0 + lane, chunks - 1)])) >= bound;
       // a step of the warp: a vector a lane, of 32 chunks (FINE) or of one
       for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0 && n < K; in = FINE ? 0u : in & (in - 1)) {
         const int i = FINE ? c0 + lane : (c0 + __ffs(in) - 1) * kVecs + lane;
@@ -372,23 +401,23 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
   }
 }
 
-// A slice of a row, tiles [t0, t1) of 32 vectors: its sums, and its chunks' maxima.  Tiles that
-// lie inside the row go in groups of U a warp, the next group's loads ahead of this one's
-// arithmetic, in packed pairs.
-template <typename T, int NT, bool TOP, bool FINE>
-__device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, float* s_max) {
-  constexpr int N = LpVec<T>::N, P = N / 2, U = 4, kStep = NT / 32 * U;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// A warp's tiles [t0, t1) of 32 vectors of a row: its sums, and its chunks' maxima.  Tiles that
+// lie inside the row go in groups of U, the next group's loads ahead of this one's arithmetic,
+// in packed pairs.
+template <typename T, bool TOP, bool FINE>
+__device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, T* s_max) {
+  constexpr int N = LpVec<T>::N, P = N / 2, U = 4;
+  const int lane = threadIdx.x & 31;
   const float behind = kLpBehind / scale;
   float m = -INFINITY;
   uint64_t s2 = 0ull, a2 = 0ull;
   auto chunk = [&](const LpVec<T>& v, int tile, float top) {
     if constexpr (TOP && FINE) {
-      if (tile * 32 + lane < row.vecs) s_max[tile * 32 + lane] = top;
+      if (tile * 32 + lane < row.vecs) s_max[tile * 32 + lane] = from_f32<T>(top);   // (exact: a value of the type)
     } else if constexpr (TOP) {
       float all;
       asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
-      if (lane == 0) s_max[tile] = all;
+      if (lane == 0) s_max[tile] = from_f32<T>(all);
     }
   };
   auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
@@ -429,7 +458,7 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
       }
     }
   };
-  int t = t0 + warp * U;
+  int t = t0;
   auto inside = [&](int t) { return t + U <= t1 && row.inside(t * 32, 32 * U); };
   auto fetch = [&](LpVec<T> (&r)[U], int t) {
 #pragma unroll
@@ -444,7 +473,7 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
 #pragma unroll
         for (int j = 0; j < U; ++j) r[j] = next[j];
         const int here = t;
-        t += kStep;
+        t += U;
         const bool more = inside(t);
         if (more) fetch(next, t);
         add(r, here, U);
@@ -455,7 +484,7 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
 #pragma unroll
       for (int j = 0; j < U; ++j) r[j] = row.load((t + j) * 32 + lane);
       add(r, t, min(U, t1 - t));
-      t += kStep;
+      t += U;
     }
   }
   float lo, hi;
@@ -496,17 +525,25 @@ __device__ LpSums lp_far(const LpRow<T>& row, float scale, LpSums* s_part) {
 // A block (a cluster of them, each with a slice of the columns, where there are fewer rows
 // than places) works on one row.
 template <typename T, int NT, bool TOP, bool FINE>
-__global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__ LogprobParams p) {
+__global__ void __launch_bounds__(NT, 1024 / NT) logprob_fwd_kernel(const __grid_constant__ LogprobParams p) {
   constexpr int kWarps = NT / 32;
   namespace cg = cooperative_groups;
   auto cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
-  extern __shared__ float lp_smem[];   // chunks' maxima (rank 0: of the whole row), the list
+  extern __shared__ __align__(16) uint8_t lp_smem[];   // the list; chunks' maxima (rank 0: of the whole row)
+  T* const own_max = reinterpret_cast<T*>(lp_smem + (TOP ? 8 * (kLpCandidates + p.K) : 0));
   __shared__ LpSums s_part[8 * kWarps];
   __shared__ uint32_t s_n[3], s_count;
+  __shared__ LpSums s_row;
+  __shared__ LpLog s_log;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.x / (unsigned)csize;
+  const LpRow<T> row(p.z, m, p.stride, (int)p.V);
+  // consecutive tiles to a warp, as equal as they can be
+  const int tiles = (row.vecs + 31) / 32, part = crank * kWarps + warp, parts = csize * kWarps;
+  const int t0 = (int)((int64_t)tiles * part / parts), t1 = (int)((int64_t)tiles * (part + 1) / parts);
   const int64_t y = p.targets != nullptr ? p.targets[m] : 0;
+  row.ahead(t0 * 32 + lane);   // on its way while the target is read
   auto nothing = [&] {   // the row does not count
     for (int i = tid; i < p.K; i += NT) p.ids[m * p.K + i] = -1, p.top[m * p.K + i] = 0.0f;
     if (tid == 0) {
@@ -519,18 +556,16 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__
     if (crank == 0) nothing();
     return;
   }
-  const LpRow<T> row(p.z, m, p.stride, (int)p.V);
-  float* s_max = lp_smem;
+  const float zy = tid == 0 && p.targets != nullptr ? to_f32<T>(row.z[y]) : 0.0f;
+  T* s_max = own_max;
   LpSums* to = s_part;
   if (csize > 1) {
-    s_max = cluster.map_shared_rank(lp_smem, 0);
+    s_max = cluster.map_shared_rank(own_max, 0);
     to = cluster.map_shared_rank(s_part, 0);
     cluster.sync();   // rank 0, to which the others write, is there
   }
-  const int tiles = (row.vecs + 31) / 32, per = (tiles + csize - 1) / csize;
-  const int t0 = min(tiles, per * crank), t1 = min(tiles, t0 + per);
   const float scale = p.scale;
-  LpSums x = lp_warp_join<true>(lp_slice<T, NT, TOP, FINE>(row, t0, t1, scale, s_max), scale);
+  LpSums x = lp_warp_join<true>(lp_slice<T, TOP, FINE>(row, t0, t1, scale, s_max), scale);
   if (lane == 0) to[crank * kWarps + warp] = x;
   if (csize > 1) {
     cluster.sync();
@@ -538,25 +573,33 @@ __global__ void __launch_bounds__(NT) logprob_fwd_kernel(const __grid_constant__
   } else {
     __syncthreads();
   }
-  x = s_part[0];
-  for (int i = 1; i < csize * kWarps; ++i) x = lp_join<true>(x, s_part[i], scale);   // the same in every thread
+  // the first warp joins the parts (at most 64), the others wait
+  if (warp == 0) {
+    x = lane < parts ? s_part[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
+    if (lane + 32 < parts) x = lp_join<true>(x, s_part[lane + 32], scale);
+    x = lp_warp_join<true>(x, scale);
+    if (lane == 0) s_row = x;
+  }
+  __syncthreads();
+  x = s_row;
   const bool plain = lp_plain(x.m, scale);
   if (!plain) x = lp_far<T, NT>(row, scale, s_part);
   if (x.m == -INFINITY && x.s == x.s) return nothing();   // no logit above -inf
   const bool nan = !(x.s < INFINITY) || !(x.m < INFINITY);
-  const LpLog log{plain ? -(double)lp_shift(x.m, scale) / (double)scale : (double)x.m, ::log((double)x.s), p.tau};
   if (tid == 0) {
-    const double l2 = log2((double)x.s);
-    const float h = nan ? NAN : fmaxf(0.0f, (float)((l2 - (double)x.a / (double)x.s) * 0.6931471805599453));
-    if (p.targets != nullptr) p.logp[m] = nan ? NAN : log.of(to_f32<T>(row.z[y]));
+    const LpLog log{plain ? -(double)lp_shift(x.m, scale) / (double)scale : (double)x.m, ::log((double)x.s), p.tau};
+    const double l2 = log.log_s * 1.4426950408889634;
+    const float h = nan ? NAN : fmaxf(0.0f, (float)(log.log_s - (double)x.a / (double)x.s * 0.6931471805599453));
+    if (p.targets != nullptr) p.logp[m] = nan ? NAN : log.of(zy);
     p.entropy[m] = h;
     p.stats[3 * m] = nan ? NAN : x.m;
     p.stats[3 * m + 1] = nan ? NAN : (float)l2;
     p.stats[3 * m + 2] = h;
+    if constexpr (TOP) s_log = log;   // (lp_top waits before it reads it)
   }
   if constexpr (TOP) {
-    uint64_t* s_list = reinterpret_cast<uint64_t*>(lp_smem + (p.chunks + 1) / 2 * 2);
-    lp_top<T, NT, FINE>(p, row, m, lp_smem, FINE ? row.vecs : tiles, log, nan, s_n, s_list, &s_count);
+    lp_top<T, NT, FINE>(p, row, m, own_max, FINE ? row.vecs : tiles, s_log, nan, s_n, reinterpret_cast<uint64_t*>(lp_smem),
+                        &s_count);
   }
 }
 
@@ -591,7 +634,7 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __g
     g = warp_sum(g);
   }
   // dz = p (c0 + c1 log2 p) + g terms
-  const float inv = (float)(1.0 / p.tau);
+  const float inv = p.inv_tau;
   const float c0 = -(g + gy + gh * h) * inv, c1 = -gh * kLpLn2 * inv;
   const bool plain = lp_plain(high, p.scale);
   const float shift = lp_shift(high, p.scale);
@@ -690,6 +733,7 @@ LogprobParams lp_params(const at::Tensor& z, const c10::optional<at::Tensor>& ta
   p.V = vocab;
   p.scale = (float)(1.4426950408889634 / temperature);
   p.tau = temperature;
+  p.inv_tau = (float)(1.0 / temperature);
   return p;
 }
 
@@ -700,7 +744,7 @@ void lp_launch(LogprobParams& p, cudaStream_t stream) {
   const int64_t vecs = (p.V + 2 * N - 2) / N;   // at the worst alignment
   p.chunks = FINE ? (int)vecs : (int)((vecs + 31) / 32);
   auto kern = logprob_fwd_kernel<T, NT, TOP, FINE>;
-  const size_t smem = TOP ? ((size_t)p.chunks + 1) / 2 * 8 + 8 * (size_t)(kLpCandidates + p.K) : 0;
+  const size_t smem = TOP ? (size_t)p.chunks * sizeof(T) + 8 * (size_t)(kLpCandidates + p.K) : 0;
   // a cluster to a row where that leaves SMs without a block, down to 4 warp tiles a warp
   int csize = 1;
   while (csize < 8 && p.M * csize * 2 <= 2 * sms && vecs / (2 * csize) >= 4 * NT) csize *= 2;
@@ -715,7 +759,7 @@ void lp_launch(LogprobParams& p, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (smem > 48 * 1024)
+  if (smem > 32 * 1024)   // (48 KB with the static arrays go without)
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
 }
@@ -748,9 +792,18 @@ void logprob_fwd(at::Tensor z, c10::optional<at::Tensor> targets, c10::optional<
   const c10::cuda::CUDAGuard guard(z.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   ZQ_LP_TYPES(z.scalar_type(), {
-    if (p.K == 0) lp_launch<T, 256, false, false>(p, stream);
-    else if (p.V <= kLpFine) lp_launch<T, 256, true, true>(p, stream);
-    else lp_launch<T, 256, true, false>(p, stream);
+    // What a row costs beside its columns (a load before the first, joins, the alternatives) is
+    // latency: blocks of 4 warps leave more of them on an SM to cover it (8192 x 152064: 683 us
+    // with 8 warps), where there are rows for twice as many.
+    const bool many = p.M >= 8 * (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    auto shape = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      if (p.K == 0) lp_launch<T, NT, false, false>(p, stream);
+      else if (p.V <= kLpFine) lp_launch<T, NT, true, true>(p, stream);
+      else lp_launch<T, NT, true, false>(p, stream);
+    };
+    if (many) shape(std::integral_constant<int, 128>{});
+    else shape(std::integral_constant<int, 256>{});
   });
 }
 
