@@ -15,9 +15,9 @@
 // and the same one wherever it enters, so t carries one rounding of a small number and no
 // error of the size of m s.  Rows whose maximum is far from 0 (all masked by the type's lowest
 // value) are summed again from differences.  The top alternatives cost that pass the maximum of every
-// chunk of columns (8 of them, or a warp's tile where the row is long): the k best of the row
-// lie in the k chunks with the best maxima, so the k-th best of those is a bound, and only
-// chunks above it are looked at again.
+// chunk of columns and of every warp's tile: the k best of the row lie in the k tiles (or chunks)
+// with the best maxima, so the k-th best of those is a bound, and only chunks that reach it are
+// looked at again.
 // Backward: one pass, p from the row's m, S and H; the columns with a g term are written a
 // second time by their block (each sum rounded once; no atomics).
 //
@@ -35,7 +35,7 @@ namespace zq {
 
 constexpr int kLpMaxTop = 256;
 constexpr int kLpCandidates = 512;      // of the list in shared memory, besides k ties
-constexpr int kLpFine = 65536;           // rows of at most this many columns: chunks of 8
+constexpr int kLpHits = 512;             // chunks of the list of those that reach the bound
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpLn2 = 0.6931471805599453f;
 
@@ -49,9 +49,9 @@ struct LogprobParams {
   const float *gp, *gh, *gt;   // gradients, or null
   void* dz;
   int64_t M, stride, gstride, width, V;
-  int K, chunks;            // chunks of a row at most
-  float scale, inv_tau;     // log2(e) / τ, 1 / τ
-  double tau;
+  int K;
+  float scale;              // log2(e) / τ
+  double inv_tau, inv_scale;
 };
 
 __device__ __forceinline__ float lp_exp2(float x) {
@@ -233,12 +233,18 @@ __device__ __forceinline__ LpSums lp_warp_join(LpSums x, float scale) {
   return x;
 }
 
-// A row's sums for its few numbers in 64 bits: l = (z - m) / τ - log S.  (PLAIN sums are
-// relative to the rounded shift: m is what it stands for.)
+// A row's few numbers, in 64 bits (sums and products; divisions and logarithms would take longer
+// than a short row): l = (z - m) / τ - log S.  PLAIN sums are relative to the rounded shift: m is
+// what it stands for.
 struct LpLog {
-  double m, log_s, tau;
-  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) / tau - log_s); }
+  double m, log_s, inv_tau;
+  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) * inv_tau - log_s); }
 };
+// log of a positive number: its exponent's part in 64 bits, its mantissa's (below 0.35) in 32
+__device__ __forceinline__ double lp_log(float s) {
+  const int e = (__float_as_int(s) - 0x3f3504f3) >> 23;   // mantissa in [sqrt(1/2), sqrt(2))
+  return (double)e * 0.69314718055994531 + (double)logf(__int_as_float(__float_as_int(s) - (e << 23)));
+}
 
 // Whole numbers in the values' order (0 and -0 equal, NaN above all), without the places that
 // are the same for all values of the type.
@@ -251,45 +257,93 @@ struct LpKey {
     const uint32_t b = __float_as_uint(v + 0.0f);
     return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kLow;
   }
+  static __device__ __forceinline__ float value(uint32_t key) {
+    if (key == 0xffffffffu >> kLow) return NAN;
+    const uint32_t b = key << kLow;
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~(b | ((1u << kLow) - 1u)));
+  }
 };
 
-template <int NT>
-__device__ __forceinline__ uint32_t lp_block_sum(uint32_t v, uint32_t* s_n, int turn) {
-  // s_n[3]: the word of two turns ahead is cleared while this one's is in use
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) atomicAdd(&s_n[turn % 3], v);
-  __syncthreads();
-  if (threadIdx.x == 0) s_n[(turn + 2) % 3] = 0u;
-  return s_n[turn % 3];
-}
+// What a block keeps of a row for its top alternatives, behind one another in shared memory:
+// the lists; the maxima of its chunks, each the vectors of G lanes (4, or 1 where the row is
+// short); with G = 4 the maxima of its tiles of 32 vectors.
+struct LpLists {
+  uint64_t cand[kLpCandidates + kLpMaxTop];
+  uint32_t hits[kLpHits];
+  uint32_t n_cand, n_hits;
+};
+template <typename T, int G>
+struct LpMaxima {
+  T *chunk, *tile;
+  static __host__ __device__ constexpr size_t bytes(int64_t vecs) {
+    return ((size_t)((vecs + G - 1) / G) + (G > 1 ? (size_t)((vecs + 31) / 32) : 0)) * sizeof(T);
+  }
+};
 
-// The top alternatives of a row, by the block that has all chunks' maxima.
-template <typename T, int NT, bool FINE>
-__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const T* s_max, int chunks, const LpLog& log,
-                       bool nan, uint32_t* s_n, uint64_t* s_list, uint32_t* s_count) {
-  constexpr int N = LpVec<T>::N, kVecs = FINE ? 1 : 32;   // vectors of a chunk
+// The top alternatives of a row, by one warp (the others' barriers would cost more than their
+// help).
+template <typename T, int G>
+__device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const LpMaxima<T, G>& s_max, const LpLog& log,
+                       bool nan, LpLists& list) {
+  constexpr int N = LpVec<T>::N;
   using Key = LpKey<T>;
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int lane = threadIdx.x & 31, chunks = (row.vecs + G - 1) / G, tiles = (row.vecs + 31) / 32;
   const uint32_t K = (uint32_t)p.K;
-  if (tid < 3) s_n[tid] = 0u;
-  if (tid == 0) *s_count = 0u;
-  __syncthreads();
-  int turn = 0;
-  // the K-th best of the chunks' maxima (0, below all, where there are fewer chunks)
+  auto chunk_key = [&](int i) { return Key::of(to_f32<T>(s_max.chunk[i])); };
+  if (lane == 0) list.n_cand = list.n_hits = 0u;
+  // The K-th best of the tiles' maxima, or of the chunks' (0, below all, where there are fewer).
+  // Of n parts with the K best among them some -n log(1 - K / n) elements reach it.
+  const bool by_tile = G > 1 && 2 * tiles >= 3 * p.K;
+  const T* parts = by_tile ? s_max.tile : s_max.chunk;
+  const int n_parts = by_tile ? tiles : chunks;
+  auto part_key = [&](int i) { return Key::of(to_f32<T>(parts[i])); };
   uint32_t bound = 0;
-  if (chunks >= p.K) {
+  if (n_parts >= p.K) {
+    constexpr int kOwn = 24;   // parts of a lane whose keys it holds
+    const bool own = n_parts <= kOwn * 32;
+    uint32_t key[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) key[i] = own && i * 32 + lane < n_parts ? part_key(i * 32 + lane) : 0u;
 #pragma unroll 1
     for (int bit = Key::kBits - 1; bit >= 0; --bit) {
-      const uint32_t up = bound | (1u << bit);
+      const uint32_t up = bound | (1u << bit);   // (above 0, the key of no part)
       uint32_t n = 0;
-      for (int i = tid; i < chunks; i += NT) n += Key::of(to_f32<T>(s_max[i])) >= up ? 1u : 0u;
-      if (lp_block_sum<NT>(n, s_n, turn++) >= K) bound = up;
+      if (own) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) n += key[i] >= up ? 1u : 0u;
+      } else {
+        for (int i = lane; i < n_parts; i += 32) n += part_key(i) >= up ? 1u : 0u;
+      }
+      if (__reduce_add_sync(0xffffffffu, n) >= K) bound = up;
     }
   }
-  // Elements that reach the bound, in any order (they are ranked below).  Where they do not fit
-  // the list, those above it, and then those at it in the order of their columns as far as they
-  // are wanted (a row of many equal ones); where the former do not fit either (a row whose best
-  // lie side by side), the bound rises to the K-th best element before.
+  __syncwarp();
+  // the chunks that reach it
+  auto hit = [&](int i) {
+    if (i < chunks && chunk_key(i) >= bound) {
+      const uint32_t at = atomicAdd(&list.n_hits, 1u);
+      if (at < kLpHits) list.hits[at] = (uint32_t)i;
+    }
+  };
+  if (by_tile) {
+    constexpr int kOf = 32 / G;   // chunks of a tile: those of four tiles (G = 4) at a time
+    for (int i0 = 0; i0 < tiles; i0 += 32) {
+      uint32_t in = __ballot_sync(0xffffffffu, i0 + lane < tiles && part_key(min(i0 + lane, tiles - 1)) >= bound);
+      while (in != 0) {
+        int mine = -1;
+#pragma unroll
+        for (int j = 0; j < 32 / kOf; ++j) {
+          if (in != 0 && lane / kOf == j) mine = i0 + __ffs(in) - 1;
+          in &= in - 1;
+        }
+        if (mine >= 0) hit(mine * kOf + lane % kOf);
+      }
+    }
+  } else {
+    for (int i = lane; i < chunks; i += 32) hit(i);
+  }
+  __syncwarp();
+  const int hits = (int)list.n_hits;
   auto elements = [&](int i, const LpVec<T>& r, auto&& f) {
     float v[N];
     r.values(v);
@@ -299,104 +353,89 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
       if (col >= 0 && col < row.V) f(Key::of(v[j]), (uint32_t)col);
     }
   };
-  auto vector = [&](int i, auto&& f) {
-    if (i < row.vecs) elements(i, row.load(i), f);
-  };
-  auto each = [&](uint32_t at_least, auto&& f) {   // elements of chunks whose maximum reaches it
-    for (int c0 = tid - lane; c0 < chunks; c0 += NT) {
-      const bool look = c0 + lane < chunks && Key::of(to_f32<T>(s_max[min(c0 + lane, chunks - 1)])) >= at_least;
-      if constexpr (FINE) {
-        if (look) vector(c0 + lane, f);
-      } else {
-        constexpr int A = 4;   // chunks under way
-        for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0;) {
-          LpVec<T> r[A];
-          int i[A];
+  // elements that may reach `at_least` (no less than the bound of the list of chunks)
+  auto each = [&](uint32_t at_least, auto&& f) {
+    const bool listed = hits <= kLpHits;   // (otherwise many equal maxima: all chunks)
+    const int vecs = listed ? hits * G : row.vecs;
+    constexpr int A = 4;   // vectors of a lane under way
+    for (int v0 = lane; v0 < vecs; v0 += 32 * A) {
+      LpVec<T> r[A];
+      int i[A];
 #pragma unroll
-          for (int j = 0; j < A; ++j) {
-            i[j] = in != 0 ? (c0 + __ffs(in) - 1) * kVecs + lane : row.vecs;
-            in &= in - 1;   // (0 stays 0)
-            if (i[j] < row.vecs) r[j] = row.load(i[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < A; ++j)
-            if (i[j] < row.vecs) elements(i[j], r[j], f);
-        }
+      for (int j = 0; j < A; ++j) {
+        const int v = v0 + j * 32;
+        i[j] = v >= vecs ? row.vecs : listed ? (int)list.hits[v / G] * G + v % G : v;
+        if (i[j] < row.vecs) r[j] = row.load(i[j]);
       }
+#pragma unroll
+      for (int j = 0; j < A; ++j)
+        if (i[j] < row.vecs && Key::of(r[j].largest()) >= at_least) elements(i[j], r[j], f);
     }
   };
   auto collect = [&](uint32_t from) {
+    __syncwarp();
+    if (lane == 0) list.n_cand = 0u;
+    __syncwarp();
     each(from, [&](uint32_t key, uint32_t col) {
       if (key >= from) {
-        const uint32_t at = atomicAdd(s_count, 1u);
-        if (at < kLpCandidates) s_list[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+        const uint32_t at = atomicAdd(&list.n_cand, 1u);
+        if (at < kLpCandidates) list.cand[at] = ((uint64_t)key << 32) | (uint32_t)~col;
       }
     });
-    __syncthreads();
+    __syncwarp();
+    return list.n_cand;
   };
-  auto clear = [&] {
-    __syncthreads();
-    if (tid == 0) *s_count = 0u;
-    __syncthreads();
-  };
-  collect(bound);
-  const bool all = *s_count <= kLpCandidates;
-  if (!all && bound < 0xffffffffu) {
-    clear();
-    collect(bound + 1);
-    if (*s_count > kLpCandidates) {
+  // Elements that reach the bound, in any order (they are ranked below).  Where they do not fit
+  // the list, those above it, and then those at it in the order of their columns as far as they
+  // are wanted (a row of many equal ones); where the former do not fit either (a row whose best
+  // lie side by side), the bound rises to the K-th best element before.
+  uint32_t n = collect(bound);
+  if (n > kLpCandidates) {
+    auto above = [&] { return bound < 0xffffffffu ? collect(bound + 1) : 0u; };   // (the largest key: NaN)
+    n = above();
+    if (n > kLpCandidates) {
       uint32_t t = 0;
 #pragma unroll 1
       for (int bit = Key::kBits - 1; bit >= 0; --bit) {
         const uint32_t up = t | (1u << bit);
-        uint32_t n = 0;
-        each(up, [&](uint32_t key, uint32_t) { n += key >= up ? 1u : 0u; });
-        if (lp_block_sum<NT>(n, s_n, turn++) >= K) t = up;
+        uint32_t c = 0;
+        each(up, [&](uint32_t key, uint32_t) { c += key >= up ? 1u : 0u; });
+        if (__reduce_add_sync(0xffffffffu, c) >= K) t = up;
       }
       bound = t;
-      clear();
-      if (bound < 0xffffffffu) collect(bound + 1);   // fewer than K
+      n = above();   // fewer than K
     }
-  } else if (!all) {   // (nothing is above the largest key)
-    clear();
-  }
-  const uint32_t above = *s_count;
-  // elements at the bound, in the order of their columns, until there are K
-  uint32_t n = above;
-  if (!all && tid < 32 && n < K) {
-    for (int c0 = 0; c0 < chunks && n < K; c0 += 32) {
-      const bool look = c0 + lane < chunks && Key::of(to_f32<T>(s_max[min(c0 + lane, chunks - 1)])) >= bound;
-      // a step of the warp: a vector a lane, of 32 chunks (FINE) or of one
-      for (uint32_t in = __ballot_sync(0xffffffffu, look); in != 0 && n < K; in = FINE ? 0u : in & (in - 1)) {
-        const int i = FINE ? c0 + lane : (c0 + __ffs(in) - 1) * kVecs + lane;
-        uint32_t ties = 0;
-        if (!FINE || look) vector(i, [&](uint32_t key, uint32_t col) { ties |= (key == bound ? 1u : 0u) << (int)(col - row.col(i)); });
-        uint32_t before = __popc(ties);   // of lower lanes
+    // a vector a lane at a time, until there are K
+    for (int i0 = 0; i0 < row.vecs && n < K; i0 += 32) {
+      const int i = i0 + lane;
+      uint32_t ties = 0;
+      if (i < row.vecs && chunk_key(i / G) >= bound)
+        elements(i, row.load(i), [&](uint32_t key, uint32_t col) { ties |= (key == bound ? 1u : 0u) << (int)(col - row.col(i)); });
+      if (!__any_sync(0xffffffffu, ties != 0)) continue;
+      uint32_t before = __popc(ties);   // of lower lanes
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += up;
-        }
-        const uint32_t all = __shfl_sync(0xffffffffu, before, 31);
-        uint32_t at = n + before - __popc(ties);
-        for (; ties != 0 && at < K; ties &= ties - 1, ++at)
-          s_list[at] = ((uint64_t)bound << 32) | (uint32_t)~(uint32_t)(row.col(i) + __ffs(ties) - 1);
-        n = min(K, n + all);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
       }
+      const uint32_t sum = __shfl_sync(0xffffffffu, before, 31);
+      uint32_t at = n + before - __popc(ties);
+      for (; ties != 0 && at < K; ties &= ties - 1, ++at)
+        list.cand[at] = ((uint64_t)bound << 32) | (uint32_t)~(uint32_t)(row.col(i) + __ffs(ties) - 1);
+      n = min(K, n + sum);
     }
+    __syncwarp();
   }
-  if (tid == 0) *s_count = max(n, above);   // (above K only where the list holds it)
-  __syncthreads();
-  n = *s_count;
   // each candidate's rank is the number of better ones: all keys differ by their column
-  for (uint32_t i = tid; i < n; i += NT) {
-    const uint64_t mine = s_list[i];
+  for (uint32_t i = lane; i < n; i += 32) {
+    const uint64_t mine = list.cand[i];
+    const uint32_t col = ~(uint32_t)mine;
     uint32_t rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += s_list[j] > mine ? 1u : 0u;
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) rank += list.cand[j] > mine ? 1u : 0u;
     if (rank < K) {
-      const uint32_t col = ~(uint32_t)mine;
       p.ids[m * p.K + rank] = col;
-      p.top[m * p.K + rank] = nan ? NAN : log.of(to_f32<T>(row.z[col]));
+      p.top[m * p.K + rank] = nan ? NAN : log.of(Key::value((uint32_t)(mine >> 32)));
     }
   }
 }
@@ -404,20 +443,23 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
 // A warp's tiles [t0, t1) of 32 vectors of a row: its sums, and its chunks' maxima.  Tiles that
 // lie inside the row go in groups of U, the next group's loads ahead of this one's arithmetic,
 // in packed pairs.
-template <typename T, bool TOP, bool FINE>
-__device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, T* s_max) {
+template <typename T, int G>
+__device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, const LpMaxima<T, G>& s_max) {
   constexpr int N = LpVec<T>::N, P = N / 2, U = 4;
   const int lane = threadIdx.x & 31;
   const float behind = kLpBehind / scale;
   float m = -INFINITY;
   uint64_t s2 = 0ull, a2 = 0ull;
-  auto chunk = [&](const LpVec<T>& v, int tile, float top) {
-    if constexpr (TOP && FINE) {
-      if (tile * 32 + lane < row.vecs) s_max[tile * 32 + lane] = from_f32<T>(top);   // (exact: a value of the type)
-    } else if constexpr (TOP) {
+  auto chunk = [&](int tile, float top) {   // (exact in the type: one of its values)
+    if constexpr (G == 1) {
+      if (tile * 32 + lane < row.vecs) s_max.chunk[tile * 32 + lane] = from_f32<T>(top);
+    } else if constexpr (G > 1) {
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane % G == 0 && tile * 32 + lane < row.vecs) s_max.chunk[tile * (32 / G) + lane / G] = from_f32<T>(top);
       float all;
       asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
-      if (lane == 0) s_max[tile] = from_f32<T>(all);
+      if (lane == 0) s_max.tile[tile] = from_f32<T>(all);
     }
   };
   auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
@@ -426,7 +468,7 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
     for (int j = 0; j < U; ++j) {
       if (j < n) {
         top[j] = r[j].largest();
-        chunk(r[j], tile + j, top[j]);
+        chunk(tile + j, top[j]);
         cm = fmaxf(cm, top[j]);
       }
     }
@@ -524,21 +566,23 @@ __device__ LpSums lp_far(const LpRow<T>& row, float scale, LpSums* s_part) {
 
 // A block (a cluster of them, each with a slice of the columns, where there are fewer rows
 // than places) works on one row.
-template <typename T, int NT, bool TOP, bool FINE>
-__global__ void __launch_bounds__(NT, 1024 / NT) logprob_fwd_kernel(const __grid_constant__ LogprobParams p) {
+template <typename T, int NT, int G>   // G: 0 without alternatives
+__global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_kernel(const __grid_constant__ LogprobParams p) {
   constexpr int kWarps = NT / 32;
   namespace cg = cooperative_groups;
   auto cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
-  extern __shared__ __align__(16) uint8_t lp_smem[];   // the list; chunks' maxima (rank 0: of the whole row)
-  T* const own_max = reinterpret_cast<T*>(lp_smem + (TOP ? 8 * (kLpCandidates + p.K) : 0));
+  extern __shared__ __align__(16) uint8_t lp_smem[];   // the lists; chunks' maxima (rank 0: of the whole row)
+  LpMaxima<T, G> own_max{};
   __shared__ LpSums s_part[8 * kWarps];
-  __shared__ uint32_t s_n[3], s_count;
   __shared__ LpSums s_row;
-  __shared__ LpLog s_log;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.x / (unsigned)csize;
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
+  if constexpr (G > 0) {
+    own_max.chunk = reinterpret_cast<T*>(lp_smem + sizeof(LpLists));
+    own_max.tile = own_max.chunk + (row.vecs + G - 1) / G;
+  }
   // consecutive tiles to a warp, as equal as they can be
   const int tiles = (row.vecs + 31) / 32, part = crank * kWarps + warp, parts = csize * kWarps;
   const int t0 = (int)((int64_t)tiles * part / parts), t1 = (int)((int64_t)tiles * (part + 1) / parts);
@@ -557,15 +601,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprob_fwd_kernel(const __grid
     return;
   }
   const float zy = tid == 0 && p.targets != nullptr ? to_f32<T>(row.z[y]) : 0.0f;
-  T* s_max = own_max;
+  LpMaxima<T, G> s_max = own_max;
   LpSums* to = s_part;
   if (csize > 1) {
-    s_max = cluster.map_shared_rank(own_max, 0);
+    if constexpr (G > 0) {
+      s_max.chunk = cluster.map_shared_rank(own_max.chunk, 0);
+      s_max.tile = cluster.map_shared_rank(own_max.tile, 0);
+    }
     to = cluster.map_shared_rank(s_part, 0);
     cluster.sync();   // rank 0, to which the others write, is there
   }
   const float scale = p.scale;
-  LpSums x = lp_warp_join<true>(lp_slice<T, TOP, FINE>(row, t0, t1, scale, s_max), scale);
+  LpSums x = lp_warp_join<true>(lp_slice<T, G>(row, t0, t1, scale, s_max), scale);
   if (lane == 0) to[crank * kWarps + warp] = x;
   if (csize > 1) {
     cluster.sync();
@@ -586,21 +633,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprob_fwd_kernel(const __grid
   if (!plain) x = lp_far<T, NT>(row, scale, s_part);
   if (x.m == -INFINITY && x.s == x.s) return nothing();   // no logit above -inf
   const bool nan = !(x.s < INFINITY) || !(x.m < INFINITY);
-  if (tid == 0) {
-    const LpLog log{plain ? -(double)lp_shift(x.m, scale) / (double)scale : (double)x.m, ::log((double)x.s), p.tau};
-    const double l2 = log.log_s * 1.4426950408889634;
-    const float h = nan ? NAN : fmaxf(0.0f, (float)(log.log_s - (double)x.a / (double)x.s * 0.6931471805599453));
+  if (warp > 0) return;
+  const LpLog log{plain ? -(double)lp_shift(x.m, scale) * p.inv_scale : (double)x.m, nan ? 0.0 : lp_log(x.s), p.inv_tau};
+  if (lane == 0) {
+    const float h = nan ? NAN : fmaxf(0.0f, (float)(log.log_s - (double)(x.a / x.s) * 0.69314718055994531));
     if (p.targets != nullptr) p.logp[m] = nan ? NAN : log.of(zy);
     p.entropy[m] = h;
     p.stats[3 * m] = nan ? NAN : x.m;
-    p.stats[3 * m + 1] = nan ? NAN : (float)l2;
+    p.stats[3 * m + 1] = nan ? NAN : (float)(log.log_s * 1.4426950408889634);
     p.stats[3 * m + 2] = h;
-    if constexpr (TOP) s_log = log;   // (lp_top waits before it reads it)
   }
-  if constexpr (TOP) {
-    lp_top<T, NT, FINE>(p, row, m, own_max, FINE ? row.vecs : tiles, s_log, nan, s_n, reinterpret_cast<uint64_t*>(lp_smem),
-                        &s_count);
-  }
+  if constexpr (G > 0) lp_top<T, G>(p, row, m, own_max, log, nan, *reinterpret_cast<LpLists*>(lp_smem));
 }
 
 // Gradient: a warp takes U tiles of 32 vectors of a row and needs no other: it sums the row's
@@ -634,7 +677,7 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __g
     g = warp_sum(g);
   }
   // dz = p (c0 + c1 log2 p) + g terms
-  const float inv = p.inv_tau;
+  const float inv = (float)p.inv_tau;
   const float c0 = -(g + gy + gh * h) * inv, c1 = -gh * kLpLn2 * inv;
   const bool plain = lp_plain(high, p.scale);
   const float shift = lp_shift(high, p.scale);
@@ -732,19 +775,19 @@ LogprobParams lp_params(const at::Tensor& z, const c10::optional<at::Tensor>& ta
   p.width = z.size(1);
   p.V = vocab;
   p.scale = (float)(1.4426950408889634 / temperature);
-  p.tau = temperature;
-  p.inv_tau = (float)(1.0 / temperature);
+  p.inv_tau = 1.0 / temperature;
+  p.inv_scale = 1.0 / (double)p.scale;
   return p;
 }
 
-template <typename T, int NT, bool TOP, bool FINE>
+template <typename T, int NT, int G>
 void lp_launch(LogprobParams& p, cudaStream_t stream) {
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   constexpr int N = LpVec<T>::N;
   const int64_t vecs = (p.V + 2 * N - 2) / N;   // at the worst alignment
-  p.chunks = FINE ? (int)vecs : (int)((vecs + 31) / 32);
-  auto kern = logprob_fwd_kernel<T, NT, TOP, FINE>;
-  const size_t smem = TOP ? (size_t)p.chunks * sizeof(T) + 8 * (size_t)(kLpCandidates + p.K) : 0;
+  auto kern = logprob_fwd_kernel<T, NT, G>;
+  size_t smem = 0;
+  if constexpr (G > 0) smem = sizeof(LpLists) + LpMaxima<T, G>::bytes(vecs);
   // a cluster to a row where that leaves SMs without a block, down to 4 warp tiles a warp
   int csize = 1;
   while (csize < 8 && p.M * csize * 2 <= 2 * sms && vecs / (2 * csize) >= 4 * NT) csize *= 2;
@@ -758,7 +801,7 @@ void lp_launch(LogprobParams& p, cudaStream_t stream) {
   attr[0].val.clusterDim.x = (unsigned)csize;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = csize > 1 ? 1 : 0;
   if (smem > 32 * 1024)   // (48 KB with the static arrays go without)
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
@@ -793,16 +836,18 @@ void logprob_fwd(at::Tensor z, c10::optional<at::Tensor> targets, c10::optional<
   auto stream = at::cuda::getCurrentCUDAStream();
   ZQ_LP_TYPES(z.scalar_type(), {
     // What a row costs beside its columns (a load before the first, joins, the alternatives) is
-    // latency: blocks of 4 warps leave more of them on an SM to cover it (8192 x 152064: 683 us
-    // with 8 warps), where there are rows for twice as many.
-    const bool many = p.M >= 8 * (int64_t)at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    // latency, about 5 us: blocks of 4 warps, or of one for short rows, leave more of them on an
+    // SM to cover it, where there are rows for twice as many (8192 x 152064 with 32 alternatives:
+    // 683 us with 8 warps, 582 with 4; 16384 x 1000 with 20: 188 us with 4).
+    const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     auto shape = [&](auto nt) {
       constexpr int NT = decltype(nt)::value;
-      if (p.K == 0) lp_launch<T, NT, false, false>(p, stream);
-      else if (p.V <= kLpFine) lp_launch<T, NT, true, true>(p, stream);
-      else lp_launch<T, NT, true, false>(p, stream);
+      if (p.K == 0) lp_launch<T, NT, 0>(p, stream);
+      else if (2 * (p.V / (32 * LpVec<T>::N)) >= 3 * p.K) lp_launch<T, NT, 4>(p, stream);
+      else lp_launch<T, NT, 1>(p, stream);
     };
-    if (many) shape(std::integral_constant<int, 128>{});
+    if (p.V <= 4096 && p.M >= 4 * sms) shape(std::integral_constant<int, 32>{});
+    else if (p.M >= 8 * sms) shape(std::integral_constant<int, 128>{});
     else shape(std::integral_constant<int, 256>{});
   });
 }
