@@ -264,20 +264,23 @@ struct LpKey {
   }
 };
 
-// What a block keeps of a row for its top alternatives, behind one another in shared memory:
-// the lists; the maxima of its chunks, each the vectors of G lanes (4, or 1 where the row is
-// short); with G = 4 the maxima of its tiles of 32 vectors.
+// What a block keeps of a row for its top alternatives, behind one another in shared memory: the
+// lists; the maxima of its chunks; with G = 4 the maxima of its tiles of 32 vectors.  A chunk is
+// a vector (G = 1, short rows), or a lane's vectors of the four tiles that a warp takes at a time.
 struct LpLists {
   uint64_t cand[kLpCandidates + kLpMaxTop];
   uint32_t hits[kLpHits];
-  uint32_t n_cand, n_hits;
 };
 template <typename T, int G>
 struct LpMaxima {
   T *chunk, *tile;
-  static __host__ __device__ constexpr size_t bytes(int64_t vecs) {
-    return ((size_t)((vecs + G - 1) / G) + (G > 1 ? (size_t)((vecs + 31) / 32) : 0)) * sizeof(T);
+  static __host__ __device__ constexpr int tiles(int vecs) { return (vecs + 31) / 32; }
+  static __host__ __device__ constexpr int chunks(int vecs) { return G == 1 ? vecs : (tiles(vecs) + 3) / 4 * 32; }
+  static __host__ __device__ constexpr size_t bytes(int vecs) {
+    return ((size_t)chunks(vecs) + (G > 1 ? tiles(vecs) : 0)) * sizeof(T);
   }
+  static __device__ __forceinline__ int vector(int c, int j) { return G == 1 ? c : (c / 32 * 4 + j) * 32 + c % 32; }
+  static __device__ __forceinline__ int chunk_of(int i) { return G == 1 ? i : i / 128 * 32 + i % 32; }
 };
 
 // The top alternatives of a row, by one warp (the others' barriers would cost more than their
@@ -287,10 +290,10 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
                        bool nan, LpLists& list) {
   constexpr int N = LpVec<T>::N;
   using Key = LpKey<T>;
-  const int lane = threadIdx.x & 31, chunks = (row.vecs + G - 1) / G, tiles = (row.vecs + 31) / 32;
-  const uint32_t K = (uint32_t)p.K;
+  using Max = LpMaxima<T, G>;
+  const int lane = threadIdx.x & 31, chunks = Max::chunks(row.vecs), tiles = Max::tiles(row.vecs);
+  const uint32_t K = (uint32_t)p.K, below = (1u << lane) - 1u;
   auto chunk_key = [&](int i) { return Key::of(to_f32<T>(s_max.chunk[i])); };
-  if (lane == 0) list.n_cand = list.n_hits = 0u;
   // The K-th best of the tiles' maxima, or of the chunks' (0, below all, where there are fewer).
   // Of n parts with the K best among them some -n log(1 - K / n) elements reach it.
   const bool by_tile = G > 1 && 2 * tiles >= 3 * p.K;
@@ -317,73 +320,86 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
       if (__reduce_add_sync(0xffffffffu, n) >= K) bound = up;
     }
   }
-  __syncwarp();
   // the chunks that reach it
-  auto hit = [&](int i) {
-    if (i < chunks && chunk_key(i) >= bound) {
-      const uint32_t at = atomicAdd(&list.n_hits, 1u);
-      if (at < kLpHits) list.hits[at] = (uint32_t)i;
-    }
+  int hits = 0;
+  auto hit = [&](int i) {   // (every lane)
+    const bool in = i < chunks && chunk_key(min(i, chunks - 1)) >= bound;
+    const uint32_t all = __ballot_sync(0xffffffffu, in);
+    const int at = hits + __popc(all & below);
+    if (in && at < kLpHits) list.hits[at] = (uint32_t)i;
+    hits += __popc(all);
   };
-  if (by_tile) {
-    constexpr int kOf = 32 / G;   // chunks of a tile: those of four tiles (G = 4) at a time
+  if (by_tile) {   // a group of four tiles has 32 chunks
     for (int i0 = 0; i0 < tiles; i0 += 32) {
       uint32_t in = __ballot_sync(0xffffffffu, i0 + lane < tiles && part_key(min(i0 + lane, tiles - 1)) >= bound);
       while (in != 0) {
-        int mine = -1;
-#pragma unroll
-        for (int j = 0; j < 32 / kOf; ++j) {
-          if (in != 0 && lane / kOf == j) mine = i0 + __ffs(in) - 1;
-          in &= in - 1;
-        }
-        if (mine >= 0) hit(mine * kOf + lane % kOf);
+        const int group = (__ffs(in) - 1) / 4;
+        hit((i0 / 4 + group) * 32 + lane);
+        in &= ~(0xfu << (group * 4));
       }
     }
   } else {
-    for (int i = lane; i < chunks; i += 32) hit(i);
+    for (int i0 = 0; i0 < chunks; i0 += 32) hit(i0 + lane);
   }
   __syncwarp();
-  const int hits = (int)list.n_hits;
-  auto elements = [&](int i, const LpVec<T>& r, auto&& f) {
-    float v[N];
-    r.values(v);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int col = row.col(i) + j;
-      if (col >= 0 && col < row.V) f(Key::of(v[j]), (uint32_t)col);
-    }
-  };
-  // elements that may reach `at_least` (no less than the bound of the list of chunks)
+  // A lane's vector of those that may hold elements that reach `at_least` (no less than the
+  // bound of the list of chunks): f(vector, bits of its elements that do); in every lane.
   auto each = [&](uint32_t at_least, auto&& f) {
     const bool listed = hits <= kLpHits;   // (otherwise many equal maxima: all chunks)
     const int vecs = listed ? hits * G : row.vecs;
     constexpr int A = 4;   // vectors of a lane under way
-    for (int v0 = lane; v0 < vecs; v0 += 32 * A) {
+    for (int v0 = 0; v0 < vecs; v0 += 32 * A) {
       LpVec<T> r[A];
       int i[A];
 #pragma unroll
       for (int j = 0; j < A; ++j) {
-        const int v = v0 + j * 32;
-        i[j] = v >= vecs ? row.vecs : listed ? (int)list.hits[v / G] * G + v % G : v;
+        const int v = v0 + j * 32 + lane;
+        i[j] = v >= vecs ? row.vecs : listed ? Max::vector((int)list.hits[v / G], v % G) : v;
         if (i[j] < row.vecs) r[j] = row.load(i[j]);
       }
 #pragma unroll
-      for (int j = 0; j < A; ++j)
-        if (i[j] < row.vecs && Key::of(r[j].largest()) >= at_least) elements(i[j], r[j], f);
+      for (int j = 0; j < A; ++j) {
+        uint32_t bits = 0;
+        float v[N];
+        if (i[j] < row.vecs) {
+          r[j].values(v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const int col = row.col(i[j]) + e;
+            bits |= (Key::of(v[e]) >= at_least && col >= 0 && col < row.V ? 1u : 0u) << e;
+          }
+        }
+        if (__any_sync(0xffffffffu, bits != 0)) f(i[j], v, bits);
+      }
     }
   };
+  // Places for the lanes' numbers of elements, in the order of the lanes; all of them in `sum`.
+  auto places = [&](uint32_t count, uint32_t& sum) {
+    uint32_t to = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += up;
+    }
+    sum = __shfl_sync(0xffffffffu, to, 31);
+    return to - count;
+  };
   auto collect = [&](uint32_t from) {
+    uint32_t n = 0;
     __syncwarp();
-    if (lane == 0) list.n_cand = 0u;
-    __syncwarp();
-    each(from, [&](uint32_t key, uint32_t col) {
-      if (key >= from) {
-        const uint32_t at = atomicAdd(&list.n_cand, 1u);
-        if (at < kLpCandidates) list.cand[at] = ((uint64_t)key << 32) | (uint32_t)~col;
+    each(from, [&](int i, const float (&v)[N], uint32_t bits) {
+      uint32_t sum, at = n + places(__popc(bits), sum);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (bits >> e & 1u) {
+          if (at < kLpCandidates) list.cand[at] = ((uint64_t)Key::of(v[e]) << 32) | (uint32_t)~(uint32_t)(row.col(i) + e);
+          ++at;
+        }
       }
+      n += sum;
     });
     __syncwarp();
-    return list.n_cand;
+    return n;
   };
   // Elements that reach the bound, in any order (they are ranked below).  Where they do not fit
   // the list, those above it, and then those at it in the order of their columns as far as they
@@ -399,7 +415,7 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
       for (int bit = Key::kBits - 1; bit >= 0; --bit) {
         const uint32_t up = t | (1u << bit);
         uint32_t c = 0;
-        each(up, [&](uint32_t key, uint32_t) { c += key >= up ? 1u : 0u; });
+        each(up, [&](int, const float (&)[N], uint32_t bits) { c += __popc(bits); });
         if (__reduce_add_sync(0xffffffffu, c) >= K) t = up;
       }
       bound = t;
@@ -409,17 +425,17 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
     for (int i0 = 0; i0 < row.vecs && n < K; i0 += 32) {
       const int i = i0 + lane;
       uint32_t ties = 0;
-      if (i < row.vecs && chunk_key(i / G) >= bound)
-        elements(i, row.load(i), [&](uint32_t key, uint32_t col) { ties |= (key == bound ? 1u : 0u) << (int)(col - row.col(i)); });
-      if (!__any_sync(0xffffffffu, ties != 0)) continue;
-      uint32_t before = __popc(ties);   // of lower lanes
+      if (i < row.vecs && chunk_key(Max::chunk_of(i)) >= bound) {
+        float v[N];
+        row.load(i).values(v);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += up;
+        for (int e = 0; e < N; ++e) {
+          const int col = row.col(i) + e;
+          ties |= (Key::of(v[e]) == bound && col >= 0 && col < row.V ? 1u : 0u) << e;
+        }
       }
-      const uint32_t sum = __shfl_sync(0xffffffffu, before, 31);
-      uint32_t at = n + before - __popc(ties);
+      if (!__any_sync(0xffffffffu, ties != 0)) continue;
+      uint32_t sum, at = n + places(__popc(ties), sum);
       for (; ties != 0 && at < K; ties &= ties - 1, ++at)
         list.cand[at] = ((uint64_t)bound << 32) | (uint32_t)~(uint32_t)(row.col(i) + __ffs(ties) - 1);
       n = min(K, n + sum);
@@ -440,8 +456,8 @@ __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, c
   }
 }
 
-// A warp's tiles [t0, t1) of 32 vectors of a row: its sums, and its chunks' maxima.  Tiles that
-// lie inside the row go in groups of U, the next group's loads ahead of this one's arithmetic,
+// A warp's tiles [t0, t1) of 32 vectors of a row (t0 a multiple of 4): its sums, and its chunks'
+// maxima.  Tiles that lie inside the row go in groups of U, the next group's loads ahead of this one's arithmetic,
 // in packed pairs.
 template <typename T, int G>
 __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, float scale, const LpMaxima<T, G>& s_max) {
@@ -450,29 +466,27 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
   const float behind = kLpBehind / scale;
   float m = -INFINITY;
   uint64_t s2 = 0ull, a2 = 0ull;
-  auto chunk = [&](int tile, float top) {   // (exact in the type: one of its values)
+  auto keep_tile = [&](int tile, float top) {   // (exact in the type: one of its values)
     if constexpr (G == 1) {
       if (tile * 32 + lane < row.vecs) s_max.chunk[tile * 32 + lane] = from_f32<T>(top);
     } else if constexpr (G > 1) {
-#pragma unroll
-      for (int o = 1; o < G; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (lane % G == 0 && tile * 32 + lane < row.vecs) s_max.chunk[tile * (32 / G) + lane / G] = from_f32<T>(top);
       float all;
       asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
       if (lane == 0) s_max.tile[tile] = from_f32<T>(all);
     }
   };
   auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
-    float top[U], cm = -INFINITY;
+    float cm = -INFINITY;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (j < n) {
-        top[j] = r[j].largest();
-        chunk(tile + j, top[j]);
-        cm = fmaxf(cm, top[j]);
+        const float top = r[j].largest();
+        keep_tile(tile + j, top);
+        cm = max_nan(cm, top);
       }
     }
-    cm = fmaxf(cm, kLpFloor);
+    if constexpr (G > 1) s_max.chunk[tile / U * 32 + lane] = from_f32<T>(cm);
+    cm = fmaxf(cm, kLpFloor);   // (a NaN is left to the sums)
     if (cm > m + behind || m == -INFINITY) {
       float s, a, lo, hi;
       f2_unpack(s2, lo, hi), s = lo + hi;
@@ -581,11 +595,11 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_ker
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
   if constexpr (G > 0) {
     own_max.chunk = reinterpret_cast<T*>(lp_smem + sizeof(LpLists));
-    own_max.tile = own_max.chunk + (row.vecs + G - 1) / G;
+    own_max.tile = own_max.chunk + LpMaxima<T, G>::chunks(row.vecs);
   }
-  // consecutive tiles to a warp, as equal as they can be
-  const int tiles = (row.vecs + 31) / 32, part = crank * kWarps + warp, parts = csize * kWarps;
-  const int t0 = (int)((int64_t)tiles * part / parts), t1 = (int)((int64_t)tiles * (part + 1) / parts);
+  // consecutive groups of four tiles to a warp, as equal as they can be
+  const int tiles = (row.vecs + 31) / 32, groups = (tiles + 3) / 4, part = crank * kWarps + warp, parts = csize * kWarps;
+  const int t0 = 4 * (int)((int64_t)groups * part / parts), t1 = min(tiles, 4 * (int)((int64_t)groups * (part + 1) / parts));
   const int64_t y = p.targets != nullptr ? p.targets[m] : 0;
   row.ahead(t0 * 32 + lane);   // on its way while the target is read
   auto nothing = [&] {   // the row does not count
@@ -787,7 +801,7 @@ void lp_launch(LogprobParams& p, cudaStream_t stream) {
   const int64_t vecs = (p.V + 2 * N - 2) / N;   // at the worst alignment
   auto kern = logprob_fwd_kernel<T, NT, G>;
   size_t smem = 0;
-  if constexpr (G > 0) smem = sizeof(LpLists) + LpMaxima<T, G>::bytes(vecs);
+  if constexpr (G > 0) smem = sizeof(LpLists) + LpMaxima<T, G>::bytes((int)vecs);
   // a cluster to a row where that leaves SMs without a block, down to 4 warp tiles a warp
   int csize = 1;
   while (csize < 8 && p.M * csize * 2 <= 2 * sms && vecs / (2 * csize) >= 4 * NT) csize *= 2;
