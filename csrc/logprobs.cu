@@ -45,7 +45,9 @@ struct LogprobParams {
   float *logp, *entropy;    // [M]
   float* top;               // [M, K]
   int64_t* ids;             // [M, K]
-  float* stats;             // [M, 3]: m, log2 S, H of counted rows; log2 S = inf of the others
+  float* stats;             // [M, 3]: m, S, H of counted rows; S = inf of the others
+  uint8_t* maxima;          // [M, row_maxima] bytes: see LpMaxima
+  int64_t row_maxima;
   const float *gp, *gh, *gt;   // gradients, or null
   void* dz;
   int64_t M, stride, gstride, width, V;
@@ -233,18 +235,21 @@ __device__ __forceinline__ LpSums lp_warp_join(LpSums x, float scale) {
   return x;
 }
 
-// A row's few numbers, in 64 bits (sums and products; divisions and logarithms would take longer
-// than a short row): l = (z - m) / τ - log S.  PLAIN sums are relative to the rounded shift: m is
-// what it stands for.
-struct LpLog {
-  double m, log_s, inv_tau;
-  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) * inv_tau - log_s); }
-};
 // log of a positive number: its exponent's part in 64 bits, its mantissa's (below 0.35) in 32
 __device__ __forceinline__ double lp_log(float s) {
   const int e = (__float_as_int(s) - 0x3f3504f3) >> 23;   // mantissa in [sqrt(1/2), sqrt(2))
   return (double)e * 0.69314718055994531 + (double)logf(__int_as_float(__float_as_int(s) - (e << 23)));
 }
+// A row's few numbers, in 64 bits (sums and products; divisions and logarithms would take longer
+// than a short row): l = (z - m) / τ - log S.  Plain sums are relative to the rounded shift: m is
+// what it stands for.
+struct LpLog {
+  double m, log_s, inv_tau;
+  __device__ __forceinline__ LpLog(const LogprobParams& p, float high, float sum)
+      : m(lp_plain(high, p.scale) ? -(double)lp_shift(high, p.scale) * p.inv_scale : (double)high),
+        log_s(sum < INFINITY ? lp_log(sum) : 0.0), inv_tau(p.inv_tau) {}
+  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) * inv_tau - log_s); }
+};
 
 // Whole numbers in the values' order (0 and -0 equal, NaN above all), without the places that
 // are the same for all values of the type.
@@ -264,10 +269,11 @@ struct LpKey {
   }
 };
 
-// What a block keeps of a row for its top alternatives, behind one another in shared memory: the
-// lists; the maxima of its chunks; with G = 4 the maxima of its tiles of 32 vectors.  A chunk is
-// a vector (G = 1, short rows), or a lane's vectors of the four tiles that a warp takes at a time.
-struct LpLists {
+// What the pass over a row keeps for its top alternatives: the maxima of its chunks; with G = 4
+// the maxima of its tiles of 32 vectors, behind them.  A chunk is a vector (G = 1, short rows), or
+// a lane's vectors of the four tiles that a warp takes at a time.  For one row of 152064 columns
+// of bf16 they are 10.7 KB.
+struct LpLists {   // of a warp that ranks a row's alternatives
   uint64_t cand[kLpCandidates + kLpMaxTop];
   uint32_t hits[kLpHits];
 };
@@ -280,11 +286,14 @@ struct LpMaxima {
     return ((size_t)chunks(vecs) + (G > 1 ? tiles(vecs) : 0)) * sizeof(T);
   }
   static __device__ __forceinline__ int vector(int c, int j) { return G == 1 ? c : (c / 32 * 4 + j) * 32 + c % 32; }
+  __device__ __forceinline__ LpMaxima(const LogprobParams& p, int64_t m, int vecs)
+      : chunk(reinterpret_cast<T*>(p.maxima + m * p.row_maxima)), tile(chunk + chunks(vecs)) {}
   static __device__ __forceinline__ int chunk_of(int i) { return G == 1 ? i : i / 128 * 32 + i % 32; }
 };
 
-// The top alternatives of a row, by one warp (the others' barriers would cost more than their
-// help).
+// The top alternatives of a row, by one warp, in a launch of its own: what it waits for (a row's
+// maxima, its candidates from memory under load) is 10 to 20 us, in which the pass over the
+// logits would have one warp of its blocks at work (8192 x 152064 with 32 alternatives: 542 us).
 template <typename T, int G>
 __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const LpMaxima<T, G>& s_max, const LpLog& log,
                        bool nan, LpLists& list) {
@@ -586,24 +595,18 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_ker
   namespace cg = cooperative_groups;
   auto cluster = cg::this_cluster();
   const int csize = (int)cluster.num_blocks(), crank = (int)cluster.block_rank();
-  extern __shared__ __align__(16) uint8_t lp_smem[];   // the lists; chunks' maxima (rank 0: of the whole row)
-  LpMaxima<T, G> own_max{};
   __shared__ LpSums s_part[8 * kWarps];
   __shared__ LpSums s_row;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.x / (unsigned)csize;
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
-  if constexpr (G > 0) {
-    own_max.chunk = reinterpret_cast<T*>(lp_smem + sizeof(LpLists));
-    own_max.tile = own_max.chunk + LpMaxima<T, G>::chunks(row.vecs);
-  }
+  const LpMaxima<T, G> s_max(p, m, row.vecs);
   // consecutive groups of four tiles to a warp, as equal as they can be
   const int tiles = (row.vecs + 31) / 32, groups = (tiles + 3) / 4, part = crank * kWarps + warp, parts = csize * kWarps;
   const int t0 = 4 * (int)((int64_t)groups * part / parts), t1 = min(tiles, 4 * (int)((int64_t)groups * (part + 1) / parts));
   const int64_t y = p.targets != nullptr ? p.targets[m] : 0;
   row.ahead(t0 * 32 + lane);   // on its way while the target is read
   auto nothing = [&] {   // the row does not count
-    for (int i = tid; i < p.K; i += NT) p.ids[m * p.K + i] = -1, p.top[m * p.K + i] = 0.0f;
     if (tid == 0) {
       if (p.targets != nullptr) p.logp[m] = 0.0f;
       p.entropy[m] = 0.0f;
@@ -615,13 +618,8 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_ker
     return;
   }
   const float zy = tid == 0 && p.targets != nullptr ? to_f32<T>(row.z[y]) : 0.0f;
-  LpMaxima<T, G> s_max = own_max;
   LpSums* to = s_part;
   if (csize > 1) {
-    if constexpr (G > 0) {
-      s_max.chunk = cluster.map_shared_rank(own_max.chunk, 0);
-      s_max.tile = cluster.map_shared_rank(own_max.tile, 0);
-    }
     to = cluster.map_shared_rank(s_part, 0);
     cluster.sync();   // rank 0, to which the others write, is there
   }
@@ -647,25 +645,40 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_ker
   if (!plain) x = lp_far<T, NT>(row, scale, s_part);
   if (x.m == -INFINITY && x.s == x.s) return nothing();   // no logit above -inf
   const bool nan = !(x.s < INFINITY) || !(x.m < INFINITY);
-  if (warp > 0) return;
-  const LpLog log{plain ? -(double)lp_shift(x.m, scale) * p.inv_scale : (double)x.m, nan ? 0.0 : lp_log(x.s), p.inv_tau};
-  if (lane == 0) {
+  if (tid == 0) {
+    const LpLog log(p, x.m, x.s);
     const float h = nan ? NAN : fmaxf(0.0f, (float)(log.log_s - (double)(x.a / x.s) * 0.69314718055994531));
     if (p.targets != nullptr) p.logp[m] = nan ? NAN : log.of(zy);
     p.entropy[m] = h;
     p.stats[3 * m] = nan ? NAN : x.m;
-    p.stats[3 * m + 1] = nan ? NAN : (float)(log.log_s * 1.4426950408889634);
+    p.stats[3 * m + 1] = nan ? NAN : x.s;
     p.stats[3 * m + 2] = h;
   }
-  if constexpr (G > 0) lp_top<T, G>(p, row, m, own_max, log, nan, *reinterpret_cast<LpLists*>(lp_smem));
+}
+
+constexpr int kLpTopWarps = 4;   // rows of a block
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kLpTopWarps * 32) logprob_top_kernel(const __grid_constant__ LogprobParams p) {
+  __shared__ LpLists s_lists[kLpTopWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t m = (int64_t)blockIdx.x * kLpTopWarps + warp;
+  if (m >= p.M) return;
+  const float high = p.stats[3 * m], sum = p.stats[3 * m + 1];
+  if (sum == INFINITY) {   // the row does not count
+    for (int i = lane; i < p.K; i += 32) p.ids[m * p.K + i] = -1, p.top[m * p.K + i] = 0.0f;
+    return;
+  }
+  const LpRow<T> row(p.z, m, p.stride, (int)p.V);
+  lp_top<T, G>(p, row, m, LpMaxima<T, G>(p, m, row.vecs), LpLog(p, high, sum), sum != sum, s_lists[warp]);
 }
 
 // Gradient: a warp takes U tiles of 32 vectors of a row and needs no other: it sums the row's
 // entries of g itself, and the columns of its tiles with a g term it writes a second time.
-constexpr int kLpBwdWarps = 8, kLpBwdTiles = 4;
+constexpr int kLpBwdWarps = 8, kLpBwdTiles = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __grid_constant__ LogprobParams p, uint32_t segs) {
+__global__ void __launch_bounds__(kLpBwdWarps * 32, 3) logprob_bwd_kernel(const __grid_constant__ LogprobParams p, uint32_t segs) {
   constexpr int N = LpVec<T>::N, P = N / 2, U = kLpBwdTiles;
   const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * kLpBwdWarps + (threadIdx.x >> 5);
@@ -675,22 +688,27 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __g
   // the gradient's row has the logits' alignment; its vectors, the columns behind V among them
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
   T* out = reinterpret_cast<T*>(p.dz) + m * p.gstride;
-  const float high = p.stats[3 * m], l2 = p.stats[3 * m + 1], h = p.stats[3 * m + 2];
-  const bool counted = !(l2 == INFINITY);
+  const float high = p.stats[3 * m], sum = p.stats[3 * m + 1], h = p.stats[3 * m + 2];
+  const int64_t y = p.gp != nullptr && p.targets != nullptr ? p.targets[m] : -1;
+  const float gh = p.gh != nullptr ? p.gh[m] : 0.0f, gy = p.gp != nullptr ? p.gp[m] : 0.0f;
+  // the first 32 alternatives, one a lane
+  const bool mine = p.gt != nullptr && lane < p.K;
+  const float gt = mine ? p.gt[m * p.K + lane] : 0.0f;
+  const int64_t id = mine ? p.ids[m * p.K + lane] : -1;
+  const bool counted = !(sum == INFINITY);
   LpVec<T> r[U];
   const bool inside = row.inside(i0, 32 * U);
   if (counted) {
 #pragma unroll
     for (int j = 0; j < U; ++j) r[j] = inside ? row.load_whole(i0 + j * 32 + lane) : row.load(i0 + j * 32 + lane);
   }
-  const int64_t y = p.gp != nullptr && p.targets != nullptr ? p.targets[m] : -1;
-  const float gh = p.gh != nullptr ? p.gh[m] : 0.0f, gy = p.gp != nullptr ? p.gp[m] : 0.0f;
-  float g = 0.0f;   // of all entries
+  float g = gt;   // of all entries
   if (p.gt != nullptr) {
-    for (int i = lane; i < p.K; i += 32) g += p.gt[m * p.K + i];
+    for (int i = lane + 32; i < p.K; i += 32) g += p.gt[m * p.K + i];
     g = warp_sum(g);
   }
   // dz = p (c0 + c1 log2 p) + g terms
+  const float l2 = log2f(sum);
   const float inv = (float)p.inv_tau;
   const float c0 = -(g + gy + gh * h) * inv, c1 = -gh * kLpLn2 * inv;
   const bool plain = lp_plain(high, p.scale);
@@ -741,14 +759,15 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32) logprob_bwd_kernel(const __g
   // columns with g terms: this warp's, once its vectors are written
   const int c_begin = max(0, row.col(i0)), c_end = row.col(i0 + 32 * U);
   bool hit = false;
+  auto again = [&](int64_t c, float more) {
+    hit = hit || c == y;
+    if (c >= c_begin && c < c_end)
+      out[c] = from_f32<T>(smooth(to_f32<T>(row.z[c])) + (more + (c == y ? gy : 0.0f)) * inv);
+  };
   __syncwarp();
   if (p.gt != nullptr) {
-    for (int i = lane; i < p.K; i += 32) {
-      const int64_t c = p.ids[m * p.K + i];
-      hit = hit || c == y;
-      if (c < c_begin || c >= c_end) continue;
-      out[c] = from_f32<T>(smooth(to_f32<T>(row.z[c])) + (p.gt[m * p.K + i] + (c == y ? gy : 0.0f)) * inv);
-    }
+    if (mine) again(id, gt);
+    for (int i = lane + 32; i < p.K; i += 32) again(p.ids[m * p.K + i], p.gt[m * p.K + i]);
     hit = __any_sync(0xffffffffu, hit);
   }
   if (lane == 0 && !hit && y >= c_begin && y < c_end) out[y] = from_f32<T>(smooth(to_f32<T>(row.z[y])) + gy * inv);
@@ -795,20 +814,17 @@ LogprobParams lp_params(const at::Tensor& z, const c10::optional<at::Tensor>& ta
 }
 
 template <typename T, int NT, int G>
-void lp_launch(LogprobParams& p, cudaStream_t stream) {
+void lp_launch(LogprobParams& p, const at::Tensor& like, cudaStream_t stream) {
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   constexpr int N = LpVec<T>::N;
   const int64_t vecs = (p.V + 2 * N - 2) / N;   // at the worst alignment
   auto kern = logprob_fwd_kernel<T, NT, G>;
-  size_t smem = 0;
-  if constexpr (G > 0) smem = sizeof(LpLists) + LpMaxima<T, G>::bytes((int)vecs);
   // a cluster to a row where that leaves SMs without a block, down to 4 warp tiles a warp
   int csize = 1;
   while (csize < 8 && p.M * csize * 2 <= 2 * sms && vecs / (2 * csize) >= 4 * NT) csize *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.M * csize));
   cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -816,9 +832,17 @@ void lp_launch(LogprobParams& p, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = csize > 1 ? 1 : 0;
-  if (smem > 32 * 1024)   // (48 KB with the static arrays go without)
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  at::Tensor maxima;
+  if constexpr (G > 0) {
+    p.row_maxima = (int64_t)(LpMaxima<T, G>::bytes((int)vecs) + 15) / 16 * 16;
+    maxima = at::empty({p.M * p.row_maxima}, like.options().dtype(at::kByte));
+    p.maxima = reinterpret_cast<uint8_t*>(maxima.data_ptr());
+  }
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+  if constexpr (G > 0) {
+    logprob_top_kernel<T, G><<<(unsigned)((p.M + kLpTopWarps - 1) / kLpTopWarps), kLpTopWarps * 32, 0, stream>>>(p);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
 }
 
 }  // namespace
@@ -849,16 +873,15 @@ void logprob_fwd(at::Tensor z, c10::optional<at::Tensor> targets, c10::optional<
   const c10::cuda::CUDAGuard guard(z.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   ZQ_LP_TYPES(z.scalar_type(), {
-    // What a row costs beside its columns (a load before the first, joins, the alternatives) is
-    // latency, about 5 us: blocks of 4 warps, or of one for short rows, leave more of them on an
-    // SM to cover it, where there are rows for twice as many (8192 x 152064 with 32 alternatives:
-    // 683 us with 8 warps, 582 with 4; 16384 x 1000 with 20: 188 us with 4).
+    // What a row costs beside its columns (a load before the first, joins) is latency: blocks of
+    // 4 warps, or of one for short rows, leave more of them on an SM to cover it, where there are
+    // rows for twice as many (4096 x 50257: 86 us with 8 warps, 78 with 4).
     const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     auto shape = [&](auto nt) {
       constexpr int NT = decltype(nt)::value;
-      if (p.K == 0) lp_launch<T, NT, 0>(p, stream);
-      else if (2 * (p.V / (32 * LpVec<T>::N)) >= 3 * p.K) lp_launch<T, NT, 4>(p, stream);
-      else lp_launch<T, NT, 1>(p, stream);
+      if (p.K == 0) lp_launch<T, NT, 0>(p, z, stream);
+      else if (2 * (p.V / (32 * LpVec<T>::N)) >= 3 * p.K) lp_launch<T, NT, 4>(p, z, stream);
+      else lp_launch<T, NT, 1>(p, z, stream);
     };
     if (p.V <= 4096 && p.M >= 4 * sms) shape(std::integral_constant<int, 32>{});
     else if (p.M >= 8 * sms) shape(std::integral_constant<int, 128>{});
