@@ -15,9 +15,8 @@
 // and the same one wherever it enters, so t carries one rounding of a small number and no
 // error of the size of m s.  Rows whose maximum is far from 0 (all masked by the type's lowest
 // value) are summed again from differences.  The top alternatives cost that pass the maximum of every
-// chunk of columns and of every warp's tile: the k best of the row lie in the k tiles (or chunks)
-// with the best maxima, so the k-th best of those is a bound, and only chunks that reach it are
-// looked at again.
+// chunk of columns: the k best of the row lie in the k chunks with the best maxima, so the k-th
+// best of those is a bound, and a second launch looks at the chunks that reach it alone.
 // Backward: one pass, p from the row's m, S and H; the columns with a g term are written a
 // second time by their block (each sum rounded once; no atomics).
 //
@@ -269,117 +268,163 @@ struct LpKey {
   }
 };
 
-// What the pass over a row keeps for its top alternatives: the maxima of its chunks; with G = 4
-// the maxima of its tiles of 32 vectors, behind them.  A chunk is a vector (G = 1, short rows), or
-// a lane's vectors of the four tiles that a warp takes at a time.  For one row of 152064 columns
-// of bf16 they are 10.7 KB.
-struct LpLists {   // of a warp that ranks a row's alternatives
-  uint64_t cand[kLpCandidates + kLpMaxTop];
-  uint32_t hits[kLpHits];
-};
+// What the pass over a row keeps for its top alternatives: the maxima of its chunks.  A chunk is a
+// vector (G = 1, rows of few vectors for the alternatives wanted), or a lane's vectors of the four
+// tiles that a warp takes at a time (G = 4); 9.5 KB for a row of 152064 columns of bf16.
 template <typename T, int G>
 struct LpMaxima {
-  T *chunk, *tile;
-  static __host__ __device__ constexpr int tiles(int vecs) { return (vecs + 31) / 32; }
-  static __host__ __device__ constexpr int chunks(int vecs) { return G == 1 ? vecs : (tiles(vecs) + 3) / 4 * 32; }
-  static __host__ __device__ constexpr size_t bytes(int vecs) {
-    return ((size_t)chunks(vecs) + (G > 1 ? tiles(vecs) : 0)) * sizeof(T);
+  static constexpr int kPad = 16 / (int)sizeof(T);
+  T* chunk;
+  static __host__ __device__ constexpr int chunks(int vecs) { return G == 1 ? vecs : (vecs + 127) / 128 * 32; }
+  static __host__ __device__ constexpr int64_t bytes(int vecs) {   // of a row
+    return (int64_t)((chunks(vecs) + kPad - 1) / kPad * kPad) * (int64_t)sizeof(T);
   }
+  __device__ __forceinline__ LpMaxima(const LogprobParams& p, int64_t m) : chunk(reinterpret_cast<T*>(p.maxima + m * p.row_maxima)) {}
   static __device__ __forceinline__ int vector(int c, int j) { return G == 1 ? c : (c / 32 * 4 + j) * 32 + c % 32; }
-  __device__ __forceinline__ LpMaxima(const LogprobParams& p, int64_t m, int vecs)
-      : chunk(reinterpret_cast<T*>(p.maxima + m * p.row_maxima)), tile(chunk + chunks(vecs)) {}
   static __device__ __forceinline__ int chunk_of(int i) { return G == 1 ? i : i / 128 * 32 + i % 32; }
 };
 
-// The top alternatives of a row, by one warp, in a launch of its own: what it waits for (a row's
-// maxima, its candidates from memory under load) is 10 to 20 us, in which the pass over the
-// logits would have one warp of its blocks at work (8192 x 152064 with 32 alternatives: 542 us).
+constexpr int kLpParts = 512;   // a row's chunks in at most this many parts
+struct LpLists {                 // of a warp that ranks a row's alternatives
+  uint64_t cand[kLpCandidates + kLpMaxTop];
+  uint32_t key[kLpParts];        // of the parts; then the parts that reach the bound
+  uint32_t hits[kLpHits];        // chunks that do
+  uint32_t vecs[128];            // vectors that do, of a step
+};
+
+// 16 bytes where `there`, without a branch: several such loads are under way at once
+__device__ __forceinline__ uint4 lp_load_if(const void* p, bool there) {
+  uint4 r = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  setp.ne.u32 p, %5, 0;\n"
+      "  @p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+      "}\n"
+      : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+      : "l"(p), "r"((uint32_t)there));
+  return r;
+}
+
+// The top alternatives of a row, by one warp, in a launch of its own: what it waits for (the
+// row's maxima, its candidates from memory) is 5 to 10 us, in which the pass over the logits would
+// have one warp of its blocks at work (8192 x 152064 with 32 alternatives: 542 us).
 template <typename T, int G>
 __device__ void lp_top(const LogprobParams& p, const LpRow<T>& row, int64_t m, const LpMaxima<T, G>& s_max, const LpLog& log,
                        bool nan, LpLists& list) {
   constexpr int N = LpVec<T>::N;
   using Key = LpKey<T>;
   using Max = LpMaxima<T, G>;
-  const int lane = threadIdx.x & 31, chunks = Max::chunks(row.vecs), tiles = Max::tiles(row.vecs);
+  const int lane = threadIdx.x & 31, chunks = Max::chunks(row.vecs);
   const uint32_t K = (uint32_t)p.K, below = (1u << lane) - 1u;
   auto chunk_key = [&](int i) { return Key::of(to_f32<T>(s_max.chunk[i])); };
-  // The K-th best of the tiles' maxima, or of the chunks' (0, below all, where there are fewer).
-  // Of n parts with the K best among them some -n log(1 - K / n) elements reach it.
-  const bool by_tile = G > 1 && 2 * tiles >= 3 * p.K;
-  const T* parts = by_tile ? s_max.tile : s_max.chunk;
-  const int n_parts = by_tile ? tiles : chunks;
-  auto part_key = [&](int i) { return Key::of(to_f32<T>(parts[i])); };
-  uint32_t bound = 0;
-  if (n_parts >= p.K) {
-    constexpr int kOwn = 24;   // parts of a lane whose keys it holds
-    const bool own = n_parts <= kOwn * 32;
-    uint32_t key[kOwn];
+  // Parts of `size` consecutive chunks.  The K-th best of the parts' maxima (0, below all, where
+  // there are fewer) is the bound: of n parts some -n log(1 - K / n) elements reach it.
+  // (One warp at work waits for its instructions too: loops here are short and rolled.)
+  int shift = 0;
+  while ((kLpParts << shift) < chunks) ++shift;
+  const int size = 1 << shift, parts = (chunks + size - 1) >> shift;
+  for (int i = lane; i < parts; i += 32) list.key[i] = 0u;
+  __syncwarp();
+  constexpr int A = 4;   // loads of a lane under way
+  for (int c0 = 0; c0 < chunks; c0 += 32 * N * A) {   // (a row's chunks end in a whole vector)
+    LpVec<T> r[A];
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) key[i] = own && i * 32 + lane < n_parts ? part_key(i * 32 + lane) : 0u;
+    for (int j = 0; j < A; ++j) {
+      const int c = c0 + (j * 32 + lane) * N;
+      r[j].u = lp_load_if(s_max.chunk + c, c < chunks);
+    }
+#pragma unroll
+    for (int j = 0; j < A; ++j) {
+      const int c = c0 + (j * 32 + lane) * N;
+      if (c >= chunks) continue;
+      if (size >= N) {
+        atomicMax(&list.key[c >> shift], Key::of(r[j].largest()));
+      } else {
+        float v[N];
+        r[j].values(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (c + e < chunks) atomicMax(&list.key[(c + e) >> shift], Key::of(v[e]));
+      }
+    }
+  }
+  __syncwarp();
+  uint32_t bound = 0;
+  if (parts >= p.K) {
 #pragma unroll 1
     for (int bit = Key::kBits - 1; bit >= 0; --bit) {
       const uint32_t up = bound | (1u << bit);   // (above 0, the key of no part)
       uint32_t n = 0;
-      if (own) {
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) n += key[i] >= up ? 1u : 0u;
-      } else {
-        for (int i = lane; i < n_parts; i += 32) n += part_key(i) >= up ? 1u : 0u;
-      }
+#pragma unroll 8
+      for (int i = lane; i < parts; i += 32) n += list.key[i] >= up ? 1u : 0u;
       if (__reduce_add_sync(0xffffffffu, n) >= K) bound = up;
     }
   }
-  // the chunks that reach it
-  int hits = 0;
-  auto hit = [&](int i) {   // (every lane)
-    const bool in = i < chunks && chunk_key(min(i, chunks - 1)) >= bound;
+  // the parts that reach it, and their chunks that do
+  auto push = [&](bool in, uint32_t what, uint32_t* to, int& n, int room) {
     const uint32_t all = __ballot_sync(0xffffffffu, in);
-    const int at = hits + __popc(all & below);
-    if (in && at < kLpHits) list.hits[at] = (uint32_t)i;
-    hits += __popc(all);
+    const int at = n + __popc(all & below);
+    if (in && at < room) to[at] = what;
+    n += __popc(all);
   };
-  if (by_tile) {   // a group of four tiles has 32 chunks
-    for (int i0 = 0; i0 < tiles; i0 += 32) {
-      uint32_t in = __ballot_sync(0xffffffffu, i0 + lane < tiles && part_key(min(i0 + lane, tiles - 1)) >= bound);
-      while (in != 0) {
-        const int group = (__ffs(in) - 1) / 4;
-        hit((i0 / 4 + group) * 32 + lane);
-        in &= ~(0xfu << (group * 4));
-      }
+  int n_parts = 0, hits = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < parts; i0 += 32) {   // (in place: no further than what has been read)
+    const bool in = i0 + lane < parts && list.key[min(i0 + lane, kLpParts - 1)] >= bound;
+    __syncwarp();
+    push(in, (uint32_t)(i0 + lane), list.key, n_parts, kLpParts);
+    __syncwarp();
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 < n_parts << shift; i0 += 32 * A) {
+    uint32_t k[A];
+    int c[A];
+#pragma unroll
+    for (int j = 0; j < A; ++j) {
+      const int i = i0 + j * 32 + lane;
+      c[j] = i < n_parts << shift ? ((int)list.key[min(i >> shift, n_parts - 1)] << shift) + (i & (size - 1)) : chunks;
+      k[j] = chunk_key(min(c[j], chunks - 1));
     }
-  } else {
-    for (int i0 = 0; i0 < chunks; i0 += 32) hit(i0 + lane);
+#pragma unroll
+    for (int j = 0; j < A; ++j) push(c[j] < chunks && k[j] >= bound, (uint32_t)c[j], list.hits, hits, kLpHits);
   }
   __syncwarp();
-  // A lane's vector of those that may hold elements that reach `at_least` (no less than the
-  // bound of the list of chunks): f(vector, bits of its elements that do); in every lane.
+  // A lane's vector of those that hold elements that reach `at_least` (no less than the bound of
+  // the list of chunks): f(vector, values, bits of its elements that do); in every lane.
   auto each = [&](uint32_t at_least, auto&& f) {
     const bool listed = hits <= kLpHits;   // (otherwise many equal maxima: all chunks)
     const int vecs = listed ? hits * G : row.vecs;
-    constexpr int A = 4;   // vectors of a lane under way
+#pragma unroll 1
     for (int v0 = 0; v0 < vecs; v0 += 32 * A) {
       LpVec<T> r[A];
-      int i[A];
+      int i[A], n = 0;
 #pragma unroll
       for (int j = 0; j < A; ++j) {
         const int v = v0 + j * 32 + lane;
         i[j] = v >= vecs ? row.vecs : listed ? Max::vector((int)list.hits[v / G], v % G) : v;
-        if (i[j] < row.vecs) r[j] = row.load(i[j]);
+        r[j].u = lp_load_if(row.z + row.col(i[j]), row.whole(i[j]));
       }
 #pragma unroll
-      for (int j = 0; j < A; ++j) {
+      for (int j = 0; j < A; ++j)   // (the row's edges are looked at below)
+        push(i[j] < row.vecs && (!row.whole(i[j]) || Key::of(r[j].largest()) >= at_least), (uint32_t)i[j], list.vecs, n, 128);
+      __syncwarp();
+#pragma unroll 1
+      for (int u = 0; u < n; u += 32) {
         uint32_t bits = 0;
+        const int at = u + lane < n ? (int)list.vecs[u + lane] : row.vecs;
         float v[N];
-        if (i[j] < row.vecs) {
-          r[j].values(v);
+        if (at < row.vecs) {
+          row.load(at).values(v);
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            const int col = row.col(i[j]) + e;
+            const int col = row.col(at) + e;
             bits |= (Key::of(v[e]) >= at_least && col >= 0 && col < row.V ? 1u : 0u) << e;
           }
         }
-        if (__any_sync(0xffffffffu, bits != 0)) f(i[j], v, bits);
+        f(at, v, bits);
       }
+      __syncwarp();
     }
   };
   // Places for the lanes' numbers of elements, in the order of the lanes; all of them in `sum`.
@@ -475,22 +520,14 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
   const float behind = kLpBehind / scale;
   float m = -INFINITY;
   uint64_t s2 = 0ull, a2 = 0ull;
-  auto keep_tile = [&](int tile, float top) {   // (exact in the type: one of its values)
-    if constexpr (G == 1) {
-      if (tile * 32 + lane < row.vecs) s_max.chunk[tile * 32 + lane] = from_f32<T>(top);
-    } else if constexpr (G > 1) {
-      float all;
-      asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(top));
-      if (lane == 0) s_max.tile[tile] = from_f32<T>(all);
-    }
-  };
   auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
     float cm = -INFINITY;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (j < n) {
         const float top = r[j].largest();
-        keep_tile(tile + j, top);
+        if constexpr (G == 1)   // (exact: one of the type's values; -inf up to a whole vector of them)
+          if ((tile + j) * 32 + lane < (row.vecs + N - 1) / N * N) s_max.chunk[(tile + j) * 32 + lane] = from_f32<T>(top);
         cm = max_nan(cm, top);
       }
     }
@@ -600,7 +637,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) logprob_fwd_ker
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t m = blockIdx.x / (unsigned)csize;
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
-  const LpMaxima<T, G> s_max(p, m, row.vecs);
+  const LpMaxima<T, G> s_max(p, m);
   // consecutive groups of four tiles to a warp, as equal as they can be
   const int tiles = (row.vecs + 31) / 32, groups = (tiles + 3) / 4, part = crank * kWarps + warp, parts = csize * kWarps;
   const int t0 = 4 * (int)((int64_t)groups * part / parts), t1 = min(tiles, 4 * (int)((int64_t)groups * (part + 1) / parts));
@@ -670,7 +707,7 @@ __global__ void __launch_bounds__(kLpTopWarps * 32) logprob_top_kernel(const __g
     return;
   }
   const LpRow<T> row(p.z, m, p.stride, (int)p.V);
-  lp_top<T, G>(p, row, m, LpMaxima<T, G>(p, m, row.vecs), LpLog(p, high, sum), sum != sum, s_lists[warp]);
+  lp_top<T, G>(p, row, m, LpMaxima<T, G>(p, m), LpLog(p, high, sum), sum != sum, s_lists[warp]);
 }
 
 // Gradient: a warp takes U tiles of 32 vectors of a row and needs no other: it sums the row's
@@ -834,7 +871,7 @@ void lp_launch(LogprobParams& p, const at::Tensor& like, cudaStream_t stream) {
   cfg.numAttrs = csize > 1 ? 1 : 0;
   at::Tensor maxima;
   if constexpr (G > 0) {
-    p.row_maxima = (int64_t)(LpMaxima<T, G>::bytes((int)vecs) + 15) / 16 * 16;
+    p.row_maxima = LpMaxima<T, G>::bytes((int)vecs);
     maxima = at::empty({p.M * p.row_maxima}, like.options().dtype(at::kByte));
     p.maxima = reinterpret_cast<uint8_t*>(maxima.data_ptr());
   }
@@ -880,7 +917,7 @@ void logprob_fwd(at::Tensor z, c10::optional<at::Tensor> targets, c10::optional<
     auto shape = [&](auto nt) {
       constexpr int NT = decltype(nt)::value;
       if (p.K == 0) lp_launch<T, NT, 0>(p, z, stream);
-      else if (2 * (p.V / (32 * LpVec<T>::N)) >= 3 * p.K) lp_launch<T, NT, 4>(p, z, stream);
+      else if (2 * (p.V / (4 * LpVec<T>::N)) >= 3 * p.K) lp_launch<T, NT, 4>(p, z, stream);
       else lp_launch<T, NT, 1>(p, z, stream);
     };
     if (p.V <= 4096 && p.M >= 4 * sms) shape(std::integral_constant<int, 32>{});
