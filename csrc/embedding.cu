@@ -4,13 +4,15 @@
 //   dW_v = s sum over i with id_i = v of dy_i, in 32 bits, rounded once; other rows 0
 //
 // Backward.  The (id, token) pairs are sorted by id, equal ids in token order (a radix sort of
-// 8-bit digits, least significant first, each pass stable): in one block's shared memory up
-// to kSortBlock tokens, in passes over all blocks' tiles above that.  Blocks beyond the sort's
-// write the table's zeros meanwhile.  Then a warp takes kPiece sorted tokens and 256 columns
-// and adds the tokens' rows up in order; a run of one id inside a piece is a finished row of
-// dW.  Runs that cross pieces leave partial sums, which a last kernel adds in piece order.  No
-// atomics on values, so a gradient is the same bits from run to run, and no run is longer than
-// a piece for any warp, however often an id occurs.
+// 9-bit digits, least significant first, each pass stable): in one block's shared memory up
+// to kSortTile tokens, in passes over all blocks' tiles above that.  Then a warp takes kPiece
+// sorted tokens and 256 columns and adds the tokens' rows up in order; a run of one id inside a
+// piece is a finished row of dW.  Blocks beyond these write zeros over the rows that no token
+// has (each lane looks its row up among the sorted ids); the table's first rows are filled with
+// zeros as a whole by blocks beyond the sort's, as many as memory takes while it sorts.  Runs that cross pieces leave partial
+// sums, which a last kernel adds in piece order.  No atomics on values, so a gradient is the same
+// bits from run to run, and no run is longer than a piece for any warp, however often an id
+// occurs.
 //
 // What bounds it: memory; the zeros of a large table are most of it.
 #include <ATen/ATen.h>
@@ -25,7 +27,7 @@ namespace zq {
 
 constexpr int kEmbWarps = 8;
 constexpr int kPiece = 32;             // sorted tokens of a warp
-constexpr int kRadixBits = 8, kRadix = 1 << kRadixBits;
+constexpr int kRadixBits = 9, kRadix = 1 << kRadixBits;
 constexpr int kSortWarps = 32, kSortItems = 8;
 constexpr int kSortTile = kSortWarps * 32 * kSortItems;   // tokens that a block ranks: 8192
 
@@ -105,22 +107,36 @@ __device__ __forceinline__ uint32_t rank_step(uint16_t* mine, uint32_t digit, bo
   return before + r.peers_before;
 }
 
-// Zeros over the table by blocks [first, gridDim.x).
-__device__ __forceinline__ void zero_table(void* dw, int64_t bytes, int first) {
-  const int64_t vecs = bytes / 16, step = (int64_t)(gridDim.x - first) * blockDim.x;
-  uint4* p = reinterpret_cast<uint4*>(dw);
+// Zeros over `bytes` bytes by a warp.
+__device__ __forceinline__ void zero_range(uint8_t* p, int64_t bytes, int lane) {
+  const int64_t head = min(bytes, (int64_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
+  for (int64_t i = lane; i < head; i += 32) p[i] = 0;
+  p += head, bytes -= head;
+  const int64_t vecs = bytes / 16;
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-  const int64_t at = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x;
-  for (int64_t i = at; i < vecs; i += step) p[i] = z;
-  if (at == 0)
-    for (int64_t i = vecs * 16; i < bytes; ++i) reinterpret_cast<uint8_t*>(dw)[i] = 0;
+#pragma unroll 4
+  for (int64_t i = lane; i < vecs; i += 32) reinterpret_cast<uint4*>(p)[i] = z;
+  for (int64_t i = vecs * 16 + lane; i < bytes; i += 32) p[i] = 0;
+}
+
+// Zeros over `bytes` bytes by the blocks from `first` on.
+struct ZeroShare {
+  uint8_t* p;
+  int64_t bytes;
+};
+constexpr int64_t kZeroChunk = 16384;
+__device__ __forceinline__ void zero_share(const ZeroShare& z, int first) {
+  const int warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  const int64_t step = (int64_t)(gridDim.x - first) * warps * kZeroChunk;
+  for (int64_t at = ((int64_t)(blockIdx.x - first) * warps + threadIdx.x / 32) * kZeroChunk; at < z.bytes; at += step)
+    zero_range(z.p + at, min(kZeroChunk, z.bytes - at), lane);
 }
 
 // Exclusive sums of s_count[warp][digit] in the order digit, warp (u16: at most kSortTile),
-// by 1024 threads: each takes a digit's run of 8 warps.
+// by 1024 threads: each takes a digit's run of kRun warps.
 __device__ __forceinline__ void scan_counts(uint16_t (*s_count)[kRadix], uint32_t* s_sum) {
-  constexpr int kRun = kSortWarps * kRadix / (kSortWarps * 32);   // counters of a thread: 8
-  constexpr int kRuns = kSortWarps / kRun;                        // threads of a digit: 4
+  constexpr int kRun = kSortWarps * kRadix / (kSortWarps * 32);   // counters of a thread: 16
+  constexpr int kRuns = kSortWarps / kRun;                        // threads of a digit: 2
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int digit = tid / kRuns, w0 = (tid % kRuns) * kRun;
   uint32_t sum = 0, v[kRun];
@@ -150,14 +166,15 @@ __device__ __forceinline__ void scan_counts(uint16_t (*s_count)[kRadix], uint32_
   __syncthreads();
 }
 
-// Block 0 sorts up to kSortTile tokens; the others write zeros.
+// One block sorts up to kSortTile tokens.  (n_cross: see the sums)
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_block_kernel(const void* __restrict__ ids, int ids64, int T,
                                                                                int V, int passes, int32_t* __restrict__ keys,
                                                                                int32_t* __restrict__ order,
-                                                                               void* __restrict__ dw, int64_t dw_bytes) {
-  if (blockIdx.x > 0) return zero_table(dw, dw_bytes, 1);
+                                                                               int32_t* __restrict__ n_cross, const ZeroShare zero) {
+  if (blockIdx.x > 0) return zero_share(zero, 1);
+  if (threadIdx.x == 0) *n_cross = 0;
   extern __shared__ uint8_t emb_smem[];
-  uint16_t(*s_count)[kRadix] = reinterpret_cast<uint16_t(*)[kRadix]>(emb_smem);           // 16 KB
+  uint16_t(*s_count)[kRadix] = reinterpret_cast<uint16_t(*)[kRadix]>(emb_smem);           // 32 KB
   uint32_t* s_key = reinterpret_cast<uint32_t*>(emb_smem + kSortWarps * kRadix * 2);      // 32 KB
   uint16_t* s_at = reinterpret_cast<uint16_t*>(s_key + kSortTile);                        // 16 KB
   __shared__ uint32_t s_sum[32];
@@ -202,14 +219,15 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_block_kernel(c
   for (int i = tid; i < T; i += blockDim.x) keys[i] = (int32_t)s_key[i], order[i] = (int32_t)s_at[i];
 }
 
-// One pass over many tiles: the tiles' counts of a digit's values (blocks beyond the tiles
-// write zeros) ...
+// One pass over many tiles: the tiles' counts of a digit's values ...
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_count_kernel(const void* __restrict__ ids, int ids64, int64_t T,
-                                                                          int V, int shift, int tiles,
+                                                                          int V, int shift,
                                                                           uint32_t* __restrict__ counts,
-                                                                          void* __restrict__ dw, int64_t dw_bytes) {
-  if ((int)blockIdx.x >= tiles) return zero_table(dw, dw_bytes, tiles);
+                                                                          int32_t* __restrict__ n_cross, int tiles,
+                                                                          const ZeroShare zero) {
+  if ((int)blockIdx.x >= tiles) return zero_share(zero, tiles);
+  if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *n_cross = 0;
   __shared__ uint32_t s_n[kRadix];
   const int tid = threadIdx.x;
   if (tid < kRadix) s_n[tid] = 0u;
@@ -224,7 +242,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_count_kernel(const 
     }
   }
   __syncthreads();
-  if (tid < kRadix) counts[(int64_t)tid * tiles + blockIdx.x] = s_n[tid];
+  if (tid < kRadix) counts[(int64_t)blockIdx.x * kRadix + tid] = s_n[tid];
 }
 
 // ... and the tiles' items to their places: each block sums the counts before its own.
@@ -234,22 +252,21 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_place_kernel(const 
                                                                           int shift, int tiles,
                                                                           const uint32_t* __restrict__ counts,
                                                                           int32_t* __restrict__ keys,
-                                                                          int32_t* __restrict__ order) {
+                                                                          int32_t* __restrict__ order, const ZeroShare zero) {
+  if ((int)blockIdx.x >= tiles) return zero_share(zero, tiles);
   extern __shared__ uint8_t emb_smem[];
   uint16_t(*s_count)[kRadix] = reinterpret_cast<uint16_t(*)[kRadix]>(emb_smem);
   __shared__ uint32_t s_base[kRadix], s_total[kRadix];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // a warp sums a digit's tiles: those before this one, and all
-  for (int d = warp; d < kRadix; d += kSortWarps) {
+  if (tid < kRadix) {   // a digit's tiles: those before this one, and all
     uint32_t before = 0, all = 0;
-    for (int t = lane; t < tiles; t += 32) {
-      const uint32_t c = counts[(int64_t)d * tiles + t];
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+      const uint32_t c = counts[(int64_t)t * kRadix + tid];
       all += c;
       before += t < (int)blockIdx.x ? c : 0u;
     }
-    before = __reduce_add_sync(0xffffffffu, before);
-    all = __reduce_add_sync(0xffffffffu, all);
-    if (lane == 0) s_base[d] = before, s_total[d] = all;
+    s_base[tid] = before, s_total[tid] = all;
   }
   const int64_t first = (int64_t)blockIdx.x * kSortTile + warp * kSortItems * 32;
   uint32_t key[kSortItems], token[kSortItems], rank[kSortItems];
@@ -305,16 +322,45 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_place_kernel(const 
 // ---------------------------------------------------------------------------
 // sums
 // ---------------------------------------------------------------------------
-// partial sums [pieces, 2, D]: of the run that a piece starts with and that began before it
+// 32 rows of the table from `first` on: zeros over those that no token has.
+__device__ __forceinline__ void zero_rows(const int32_t* __restrict__ keys, int64_t tokens, uint8_t* dw, int64_t row_bytes,
+                                          int64_t first, int V, int lane) {
+  const int64_t row = first + lane;
+  int64_t lo = 0, hi = tokens;   // first token whose id is not below the row's
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  uint32_t absent = __ballot_sync(0xffffffffu, row < V && (lo == tokens || keys[lo] != row));
+  while (absent != 0) {   // consecutive ones are one range
+    const int from = __ffs(absent) - 1;
+    const uint32_t run = ~(absent >> from);
+    const int n = run == 0u ? 32 : __ffs(run) - 1;
+    zero_range(dw + (first + from) * row_bytes, n * row_bytes, lane);
+    absent = from + n >= 32 ? 0u : absent >> (from + n) << (from + n);
+  }
+}
+
+// Partial sums [pieces, 2, D]: of the run that a piece starts with and that began before it
 // (0; also where it goes on behind the piece), and of the one that it starts and that goes
-// on behind it (1)
+// on behind it (1).  Pieces with one of the latter are listed for the join (in any order).
+// Warps behind the pieces' write zeros.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbWarps * 32) embedding_sum_kernel(const int32_t* __restrict__ keys,
                                                                        const int32_t* __restrict__ order, int64_t tokens,
                                                                        const T* __restrict__ dy, int64_t dys,
                                                                        T* __restrict__ dw, float* __restrict__ part,
-                                                                       int tiles, int V, int D, float scale) {
+                                                                       int32_t* __restrict__ n_cross,
+                                                                       int32_t* __restrict__ cross, int sum_blocks,
+                                                                       int64_t zero_from, int tiles,
+                                                                       int V, int D, float scale) {
   const int lane = threadIdx.x & 31;
+  if ((int)blockIdx.x >= sum_blocks) {
+    const int64_t first = zero_from + ((int64_t)(blockIdx.x - sum_blocks) * kEmbWarps + (threadIdx.x >> 5)) * 32;
+    if (first < V) zero_rows(keys, tokens, reinterpret_cast<uint8_t*>(dw), (int64_t)D * sizeof(T), first, V, lane);
+    return;
+  }
   const int64_t unit = (int64_t)blockIdx.x * kEmbWarps + (threadIdx.x >> 5);
   const int64_t piece = unit / tiles, begin = piece * kPiece;
   if (begin >= tokens) return;
@@ -353,6 +399,7 @@ __global__ void __launch_bounds__(kEmbWarps * 32) embedding_sum_kernel(const int
           if (k < V) {
             const bool began_before = run == 0 && before == k, goes_on = at + 1 == n && next == k;
             if (began_before || goes_on) {
+              if (!began_before && base == 0 && lane == 0) cross[atomicAdd(n_cross, 1)] = (int32_t)piece;
               store_tile<float, VEC>(part + (piece * 2 + (began_before ? 0 : 1)) * D, base, lane, D, sum);
             } else {
 #pragma unroll
@@ -369,51 +416,55 @@ __global__ void __launch_bounds__(kEmbWarps * 32) embedding_sum_kernel(const int
   }
 }
 
-// A block takes a piece and 256 columns: where a run starts in the piece and goes on, the
-// pieces' partial sums of that run.  Its warps take the pieces in turn and are added in warp
-// order.
+// A block takes a listed piece and 256 columns: the pieces' partial sums of the run that starts
+// there and goes on.  Its warps take the pieces in turn and are added in warp order.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kEmbWarps * 32) embedding_join_kernel(const int32_t* __restrict__ keys, int64_t tokens,
                                                                         const float* __restrict__ part, T* __restrict__ dw,
-                                                                        int tiles, int V, int D, float scale) {
+                                                                        const int32_t* __restrict__ n_cross,
+                                                                        const int32_t* __restrict__ cross, int tiles, int D,
+                                                                        float scale) {
   __shared__ float s_sum[kEmbWarps][kTile];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t piece = blockIdx.x / (unsigned)tiles, begin = piece * kPiece, end = begin + kPiece;
-  const int base = (int)(blockIdx.x - piece * tiles) * kTile;
-  if (end >= tokens) return;                       // nothing behind the last piece
-  const int k = keys[end - 1];
-  if (k >= V || keys[end] != k) return;            // no run goes on behind this one
-  if (begin > 0 && keys[begin] == k && keys[begin - 1] == k) return;   // it began before
-  // pieces behind this one that the run goes through or ends in: those that start with k
-  const int64_t pieces = (tokens + kPiece - 1) / kPiece;
-  int64_t n = 0;
-  for (;;) {
-    const int64_t q = piece + 1 + n + lane;
-    const uint32_t in = __ballot_sync(0xffffffffu, q < pieces && keys[q * kPiece] == k);
-    const int got = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-    n += got;
-    if (got < 32) break;
+  const int64_t units = (int64_t)*n_cross * tiles;
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t piece = cross[unit / tiles];
+    const int base = (int)(unit % tiles) * kTile;
+    const int k = keys[(piece + 1) * kPiece - 1];
+    // pieces behind this one that the run goes through or ends in: those that start with k
+    const int64_t pieces = (tokens + kPiece - 1) / kPiece;
+    int64_t n = 0;
+    for (;;) {
+      const int64_t q = piece + 1 + n + lane;
+      const uint32_t in = __ballot_sync(0xffffffffu, q < pieces && keys[q * kPiece] == k);
+      const int got = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+      n += got;
+      if (got < 32) break;
+    }
+    float sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+    for (int64_t j = warp; j <= n; j += kEmbWarps) {
+      RawTile<float, VEC> t;
+      t.load(part + ((piece + j) * 2 + (j == 0 ? 1 : 0)) * D, base, lane, D);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += __uint_as_float(t.w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_sum[warp][i * 32 + lane] = sum[i];
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 1; w < kEmbWarps; ++w)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += s_sum[w][i * 32 + lane];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] *= scale;
+      store_tile<T, VEC>(dw + (int64_t)k * D, base, lane, D, sum);
+    }
+    __syncthreads();   // (before the next one's sums)
   }
-  float sum[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
-  for (int64_t j = warp; j <= n; j += kEmbWarps) {
-    RawTile<float, VEC> t;
-    t.load(part + ((piece + j) * 2 + (j == 0 ? 1 : 0)) * D, base, lane, D);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += __uint_as_float(t.w[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s_sum[warp][i * 32 + lane] = sum[i];
-  __syncthreads();
-  if (warp > 0) return;
-#pragma unroll
-  for (int w = 1; w < kEmbWarps; ++w)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += s_sum[w][i * 32 + lane];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum[i] *= scale;
-  store_tile<T, VEC>(dw + (int64_t)k * D, base, lane, D, sum);
 }
 
 }  // namespace zq
@@ -487,17 +538,26 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor dw, double scale) {
   const int64_t T_ = ids.numel();
   const int V = (int)dw.size(0), D = (int)dw.size(1), tiles = (D + kTile - 1) / kTile;
   const int ids64 = ids.scalar_type() == at::kLong;
-  const int64_t bytes = dw.numel() * dw.element_size();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   int passes = 1;   // digits of 0 .. V
   while (passes < 4 && ((uint64_t)V >> (passes * kRadixBits)) != 0) ++passes;
   const int64_t pieces = (T_ + kPiece - 1) / kPiece;
   TORCH_CHECK(pieces * tiles < (1LL << 31), "embedding: too many tokens");
-  // zeros: blocks of 1024 threads, two to an SM
-  const int zero_blocks = (int)std::min<int64_t>(2 * sms, (bytes + 16383) / 16384);
   const auto i32 = ids.options().dtype(at::kInt);
-  at::Tensor sorted;
-  int32_t *keys, *order;
+  at::Tensor sorted, crossing = at::empty({1 + pieces}, i32);
+  int32_t *keys, *order, *n_cross = crossing.data_ptr<int32_t>(), *cross = n_cross + 1;
+  // the table's first rows, zeroed meanwhile: `bytes` a launch
+  const int64_t row_bytes = (int64_t)D * dw.element_size();
+  int64_t zeroed = 0;   // rows
+  auto share = [&](int64_t bytes) {
+    const int64_t rows = std::min<int64_t>(V - zeroed, bytes / row_bytes);
+    const ZeroShare z{reinterpret_cast<uint8_t*>(dw.data_ptr()) + zeroed * row_bytes, rows * row_bytes};
+    zeroed += rows;
+    return z;
+  };
+  auto share_blocks = [&](const ZeroShare& z) {
+    return (unsigned)std::min<int64_t>(2 * sms, (z.bytes + 32 * kZeroChunk - 1) / (32 * kZeroChunk));
+  };
   if (T_ <= kSortTile) {
     sorted = at::empty({2 * T_}, i32);
     keys = sorted.data_ptr<int32_t>();
@@ -509,8 +569,10 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor dw, double scale) {
       C10_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       configured[dev] = true;
     }
-    embedding_sort_block_kernel<<<1 + zero_blocks, kSortWarps * 32, smem, stream>>>(ids.data_ptr(), ids64, (int)T_, V, passes,
-                                                                                    keys, order, dw.data_ptr(), bytes);
+    // (8192 tokens in two passes take 19 us)
+    const ZeroShare z = share((int64_t)passes * 3500 * (T_ + 4096));
+    embedding_sort_block_kernel<<<1 + share_blocks(z), kSortWarps * 32, smem, stream>>>(ids.data_ptr(), ids64, (int)T_, V, passes,
+                                                                                        keys, order, n_cross, z);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   } else {
     const int64_t n = (T_ + kSortTile - 1) / kSortTile;
@@ -518,21 +580,21 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor dw, double scale) {
     int32_t* buf[2] = {sorted.data_ptr<int32_t>(), sorted.data_ptr<int32_t>() + 2 * T_};
     uint32_t* counts = reinterpret_cast<uint32_t*>(buf[1] + 2 * T_);
     constexpr int smem = kSortWarps * kRadix * 2;
-    for (int pass = 0; pass < passes; ++pass) {
+    for (int pass = 0; pass < passes; ++pass) {   // (6 and 4 us to count, 17 and 13 to place)
+      const ZeroShare z0 = share(24 << 20), z1 = share(72 << 20);
+      const unsigned b0 = (unsigned)n + share_blocks(z0), b1 = (unsigned)n + share_blocks(z1);
       int32_t *in = buf[pass & 1], *out = buf[(pass + 1) & 1];
       const int shift = pass * kRadixBits;
       if (pass == 0) {
-        embedding_count_kernel<true><<<(unsigned)n + zero_blocks, kSortWarps * 32, 0, stream>>>(
-            ids.data_ptr(), ids64, T_, V, shift, (int)n, counts, dw.data_ptr(), bytes);
+        embedding_count_kernel<true><<<b0, kSortWarps * 32, 0, stream>>>(ids.data_ptr(), ids64, T_, V, shift, counts, n_cross, (int)n, z0);
         C10_CUDA_KERNEL_LAUNCH_CHECK();
-        embedding_place_kernel<true><<<(unsigned)n, kSortWarps * 32, smem, stream>>>(ids.data_ptr(), ids64, nullptr, T_, V,
-                                                                                     shift, (int)n, counts, out, out + T_);
+        embedding_place_kernel<true><<<b1, kSortWarps * 32, smem, stream>>>(ids.data_ptr(), ids64, nullptr, T_, V, shift, (int)n,
+                                                                             counts, out, out + T_, z1);
       } else {
-        embedding_count_kernel<false><<<(unsigned)n, kSortWarps * 32, 0, stream>>>(in, 0, T_, V, shift, (int)n, counts,
-                                                                                   nullptr, 0);
+        embedding_count_kernel<false><<<b0, kSortWarps * 32, 0, stream>>>(in, 0, T_, V, shift, counts, nullptr, (int)n, z0);
         C10_CUDA_KERNEL_LAUNCH_CHECK();
-        embedding_place_kernel<false><<<(unsigned)n, kSortWarps * 32, smem, stream>>>(in, 0, in + T_, T_, V, shift, (int)n,
-                                                                                      counts, out, out + T_);
+        embedding_place_kernel<false><<<b1, kSortWarps * 32, smem, stream>>>(in, 0, in + T_, T_, V, shift, (int)n, counts, out,
+                                                                              out + T_, z1);
       }
       C10_CUDA_KERNEL_LAUNCH_CHECK();
     }
@@ -541,14 +603,18 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor dw, double scale) {
   }
   at::Tensor part = at::empty({pieces * 2 * D}, ids.options().dtype(at::kFloat));
   float* pp = part.data_ptr<float>();
-  const unsigned sums = (unsigned)((pieces * tiles + kEmbWarps - 1) / kEmbWarps);
+  const int64_t sums = (pieces * tiles + kEmbWarps - 1) / kEmbWarps, zeros = (V - zeroed + 32 * kEmbWarps - 1) / (32 * kEmbWarps);
   ZQ_EMB_TYPES(dw.scalar_type(), {
     const T* dyp = reinterpret_cast<const T*>(dy.data_ptr());
     T* dwp = reinterpret_cast<T*>(dw.data_ptr());
     auto go = [&](auto sum, auto join) {
-      sum<<<sums, kEmbWarps * 32, 0, stream>>>(keys, order, T_, dyp, dy.stride(0), dwp, pp, tiles, V, D, (float)scale);
+      sum<<<(unsigned)(sums + zeros), kEmbWarps * 32, 0, stream>>>(keys, order, T_, dyp, dy.stride(0), dwp, pp, n_cross, cross,
+                                                                   (int)sums, zeroed, tiles, V, D, (float)scale);
       C10_CUDA_KERNEL_LAUNCH_CHECK();
-      if (pieces > 1) join<<<(unsigned)(pieces * tiles), kEmbWarps * 32, 0, stream>>>(keys, T_, pp, dwp, tiles, V, D, (float)scale);
+      if (pieces > 1) {
+        const unsigned grid = (unsigned)std::min<int64_t>(pieces * tiles, 4 * sms);
+        join<<<grid, kEmbWarps * 32, 0, stream>>>(keys, T_, pp, dwp, n_cross, cross, tiles, D, (float)scale);
+      }
     };
     if (D % 8 == 0 && emb_aligned(dy)) go(embedding_sum_kernel<T, true>, embedding_join_kernel<T, true>);
     else go(embedding_sum_kernel<T, false>, embedding_join_kernel<T, false>);
