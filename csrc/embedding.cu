@@ -612,7 +612,7 @@ void embedding_bwd(at::Tensor ids, at::Tensor dy, at::Tensor dw, double scale) {
                                                                    (int)sums, zeroed, tiles, V, D, (float)scale);
       C10_CUDA_KERNEL_LAUNCH_CHECK();
       if (pieces > 1) {
-        const unsigned grid = (unsigned)std::min<int64_t>(pieces * tiles, 4 * sms);
+        const unsigned grid = (unsigned)std::min<int64_t>(pieces * tiles, 16 * sms);
         join<<<grid, kEmbWarps * 32, 0, stream>>>(keys, T_, pp, dwp, n_cross, cross, tiles, D, (float)scale);
       }
     };

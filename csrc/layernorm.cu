@@ -118,32 +118,35 @@ __device__ __forceinline__ float ln_sum16(float v) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// Rows on their way: every thread copies its own columns of NS tensors of T (and, CODES, of the
-// 8-bit input) into its own places of shared memory, S rows ahead, and reads them back itself,
-// so no barrier belongs to it and nothing waits in registers.
-template <typename T, int K, int NS, bool CODES>
+// Rows on their way: every warp copies its own columns of NS tensors of T (and, CODES, of the 8-bit
+// input, STATS, the row's mean and deviation) into its own places of shared memory, S groups of
+// rows ahead, and reads them back itself, so no barrier belongs to it and nothing waits in
+// registers.  A lane copies its own vectors; codes go 16 bytes a lane, the few single numbers by a
+// few lanes (copies of 4 and 8 bytes by all of them took as long as the vectors).
+template <typename T, int K, int NS, bool CODES, bool STATS>
 struct LnSlots {
   static constexpr int kVecs = (int)sizeof(T) / 2;   // 16-byte vectors of a lane's 8 elements
-  static constexpr int kBytes = K * (16 * kVecs * NS + (CODES ? 12 : 0));   // of a thread
+  static constexpr int kBytes = K * (16 * kVecs * NS + (CODES ? 8 : 0)) + (CODES || STATS ? 4 : 0);   // of a thread
   uint32_t mine;       // shared address of this thread's vectors in the first slot
   uint32_t slot_bytes; // from slot to slot
   uint32_t there;      // bit k: tile k has columns here
-  int col;             // this thread's first column
+  int first;           // the warp's first column
 
-  // A warp's places in a slot: [tensor][tile][vector][lane] of 16 bytes, codes (8), steps (4).
-  static constexpr int kEight = 512 * K * kVecs * NS, kFour = kEight + 256 * K;
+  // A warp's places in a slot: [tensor][tile][vector][lane] of 16 bytes; codes [tile][256]; numbers:
+  // steps [tile][2], mean, deviation.
+  static constexpr int kCodes = 512 * K * kVecs * NS, kNumbers = kCodes + (CODES ? 256 * K : 0), kStats = CODES ? 2 * K : 0;
   static __device__ __forceinline__ uint32_t vec(int i) { return 512u * i; }
-  __device__ __forceinline__ uint32_t eight(int k) const { return kEight + 256u * k - 8u * (threadIdx.x & 31); }
-  __device__ __forceinline__ uint32_t four(int k) const { return kFour + 128u * k - 12u * (threadIdx.x & 31); }
+  static __device__ __forceinline__ int lane() { return threadIdx.x & 31; }
+  __device__ __forceinline__ uint32_t number(int i) const { return kNumbers + 4u * i - 16u * lane(); }
 
-  __device__ __forceinline__ void init(uint8_t* smem, const LnParams& p, int first, int n) {
-    col = first;
+  __device__ __forceinline__ void init(uint8_t* smem, const LnParams& p, int first_, int n) {
+    first = first_;
     there = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) there |= (col + k * p.W * kTile < p.D ? 1u : 0u) << k;
-    mine = smem_u32(smem) + (threadIdx.x >> 5) * (32u * kBytes) + 16u * (threadIdx.x & 31);
+    for (int k = 0; k < K; ++k) there |= (first + lane() * 8 + k * p.W * kTile < p.D ? 1u : 0u) << k;
+    mine = smem_u32(smem) + (threadIdx.x >> 5) * (32u * kBytes) + 16u * lane();
     slot_bytes = (uint32_t)kBytes * blockDim.x;
-    if (there + 1 != 1u << K) {   // places that are never filled hold zeros
+    if (first + ((K - 1) * p.W + 1) * kTile > p.D) {   // places that are never filled hold zeros
       for (int s = 0; s < n; ++s) {
         const uint32_t at = mine + s * slot_bytes;
 #pragma unroll
@@ -151,25 +154,26 @@ struct LnSlots {
           asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + vec(i)), "r"(0) : "memory");
         if constexpr (CODES) {
 #pragma unroll
-          for (int k = 0; k < K; ++k) {
-            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + eight(k)), "r"(0) : "memory");
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + four(k)), "r"(0) : "memory");
-          }
+          for (int k = 0; k < K; ++k)
+            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + kCodes + 256u * k - 8u * lane()), "r"(0) : "memory");
+          if (lane() < 2 * K) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + number(lane())), "r"(0) : "memory");
         }
       }
+      __syncwarp();
     }
   }
   // fetches rows [row, row + B) of M into slots [group B, group B + B), as one group of copies
   template <int B>
-  __device__ __forceinline__ void fetch(const LnParams& p, int group, int64_t first) const {
+  __device__ __forceinline__ void fetch(const LnParams& p, int group, int64_t first_row) const {
+    if constexpr (CODES || STATS) __syncwarp();   // (the slots are read)
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       const uint32_t at = mine + (group * B + b) * slot_bytes;
-      const int64_t row = first + b;
+      const int64_t row = first_row + b;
       if (row >= p.M) continue;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const T* from = reinterpret_cast<const T*>(p.src[i]) + row * p.pitch[i] + col;
+        const T* from = reinterpret_cast<const T*>(p.src[i]) + row * p.pitch[i] + first + lane() * 8;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -180,25 +184,36 @@ struct LnSlots {
                            : "memory");
       }
       if constexpr (CODES) {
-        const int8_t* codes = p.codes + row * p.P + col;
-        const float* steps = p.steps + row * p.G + col / kGroup;
+        const int8_t* codes = p.codes + row * p.P + first + lane() * 16;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (there >> k & 1u) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at + eight(k)), "l"(codes + k * p.W * kTile) : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + four(k)), "l"(steps + k * p.W * (kTile / kGroup))
+        for (int k = 0; k < K; ++k)
+          if (lane() < 16 && first + k * p.W * kTile + lane() * 16 < p.D)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + kCodes + 256u * k), "l"(codes + k * p.W * kTile)
                          : "memory");
-          }
-        }
+      }
+      if constexpr (CODES || STATS) {
+        const int group_at = (first + (lane() >> 1) * p.W * kTile) / kGroup + (lane() & 1);   // of the lane's step
+        const float* from = nullptr;
+        if (CODES && lane() < 2 * K && group_at < p.G) from = p.steps + row * p.G + group_at;
+        if (STATS && lane() == kStats) from = p.mean + row;
+        if (STATS && lane() == kStats + 1) from = p.rstd + row;
+        if (from != nullptr)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at + number(lane())), "l"(from) : "memory");
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void get_stats(int slot, float& mu, float& r) const {
+    const uint32_t at = mine + slot * slot_bytes;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(mu) : "r"(at + number(kStats)) : "memory");
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at + number(kStats + 1)) : "memory");
   }
   // until all but the last S - 1 fetches are there
   static __device__ __forceinline__ void wait(int S) {
     if (S == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else if (S == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    if constexpr (CODES || STATS) __syncwarp();   // other lanes' copies
   }
   __device__ __forceinline__ void get(int slot, int i, int k, RawTile<T, true>& t) const {
 #pragma unroll
@@ -210,8 +225,8 @@ struct LnSlots {
   }
   __device__ __forceinline__ void get(int slot, int k, RawCodes<true>& c) const {
     const uint32_t at = mine + slot * slot_bytes;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(c.w.x), "=r"(c.w.y) : "r"(at + eight(k)) : "memory");
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c.step[0]) : "r"(at + four(k)) : "memory");
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(c.w.x), "=r"(c.w.y) : "r"(at + kCodes + 256u * k - 8u * lane()) : "memory");
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c.step[0]) : "r"(at + number(2 * k + (lane() >> 4))) : "memory");
   }
 };
 
@@ -226,9 +241,9 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   const int whole = (D + kTile - 1) / kTile * kTile;
   const int64_t step = (int64_t)gridDim.x * p.R;
   int64_t row = (int64_t)blockIdx.x * p.R + team;
-  LnSlots<T, K, RES ? 2 : 1, false> rows;
+  LnSlots<T, K, RES ? 2 : 1, false, false> rows;
   if constexpr (PIPE) {
-    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile + lane * 8, S);
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile, S);
     for (int i = 0; i < S; ++i) rows.template fetch<1>(p, i, row + i * step);
   }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
@@ -348,9 +363,9 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
   const int64_t step = (int64_t)gridDim.x * p.R * B;
   int64_t row = ((int64_t)blockIdx.x * p.R + team) * B;
   constexpr int kH = 1, kX = RES ? 2 : 1;   // tensors behind dy
-  LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT> rows;
+  LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT, true> rows;
   if constexpr (PIPE) {
-    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile + lane * 8, S * B);
+    rows.init(reinterpret_cast<uint8_t*>(s_wb) + p.slots_at, p, wt * kTile, S * B);
     for (int i = 0; i < S; ++i) rows.template fetch<B>(p, i, row + i * step);
   }
   ln_stage<VEC>(s_wb, p.w, p.wt, 1.0f, D);
@@ -366,8 +381,14 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
     const bool second = row + 1 < p.M;
     float mu[B], r[B];
-    mu[0] = p.mean[row], r[0] = p.rstd[row];
-    mu[1] = second ? p.mean[row + 1] : 0.0f, r[1] = second ? p.rstd[row + 1] : 0.0f;
+    if constexpr (PIPE) {   // (of a second row that is not there: not used)
+      rows.wait(S);
+      rows.get_stats(at * B, mu[0], r[0]);
+      rows.get_stats(at * B + 1, mu[1], r[1]);
+    } else {
+      mu[0] = p.mean[row], r[0] = p.rstd[row];
+      mu[1] = second ? p.mean[row + 1] : 0.0f, r[1] = second ? p.rstd[row + 1] : 0.0f;
+    }
     auto gradient = [&](const void* from, int64_t pitch, int stream, int b, int k, uint64_t (&g)[4]) {
       RawTile<T, VEC> t;
       if constexpr (PIPE) rows.get(at * B + b, stream, k, t);
@@ -391,7 +412,6 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
         for (int i = 0; i < 4; ++i) n[i] = f2_fma(n[i], f2_pack(r[b], r[b]), f2_pack(off, off));
       }
     };
-    if constexpr (PIPE) rows.wait(S);
     float s[2 * B];   // sums of a and a n of each row
     {
       uint64_t t[2 * B];
@@ -682,7 +702,7 @@ static void ln_fwd_launch(LnParams& p, cudaStream_t stream) {
     if constexpr (VEC) {
       p.src[0] = p.x, p.pitch[0] = p.xs;
       p.src[1] = p.delta, p.pitch[1] = p.ds;
-      const size_t smem = ln_block(p, front, LnSlots<T, K, RES ? 2 : 1, false>::kBytes, 8, 1, 3);
+      const size_t smem = ln_block(p, front, LnSlots<T, K, RES ? 2 : 1, false, false>::kBytes, 8, 1, 3);
       if (smem > 0) return go(ln_fwd_kernel<T, VEC, K, RES, KEEP, true>, smem);
     }
     if constexpr (!VEC || K == 4) {
@@ -767,7 +787,7 @@ static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::T
       p.src[0] = p.dy, p.pitch[0] = p.dys;
       p.src[1] = RES ? p.dh : p.x, p.pitch[1] = RES ? p.dhs : p.xs;
       p.src[2] = p.x, p.pitch[2] = p.xs;
-      constexpr int kBytes = LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT>::kBytes;
+      constexpr int kBytes = LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT, true>::kBytes;
       constexpr int kWarps = K <= 2 ? kLnBlockWarps : kLnMaxWarps;
       const size_t smem = ln_block(p, front, kBytes, kWarps, kLnRows, 1);
       if (smem > 0) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, kWarps>, smem);

@@ -147,9 +147,7 @@ __device__ __forceinline__ uint32_t code_of(float v, float inv) {
 }
 
 // Writes the codes and steps of K tiles of one warp: tile k holds columns [base[k], base[k] + 256)
-// of row `codes[k]`, `steps[k]`; tiles with base[k] >= D are none.  A group's scale is formed
-// by one lane of it (a division and its checks cost as much as the codes of eight elements)
-// and handed to the others.
+// of row `codes[k]`, `steps[k]`; tiles with base[k] >= D are none.
 template <bool VEC, int K>
 __device__ __forceinline__ void keep_tiles(const uint64_t (&v)[K][4], int8_t* const (&codes)[K], float* const (&steps)[K],
                                            const int (&base)[K], int lane, int D) {
@@ -166,19 +164,11 @@ __device__ __forceinline__ void keep_tiles(const uint64_t (&v)[K][4], int8_t* co
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) a[k] = max_nan(a[k], __shfl_xor_sync(0xffffffffu, a[k], o));
     }
-    static_assert(K <= 16, "a lane of a group for each tile");
-    float mine = a[0];
-    int at = base[0];
-    float* to = steps[0];
-#pragma unroll
-    for (int k = 1; k < K; ++k)
-      if ((lane & 15) == k) mine = a[k], at = base[k], to = steps[k];
-    const GroupScale g = group_scale(mine);
-    at += (lane & 16) * 8;   // this half's group
-    if ((lane & 15) < K && at < D) to[at / kGroup] = g.step;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float inv = __shfl_sync(0xffffffffu, g.inv, (lane & 16) | k);
+      const GroupScale g = group_scale(a[k]);
+      if ((lane & 15) == 0 && base[k] + lane * 8 < D) steps[k][(base[k] + lane * 8) / kGroup] = g.step;
+      const float inv = g.inv;
       const uint64_t inv2 = f2_pack(inv, inv);
       uint32_t c[8];
 #pragma unroll
