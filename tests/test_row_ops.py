@@ -516,7 +516,8 @@ def test_token_logprobs(device, M, V, W, k, tau, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,V,W,k", [(500, 2000, 2048, 3), (3, 50257, 50304, 128), (310, 33000, 33000, 9), (1, 65536, 65536, 256),
-                                     (2, 65537, 65540, 256), (3, 152064, 152064, 32), (1, 152063, 152063, 0), (20, 40000, 40000, 0)])
+                                     (2, 65537, 65540, 256), (700, 1000, 1000, 20),
+                                     (700, 301, 304, 0), (1300, 5000, 5056, 8), (3, 152064, 152064, 32), (1, 152063, 152063, 0), (20, 40000, 40000, 0)])
 def test_token_logprobs_sizes(cuda, M, V, W, k, dtype):
     logprob_case("cuda", logits(M, W, dtype, "cuda"), V, k)
 
