@@ -10,7 +10,9 @@
 //   swiglu: y = g sigma(g) u;        du = dy gq s,  dg = dy uq s (1 + gq (1 - s)),  s = sigma(gq)
 //
 // What bounds them: memory.  A warp takes 256 columns at a time (rows.cuh) and loads several
-// such tiles before it works on the first.
+// such tiles before it works on the first.  Measured: 16384 x 5120 bf16 50 us to keep, 45 us to
+// read back (0.77 and 0.85 of a copy's rate); SwiGLU of 8192 x 18944 213 us forward, 208 backward
+// (0.89 and 0.91).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -14,7 +14,10 @@
 // both and nothing cancels.  dw and db: a block's teams add up in team order in shared memory,
 // the blocks' rows of partial sums are added in block order by a second kernel: no atomics.
 //
-// What bounds it: memory.
+// What bounds it: memory in the plain forward (8192 x 3584 with residual 38 us, 0.95 of a copy's
+// rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 100 us,
+// 0.64) and in the backward (55 us, 0.66, and 128 us from codes, 0.50), at about half of the issue
+// slots and no pipe above 0.4.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -18,9 +18,12 @@
 // chunk of columns: the k best of the row lie in the k chunks with the best maxima, so the k-th
 // best of those is a bound, and a second launch looks at the chunks that reach it alone.
 // Backward: one pass, p from the row's m, S and H; the columns with a g term are written a
-// second time by their block (each sum rounded once; no atomics).
+// second time by their warp (each sum rounded once; no atomics).
 //
-// What bounds it: memory, next to 16 exponentials a cycle and SM.
+// What bounds it: memory, next to 16 exponentials a cycle and SM.  8192 x 152064 bf16: forward
+// 372 us (a copy's rate), 403 and 81 for the ranking with 32 alternatives; gradient 785 us (0.97).
+// 4096 x 50257 with an eighth of the rows not counted: 78 and 137 us (0.71, 0.86): a row's start and
+// end weigh more, and 3584 rows are three and a bit rounds of blocks.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
