@@ -1,0 +1,68 @@
+"""What an 8-bit checkpoint keeps in 8 bits and what it keeps as it is: gradients against those of
+the same function at the kept activations and the exact rest, to the bit."""
+
+import pytest
+import torch
+
+from zeroq_b200.ops import checkpoint_8bit, dequantize_activation, quantize_activation
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.fixture(params=DEVICES)
+def device(request):
+    if request.param == "cuda":
+        request.getfixturevalue("cuda")
+    return request.param
+
+
+def attention(h, mask, bias=None):
+    s = h @ h.transpose(-1, -2) / 8 + mask
+    return torch.softmax(s if bias is None else s + bias, -1) @ h
+
+
+def inputs(device, low, S=24):
+    torch.manual_seed(1)
+    h = torch.randn(2, S, 64).to(device).requires_grad_()
+    mask = torch.full((S, S), low).triu(1).to(device)
+    return h, mask, torch.randn(2, S, 64).to(device)
+
+
+def at_kept(h):
+    return dequantize_activation(quantize_activation(h)).requires_grad_()
+
+
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e9])
+def test_a_mask_is_kept_as_it_is(device, low):
+    """a mask in one tensor with a position bias of ordinary size, which 8 bits would lose"""
+    h, mask, dy = inputs(device, low)
+    bias = torch.randn(24, 24).to(device)
+    (got,) = torch.autograd.grad(checkpoint_8bit(attention, h, mask + bias), h, dy)
+    k = at_kept(h)
+    (want,) = torch.autograd.grad(attention(k, mask + bias), k, dy)
+    assert torch.isfinite(got).all() and torch.equal(got, want)
+    (exact,) = torch.autograd.grad(attention(h, mask + bias), h, dy)
+    assert not torch.equal(got, exact)   # (h itself is kept in 8 bits)
+
+
+def test_a_bias_with_a_gradient_is_kept_as_it_is(device):
+    """learned position biases with the mask added in: not of the hidden states' shape"""
+    h, mask, dy = inputs(device, float("-inf"))
+    table = torch.randn(24, 24).to(device).requires_grad_()
+    bias = table[None] + mask
+    got = torch.autograd.grad(checkpoint_8bit(attention, h, torch.zeros_like(mask), bias), (h, table), dy, retain_graph=True)
+    k = at_kept(h)
+    want = torch.autograd.grad(attention(k, torch.zeros_like(mask), table[None] + mask), (k, table), dy)
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_every_input_of_the_first_activations_shape_is_kept_in_8_bits(device):
+    """a residual stream and its addend"""
+    h, _, dy = inputs(device, 0.0)
+    delta = torch.randn(2, 24, 64).to(device).requires_grad_()
+    cos = torch.randn(24, 64).to(device)
+    fn = lambda h, cos, d: torch.tanh(h * cos + d)  # noqa: E731
+    got = torch.autograd.grad(checkpoint_8bit(fn, h, cos, delta), (h, delta), dy)
+    a, b = at_kept(h), at_kept(delta)
+    want = torch.autograd.grad(fn(a, cos, b), (a, b), dy)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

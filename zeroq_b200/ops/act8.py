@@ -112,10 +112,12 @@ def checkpoint_8bit(fn, *args, **kwargs):
 
     Like ``torch.utils.checkpoint.checkpoint`` (without reentrance; ``kwargs`` are ``fn``'s,
     ``preserve_rng_state`` is this function's): nothing that ``fn`` saves is held until the
-    backward, only its inputs.  Those that are activations (bf16, fp16 or fp32 tensors of at
-    least one dimension that are not parameters) are held in 8 bits, the others as they
-    are.  The outputs are those of the exact inputs; the gradients are those of ``fn`` at the
-    kept ones."""
+    backward, only its inputs.  Held in 8 bits are the activations: of the bf16, fp16 and fp32
+    tensors that take a gradient and are no parameters the first (the hidden states) and those of
+    its shape.  Everything else is held as it is - attention masks, whose lowest values would take a
+    group's step or make it NaN, position tables and biases, another sequence's states - and
+    costs nothing where layers share it.  The outputs are those of the exact inputs; the
+    gradients are those of ``fn`` at the kept ones."""
     from torch.utils.checkpoint import checkpoint
 
     preserve = kwargs.pop("preserve_rng_state", True)
@@ -124,17 +126,18 @@ def checkpoint_8bit(fn, *args, **kwargs):
 
     def activation(t):
         return (isinstance(t, torch.Tensor) and not isinstance(t, torch.nn.Parameter) and t.dtype in _FLOATS
-                and t.dim() >= 1)
+                and t.dim() >= 1 and t.requires_grad)
 
+    shape = next((t.shape for t in args if activation(t)), None)
+    in8 = [activation(t) and t.shape == shape for t in args]
     exact = list(args)      # for the call now; given up behind it
-    kept = [(quantize_activation(t), t.requires_grad) if activation(t) else t for t in args]
-    masks = [activation(t) for t in args]
+    kept = [quantize_activation(t) if m else t for t, m in zip(args, in8)]
     del args
 
     def run():
         if exact:
             return fn(*exact, **kwargs)
-        again = [dequantize_activation(k[0]).requires_grad_(k[1]) if m else k for k, m in zip(kept, masks)]
+        again = [dequantize_activation(k).requires_grad_() if m else k for k, m in zip(kept, in8)]
         return fn(*again, **kwargs)
 
     if not exact:
