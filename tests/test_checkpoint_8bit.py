@@ -66,3 +66,43 @@ def test_every_input_of_the_first_activations_shape_is_kept_in_8_bits(device):
     a, b = at_kept(h), at_kept(delta)
     want = torch.autograd.grad(fn(a, cos, b), (a, b), dy)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("args,names", [((), ("h", "d")), (("h",), ("d",))])
+def test_inputs_by_name_are_kept_like_the_others(device, args, names):
+    """called by name alone, too: recomputed, from 8 bits, and nothing exact is held"""
+    import gc
+    import weakref
+
+    leaf = torch.randn(6, 200, device=device, requires_grad=True)
+    calls = []
+
+    def fn(h, d, scale=2.0):
+        calls.append(1)
+        return torch.sin(h) * torch.exp(d) * scale
+
+    def inputs():
+        return {"h": leaf * 1.0, "d": leaf * 0.5}
+
+    now = inputs()
+    held = [weakref.ref(t) for t in now.values()]
+    y = checkpoint_8bit(fn, *(now[n] for n in args), **{n: now[n] for n in names}, scale=3.0)
+    want = fn(**inputs(), scale=3.0)
+    assert torch.equal(y, want)
+    del now
+    gc.collect()
+    assert all(r() is None for r in held)
+    calls.clear()
+    (got,) = torch.autograd.grad(y.sum(), leaf)
+    assert len(calls) == 1
+    again = {n: at_kept(t.detach().requires_grad_()) for n, t in inputs().items()}
+    a, b = torch.autograd.grad(fn(**again, scale=3.0).sum(), list(again.values()))
+    assert torch.allclose(got, a + 0.5 * b, rtol=1e-6, atol=1e-6)
+
+
+def test_a_mask_by_name_is_kept_as_it_is(device):
+    h, mask, dy = inputs(device, float("-inf"))
+    (got,) = torch.autograd.grad(checkpoint_8bit(attention, mask=mask, h=h), h, dy)
+    k = at_kept(h)
+    (want,) = torch.autograd.grad(attention(k, mask), k, dy)
+    assert torch.equal(got, want)

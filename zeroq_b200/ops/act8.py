@@ -108,11 +108,11 @@ def dequantize_activation(kept: Activation8) -> torch.Tensor:
 
 
 def checkpoint_8bit(fn, *args, **kwargs):
-    """``fn(*args)`` now, and again in the backward from its inputs kept in 8 bits.
+    """``fn(*args, **kwargs)`` now, and again in the backward from its inputs kept in 8 bits.
 
-    Like ``torch.utils.checkpoint.checkpoint`` (without reentrance; ``kwargs`` are ``fn``'s,
-    ``preserve_rng_state`` is this function's): nothing that ``fn`` saves is held until the
-    backward, only its inputs.  Held in 8 bits are the activations: of the bf16, fp16 and fp32
+    Like ``torch.utils.checkpoint.checkpoint`` (without reentrance; ``preserve_rng_state`` is
+    this function's): nothing that ``fn`` saves is held until the backward, only its inputs,
+    given by place or by name.  Held in 8 bits are the activations: of the bf16, fp16 and fp32
     tensors that take a gradient and are no parameters the first (the hidden states) and those of
     its shape.  Everything else is held as it is - attention masks, whose lowest values would take a
     group's step or make it NaN, position tables and biases, another sequence's states - and
@@ -128,20 +128,21 @@ def checkpoint_8bit(fn, *args, **kwargs):
         return (isinstance(t, torch.Tensor) and not isinstance(t, torch.nn.Parameter) and t.dtype in _FLOATS
                 and t.dim() >= 1 and t.requires_grad)
 
-    shape = next((t.shape for t in args if activation(t)), None)
-    in8 = [activation(t) and t.shape == shape for t in args]
-    exact = list(args)      # for the call now; given up behind it
-    kept = [quantize_activation(t) if m else t for t, m in zip(args, in8)]
-    del args
+    n, names = len(args), list(kwargs)
+    inputs = [*args, *kwargs.values()]
+    shape = next((t.shape for t in inputs if activation(t)), None)
+    in8 = [activation(t) and t.shape == shape for t in inputs]
+    kept = [quantize_activation(t) if m else t for t, m in zip(inputs, in8)]
+    exact = [inputs]        # for the call now; given up behind it
+    del args, kwargs, inputs
 
     def run():
         if exact:
-            return fn(*exact, **kwargs)
-        again = [dequantize_activation(k).requires_grad_() if m else k for k, m in zip(kept, in8)]
-        return fn(*again, **kwargs)
+            v = exact[0]
+        else:
+            v = [dequantize_activation(k).requires_grad_() if m else k for k, m in zip(kept, in8)]
+        return fn(*v[:n], **dict(zip(names, v[n:])))
 
-    if not exact:
-        return fn(**kwargs)
     out = checkpoint(run, use_reentrant=False, preserve_rng_state=preserve)
     exact.clear()
     return out
