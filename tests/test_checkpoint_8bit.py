@@ -106,3 +106,65 @@ def test_a_mask_by_name_is_kept_as_it_is(device):
     k = at_kept(h)
     (want,) = torch.autograd.grad(attention(k, mask), k, dy)
     assert torch.equal(got, want)
+
+
+class Block(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.lin = torch.nn.Linear(200, 200)
+        self.calls = 0
+
+    def forward(self, h, mask=None):
+        self.calls += 1
+        return torch.tanh(self.lin(h)) * (1.0 if mask is None else torch.exp(mask))
+
+
+class Stack(torch.nn.Module):
+    def __init__(self, by_name=False):
+        super().__init__()
+        self.layers = torch.nn.ModuleList([Block(), Block()])
+        self.by_name = by_name
+
+    def forward(self, h, mask=None):
+        for layer in self.layers:
+            h = layer(h=h, mask=mask) if self.by_name else layer(h, mask)
+        return h
+
+
+def stack_gradients(m, x, mask, read):
+    """by hand, every layer recomputed from `read` of its input"""
+    a = [x]
+    with torch.no_grad():
+        for layer in m.layers:
+            a.append(layer.lin(a[-1]).tanh() * torch.exp(mask))
+    g, out = torch.ones_like(x), {}
+    for i in (1, 0):
+        k = read(a[i]).requires_grad_()
+        lin = m.layers[i].lin
+        g, out[f"layers.{i}.lin.weight"], out[f"layers.{i}.lin.bias"] = torch.autograd.grad(
+            torch.tanh(lin(k)) * torch.exp(mask), [k, lin.weight, lin.bias], g)
+    return out
+
+
+@pytest.mark.parametrize("by_name", [False, True])
+@pytest.mark.parametrize("before", [None, "full", "8bit"])
+@pytest.mark.parametrize("saved", ["full", "8bit"])
+def test_enabled_checkpoints_are_what_was_asked_for_last(device, saved, before, by_name):
+    from zeroq_b200.utils.checkpoint import enable_gradient_checkpointing
+
+    torch.manual_seed(0)
+    m = Stack(by_name).to(device)
+    x = torch.randn(6, 200, device=device)
+    mask = torch.zeros(200, device=device)
+    mask[3] = float("-inf")
+    if before:
+        enable_gradient_checkpointing(m, saved=before)
+    enable_gradient_checkpointing(m, saved=saved)
+    m(x.requires_grad_(), mask).sum().backward()
+    assert [layer.calls for layer in m.layers] == [2, 2]   # (once more each, not nested)
+    full = stack_gradients(m, x.detach(), mask, lambda t: t.detach().clone())
+    kept = stack_gradients(m, x.detach(), mask, lambda t: at_kept(t).detach())
+    want, other = (kept, full) if saved == "8bit" else (full, kept)
+    for n, p in m.named_parameters():
+        assert torch.equal(p.grad, want[n]), n
+        assert not torch.equal(p.grad, other[n]) or n == "layers.1.lin.bias", n

@@ -61,13 +61,14 @@ def _get_layer_by_name(model: nn.Module, name: str) -> Optional[nn.Module]:
 
 
 def _wrap_layer_with_checkpoint(layer: nn.Module, use_reentrant: bool, saved: str = "full"):
+    layer._zq_ckpt_saved = saved   # (of a layer that is wrapped already, too)
     if getattr(layer, "_zq_ckpt_wrapped", False):
         return
     original = layer.forward
 
     def checkpointed_forward(*args, **kwargs):
         if torch.is_grad_enabled():
-            if saved == "8bit":
+            if layer._zq_ckpt_saved == "8bit":
                 return checkpoint_8bit(original, *args, **kwargs)
             return checkpoint(original, *args, use_reentrant=use_reentrant, **kwargs)
         return original(*args, **kwargs)
@@ -78,8 +79,9 @@ def _wrap_layer_with_checkpoint(layer: nn.Module, use_reentrant: bool, saved: st
 
 def enable_gradient_checkpointing(model: nn.Module, checkpoint_layers: Optional[List[str]] = None,
                                   use_reentrant: bool = False, saved: str = "full"):
-    """``saved="8bit"``: the wrapped layers keep their inputs in 8 bits
-    (:func:`~zeroq_b200.ops.act8.checkpoint_8bit`, without reentrance)."""
+    """``saved="8bit"``: the wrapped layers keep their activations in 8 bits
+    (:func:`~zeroq_b200.ops.act8.checkpoint_8bit`, without reentrance).  Layers that are
+    wrapped already take the ``saved`` of the last call."""
     keep8 = check_saved("enable_gradient_checkpointing", saved)
     if keep8 and use_reentrant:
         raise ValueError("enable_gradient_checkpointing: saved='8bit' goes without reentrance")
