@@ -363,3 +363,26 @@ def test_gpu_forward_mode_is_refused(cuda):
 def test_a_copied_model_keeps_its_choices():
     m = copy.deepcopy(model(saved_activations="8bit"))
     assert m.embed_tokens.scale == 8.0 and m.norm.saved == "8bit" and m.layers[0].act_saved == "8bit"
+
+
+def test_layer_norm_biases_go_through_checkpoint_files(tmp_path):
+    from zeroq_b200.utils.loading import hf_to_decoder_name, save_hf_checkpoint, stream_load
+
+    m = model(vocab_size=256)
+    g = torch.Generator().manual_seed(4)
+    for n, p in m.named_parameters():
+        if "norm" in n:
+            p.data += torch.randn(p.shape, generator=g)
+    path = str(tmp_path / "model.safetensors")
+    save_hf_checkpoint(m, path)
+    again = model(seed=1, vocab_size=256)
+    counts = stream_load(again, path)
+    assert counts["skipped"] == 0 and counts["copied"] == len(list(m.parameters()))
+    for (n, a), b in zip(m.named_parameters(), again.parameters()):
+        assert torch.equal(a, b), n
+    ids, _ = batch()
+    assert torch.equal(m(ids), again(ids))
+    assert hf_to_decoder_name("model.layers.1.input_layernorm.bias") == "layers.1.attn_norm.bias"
+    assert hf_to_decoder_name("model.norm.bias") == "norm.bias"
+    # into a decoder whose norms have none
+    assert stream_load(model(seed=1, vocab_size=256, norm="rmsnorm"), path)["skipped"] == 5

@@ -13,7 +13,8 @@ does the same for :class:`zeroq_b200.models.DecoderLM`:
   weight registered with the coordinator is quantised and sharded on arrival
   (this rank keeps only its shard), anything else (norms, embeddings, the head,
   biases that are not registered) is copied into the module; the vocabulary
-  padding rows stay zero.
+  padding rows stay zero.  The kind of norm and the embedding's scale come from the
+  model's config, not from the file.
 """
 
 from __future__ import annotations
@@ -29,7 +30,9 @@ import torch.nn as nn
 _LAYER = re.compile(r"^model\.layers\.(\d+)\.(.+)$")
 _SUFFIX = {
     "input_layernorm.weight": "attn_norm.weight",
+    "input_layernorm.bias": "attn_norm.bias",
     "post_attention_layernorm.weight": "mlp_norm.weight",
+    "post_attention_layernorm.bias": "mlp_norm.bias",
     "self_attn.q_proj.weight": "q_proj.weight",
     "self_attn.k_proj.weight": "k_proj.weight",
     "self_attn.v_proj.weight": "v_proj.weight",
@@ -47,8 +50,8 @@ def hf_to_decoder_name(name: str) -> Optional[str]:
     """Hugging Face Llama/Qwen2 parameter name -> DecoderLM name (None if unused)."""
     if name == "model.embed_tokens.weight":
         return "embed_tokens.weight"
-    if name == "model.norm.weight":
-        return "norm.weight"
+    if name in ("model.norm.weight", "model.norm.bias"):
+        return name[len("model."):]
     if name == "lm_head.weight":
         return "lm_head.weight"
     m = _LAYER.match(name)
@@ -146,6 +149,7 @@ def save_hf_checkpoint(model: nn.Module, path: str, vocab_size: Optional[int] = 
             inv[f"layers.{i}.{ours}"] = f"model.layers.{i}.{hf}"
     inv["embed_tokens.weight"] = "model.embed_tokens.weight"
     inv["norm.weight"] = "model.norm.weight"
+    inv["norm.bias"] = "model.norm.bias"
     inv["lm_head.weight"] = "lm_head.weight"
     out = {}
     for name, p in model.named_parameters():
