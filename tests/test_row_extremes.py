@@ -1,0 +1,62 @@
+"""Ends of the ranges of the row operators."""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_row_ops import DEVICES, TYPES, U, near, randn
+from zeroq_b200.ops import token_logprobs
+
+
+@pytest.fixture(params=DEVICES)
+def device(request):
+    if request.param == "cuda":
+        request.getfixturevalue("cuda")
+    return request.param
+
+
+# ---------------------------------------------------------------------------
+# token log probabilities
+# ---------------------------------------------------------------------------
+def entropy_gradient(z, tau, g):
+    """dz of g . H against -g p (l + H) / tau in 64 bits; the bounds of the formula's other tests"""
+    z = z.requires_grad_()
+    M, V = z.shape
+    out = token_logprobs(z, None, temperature=tau)
+    (dz,) = torch.autograd.grad(out.entropy, z, g)
+    Z, G = z.detach().double().cpu(), g.double().cpu()[:, None]
+    high = Z.amax(-1, keepdim=True)
+    t = (Z - high) / tau
+    l = torch.log_softmax(t, -1)
+    p = l.exp()
+    l0, t0 = torch.where(p > 0, l, 0.0), torch.where(p > 0, t.abs(), 0.0)
+    H = -(p * l0).sum(-1, keepdim=True)
+    spread = (p * t0).sum(-1, keepdim=True)
+    # S: V / 256 sums in a row and their joins, 2^-22 an exponential; its argument's error; H's
+    es = (V / 256 + 64) * U
+    more = p * G.abs() * ((l0.abs() + H) * (2 * es + 2.0 ** -20 * (1 + t0)) + 4 * es * (1 + spread + H)) / tau
+    # a p below 32 bits' normal range, 2^-126, is 0 (with its error, from 2^-125 down it may be), times
+    # the same factor
+    more = more + 2.0 ** -125 * G.abs() * (l0.abs() + H) / tau
+    want = -G * p * (l0 + H) / tau
+    # (an entry whose bounds reach past the type's range may be there; near() takes the others)
+    tol = torch.finfo(z.dtype).eps / 2 * want.abs() + more
+    low, high, got = (want - tol).to(z.dtype), (want + tol).to(z.dtype), dz.cpu()
+    edge = low.isinf() | high.isinf()
+    assert ((low <= got) & (got <= high))[edge].all()
+    near(torch.where(edge, 0.0, got), torch.where(edge, 0.0, want), more + 2.0 ** -126)
+
+
+@pytest.mark.parametrize("V", [600, pytest.param(70001, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau,g", [(0.01, 65536.0), (1e-3, 400.0), (1e-4, 10.0), (1e-5, 0.1), (1e-5, 1e5), (1e-6, 1.0)])
+def test_entropy_gradient_of_masked_logits(device, tau, g, dtype, V):
+    z = randn(9, V, seed=V) * tau            # several of a row weigh something
+    z[5:] = randn(4, V, seed=1).clamp(max=0.5)
+    z[5:, 7] = torch.tensor([0.6, 1.0, 3.0, 5.0])   # one has all the weight
+    z = z.to(device=device, dtype=dtype)
+    gone = torch.rand(9, V, generator=torch.Generator().manual_seed(2)) < 0.3
+    gone[:, 7] = False
+    for low in (-math.inf, torch.finfo(dtype).min, max(-1e9, torch.finfo(dtype).min)):
+        entropy_gradient(torch.where(gone.to(device), low, z), tau, g * randn(9, seed=3, device=device))
