@@ -254,7 +254,8 @@ struct LpLog {
   __device__ __forceinline__ LpLog(const LogprobParams& p, float high, float sum)
       : m(lp_plain(high, p.scale) ? -(double)lp_shift(high, p.scale) * p.inv_scale : (double)high),
         log_s(sum < INFINITY ? lp_log(sum) : 0.0), inv_tau(p.inv_tau) {}
-  __device__ __forceinline__ float of(float z) const { return (float)(((double)z - m) * inv_tau - log_s); }
+  // At most 0, as p is at most 1: a certain token's S may be below 1 by the exponential's error.
+  __device__ __forceinline__ float of(float z) const { return (float)fmin(((double)z - m) * inv_tau - log_s, 0.0); }
 };
 
 // Whole numbers in the values' order (0 and -0 equal, NaN above all), without the places that

@@ -60,3 +60,18 @@ def test_entropy_gradient_of_masked_logits(device, tau, g, dtype, V):
     gone[:, 7] = False
     for low in (-math.inf, torch.finfo(dtype).min, max(-1e9, torch.finfo(dtype).min)):
         entropy_gradient(torch.where(gone.to(device), low, z), tau, g * randn(9, seed=3, device=device))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [300, 5003, pytest.param(70000, marks=pytest.mark.gpu)])
+def test_log_probabilities_are_at_most_0(device, V, dtype):
+    """a certain token's: neither the exponential's error nor a sum's rounding shows above 0"""
+    M = 400 if V < 60000 else 40
+    z = randn(M, V, seed=V)
+    z[torch.arange(M), torch.arange(M) % V] += torch.linspace(0, 30, M)
+    z[: M // 4] = -math.inf                      # no other token at all
+    z[torch.arange(M), torch.arange(M) % V] = z[torch.arange(M), torch.arange(M) % V].nan_to_num(neginf=3.3)
+    z[: M // 4, :3] = z[: M // 4, :3].clamp(min=-30.0)
+    for tau in (1.0, 0.7, 1e-3):
+        out = token_logprobs(z.to(device=device, dtype=dtype), torch.arange(M, device=device) % V, top_k=3, temperature=tau)
+        assert (out.logprobs <= 0).all() and (out.top_logprobs <= 0).all() and (out.entropy >= 0).all()
