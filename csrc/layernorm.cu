@@ -592,7 +592,8 @@ LnParams ln_base(const at::Tensor& x, const c10::optional<at::Tensor>& w, const 
   p.G = (D + kGroup - 1) / kGroup;
   at::ScalarType wt = at::kFloat;
   if (w.has_value()) wt = w->scalar_type();
-  TORCH_CHECK(wt == at::kFloat || wt == at::kBFloat16 || wt == at::kHalf, "layer_norm: weight in fp32, bf16 or fp16");
+  else if (b.has_value()) wt = b->scalar_type();
+  TORCH_CHECK(wt == at::kFloat || wt == at::kBFloat16 || wt == at::kHalf, "layer_norm: weight and bias in fp32, bf16 or fp16");
   if (w.has_value()) ln_vector(*w, x, wt, "weight"), p.w = w->data_ptr();
   if (b.has_value()) ln_vector(*b, x, wt, "bias"), p.b = b->data_ptr();
   p.wt = wt == at::kFloat ? 0 : wt == at::kBFloat16 ? 1 : 2;

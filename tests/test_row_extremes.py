@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_row_ops import DEVICES, TYPES, U, near, randn
+from tests.test_row_ops import DEVICES, TYPES, U, near, norm_case, randn
 from zeroq_b200.ops import token_logprobs
 
 
@@ -75,3 +75,14 @@ def test_log_probabilities_are_at_most_0(device, V, dtype):
     for tau in (1.0, 0.7, 1e-3):
         out = token_logprobs(z.to(device=device, dtype=dtype), torch.arange(M, device=device) % V, top_k=3, temperature=tau)
         assert (out.logprobs <= 0).all() and (out.top_logprobs <= 0).all() and (out.entropy >= 0).all()
+
+
+# ---------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("wtype", TYPES)
+def test_layer_norm_with_a_bias_alone(device, wtype):
+    for dtype in TYPES:
+        for D in (72, 1001):
+            norm_case(device, 40, D, dtype, wtype=wtype, weight=False)
+            norm_case(device, 40, D, dtype, wtype=wtype, weight=False, residual=True, saved="8bit")
