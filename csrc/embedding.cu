@@ -51,12 +51,14 @@ __global__ void __launch_bounds__(kEmbWarps * 32) embedding_fwd_kernel(const voi
   uint32_t row = (uint32_t)first / (uint32_t)tiles, tile = (uint32_t)first - row * (uint32_t)tiles;
   int64_t at[U];
   int base[U], id[U];
+  uint32_t here = 0;   // bit j: the id is in the table
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     at[j] = row;
     base[j] = (int)tile * kTile;
     if (++tile == (uint32_t)tiles) tile = 0, ++row;
     id[j] = j < n ? emb_id(ids, ids64, at[j], V) : -1;
+    here |= (id[j] >= 0 ? 1u : 0u) << j;
   }
   RawTile<T, VEC> t[U];
 #pragma unroll
@@ -66,8 +68,10 @@ __global__ void __launch_bounds__(kEmbWarps * 32) embedding_fwd_kernel(const voi
     if (j < n) {
       float v[8];
       t[j].values(v);
+      // (an absent id's zeros times a scale that is not finite, or negative, would be NaN or -0)
+      const float s = here >> j & 1u ? scale : 1.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= scale;
+      for (int i = 0; i < 8; ++i) v[i] *= s;
       store_tile<T, VEC>(y + at[j] * D, base[j], lane, D, v);
     }
   }

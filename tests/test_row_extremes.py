@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_row_ops import DEVICES, TYPES, U, near, norm_case, randn
-from zeroq_b200.ops import token_logprobs
+from zeroq_b200.ops import embedding, token_logprobs
 
 
 @pytest.fixture(params=DEVICES)
@@ -86,3 +86,23 @@ def test_layer_norm_with_a_bias_alone(device, wtype):
         for D in (72, 1001):
             norm_case(device, 40, D, dtype, wtype=wtype, weight=False)
             norm_case(device, 40, D, dtype, wtype=wtype, weight=False, residual=True, saved="8bit")
+
+
+# ---------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [256, 1001])
+@pytest.mark.parametrize("scale", [-2.0, 0.0, math.inf, -math.inf, math.nan])
+def test_rows_of_absent_ids_are_0(device, scale, D, dtype):
+    """whatever the scale, and without a sign"""
+    ids = torch.tensor([3, -1, 8, 7, 1 << 40, -100], device=device)
+    w = randn(8, D, seed=1, dtype=dtype, device=device).requires_grad_()
+    y = embedding(ids, w, scale)
+    absent = y.detach()[[1, 2, 4, 5]]
+    assert (absent == 0).all() and not torch.signbit(absent).any()
+    here = (w.detach().float() * scale).to(dtype)[[3, 7]]
+    assert torch.equal(y.detach()[[0, 3]].nan_to_num(nan=5.0), here.nan_to_num(nan=5.0))
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    rows = dw[[0, 1, 2, 4, 5, 6]]
+    assert (rows == 0).all() and not torch.signbit(rows).any()
