@@ -6,18 +6,22 @@
 // and with a = dy w (n from the kept h, which may be the 8-bit one):
 //   dx = r (a - mean a - n mean(a n)) (+ dh);  dw = sum over rows dy n;  db = sum over rows dy
 //
-// A team of W warps takes one row at a time and holds it in registers, K tiles of 256 columns
-// a warp (the backward with its sums of dw and db beside it; w and b are in shared memory);
-// teams go over the rows with a fixed stride, and the loads of the next row are under way while
-// this one is reduced.  The variance is the joined sum of squares about each warp's own mean
-// (columns n_i, mean m_i, squares q_i: q = sum q_i + n_i (m_i - mu)^2), so one exchange gives
-// both and nothing cancels.  dw and db: a block's teams add up in team order in shared memory,
-// the blocks' rows of partial sums are added in block order by a second kernel: no atomics.
+// Forward: a team of W warps takes one row at a time and holds it in registers, K tiles of 256
+// columns a warp; w and b are in shared memory.  Backward: a team takes two rows at a time, holds
+// their sums and those of dw and db, and reads the rows twice from shared memory.  Teams go over
+// the rows with a fixed stride, and the loads of the next row are under way while this one is
+// reduced.  A mean that is large next to the deviation costs nothing but its own roundings: a warp's
+// sums are of differences from its first value, the row's mean is formed by differences from the
+// first warp's, and n by subtracting before r is multiplied (r h - r mu rounds r mu: n = 0.08 in a
+// row of 10000).  A row of one value has n = 0.  The variance is the joined sum of squares about
+// each warp's own mean (columns n_i, mean m_i, squares q_i: q = sum q_i + n_i (m_i - mu)^2), so
+// one exchange gives both and nothing cancels.  dw and db: a block's teams add up in team order in
+// shared memory, the blocks' rows of partial sums are added in block order by a second kernel: no
+// atomics.
 //
 // What bounds it: memory in the plain forward (8192 x 3584 with residual 38 us, 0.95 of a copy's
-// rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 100 us,
-// 0.64) and in the backward (55 us, 0.66, and 128 us from codes, 0.50), at about half of the issue
-// slots and no pipe above 0.4.
+// rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 106 us,
+// 0.61) and in the backward (52 us, 0.70, and 112 us from codes, 0.57).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -29,7 +33,7 @@
 namespace zq {
 
 constexpr int kLnMaxWarps = 16;     // of a team
-constexpr int kLnBlockWarps = 24;   // of a block: 80 registers a thread
+constexpr int kLnBlockWarps = 24;   // of a block at most: 80 registers a thread (20: 96, 16: 128)
 constexpr int kLnMaxTeams = kLnBlockWarps / 2;   // of several warps
 
 struct LnParams {
@@ -283,49 +287,10 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
         t.pairs(v[k]);   // as the next layer and the backward see it
       }
     }
-    uint64_t s = 0ull;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = f2_add(s, v[k][i]);
-    float mu = warp_sum(f2_sum(s)) * inv_cols, q = 0.0f;
     if constexpr (PIPE) {   // the slot is read
       rows.template fetch<1>(p, at, row + S * step);
       at = at + 1 == S ? 0 : at + 1;
     }
-    {
-      const uint64_t away = f2_pack(-mu, -mu);
-      uint64_t q2 = 0ull;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int base = (wt + k * W) * kTile;
-        if (base + kTile <= D) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t d = f2_add(v[k][i], away);
-            q2 = f2_fma(d, d, q2);
-          }
-        } else if (base < D) {   // the row ends in this tile
-          const uint32_t mask = ln_mask<VEC>(base, lane, D);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float a, b;
-            f2_unpack(f2_add(v[k][i], away), a, b);
-            if (mask >> (2 * i) & 1u) q = fmaf(a, a, q);
-            if (mask >> (2 * i + 1) & 1u) q = fmaf(b, b, q);
-          }
-        }
-      }
-      q = warp_sum(q + f2_sum(q2));
-    }
-    if (W > 1) {
-      const float2 o = ln_exchange(s_red[team][turn], make_float2(mu, q), wt, lane, team, W);
-      mu = ln_sum16(cols_of * o.x) * inv_d;
-      const float d = o.x - mu;
-      q = ln_sum16(lane < W ? fmaf(cols_of * d, d, o.y) : 0.0f);
-    }
-    const float r = rsqrtf(fmaf(q, inv_d, p.eps));
-    if (wt == 0 && lane == 0 && p.mean != nullptr) p.mean[row] = mu, p.rstd[row] = r;
     if constexpr (KEEP) {
       int8_t* c[K];
       float* t[K];
@@ -334,7 +299,57 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       for (int k = 0; k < K; ++k) c[k] = p.codes + row * p.P, t[k] = p.steps + row * p.G, base[k] = (wt + k * W) * kTile;
       keep_tiles<VEC, K>(v, c, t, base, lane, D);
     }
-    const float off = -mu * r;
+    // The warp's mean and its sum of squares about it, from differences from its first value, which are
+    // small or exact: one pass and one reduction.  q = sum d^2 - n (mean d)^2 cancels where that value
+    // lies far out; from 2.8 deviations on once more, from the mean, so that the 22 roundings of a sum
+    // weigh 9-fold at most (16384 x 5120 kept in 8 bits: 107 us from 2 deviations on, 104 from 5.5).
+    // v: the differences.
+    float mu, q, from, rest;
+    f2_unpack(v[0][0], from, rest);
+    from = __shfl_sync(0xffffffffu, from, 0);
+    float away = -from;
+    for (bool again = false;; again = true) {
+      const uint64_t away2 = f2_pack(away, away);
+      uint64_t s2 = 0ull, q2 = 0ull;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int base = (wt + k * W) * kTile;
+        if (base + kTile <= D) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[k][i] = f2_add(v[k][i], away2);
+        } else if (base < D) {   // the row ends in this tile: 0 behind it
+          const uint32_t mask = ln_mask<VEC>(base, lane, D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a, b;
+            f2_unpack(f2_add(v[k][i], away2), a, b);
+            v[k][i] = f2_pack(mask >> (2 * i) & 1u ? a : 0.0f, mask >> (2 * i + 1) & 1u ? b : 0.0f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s2 = f2_add(s2, v[k][i]);
+          q2 = f2_fma(v[k][i], v[k][i], q2);
+        }
+      }
+      const float d = warp_sum(f2_sum(s2)) * inv_cols, nd2 = cols * d * d;
+      q = warp_sum(f2_sum(q2)) - nd2;
+      mu = from + d;
+      if (again || nd2 <= 8.0f * q) break;   // (sums beyond 32 bits, too: infinity - infinity is NaN)
+      away = from - mu;
+      from = mu;
+    }
+    q = max_nan(q, 0.0f);
+    if (W > 1) {
+      const float2 o = ln_exchange(s_red[team][turn], make_float2(mu, q), wt, lane, team, W);
+      const float first = __shfl_sync(0xffffffffu, o.x, 0);   // (again from differences)
+      mu = fmaf(ln_sum16(lane < W ? cols_of * (o.x - first) : 0.0f), inv_d, first);
+      const float d = o.x - mu;
+      q = ln_sum16(lane < W ? fmaf(cols_of * d, d, o.y) : 0.0f);
+    }
+    const float r = rsqrtf(fmaf(q, inv_d, p.eps));
+    if (wt == 0 && lane == 0 && p.mean != nullptr) p.mean[row] = mu, p.rstd[row] = r;
+    const float off = (from - mu) * r;   // (of a few deviations' size)
     const uint64_t off2 = f2_pack(off, off), r2 = f2_pack(r, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -398,24 +413,23 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
       else t.load(reinterpret_cast<const T*>(from) + (row + b) * pitch, (wt + k * W) * kTile, lane, D);
       t.pairs(g);
     };
-    auto normal = [&](int b, int k, uint64_t (&n)[4]) {   // (h - mu) r
+    auto away = [&](int b, int k, uint64_t (&d)[4]) {   // h - mu
       const int base = (wt + k * W) * kTile;
-      const float off = -mu[b] * r[b];
       if constexpr (KEPT) {
         RawCodes<VEC> c;
         if constexpr (PIPE) rows.get(at * B + b, k, c);
         else c.load(p.codes + (row + b) * p.P, p.steps + (row + b) * p.G, base, lane, D);
-        c.scaled(r[b], off, n);
+        c.away(mu[b], d);
       } else {
         RawTile<T, VEC> t;
         if constexpr (PIPE) rows.get(at * B + b, kX, k, t);
         else t.load(reinterpret_cast<const T*>(p.x) + (row + b) * p.xs, base, lane, D);
-        t.pairs(n);
+        t.pairs(d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = f2_fma(n[i], f2_pack(r[b], r[b]), f2_pack(off, off));
+        for (int i = 0; i < 4; ++i) d[i] = f2_add(d[i], f2_pack(-mu[b], -mu[b]));
       }
     };
-    float s[2 * B];   // sums of a and a n of each row
+    float s[2 * B];   // sums of a and a (h - mu) of each row
     {
       uint64_t t[2 * B];
 #pragma unroll
@@ -429,16 +443,17 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
 #pragma unroll
         for (int b = 0; b < B; ++b) {
           if (b > 0 && !second) continue;
-          uint64_t g[4], n[4];
+          uint64_t g[4], d[4];
           gradient(p.dy, p.dys, 0, b, k, g);
-          normal(b, k, n);
+          away(b, k, d);
+          const uint64_t r2 = f2_pack(r[b], r[b]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {   // (past the row's end dy and w are 0)
-            dw[k][i] = f2_fma(g[i], n[i], dw[k][i]);
+            dw[k][i] = f2_fma(g[i], f2_mul(d[i], r2), dw[k][i]);
             db[k][i] = f2_add(db[k][i], g[i]);
             g[i] = f2_mul(g[i], w[i]);
             t[2 * b] = f2_add(t[2 * b], g[i]);
-            t[2 * b + 1] = f2_fma(g[i], n[i], t[2 * b + 1]);
+            t[2 * b + 1] = f2_fma(g[i], d[i], t[2 * b + 1]);
           }
         }
       }
@@ -472,7 +487,7 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
     }
 #pragma unroll
     for (int i = 0; i < 2 * B; ++i) s[i] = __shfl_sync(0xffffffffu, v, i) * inv_d;
-    // dx = r a - r mean a - n r mean(a n)
+    // dx = r a - r mean a - (h - mu) r^2 mean(a n)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int base = (wt + k * W) * kTile;
@@ -482,13 +497,13 @@ __global__ void __launch_bounds__(WARPS * 32) ln_bwd_kernel(const __grid_constan
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         if (b > 0 && !second) continue;
-        const float c0 = -r[b] * s[2 * b], c1 = -r[b] * s[2 * b + 1];
+        const float c0 = -r[b] * s[2 * b], c1 = -r[b] * (r[b] * (r[b] * s[2 * b + 1]));
         const uint64_t c02 = f2_pack(c0, c0), c12 = f2_pack(c1, c1), r2 = f2_pack(r[b], r[b]);
-        uint64_t g[4], n[4];
+        uint64_t g[4], d[4];
         gradient(p.dy, p.dys, 0, b, k, g);
-        normal(b, k, n);
+        away(b, k, d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(n[i], c12, c02));
+        for (int i = 0; i < 4; ++i) g[i] = f2_fma(f2_mul(g[i], w[i]), r2, f2_fma(d[i], c12, c02));
         if constexpr (RES) {
           uint64_t h[4];
           gradient(p.dh, p.dhs, kH, b, k, h);
@@ -792,8 +807,12 @@ static void ln_bwd_launch(LnParams& p, const at::Tensor& dy, c10::optional<at::T
       p.src[1] = RES ? p.dh : p.x, p.pitch[1] = RES ? p.dhs : p.xs;
       p.src[2] = p.x, p.pitch[2] = p.xs;
       constexpr int kBytes = LnSlots<T, K, 1 + (RES ? 1 : 0) + (KEPT ? 0 : 1), KEPT, true>::kBytes;
-      constexpr int kWarps = K <= 2 ? kLnBlockWarps : kLnMaxWarps;
+      // as many warps as two groups of rows leave room for, and the registers that they do
+      constexpr int kRoom = 227 * 1024 / (kBytes * 32 * kLnRows * 2);
+      constexpr int kWarps = K > 2 || kRoom <= kLnMaxWarps ? kLnMaxWarps : kRoom < kLnBlockWarps ? 20 : kLnBlockWarps;
       const size_t smem = ln_block(p, front, kBytes, kWarps, kLnRows, 1);
+      if constexpr (K == 2 && kWarps > 20)   // (16384 x 5120 from codes, 20 warps: 131 us with 80 registers, 112 with 96)
+        if (smem > 0 && p.W * p.R <= 20) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, 20>, smem);
       if (smem > 0) return go(ln_bwd_kernel<T, VEC, K, KEPT, RES, true, kWarps>, smem);
     }
     p.R = VEC ? 1 : ln_teams(p, kLnRows);

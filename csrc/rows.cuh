@@ -240,17 +240,17 @@ struct RawCodes {
       v[i] = __fmul_rn(__fadd_rn(f, -8388736.0f), step[VEC ? 0 : i / 4]);
     }
   }
-  // code * (step * a) + b, in packed pairs
-  __device__ __forceinline__ void scaled(float a, float b, uint64_t (&v)[4]) const {
+  // code * step - mu, rounded once, in packed pairs
+  __device__ __forceinline__ void away(float mu, uint64_t (&v)[4]) const {
     const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
-    const uint64_t away = f2_pack(-8388736.0f, -8388736.0f), b2 = f2_pack(b, b);
+    const uint64_t back = f2_pack(-8388736.0f, -8388736.0f), mu2 = f2_pack(-mu, -mu);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t s = i < 2 ? x : y;
       const float lo = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + (2 * i & 3)));
       const float hi = __uint_as_float(__byte_perm(s, 0x4b000000u, 0x7540u + ((2 * i + 1) & 3)));
-      const float t = step[VEC ? 0 : i / 2] * a;
-      v[i] = f2_fma(f2_add(f2_pack(lo, hi), away), f2_pack(t, t), b2);
+      const float t = step[VEC ? 0 : i / 2];
+      v[i] = f2_fma(f2_add(f2_pack(lo, hi), back), f2_pack(t, t), mu2);
     }
   }
 };

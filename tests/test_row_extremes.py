@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_row_ops import DEVICES, TYPES, U, near, norm_case, randn
-from zeroq_b200.ops import embedding, token_logprobs
+from zeroq_b200.ops import add_layer_norm, embedding, layer_norm, token_logprobs
 
 
 @pytest.fixture(params=DEVICES)
@@ -80,6 +80,69 @@ def test_log_probabilities_are_at_most_0(device, V, dtype):
 # ---------------------------------------------------------------------------
 # layer norm
 # ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1, 8, 33, 256, 264, 1000, 1001, 1032, 3584, 5120, 8200, 12289, 16384])
+def test_layer_norm_of_rows_of_one_value(cuda, D, dtype, residual):
+    """differences from the mean are 0 to the bit: y is the bias, dw is 0"""
+    c = torch.tensor([10000.0, 0.1, -777.7, 3.0, 1e-3, 60000.0], device=cuda)[:, None]
+    x = c.expand(6, D).to(dtype).contiguous().requires_grad_()
+    w, b = randn(D, seed=8, device=cuda).requires_grad_(), randn(D, seed=9, device=cuda)
+    y = add_layer_norm(x, torch.zeros_like(x), w, b, eps=1e-5)[1] if residual else layer_norm(x, w, b, eps=1e-5)
+    assert torch.equal(y, b.to(dtype).expand(6, D))
+    dw, dx = torch.autograd.grad(y, [w, x], randn(6, D, seed=10, dtype=dtype, device=cuda))
+    assert (dw == 0).all() and torch.isfinite(dx).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [0.0, 50.0])
+@pytest.mark.parametrize("D", [520, 4100, 4101, 12000])
+@pytest.mark.parametrize("mean,dev", [(10000.0, 1e-2), (-3e5, 1.0), (1e3, 1e-3), (1.0, 1e-6), (0.0, 1.0)])
+def test_layer_norm_rounds_the_mean_alone(cuda, mean, dev, D, first):
+    """Rows far from 0 in fp32, with and without a first value far out.  The mean is off by two roundings
+    of its own (a warp's, the row's) and by a row's length in roundings of the deviations; the
+    differences from it by one of theirs."""
+    z = randn(6, D, seed=D).double()
+    z[::2, 0] += first
+    x = (mean + dev * z).float().to(cuda)
+    w = torch.ones(D, device=cuda, requires_grad=True)
+    y = layer_norm(x, w, None, eps=1e-12)
+    X = x.double().cpu()
+    mu = X.mean(-1, keepdim=True)
+    d = X - mu
+    r = (d.square().mean(-1, keepdim=True) + 1e-12).rsqrt()
+    dmu = 2 * U * mu.abs() + 64 * U * (d.abs().mean(-1, keepdim=True) + d.abs().amax(-1, keepdim=True))
+    # r: half of what its sum of squares is off by - 22 roundings (of a lane's values, of the lanes) nine
+    # times, as up to 8/9 of the sum are taken off again, and those over warps - and of dmu squared
+    dn = r * dmu + (d * r).abs() * (128 * U + 0.5 * (r * dmu).square())
+    near(y, d * r, dn)
+    dy = randn(6, D, seed=10, device=cuda)
+    (dw,) = torch.autograd.grad(y, w, dy)
+    g = dy.double().cpu()
+    # 2 more: of the mean that the backward is given, and of its use
+    near(dw, (g * d * r).sum(0), (g.abs() * (dn + 2 * U * mu.abs() * r)).sum(0) + 10 * U * (g * d * r).abs().sum(0))
+
+
+@pytest.mark.parametrize("D", [8, 300, 301, 4100, pytest.param(16384, marks=pytest.mark.gpu)])
+def test_layer_norm_of_rows_with_infinities(device, D):
+    """NaN throughout, wherever they are, and their gradients; the rows beside them are not touched"""
+    for dtype in TYPES:
+        x = randn(9, D, seed=D, dtype=dtype, device=device)
+        for i, (c, v) in enumerate([(0, math.inf), (D // 2, -math.inf), (D - 1, math.inf), (0, math.nan), (D - 1, math.nan)]):
+            x[i, c] = v
+        x[5] = math.inf
+        x.requires_grad_()
+        y = layer_norm(x)
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert y[:6].isnan().all() and dx[:6].isnan().all()
+        assert torch.equal(y[6:], layer_norm(x[6:])) and torch.isfinite(dx[6:]).all()
+    # squares beyond 32 bits: a deviation without end
+    x = torch.full((2, D), 1e25, device=device)
+    x[:, ::2] = -3e25
+    assert (layer_norm(x) == 0).all()
+
+
 @pytest.mark.parametrize("wtype", TYPES)
 def test_layer_norm_with_a_bias_alone(device, wtype):
     for dtype in TYPES:
