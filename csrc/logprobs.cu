@@ -55,8 +55,6 @@ struct LogprobParams {
   int64_t M, stride, gstride, width, V;
   int K;
   float scale;              // log2(e) / τ
-  float floor;              // of the logits in the gradient
-  __nv_bfloat162 low;       // the same, twice
   double inv_tau, inv_scale;
 };
 
@@ -76,13 +74,11 @@ __device__ __forceinline__ float lp_t(float z, float m, float scale) { return ma
 __device__ __forceinline__ float lp_shift(float m, float scale) { return __fmul_rd(-m, scale); }
 
 // Logits from here down are taken as this: they weigh 0 in a row whose reference is in the range
-// where what the shift's rounding leaves is small (temperatures of 1e-6 to 1e6), and t stays
-// finite.  Other rows take the form above.  The gradient's floor is nearer: there t is multiplied by
-// up to |g_H| / τ before 2^t = 0 is, and 0 times what overflows is NaN (t of -1e30 s at a τ of 1e-4
-// and a g_H of 4).  From -4e6 powers of two down, rounded to bf16 or not, t lies below -2.9e6 in
-// a row whose reference is less than 1e6 of them from 0, and above -5.1e6.
-constexpr float kLpFloor = -1e30f;
-constexpr float kLpGradientFloor = -4e6f;   // times 1 / s; a launch argument
+// where what the shift's rounding leaves is small (t < -1.3e7 at a temperature of 1e6), and t stays
+// finite, also times up to |g_H| / τ in the gradient: 2^t = 0 times what overflows would be NaN
+// (-1e13 · 1.44 ln 2 |g_H| / τ² does from |g_H| / τ² = 3e25 on, -1e30 did from 3e8).  Other rows take
+// the form above.
+constexpr float kLpFloor = -1e13f;
 __device__ __forceinline__ bool lp_plain(float m, float scale) { return fabsf(m * scale) < 1e6f; }
 
 // 16 bytes of a row
@@ -117,11 +113,13 @@ struct LpVec {
       return max_nan(to_f32<T>(c.x), to_f32<T>(c.y));
     }
   }
-  // bounded from below by the floor (of bf16 by `low`, before the values are spread); NaN stays
-  __device__ __forceinline__ void floored_pairs(uint64_t (&p)[N / 2], float floor, const __nv_bfloat162& low) const {
+  // bounded from below by the floor (bf16 has it: before the values are spread); NaN stays
+  __device__ __forceinline__ void floored_pairs(uint64_t (&p)[N / 2]) const {
     float v[N];
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      __nv_bfloat162 low;
+      low.x = low.y = __float2bfloat16_rn(kLpFloor);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), low);
@@ -131,7 +129,7 @@ struct LpVec {
     } else {
       values(v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = max_nan(v[i], floor);
+      for (int i = 0; i < N; ++i) v[i] = max_nan(v[i], kLpFloor);
     }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) p[i] = f2_pack(v[2 * i], v[2 * i + 1]);
@@ -527,8 +525,6 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
   const int lane = threadIdx.x & 31;
   const float behind = kLpBehind / scale;
   float m = -INFINITY;
-  __nv_bfloat162 low;
-  low.x = low.y = __float2bfloat16_rn(kLpFloor);
   uint64_t s2 = 0ull, a2 = 0ull;
   auto add = [&](const LpVec<T> (&r)[U], int tile, int n) {
     float cm = -INFINITY;
@@ -557,7 +553,7 @@ __device__ __forceinline__ LpSums lp_slice(const LpRow<T>& row, int t0, int t1, 
     for (int j = 0; j < U; ++j) {
       if (j < n) {
         uint64_t z[P];
-        r[j].floored_pairs(z, kLpFloor, low);
+        r[j].floored_pairs(z);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const uint64_t t = f2_fma(z[i], sc, sh);
@@ -761,7 +757,7 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32, 3) logprob_bwd_kernel(const 
   const bool plain = lp_plain(high, p.scale);
   const float shift = lp_shift(high, p.scale);
   auto smooth = [&](float z) {
-    const float t = plain ? fmaf(max_nan(z, p.floor), p.scale, shift) - l2 : max_nan((z - high) * p.scale - l2, -1000.0f);
+    const float t = plain ? fmaf(max_nan(z, kLpFloor), p.scale, shift) - l2 : max_nan((z - high) * p.scale - l2, -1000.0f);
     return lp_exp2(t) * fmaf(c1, t, c0);
   };
   if (inside && counted && plain) {
@@ -770,7 +766,7 @@ __global__ void __launch_bounds__(kLpBwdWarps * 32, 3) logprob_bwd_kernel(const 
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       uint64_t z[P];
-      r[j].floored_pairs(z, p.floor, p.low);
+      r[j].floored_pairs(z);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const uint64_t t = f2_add(f2_fma(z[i], sc, sh), l);
@@ -855,8 +851,6 @@ LogprobParams lp_params(const at::Tensor& z, const c10::optional<at::Tensor>& ta
   p.width = z.size(1);
   p.V = vocab;
   p.scale = (float)(1.4426950408889634 / temperature);
-  p.floor = kLpGradientFloor / p.scale;
-  p.low.x = p.low.y = __float2bfloat16_rn(p.floor);
   p.inv_tau = 1.0 / temperature;
   p.inv_scale = 1.0 / (double)p.scale;
   return p;
