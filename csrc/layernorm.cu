@@ -22,6 +22,8 @@
 // What bounds it: memory in the plain forward (8192 x 3584 with residual 38 us, 0.95 of a copy's
 // rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 106 us,
 // 0.61) and in the backward (52 us, 0.70, and 112 us from codes, 0.57).
+// Rows that are not whole 16-byte vectors go by single elements and without rows under way: 16384 x
+// 5003 bf16 111 us forward (0.45), 289 backward (0.26), with codes 224 and 395 (0.28, 0.16).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

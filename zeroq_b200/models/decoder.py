@@ -79,8 +79,9 @@ class DecoderConfig:
     # memory
     activation_checkpointing: bool = False
     # "8bit": what a layer keeps for the backward is held in 8 bits - the inputs of checkpointed
-    # layers; without checkpoints those of the activation function and of layer norms (the
-    # activation then runs apart from the projections' GEMMs)
+    # layers (a frozen embedding's rows, which take no gradient, as they are); without
+    # checkpoints those of the activation function and of layer norms (the activation then runs
+    # apart from the projections' GEMMs)
     saved_activations: str = "full"
     # > 0: LM head + cross-entropy over vocabulary chunks of this many columns
     # (the [tokens, vocab] logits are never materialised; frozen head only).

@@ -4,8 +4,8 @@
 fp32; the erf and exp calls are CUDA's own functions.
 
 With ``saved="8bit"`` (``csrc/act8.cu``; bf16, fp16 and fp32) the outputs are the same and
-the inputs are kept for the backward in the 8 bits of :mod:`zeroq_b200.ops.act8`: half the
-memory, and gradients at the kept values.
+the inputs are kept for the backward in the 8 bits of :mod:`zeroq_b200.ops.act8`: 1.03 bytes
+an element instead of 2 or 4, and gradients at the kept values.
 """
 
 from __future__ import annotations
