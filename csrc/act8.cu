@@ -9,10 +9,11 @@
 //   gelu:   y = x Phi(x);            dx = dy (Phi(xq) + xq phi(xq))
 //   swiglu: y = g sigma(g) u;        du = dy gq s,  dg = dy uq s (1 + gq (1 - s)),  s = sigma(gq)
 //
-// What bounds them: memory.  A warp takes 256 columns at a time (rows.cuh) and loads several
+// What bounds them: memory, but for GELU.  A warp takes 256 columns at a time (rows.cuh) and loads several
 // such tiles before it works on the first.  Measured: 16384 x 5120 bf16 50 us to keep, 45 us to
 // read back (0.77 and 0.85 of a copy's rate); SwiGLU of 8192 x 18944 213 us forward, 208 backward
-// (0.89 and 0.91).  GELU of 8192 x 18944: 210 us forward (0.57; its error function), 234 backward (0.51).
+// (0.89 and 0.91).  GELU is bound by its arithmetic: 8192 x 18944 210 us forward (0.57, at 0.85 of the
+// issue slots), 234 backward (0.51, 0.76).
 // Rows that are not whole 16-byte vectors go by single elements: 16384 x 5003 bf16 137 us to keep,
 // 128 to read back, SwiGLU 355 and 332, GELU 263 and 256 (0.24 to 0.30).
 #include <ATen/ATen.h>

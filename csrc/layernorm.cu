@@ -21,7 +21,8 @@
 //
 // What bounds it: memory in the plain forward (8192 x 3584 with residual 38 us, 0.95 of a copy's
 // rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 106 us,
-// 0.61) and in the backward (52 us, 0.70, and 112 us from codes, 0.57).
+// 0.61) and in the backward (52 us, 0.70, and 112 us from codes, 0.57), at half to two thirds of the
+// issue slots and no pipe above 0.46.
 // Rows that are not whole 16-byte vectors go by single elements and without rows under way: 16384 x
 // 5003 bf16 111 us forward (0.45), 289 backward (0.26), with codes 224 and 395 (0.28, 0.16).
 #include <ATen/ATen.h>
@@ -289,10 +290,15 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
         t.pairs(v[k]);   // as the next layer and the backward see it
       }
     }
-    if constexpr (PIPE) {   // the slot is read
-      rows.template fetch<1>(p, at, row + S * step);
-      at = at + 1 == S ? 0 : at + 1;
-    }
+    // The slot is read: the row S steps behind this one.  With a residual once the sums are formed, as h
+    // is on its way out (8192 x 5120 fp32 with residual 151 us, 170 before them; without 83, 90 behind them).
+    auto ahead = [&] {
+      if constexpr (PIPE) {
+        rows.template fetch<1>(p, at, row + S * step);
+        at = at + 1 == S ? 0 : at + 1;
+      }
+    };
+    if constexpr (!RES) ahead();
     if constexpr (KEEP) {
       int8_t* c[K];
       float* t[K];
@@ -342,6 +348,7 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       from = mu;
     }
     q = max_nan(q, 0.0f);
+    if constexpr (RES) ahead();
     if (W > 1) {
       const float2 o = ln_exchange(s_red[team][turn], make_float2(mu, q), wt, lane, team, W);
       const float first = __shfl_sync(0xffffffffu, o.x, 0);   // (again from differences)
