@@ -19,7 +19,7 @@
 // shared memory, the blocks' rows of partial sums are added in block order by a second kernel: no
 // atomics.
 //
-// What bounds it: memory in the plain forward (8192 x 3584 with residual 38 us, 0.95 of a copy's
+// What bounds it: memory in the plain forward (8192 x 3584 with residual 39 us, 0.92 of a copy's
 // rate); arithmetic and the latency of reductions and barriers with codes (16384 x 5120: 106 us,
 // 0.61) and in the backward (52 us, 0.70, and 112 us from codes, 0.57), at half to two thirds of the
 // issue slots and no pipe above 0.46.
@@ -271,34 +271,30 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
     uint64_t v[K][4];
     if constexpr (PIPE) rows.wait(S);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int base = (wt + k * W) * kTile;
+    auto tile = [&](int stream, const void* from, int64_t pitch, int k, uint64_t (&u)[4]) {
       RawTile<T, VEC> t;
-      if constexpr (PIPE) rows.get(at, 0, k, t);
-      else t.load(reinterpret_cast<const T*>(p.x) + row * p.xs, base, lane, D);
-      t.pairs(v[k]);
-      if constexpr (RES) {
-        uint64_t d[4];
-        if constexpr (PIPE) rows.get(at, 1, k, t);
-        else t.load(reinterpret_cast<const T*>(p.delta) + row * p.ds, base, lane, D);
-        t.pairs(d);
+      if constexpr (PIPE) rows.get(at, stream, k, t);
+      else t.load(reinterpret_cast<const T*>(from) + row * pitch, (wt + k * W) * kTile, lane, D);
+      t.pairs(u);
+    };
+    auto read = [&](bool again) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[k][i] = f2_add(v[k][i], d[i]);
-        t.set(v[k]);
-        if (base < D) t.store(reinterpret_cast<T*>(p.h) + row * D, base, lane, D);
-        t.pairs(v[k]);   // as the next layer and the backward see it
-      }
-    }
-    // The slot is read: the row S steps behind this one.  With a residual once the sums are formed, as h
-    // is on its way out (8192 x 5120 fp32 with residual 151 us, 170 before them; without 83, 90 behind them).
-    auto ahead = [&] {
-      if constexpr (PIPE) {
-        rows.template fetch<1>(p, at, row + S * step);
-        at = at + 1 == S ? 0 : at + 1;
+      for (int k = 0; k < K; ++k) {
+        tile(0, p.x, p.xs, k, v[k]);
+        if constexpr (RES) {
+          const int base = (wt + k * W) * kTile;
+          RawTile<T, VEC> t;
+          uint64_t d[4];
+          tile(1, p.delta, p.ds, k, d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[k][i] = f2_add(v[k][i], d[i]);
+          t.set(v[k]);
+          if (!again && base < D) t.store(reinterpret_cast<T*>(p.h) + row * D, base, lane, D);
+          t.pairs(v[k]);   // as the next layer and the backward see it
+        }
       }
     };
-    if constexpr (!RES) ahead();
+    read(false);
     if constexpr (KEEP) {
       int8_t* c[K];
       float* t[K];
@@ -308,10 +304,11 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       keep_tiles<VEC, K>(v, c, t, base, lane, D);
     }
     // The warp's mean and its sum of squares about it, from differences from its first value, which are
-    // small or exact: one pass and one reduction.  q = sum d^2 - n (mean d)^2 cancels where that value
-    // lies far out; from 2.8 deviations on once more, from the mean, so that the 22 roundings of a sum
-    // weigh 9-fold at most (16384 x 5120 kept in 8 bits: 107 us from 2 deviations on, 104 from 5.5).
-    // v: the differences.
+    // small or exact: one pass and one reduction.  q = sum d^2 - n (mean d)^2 cancels, and differences
+    // are rounded as that value is, where it lies far out; from 2.8 deviations on once more, from the
+    // mean and the row read again, so that the 22 roundings of a sum weigh 9-fold at most (16384 x 5120
+    // kept in 8 bits: 107 us from 2 deviations on, 104 from 5.5).  v: the differences.  (Read again from
+    // its slot, filled anew behind this only; from memory, with the slot given up before: 110 us.)
     float mu, q, from, rest;
     f2_unpack(v[0][0], from, rest);
     from = __shfl_sync(0xffffffffu, from, 0);
@@ -344,11 +341,15 @@ __global__ void __launch_bounds__(kLnMaxWarps * 32) ln_fwd_kernel(const __grid_c
       q = warp_sum(f2_sum(q2)) - nd2;
       mu = from + d;
       if (again || nd2 <= 8.0f * q) break;   // (sums beyond 32 bits, too: infinity - infinity is NaN)
-      away = from - mu;
+      read(true);
+      away = -mu;
       from = mu;
     }
     q = max_nan(q, 0.0f);
-    if constexpr (RES) ahead();
+    if constexpr (PIPE) {   // the slot is read
+      rows.template fetch<1>(p, at, row + S * step);
+      at = at + 1 == S ? 0 : at + 1;
+    }
     if (W > 1) {
       const float2 o = ln_exchange(s_red[team][turn], make_float2(mu, q), wt, lane, team, W);
       const float first = __shfl_sync(0xffffffffu, o.x, 0);   // (again from differences)

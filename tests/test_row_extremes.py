@@ -124,6 +124,19 @@ def test_layer_norm_rounds_the_mean_alone(cuda, mean, dev, D, first):
     near(dw, (g * d * r).sum(0), (g.abs() * (dn + 2 * U * mu.abs() * r)).sum(0) + 10 * U * (g * d * r).abs().sum(0))
 
 
+@pytest.mark.parametrize("residual,saved", [(False, "full"), (True, "full"), (False, "8bit")])
+@pytest.mark.parametrize("D", [520, 1001, 4100, pytest.param(5120, marks=pytest.mark.gpu), pytest.param(16384, marks=pytest.mark.gpu)])
+def test_layer_norm_of_rows_with_values_far_out(device, D, residual, saved):
+    """single values thousands of times the others, first in a row or in a tile: the others keep their places"""
+    x = randn(8, D, seed=D)
+    for i, c in enumerate([0, 256, 1, D - 1]):
+        x[i, c] = 1e4
+    x[4, 0], x[4, D // 2] = 1e4, -1e4
+    x[5, ::256] = 3e3
+    x[6, :8] = -2e4
+    norm_case(device, 8, D, torch.float32, x=x.to(device), residual=residual, saved=saved)
+
+
 @pytest.mark.parametrize("D", [8, 300, 301, 4100, pytest.param(16384, marks=pytest.mark.gpu)])
 def test_layer_norm_of_rows_with_infinities(device, D):
     """NaN throughout, wherever they are, and their gradients; the rows beside them are not touched"""
