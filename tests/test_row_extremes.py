@@ -169,7 +169,7 @@ def test_layer_norm_with_a_bias_alone(device, wtype):
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("D", [256, 1001])
-@pytest.mark.parametrize("scale", [-2.0, 0.0, math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("scale", [-2.0, 0.0, 1e300, math.inf, -math.inf, math.nan])
 def test_rows_of_absent_ids_are_0(device, scale, D, dtype):
     """whatever the scale, and without a sign"""
     ids = torch.tensor([3, -1, 8, 7, 1 << 40, -100], device=device)

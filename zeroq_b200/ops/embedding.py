@@ -24,10 +24,10 @@ def embedding_reference(ids: torch.Tensor, weight: torch.Tensor, scale: float = 
     if V == 0:
         return wide.new_zeros(*ids.shape, weight.shape[1]).to(weight.dtype)
     rows = wide.index_select(0, torch.where(there, ids, torch.zeros_like(ids)).reshape(-1).long())
-    rows = rows.view(*ids.shape, weight.shape[1])
-    rows = torch.where(there[..., None], rows, torch.zeros_like(rows))
-    # (0 by a scale that is not finite would be NaN, by a negative one -0, and so would their gradients)
-    return (rows * torch.full_like(there, scale, dtype=wide.dtype).masked_fill(~there, 1.0)[..., None]).to(weight.dtype)
+    rows, there = rows.view(*ids.shape, weight.shape[1]), there[..., None]
+    none = torch.zeros_like(rows)
+    # (twice: 0 by a scale that is not finite is NaN, by a negative one -0, and so it is on the way back)
+    return torch.where(there, torch.where(there, rows, none) * scale, none).to(weight.dtype)
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
